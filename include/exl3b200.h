@@ -412,6 +412,93 @@ int     exl3b200_tp_step_forward(const Exl3bTpDesc* desc, const Exl3bLayerBufs* 
                                  const float* logits, int64_t n_tok, float* out, int64_t out_pitch, void* stream,
                                  void* const* marks);
 
+/* Experts whose weights are not EXL3 records (kept in f16 / bf16, or in MXFP4), and the norms around a block. No
+ * counterpart in the reference's kernels (its engine serves protected experts and norms); serving only, no gradients.
+ *
+ * MXFP4 (dtype EXL3B_MX4): blocks of 32 values along a row, each an e2m1 code -- two a byte, the lower index in the low
+ * nibble -- times one power of two held as E8M0 (2^(byte - 127), 255 NaN). Codes [rows][cols / 2] bytes and scales
+ * [rows][cols / 32] bytes, each with its row pitch in bytes.
+ *   mx4_quantize:    x (f32 / f16 / bf16, row pitch in elements) -> codes, scales. A block's scale is
+ *                    2^(floor(log2(max |x|)) - 2), no less than 2^-127; values round to nearest, ties to even, and
+ *                    saturate at 6 times the scale. A block with a NaN or an infinity: scale 255, codes 0.
+ *   mx4_dequantize:  the values back, in f32 / f16 / bf16.
+ *   mx4_tile_scales: a weight's scales (per expert `rows` rows, expert_pitch bytes apart) into the form grouped_mm
+ *                    reads, once, when the weight is loaded; `act` as the product's. mx4_tiled_bytes sizes it (-1:
+ *                    refused).
+ * cols a multiple of 32; rows of x, y on 16-byte boundaries, codes on 4-byte ones (grouped_mm: 16). */
+enum { EXL3B_MX4 = RAD_DT_PLUGIN_BASE + 0x3B4 };
+int     exl3b200_mx4_quantize(const void* x, int x_dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* codes,
+                              int64_t codes_pitch, uint8_t* scales, int64_t scales_pitch, void* stream);
+int     exl3b200_mx4_dequantize(const uint8_t* codes, int64_t codes_pitch, const uint8_t* scales, int64_t scales_pitch,
+                                int64_t rows, int64_t cols, void* y, int y_dtype, int64_t y_pitch, void* stream);
+int64_t exl3b200_mx4_tiled_bytes(int64_t n_expert, int64_t rows, int64_t cols, int act);
+int     exl3b200_mx4_tile_scales(const uint8_t* scales, int64_t scales_pitch, int64_t expert_pitch, int64_t n_expert,
+                                 int64_t rows, int64_t cols, int act, void* tiled, void* stream);
+
+/* grouped_mm: the routing contract's rows (moe_scatter's sorted_tok and expert_offset) times their expert's weight.
+ * Sorted row i of expert e, t = sorted_tok[i] / top_k (top_k 0: the row of x is i itself):
+ *   z[n] = sum over k of x[t][k] * w[e][n][k]  in f32;  act NONE: y[i][n] = z[n] for n < n_out;
+ *   act SILU_MUL: y[i][n] = silu(z[n]) * z[n_out + n], w[e] holding n_out gate rows and then n_out up rows.
+ * Each output is rounded once to y_dtype (RAD_F32, RAD_F16, RAD_BF16, or EXL3B_MX4: codes and scales as mx4_quantize
+ * makes them of the f32 values). Rows outside [expert_offset[0], expert_offset[n_expert]) and dropped slots
+ * (sorted_tok < 0) are zero. expert_offset NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and
+ * slot i is i. dtype: RAD_F16, RAD_BF16, or EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form).
+ * Pitches in elements (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32), n_out of 8
+ * (MXFP4 out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048. */
+enum { EXL3B_ACT_NONE = 0, EXL3B_ACT_SILU_MUL = 1 };
+typedef struct Exl3bGroupedMm {
+    int64_t        n_expert, n_rows, n_out, n_in;
+    int64_t        x_rows, top_k;
+    int32_t        dtype, y_dtype, act, pad0;
+    const void*    x;
+    int64_t        x_pitch;
+    const uint8_t* x_scales;
+    int64_t        x_scales_pitch;
+    const void*    w;
+    int64_t        w_pitch, w_expert_pitch;
+    const void*    w_scales;
+    const int32_t* sorted_tok;
+    const int32_t* expert_offset;
+    void*          y;
+    int64_t        y_pitch;
+    uint8_t*       y_scales;
+    int64_t        y_scales_pitch;
+} Exl3bGroupedMm;
+int     exl3b200_grouped_mm(const Exl3bGroupedMm* mm, void* stream);
+
+/* block_norm: a block's output into the residual stream, and the next block's normed input, one pass over each row
+ * (all in f32, each output rounded once):
+ *   n = branch * rsqrt(mean(branch^2) + post_eps) * post_w      (post_w NULL: n = branch; branch NULL: n = 0)
+ *   r = res_scale * res + g * n                                 (res NULL: r = g * n)  -> out, if given (may be res)
+ *   y = r * rsqrt(mean(r^2) + pre_eps) * pre_w                  -> y and / or its MXFP4 codes and scales, if given
+ * g: 1, sigmoid(gate[row]) (TOKEN, f32 logits), gate[col] (CHANNEL), or sigmoid(gate[row][col]) (ELEMENT). res, out, y,
+ * the weights and the last two gates are of `dtype` (f32 / f16 / bf16), the branch of its own. Pitches in elements,
+ * those of codes and scales in bytes. cols <= 32768, any width and alignment (16-byte rows are faster); MXFP4 output
+ * wants cols a multiple of 32 and every row on 16-byte boundaries. */
+enum { EXL3B_GATE_NONE = 0, EXL3B_GATE_TOKEN = 1, EXL3B_GATE_CHANNEL = 2, EXL3B_GATE_ELEMENT = 3 };
+typedef struct Exl3bBlockNorm {
+    int64_t     rows, cols;
+    int32_t     dtype, branch_dtype, gate_kind;
+    float       res_scale, post_eps, pre_eps;
+    const void* branch;
+    int64_t     branch_pitch;
+    const void* post_w;
+    const void* gate;
+    int64_t     gate_pitch;
+    const void* res;
+    int64_t     res_pitch;
+    void*       out;
+    int64_t     out_pitch;
+    const void* pre_w;
+    void*       y;
+    int64_t     y_pitch;
+    uint8_t*    y_codes;
+    int64_t     y_codes_pitch;
+    uint8_t*    y_scales;
+    int64_t     y_scales_pitch;
+} Exl3bBlockNorm;
+int     exl3b200_block_norm(const Exl3bBlockNorm* norm, void* stream);
+
 /* How long a kernel that waits on another rank's flag (p2p_wait_dispatch, p2p_wait_combine, tp_reduce, tp_pull)
  * waits before it gives up, sets its status and the error word, and returns: `ns` nanoseconds, or the default 5 s
  * for ns <= 0 (more than 600 s is refused, RAD_E_INVAL). Process-wide; each launch reads it when it is enqueued

@@ -1,0 +1,181 @@
+"""dense.py -- experts whose weights are not EXL3 records (f16, bf16 or MXFP4) and the norms around a block, over torch
+tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (include/exl3b200.h).
+
+A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
+`run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). The tensors' contents may
+change between runs, their addresses may not. torch only holds memory here; every refusal is the library's own status,
+raised. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
+import ctypes as C
+
+import torch
+
+from .native import BlockNormDesc, GroupedMmDesc, Native
+
+MX4 = 1024 + 0x3B4                      # EXL3B_MX4
+DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+ACTS = {"none": 0, "silu_mul": 1}
+GATES = {"none": 0, "token": 1, "channel": 2, "element": 3}
+
+_native = None
+
+
+def native():
+    global _native
+    if _native is None:
+        _native = Native()
+    return _native
+
+
+def _dtype(t):
+    if t.dtype not in DTYPES:
+        raise ValueError(f"f32, f16 or bf16, not {t.dtype}")
+    return DTYPES[t.dtype]
+
+
+def _rows(t, name, shape=None, dtype=None):
+    """A tensor whose last dimension is dense, on a GPU, of this shape and type: (address, row pitch in elements)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on a GPU")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension is strided")
+    if t.dim() < 2:
+        return t.data_ptr(), 0
+    return t.data_ptr(), t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), t.shape[-1])
+
+
+# ------------------------------------------------------------------------------------------------ MXFP4
+def mx4_empty(rows, cols, device="cuda"):
+    """(codes, scales) for `rows` rows of `cols` values."""
+    return (torch.empty((rows, cols // 2), dtype=torch.uint8, device=device),
+            torch.empty((rows, cols // 32), dtype=torch.uint8, device=device))
+
+
+def mx4_quantize(x, codes, scales, stream=0):
+    """x [rows, cols] in f32, f16 or bf16 -> its MXFP4 codes and scales."""
+    rows, cols = x.shape
+    xp, pitch = _rows(x, "x")
+    cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
+    sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
+    native().mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch, stream)
+    return codes, scales
+
+
+def mx4_dequantize(codes, scales, y, stream=0):
+    """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
+    rows, cols = y.shape
+    yp, pitch = _rows(y, "y")
+    cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
+    sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
+    native().mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch, stream)
+    return y
+
+
+def mx4_tile_scales(scales, act="none", stream=None):
+    """A weight's scales [experts, rows, cols / 32] in the form GroupedMm reads; once, when the weight is loaded. On the
+    current stream unless another is given."""
+    n_expert, rows, blocks = scales.shape
+    sp, pitch = _rows(scales, "scales", dtype=torch.uint8)
+    out = torch.empty(native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act]), dtype=torch.uint8,
+                      device=scales.device)
+    if stream is None:
+        stream = torch.cuda.current_stream(scales.device).cuda_stream
+    native().mx4_tile_scales(sp, pitch, scales.stride(0), n_expert, rows, blocks * 32, ACTS[act], out.data_ptr(), stream)
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ plans
+class _Plan:
+    _entry = None
+
+    def _finish(self, desc, *tensors):
+        self.desc, self._keep = desc, tensors
+        self._addr, self._call = C.addressof(desc), getattr(native().lib, self._entry)
+
+    def run(self, stream=0):
+        rc = self._call(self._addr, stream)
+        if rc:
+            raise RuntimeError(f"{self._entry}: status {rc}")
+
+
+class GroupedMm(_Plan):
+    """y[i] = x[t(i)] @ w[e(i)].T for the sorted rows i of the routing contract (act "silu_mul": silu of the first half
+    of w's rows times the second).
+
+    x [x_rows, n_in] and w [experts, w_rows, n_in] in f16 or bf16; or MXFP4 codes (uint8, half as wide) with x_scales
+    [x_rows, n_in / 32] and w_scales from mx4_tile_scales. y [rows, n_out] in f32, f16 or bf16, or MXFP4 codes with
+    y_scales. expert_offset i32 [experts + 1] (None: one expert); sorted_tok i32 [rows] (None: no dropped slot). top_k:
+    row i reads x row sorted_tok[i] // top_k; 0: x is sorted already."""
+    _entry = "exl3b200_grouped_mm"
+
+    def __init__(self, *, x, w, y, expert_offset=None, sorted_tok=None, top_k=0, act="none", x_scales=None,
+                 w_scales=None, y_scales=None):
+        mx, mx_out = w.dtype == torch.uint8, y.dtype == torch.uint8
+        d = GroupedMmDesc()
+        per, per_out = 2 if mx else 1, 2 if mx_out else 1
+        if x.dtype != w.dtype:
+            raise ValueError(f"x is {x.dtype}, w {w.dtype}")
+        d.n_expert, d.n_rows, d.x_rows, d.top_k = w.shape[0], y.shape[0], x.shape[0], top_k
+        d.n_out, d.n_in, d.act = y.shape[1] * per_out, x.shape[1] * per, ACTS[act]
+        d.dtype, d.y_dtype = MX4 if mx else _dtype(x), MX4 if mx_out else _dtype(y)
+        _rows(w, "w", (d.n_expert, d.n_out * (2 if d.act else 1), x.shape[1]))
+        d.x, pitch = _rows(x, "x")
+        d.x_pitch = pitch * per
+        d.w, pitch = _rows(w, "w")
+        d.w_pitch, d.w_expert_pitch = pitch * per, w.stride(0) * per
+        d.y, pitch = _rows(y, "y")
+        d.y_pitch = pitch * per_out
+        if mx:
+            d.x_scales, d.x_scales_pitch = _rows(x_scales, "x_scales", (d.x_rows, d.n_in // 32), torch.uint8)
+            want = native().mx4_tiled_bytes(d.n_expert, w.shape[1], d.n_in, d.act)
+            d.w_scales, _ = _rows(w_scales, "w_scales", (want,), torch.uint8)
+        if mx_out:
+            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", (d.n_rows, d.n_out // 32), torch.uint8)
+        if expert_offset is not None:
+            d.expert_offset, _ = _rows(expert_offset, "expert_offset", (d.n_expert + 1,), torch.int32)
+        if sorted_tok is not None:
+            d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", (d.n_rows,), torch.int32)
+        self._finish(d, x, w, y, expert_offset, sorted_tok, x_scales, w_scales, y_scales)
+
+
+class BlockNorm(_Plan):
+    """The norm behind a block with its gate and residual scale, and the norm before the next, in one pass:
+    r = res_scale * res + g * rmsnorm(branch) * post_w -> out; rmsnorm(r) * pre_w -> y and / or (y_codes, y_scales).
+    gate_kind: "none"; "token" (f32 logits [rows]) or "element" (logits [rows, cols]) through a sigmoid; "channel"
+    ([cols], as it is). Every tensor but branch and a token gate shares one of f32, f16, bf16."""
+    _entry = "exl3b200_block_norm"
+
+    def __init__(self, *, branch=None, post_w=None, post_eps=1e-6, gate=None, gate_kind="none", res=None, res_scale=1.0,
+                 out=None, pre_w=None, pre_eps=1e-6, y=None, y_codes=None, y_scales=None):
+        d = BlockNormDesc()
+        lead = branch if branch is not None else res
+        if lead is None:
+            raise ValueError("neither branch nor res")
+        rows, cols = d.rows, d.cols = lead.shape
+        typed = next((t for t in (res, out, y, post_w, pre_w) if t is not None), lead)
+        dt = typed.dtype
+        d.dtype, d.gate_kind = _dtype(typed), GATES[gate_kind]
+        d.res_scale, d.post_eps, d.pre_eps = res_scale, post_eps, pre_eps
+        if branch is not None:
+            d.branch, d.branch_pitch = _rows(branch, "branch", (rows, cols))
+            d.branch_dtype = _dtype(branch)
+        for name, t in (("res", res), ("out", out), ("y", y)):
+            if t is not None:
+                p, pitch = _rows(t, name, (rows, cols), dt)
+                setattr(d, name, p)
+                setattr(d, name + "_pitch", pitch)
+        for name, t in (("post_w", post_w), ("pre_w", pre_w)):
+            if t is not None:
+                setattr(d, name, _rows(t, name, (cols,), dt)[0])
+        if gate is not None:
+            shape, want = {"token": ((rows,), torch.float32), "channel": ((cols,), dt),
+                           "element": ((rows, cols), dt)}.get(gate_kind, (None, None))
+            d.gate, d.gate_pitch = _rows(gate, "gate", shape, want)
+        if y_codes is not None:
+            d.y_codes, d.y_codes_pitch = _rows(y_codes, "y_codes", (rows, cols // 2), torch.uint8)
+        if y_scales is not None:
+            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", (rows, cols // 32), torch.uint8)
+        self._finish(d, branch, post_w, gate, res, out, pre_w, y, y_codes, y_scales)

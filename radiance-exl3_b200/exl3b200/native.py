@@ -56,6 +56,24 @@ class TpDesc(C.Structure):
                 ("peers", _VP), ("offs", _I64 * 4), ("epoch", _VP), ("status", _VP)]
 
 
+class GroupedMmDesc(C.Structure):
+    """Exl3bGroupedMm (include/exl3b200.h)."""
+    _fields_ = [(n, _I64) for n in ("n_expert", "n_rows", "n_out", "n_in", "x_rows", "top_k")] + [
+        (n, C.c_int32) for n in ("dtype", "y_dtype", "act", "pad0")] + [
+        ("x", _VP), ("x_pitch", _I64), ("x_scales", _VP), ("x_scales_pitch", _I64), ("w", _VP), ("w_pitch", _I64),
+        ("w_expert_pitch", _I64), ("w_scales", _VP), ("sorted_tok", _VP), ("expert_offset", _VP), ("y", _VP),
+        ("y_pitch", _I64), ("y_scales", _VP), ("y_scales_pitch", _I64)]
+
+
+class BlockNormDesc(C.Structure):
+    """Exl3bBlockNorm (include/exl3b200.h)."""
+    _fields_ = [("rows", _I64), ("cols", _I64)] + [(n, C.c_int32) for n in ("dtype", "branch_dtype", "gate_kind")] + [
+        (n, C.c_float) for n in ("res_scale", "post_eps", "pre_eps")] + [
+        ("branch", _VP), ("branch_pitch", _I64), ("post_w", _VP), ("gate", _VP), ("gate_pitch", _I64), ("res", _VP),
+        ("res_pitch", _I64), ("out", _VP), ("out_pitch", _I64), ("pre_w", _VP), ("y", _VP), ("y_pitch", _I64),
+        ("y_codes", _VP), ("y_codes_pitch", _I64), ("y_scales", _VP), ("y_scales_pitch", _I64)]
+
+
 def marks_array(events):
     """A C array of cudaEvent_t from torch.cuda.Event objects (None entries stay NULL), or None. torch creates an
     event's handle at its first record, so each is recorded once here before its handle is taken."""
@@ -142,6 +160,15 @@ class Native:
                                             _I64, _VP, _VP, _VP]
         L.exl3b200_tp_reduce.argtypes = [_VP, _VP, _I64, _I64, _I64, _I64, _I64, _VP, _VP]
         L.exl3b200_tp_pull.argtypes = [_VP, _VP, _I64, _I64, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _VP]
+
+        L.exl3b200_mx4_quantize.argtypes = [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _VP]
+        L.exl3b200_mx4_dequantize.argtypes = [_VP, _I64, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP]
+        L.exl3b200_mx4_tiled_bytes.restype = _I64
+        L.exl3b200_mx4_tiled_bytes.argtypes = [_I64, _I64, _I64, _I]
+        L.exl3b200_mx4_tile_scales.argtypes = [_VP, _I64, _I64, _I64, _I64, _I64, _I, _VP, _VP]
+        # descriptors by address: a plan takes its own once (ctypes.addressof), not a byref a call
+        L.exl3b200_grouped_mm.argtypes = [_VP, _VP]
+        L.exl3b200_block_norm.argtypes = [_VP, _VP]
 
     @staticmethod
     def _check(rc, what):
@@ -387,3 +414,28 @@ class Native:
         """out_dtype: 1 (RAD_F32) or 3 (RAD_BF16)."""
         self._check(self.lib.exl3b200_moe_block_forward(C.byref(desc), C.byref(bufs), x, logits, n_tok, out, out_dtype,
                                                         stream), "exl3b200_moe_block_forward")
+
+    # ---- experts not kept as EXL3 records, and the norms around a block (exl3b200_dense.c)
+    def mx4_quantize(self, x, x_dtype, x_pitch, rows, cols, codes, codes_pitch, scales, scales_pitch, stream=0):
+        self._check(self.lib.exl3b200_mx4_quantize(x, x_dtype, x_pitch, rows, cols, codes, codes_pitch, scales,
+                                                   scales_pitch, stream), "exl3b200_mx4_quantize")
+
+    def mx4_dequantize(self, codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype, y_pitch, stream=0):
+        self._check(self.lib.exl3b200_mx4_dequantize(codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype,
+                                                     y_pitch, stream), "exl3b200_mx4_dequantize")
+
+    def mx4_tiled_bytes(self, n_expert, rows, cols, act):
+        n = int(self.lib.exl3b200_mx4_tiled_bytes(n_expert, rows, cols, act))
+        if n < 0:
+            raise RuntimeError("exl3b200_mx4_tiled_bytes: the weight's shape was refused")
+        return n
+
+    def mx4_tile_scales(self, scales, scales_pitch, expert_pitch, n_expert, rows, cols, act, tiled, stream=0):
+        self._check(self.lib.exl3b200_mx4_tile_scales(scales, scales_pitch, expert_pitch, n_expert, rows, cols, act,
+                                                      tiled, stream), "exl3b200_mx4_tile_scales")
+
+    def grouped_mm(self, desc, stream=0):
+        self._check(self.lib.exl3b200_grouped_mm(C.addressof(desc), stream), "exl3b200_grouped_mm")
+
+    def block_norm(self, desc, stream=0):
+        self._check(self.lib.exl3b200_block_norm(C.addressof(desc), stream), "exl3b200_block_norm")
