@@ -4,20 +4,27 @@
 //   z[n] = sum over k of x[t(i)][k] * w[e][n][k]  for every sorted row i of expert e (f32 accumulators), then
 //   y[i][n] = z[n], or silu(z[n]) * z[n_out + n] (act silu_mul: w[e] holds n_out gate rows, then n_out up rows).
 //
-// The WEIGHT rows are the MMA's M (128 a block) and the sorted rows its N: experts hold a few to a few hundred rows, N
-// goes in steps of 16, so a group of 40 rows costs 48 columns where rows as M would cost 128. A block of silu_mul is 64
+// The WEIGHT rows are the MMA's M (128 a CTA) and the sorted rows its N: experts hold a few to a few hundred rows, N
+// goes in steps of 16 (PAIR: 32), so a group of 40 rows costs 48 (64) columns where rows as M would cost 128. A block of silu_mul is 64
 // gate rows and their 64 up rows, so the epilogue has both halves of every output.
 //
-// One persistent CTA an SM walks the units (expert, up to NT of its sorted rows, MT blocks), expert-major, so that the
-// CTAs working at one time share an expert's rows and weights in L2. Warps:
-//   0      weights: cp.async.bulk.tensor of the unit's rows, 128 bytes of k a stage (64 f16 / bf16, 256 MXFP4 codes),
-//          128-byte swizzled; MXFP4 scales by one bulk copy a block from their tiled form
-//   1      input rows: tile::gather4 copies (a lane four rows), so x is read through sorted_tok in place
-//   2      MMA issuer (and the TMEM allocation): tcgen05.mma kind::f16 (K 16) or kind::mxf4.block_scale (K 64), four a
-//          block and stage; for MXFP4 tcgen05.cp moves the stage's scales into tensor memory before them
-//   3      MXFP4: the input rows' scales, through registers into the layout tcgen05.cp reads
-//   4..7   epilogue: tcgen05.ld, transposed through shared memory so that a row's outputs are stored contiguously;
-//          silu_mul, and the rounding to y's type (MXFP4: with its blocks' scales), happen there
+// Two forms of one kernel, both persistent over units (expert, a group of its sorted rows, a block of weight rows),
+// expert-major, so that the CTAs working at one time share an expert's rows and weights in L2:
+//   narrow  a CTA a unit of 128 weight rows and up to 32 sorted rows, two CTAs an SM: a few rows an expert, where the
+//           weights' bytes count and units are needed to spread them over the SMs
+//   PAIR    two CTAs (a cluster) a unit of 256 weight rows and up to 256 sorted rows (MXFP4: 224, the scales take
+//           tensor memory), tcgen05 cta_group::2: each CTA brings its 128 weight rows and HALF of the sorted rows, and
+//           both multiply by all of them, 32 KB a CTA for 4.2 MFLOP against 48 KB for a CTA alone
+// Warps of a CTA:
+//   0       weights: cp.async.bulk.tensor of its 128 rows, 128 bytes of k a stage (64 f16 / bf16, 256 MXFP4 codes),
+//           128-byte swizzled; MXFP4 scales by one bulk copy from their tiled form
+//   1       MMA issuer (PAIR: of the even CTA; the odd one's reports its filled stages there): four tcgen05.mma a stage,
+//           kind::f16 (K 16) or kind::mxf4.block_scale (K 64, tcgen05.cp moving the stage's scales before them)
+//   2, 3    MXFP4: the sorted rows' scales, 128 rows a warp, through registers into the layout tcgen05.cp reads
+//   4..7    sorted rows: 16-byte cp.async through sorted_tok into the same swizzle (tile::gather4 copies took ~80 cycles
+//           for four rows: 444 against 205 us at 16 experts, 16384 rows, 1536 -> 4096)
+//   8..     epilogue, groups of four warps: tcgen05.ld, transposed through shared memory so that a row's outputs are
+//           stored contiguously; silu_mul, and the rounding to y's type (MXFP4: with its blocks' scales), happen there
 // Two accumulator buffers in tensor memory: one unit's epilogue runs under the next one's MMAs. Every wait is bounded;
 // one that gives up sets the error word, and every role then drains and leaves.
 #include <cuda.h>
@@ -32,32 +39,35 @@ using namespace exl3b;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kEpiWarp0 = 4, kEpiWarps = 4;
+constexpr int kXWarp0 = 4, kXWarps = 4, kEpiWarp0 = 8;
 constexpr int kRowB = 128;                       // bytes of k a stage: one swizzle row
-constexpr int kSlice = 16;                       // sorted rows the epilogue stages at a time
+constexpr int kW_B = 128 * kRowB;                // a CTA's weight rows of a stage
+constexpr int kSlice = 16;                       // sorted rows an epilogue group stages at a time
+constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
 constexpr int kMaxExpert = 2048;
 
-template <bool MX, int MT, int NT>
+template <bool MX, bool PAIR>
 struct Cfg {
-    static constexpr int W_B = MT * 128 * kRowB;
-    static constexpr int X_B = NT * kRowB;
-    static constexpr int SFW_B = MX ? MT * 1024 : 0;             // two 128-k halves of 512 bytes a block
-    static constexpr int SFX_B = MX ? 1024 : 0;
-    static constexpr int STAGE_B = W_B + X_B + SFW_B + SFX_B;
-    static constexpr int EPI_LD = MT * 128 + 4;                  // f32 a staged row, padded
-    static constexpr int EPI_B = kSlice * EPI_LD * 4;
-    static constexpr int ACC = MT * NT;                          // TMEM columns of one accumulator buffer
-    static constexpr int SFC = MX ? 8 * MT + 8 : 0;              // TMEM columns of a stage's scales
-    static constexpr int COLS = 2 * ACC + 2 * SFC;
-    static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static constexpr int PER_SM = TMEM <= 256 && MT == 1 ? 2 : 1;
-    static constexpr int BUDGET = (PER_SM == 2 ? 112 : 225) * 1024 - 1024 - EPI_B - 512 - kTab * 16 - (kMaxExpert + 4) * 4;
+    static constexpr int NT = !PAIR ? 32 : MX ? 224 : 256;       // sorted rows a unit at most
+    static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
+    static constexpr int EPI_G = PAIR ? 2 : 1;                   // epilogue groups of four warps
+    static constexpr int THREADS = (kEpiWarp0 + 4 * EPI_G) * 32;
+    static constexpr int X_B = NL * kRowB;
+    static constexpr int SFW_B = MX ? 1024 : 0;                  // two 128-k halves of 512 bytes
+    static constexpr int SFX_G = MX ? (NT + 127) / 128 : 0;      // 128-row groups of the sorted rows' scales
+    static constexpr int SFX_B = SFX_G * 1024;
+    static constexpr int STAGE_B = kW_B + X_B + SFW_B + SFX_B;
+    static constexpr int EPI_B = EPI_G * kSlice * kEpiLd * 4;
+    static constexpr int SFC = MX ? 8 + 8 * SFX_G : 0;           // TMEM columns of a stage's scales
+    static constexpr int COLS = 2 * NT + 2 * SFC;
+    static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 512;
+    static constexpr int PER_SM = PAIR ? 1 : 2;
+    static constexpr int BUDGET = (PAIR ? 226 : 113) * 1024 - 1024 - EPI_B - 512 - kTab * 16 - 1024 - (kMaxExpert + 4) * 4;
     static constexpr int ST = BUDGET / STAGE_B > 8 ? 8 : BUDGET / STAGE_B;
     static constexpr int SMEM = 1024 + ST * STAGE_B + EPI_B + 512;   // the unit prefix follows
-    static_assert(COLS <= 512 && ST >= 3, "tensor or shared memory");
-    static_assert(NT <= 128 && (!MX || NT <= 128), "one gather4 a lane; one column group of scales");
+    static_assert(COLS <= 512 && ST >= 4, "tensor or shared memory");
+    static_assert((3 * ST + 4) * 8 + 8 <= 512, "barriers");
 };
 
 struct Unit {
@@ -91,14 +101,14 @@ __device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* p
     const uint32_t local = unit - prefix[lo], g = local / n_mb;
     int64_t r0, r1;
     const uint32_t ng = groups<NT>(p, lo, &r0, &r1);
-    // the expert's rows split evenly over its groups, in steps of 16: no group is left with a sliver
-    const int64_t per = ((r1 - r0 + ng - 1) / ng + 15) / 16 * 16;
+    // the expert's rows split evenly over its groups, in steps of the MMA's N: no group is left with a sliver
+    const int64_t step = 16 * mt, per = ((r1 - r0 + ng - 1) / ng + step - 1) / step * step;
     Unit u;
     u.e = lo;
     u.blk = (int32_t)(local % n_mb) * mt;
     const int64_t a = r0 + g * per, left = r1 - a;
     u.r0 = (int32_t)a;
-    u.nr = (int32_t)(left < 0 ? 0 : left < per ? left : per);
+    u.nr = (int32_t)(left < per ? left : per);
     return u;
 }
 
@@ -117,42 +127,80 @@ __device__ __forceinline__ uint64_t desc_plain(uint32_t a) {      // tcgen05.cp:
     return (uint64_t)((a & 0x3FFFFu) >> 4) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
 
-// Four MMAs of K = 16 (f16 / bf16): a stage of one block. The first accumulates when acc != 0.
+// Four MMAs of K = 16 (f16 / bf16): one stage. The first accumulates when acc != 0.
+#define EXL3B_MMA4_F16(G)                                                                                          \
+    asm volatile(                                                                                                  \
+        "{\n .reg .pred p, e, t;\n .reg .b64 a, b;\n"                                                              \
+        " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"                            \
+        " @e tcgen05.mma.cta_group::" G ".kind::f16 [%0], %1, %2, %3, p;\n"                                        \
+        " add.u64 a, %1, 2; add.u64 b, %2, 2;\n @e tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n"    \
+        " add.u64 a, %1, 4; add.u64 b, %2, 4;\n @e tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n"    \
+        " add.u64 a, %1, 6; add.u64 b, %2, 6;\n @e tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n"    \
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc))
+template <bool PAIR>
 __device__ __forceinline__ void mma4_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p, e, t;\n .reg .b64 a, b;\n"
-        " setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"
-        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        " add.u64 a, %1, 2; add.u64 b, %2, 2;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
-        " add.u64 a, %1, 4; add.u64 b, %2, 4;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
-        " add.u64 a, %1, 6; add.u64 b, %2, 6;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+    if constexpr (PAIR) EXL3B_MMA4_F16("2");
+    else EXL3B_MMA4_F16("1");
 }
-// 512 bytes of scales (32 rows of 16) into four tensor-memory columns of all four lane quadrants.
+// 512 bytes of scales (32 rows of 16) into four tensor-memory columns of all four lane quadrants (PAIR: of both CTAs,
+// each from its own shared memory).
+template <bool PAIR>
 __device__ __forceinline__ void cp_scales(uint32_t t, uint64_t desc) {
-    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-                 " @e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(t), "l"(desc));
+    if constexpr (PAIR)
+        asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                     " @e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(t), "l"(desc));
+    else
+        asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                     " @e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(t), "l"(desc));
 }
-// Four MMAs of K = 64 (MXFP4): a stage of one block. Scales: two 128-k halves of four columns; within a half the first
-// MMA takes bytes 0, 1 of each column and the second bytes 2, 3 (id2: the descriptor with both scale ids at 2).
+// Four MMAs of K = 64 (MXFP4): one stage. Scales: two 128-k halves, sa and sb columns of the first, `hb` columns on for
+// sb's second; within a half the first MMA takes bytes 0, 1 of each column and the second bytes 2, 3 (id2: the
+// descriptor with both scale ids at 2).
+#define EXL3B_MMA4_MX4(G)                                                                                           \
+    asm volatile(                                                                                                   \
+        "{\n .reg .pred p, e, t;\n .reg .b64 a, b;\n .reg .b32 u, v;\n"                                             \
+        " setp.ne.b32 p, %7, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"                             \
+        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"  \
+        " add.u64 a, %1, 2; add.u64 b, %2, 2;\n"                                                                    \
+        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], t;\n"    \
+        " add.u64 a, %1, 4; add.u64 b, %2, 4; add.u32 u, %5, 4; add.u32 v, %6, %8;\n"                               \
+        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [u], [v], t;\n"      \
+        " add.u64 a, %1, 6; add.u64 b, %2, 6;\n"                                                                    \
+        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [u], [v], t;\n"      \
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "r"(sb), "r"(acc), "r"(hb))
+template <bool PAIR>
 __device__ __forceinline__ void mma4_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t id0, uint32_t id2, uint32_t sa,
-                                         uint32_t sb, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p, e, t;\n .reg .b64 a, b;\n .reg .b32 u, v;\n"
-        " setp.ne.b32 p, %7, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"
-        " @e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"
-        " add.u64 a, %1, 2; add.u64 b, %2, 2;\n"
-        " @e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], t;\n"
-        " add.u64 a, %1, 4; add.u64 b, %2, 4; add.u32 u, %5, 4; add.u32 v, %6, 4;\n"
-        " @e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [u], [v], t;\n"
-        " add.u64 a, %1, 6; add.u64 b, %2, 6;\n"
-        " @e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [u], [v], t;\n"
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "r"(sb), "r"(acc));
+                                         uint32_t sb, uint32_t hb, uint32_t acc) {
+    if constexpr (PAIR) EXL3B_MMA4_MX4("2");
+    else EXL3B_MMA4_MX4("1");
 }
+// The MMAs issued so far done -> one arrival on bar (PAIR: on both CTAs' bar of that offset).
+template <bool PAIR>
 __device__ __forceinline__ void commit_el(uint64_t* bar) {
-    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-                 " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n .reg .pred e;\n .reg .b16 m;\n mov.b16 m, 3;\n elect.sync _|e, 0xffffffff;\n"
+                     " @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}\n" ::
+                         "r"(smem_u32(bar))
+                     : "memory");
+    else
+        asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                     " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+                     : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t t, uint32_t cols) {
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float v[16]) {
     uint32_t r[16];
@@ -176,14 +224,21 @@ __device__ __forceinline__ void tma_w_el(void* dst, const CUtensorMap* map, int 
                      "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
 }
-// Four rows of x (each 128 bytes from k offset x), by the calling lane.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int r[4], uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-                 "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]),
-                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
+// 16 bytes global -> shared, or 16 zero bytes (`bytes` 0: nothing is read).
+__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Shared-memory writes this thread made or has been told of become visible to the asynchronous proxy (tcgen05's reads).
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// One arrival on the even CTA's barrier of the same offset. What it and the waits below order across the CTAs is tensor
+// core work alone, which reads each SM's own shared and tensor memory: no thread reads what one of the other CTA wrote,
+// so they keep the default (CTA) scope. Cluster scope costs a fence a stage: 805 against 356 us at 512 experts, 20480
+// rows, 2048 -> 512 silu_mul.
+__device__ __forceinline__ void arrive_even(uint64_t* bar) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n"
+                 " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(bar))
                  : "memory");
 }
-
 // The x row of sorted row i (a dropped slot reads row 0: its outputs are zeroed, not stored), never past x's rows.
 __device__ __forceinline__ int x_row(const Exl3bGmmOp& p, int64_t i) {
     if (p.top_k == 0) return (int)i;
@@ -191,60 +246,64 @@ __device__ __forceinline__ int x_row(const Exl3bGmmOp& p, int64_t i) {
     const int32_t t = f < 0 ? 0 : f / p.top_k;
     return t < p.x_rows ? t : (int)(p.x_rows - 1);
 }
-// Whether any of the epilogue's threads has `bad` set (they decide together: they meet at barriers).
-__device__ __forceinline__ bool epi_any(bool bad) {
+// Barrier over an epilogue group, and the same with a vote: whether any of its threads has `bad` set (they decide
+// together whether to go on, since they meet at barriers).
+__device__ __forceinline__ void epi_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+__device__ __forceinline__ bool epi_any(int g, bool bad) {
     uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
                  : "=r"(r)
-                 : "r"((uint32_t)bad), "n"(kEpiWarps * 32)
+                 : "r"((uint32_t)bad), "r"(1 + g)
                  : "memory");
     return r != 0;
 }
 
-template <bool MX, int MT, int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
-    k_gmm(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Exl3bGmmOp p) {
-    using C = Cfg<MX, MT, NT>;
-    constexpr int ST = C::ST;
+template <bool MX, bool PAIR>
+__global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
+    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p) {
+    using C = Cfg<MX, PAIR>;
+    constexpr int ST = C::ST, NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* w_ring = smem;                                   // [ST][MT][128 rows][128 B]
-    uint8_t* x_ring = w_ring + ST * C::W_B;                   // [ST][NT rows][128 B]
-    uint8_t* sfw_ring = x_ring + ST * C::X_B;                 // [ST][MT][2][512 B]
-    uint8_t* sfx_ring = sfw_ring + ST * C::SFW_B;             // [ST][2][512 B]
+    uint8_t* w_ring = smem;                                   // [ST][128 rows][128 B]
+    uint8_t* x_ring = w_ring + ST * kW_B;                     // [ST][NL rows][128 B]
+    uint8_t* sfw_ring = x_ring + ST * C::X_B;                 // [ST][2 halves][512 B]
+    uint8_t* sfx_ring = sfw_ring + ST * C::SFW_B;             // [ST][2 halves][SFX_G][512 B]
     float* epi = reinterpret_cast<float*>(sfx_ring + ST * C::SFX_B);
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(epi) + C::EPI_B);
-    uint64_t* full = bars;                                    // producers -> MMA (2, MXFP4 3 arrivals)
+    uint64_t* full = bars;                                    // this CTA's producers -> its MMA warp
     uint64_t* empty = full + ST;                              // MMA commit -> producers
-    uint64_t* acc_full = empty + ST;                          // MMA commit -> epilogue [2]
-    uint64_t* acc_empty = acc_full + 2;                       // epilogue -> MMA [2]
+    uint64_t* peer = empty + ST;                              // PAIR, even CTA: the odd one's stage is full
+    uint64_t* acc_full = peer + ST;                           // MMA commit -> epilogue [2]
+    uint64_t* acc_empty = acc_full + 2;                       // epilogue (PAIR: of both CTAs) -> MMA [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
     uint32_t* prefix = reinterpret_cast<uint32_t*>(bars) + 128;   // [n_expert + 1]
     __shared__ Unit utab[kTab];
-    static_assert((2 * ST + 4) * 8 + 8 <= 512, "barriers");
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;
+    const uint32_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
     const int act = p.act;
-    const int blk_out = act ? 64 : 128;                       // outputs a block
-    const uint32_t n_mb = (uint32_t)((p.n_out + blk_out * MT - 1) / (blk_out * MT));
+    const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
+    constexpr int MB = PAIR ? 2 : 1;
+    const uint32_t n_mb = (uint32_t)((p.n_out + blk_out * MB - 1) / (blk_out * MB));
     if (tid == 0) {
-        for (int s = 0; s < ST; ++s) { mbar_init(&full[s], MX ? 3 : 2); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kEpiWarps); }
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&full[s], 1 + 32 * kXWarps + C::SFX_G);
+            mbar_init(&empty[s], 1);
+            mbar_init(&peer[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * C::EPI_G * MB); }
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(C::TMEM)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
     // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts)
     {
-        __shared__ uint32_t wsum[kThreads / 32];
-        const int per = (p.n_expert + kThreads - 1) / kThreads;
-        const int e0 = tid * per, e1 = min(e0 + per, p.n_expert);
+        __shared__ uint32_t wsum[THREADS / 32];
+        const int per = (p.n_expert + THREADS - 1) / THREADS;
+        const int e0 = min(tid * per, p.n_expert), e1 = min(e0 + per, p.n_expert);
         int64_t a, b;
         uint32_t sum = 0;
         for (int e = e0; e < e1; ++e) sum += groups<NT>(p, e, &a, &b) * n_mb;
@@ -262,114 +321,127 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
             prefix[e] = acc;
             acc += groups<NT>(p, e, &a, &b) * n_mb;
         }
-        if (tid == kThreads - 1) prefix[p.n_expert] = acc;
+        if (tid == THREADS - 1) prefix[p.n_expert] = acc;
     }
     __syncthreads();
     const uint32_t n_units = prefix[p.n_expert];
-    const uint32_t n_mine = n_units > blockIdx.x ? (n_units - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
-    for (uint32_t i = tid; i < n_mine && i < kTab; i += kThreads)
-        utab[i] = find_unit<NT>(p, prefix, blockIdx.x + i * gridDim.x, n_mb, MT);
+    const uint32_t n_mine = n_units > first ? (n_units - first + stride - 1) / stride : 0;
+    for (uint32_t i = tid; i < n_mine && i < kTab; i += THREADS)
+        utab[i] = find_unit<NT>(p, prefix, first + i * stride, n_mb, MB);
     fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();                             // both CTAs' barriers and tensor memory are set up
     fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     auto unit_at = [&](uint32_t i) {
-        return i < kTab ? utab[i] : find_unit<NT>(p, prefix, blockIdx.x + i * gridDim.x, n_mb, MT);
+        return i < kTab ? utab[i] : find_unit<NT>(p, prefix, first + i * stride, n_mb, MB);
     };
     const int nck = (int)((p.n_in + (MX ? 255 : 63)) / (MX ? 256 : 64));
     volatile uint32_t* vdead = dead;
-    // a bounded wait by a whole warp; false once any wait of the CTA has given up
+    // A bounded wait by a whole warp, which reports nothing: one that gives up marks the CTA dead, every other wait of the
+    // CTA then gives up at its next try, and the roles leave at their next unit. (A result tested each stage cost up to
+    // a seventh: 205 against 192 us at 16 experts, 16067 rows, 1536 -> 4096; 92 against 79 in MXFP4.)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (mbar_wait_warp(bar, parity, p.err) && !*vdead) return true;
-        *vdead = 1;
-        return false;
+        const uint32_t a = smem_u32(bar);
+        uint64_t t0 = 0;
+        for (;;) {
+            uint32_t done;
+            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+                         " selp.u32 %0, 1, 0, p;\n}\n"
+                         : "=r"(done)
+                         : "r"(a), "r"(parity), "r"(kSuspendNs)
+                         : "memory");
+            if (done || *vdead) break;
+            const uint64_t now = globaltimer_ns();
+            if (!t0) t0 = now;
+            else if (now - t0 > kWaitLimitNs) {
+                *vdead = 1;
+                atomicOr(p.err, 1);
+                break;
+            }
+        }
+        __syncwarp();
     };
-    uint32_t issued = 0;                                      // stages a producer filled
     Pipe pipe;
 
     if (warp == 0) {
         // ---------------------------------------------------------------- weights
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
             const Unit u = unit_at(i);
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST), ++issued) {
-                if (!wait(&empty[pipe.s], pipe.ph ^ 1)) break;
-                mbar_expect_tx_el(&full[pipe.s], C::W_B + C::SFW_B);
-                uint8_t* dst = w_ring + pipe.s * C::W_B;
+            const int b = u.blk + (int)rank;
+            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+                wait(&empty[pipe.s], pipe.ph ^ 1);
+                mbar_expect_tx_el(&full[pipe.s], kW_B + C::SFW_B);
+                uint8_t* dst = w_ring + pipe.s * kW_B;
                 const int k = ck * (MX ? 128 : 64);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int b = u.blk + m;
-                    tma_w_el(dst + m * 16384, &wmap, k, b * blk_out, u.e, &full[pipe.s]);
-                    tma_w_el(dst + m * 16384 + 8192, &wmap, k, act ? (int)p.n_out + b * 64 : b * 128 + 64, u.e, &full[pipe.s]);
-                    if (MX)
-                        tma_bulk_g2s_el(sfw_ring + pipe.s * C::SFW_B + m * 1024,
-                                        p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes + ck * 1024, 1024,
-                                        &full[pipe.s]);
-                }
+                tma_w_el(dst, &wmap, k, b * blk_out, u.e, &full[pipe.s]);
+                if (act) tma_w_el(dst + kW_B / 2, &wmap, k, (int)p.n_out + b * 64, u.e, &full[pipe.s]);
+                if (MX)
+                    tma_bulk_g2s_el(sfw_ring + pipe.s * C::SFW_B,
+                                    p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes + ck * 1024, 1024,
+                                    &full[pipe.s]);
+            }
+        }
+        // after a wait that gave up: a millisecond for the copies still in flight, before the CTA's memory goes
+        if (*vdead)
+            for (int j = 0; j < 50; ++j) __nanosleep(20000);
+    } else if (warp == 1 && rank == 1) {
+        // ---------------------------------------------------------------- PAIR, odd CTA: its filled stages, reported
+        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+                wait(&full[pipe.s], pipe.ph);
+                proxy_fence();
+                if (lane == 0) arrive_even(&peer[pipe.s]);
+                __syncwarp();
             }
         }
     } else if (warp == 1) {
-        // ---------------------------------------------------------------- input rows
-        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-            const Unit u = unit_at(i);
-            const int n = (u.nr + 15) & ~15;
-            int r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = 4 * lane + j < u.nr ? x_row(p, u.r0 + 4 * lane + j) : 0;
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST), ++issued) {
-                if (!wait(&empty[pipe.s], pipe.ph ^ 1)) break;
-                mbar_expect_tx_el(&full[pipe.s], n * kRowB);
-                __syncwarp();
-                if (4 * lane < n)
-                    tma_gather4(smem_u32(x_ring + pipe.s * C::X_B) + lane * 512, &xmap, ck * (MX ? 128 : 64), r, &full[pipe.s]);
-                __syncwarp();
-            }
-        }
-    } else if (warp == 2) {
         // ---------------------------------------------------------------- MMA issuer
         const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
         const uint64_t swd0 = desc_plain(smem_u32(sfw_ring)), sxd0 = desc_plain(smem_u32(sfx_ring));
         uint32_t ab = 0, sfp = 0;
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i, ab ^= 1) {
             const Unit u = unit_at(i);
-            const uint32_t n = (u.nr + 15) & ~15;
-            // D f32, both operands K-major, M 128, N n; MXFP4: e2m1, E8M0 scales
-            const uint32_t idesc = MX ? 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | 8u << 24
-                                      : 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u) | (n >> 3) << 17 | 8u << 24;
-            if (!wait(&acc_empty[ab], ((i >> 1) & 1) ^ 1)) break;
+            const uint32_t n = (u.nr + 16 * MB - 1) & ~(16 * MB - 1);
+            // D f32, both operands K-major, M 128 (PAIR: 256), N n; MXFP4: e2m1, E8M0 scales
+            const uint32_t idesc = (n >> 3) << 17 | (8u * MB) << 24 |
+                                   (MX ? 1u << 7 | 1u << 10 | 1u << 23 : 1u << 4 | (p.bf16 ? 1u << 7 | 1u << 10 : 0u));
+            wait(&acc_empty[ab], ((i >> 1) & 1) ^ 1);
             fence_after();
+            const uint32_t d = tmem + ab * NT;
             for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
-                if (!wait(&full[pipe.s], pipe.ph)) break;
+                wait(&full[pipe.s], pipe.ph);
+                if (PAIR) wait(&peer[pipe.s], pipe.ph);
+                proxy_fence();
                 fence_after();
-                const uint64_t xd = xd0 + (uint64_t)(pipe.s * C::X_B >> 4);
-                const uint32_t sf = tmem + 2 * C::ACC + sfp * C::SFC;
-                if (MX) {
+                const uint64_t wd = wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd = xd0 + (uint64_t)(pipe.s * C::X_B >> 4);
+                if constexpr (MX) {
+                    const uint32_t sa = tmem + 2 * NT + sfp * C::SFC, sb = sa + 8;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        cp_scales(sf + 8 * MT + 4 * h, sxd0 + (uint64_t)((pipe.s * C::SFX_B + h * 512) >> 4));
+                        cp_scales<PAIR>(sa + 4 * h, swd0 + (uint64_t)((pipe.s * C::SFW_B + h * 512) >> 4));
 #pragma unroll
-                        for (int m = 0; m < MT; ++m)
-                            cp_scales(sf + 8 * m + 4 * h, swd0 + (uint64_t)((pipe.s * C::SFW_B + m * 1024 + h * 512) >> 4));
+                        for (int g = 0; g < C::SFX_G; ++g)
+                            cp_scales<PAIR>(sb + 4 * (h * C::SFX_G + g),
+                                            sxd0 + (uint64_t)((pipe.s * C::SFX_B + (h * C::SFX_G + g) * 512) >> 4));
                     }
+                    mma4_mx4<PAIR>(d, wd, xd, idesc, idesc | 2u << 4 | 2u << 29, sa, sb, 4 * C::SFX_G, ck ? 1u : 0u);
+                    sfp ^= 1;
+                } else {
+                    mma4_f16<PAIR>(d, wd, xd, idesc, ck ? 1u : 0u);
                 }
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint32_t d = tmem + ab * C::ACC + m * NT;
-                    const uint64_t wd = wd0 + (uint64_t)((pipe.s * C::W_B + m * 16384) >> 4);
-                    if (MX) mma4_mx4(d, wd, xd, idesc, idesc | 2u << 4 | 2u << 29, sf + 8 * m, sf + 8 * MT, ck ? 1u : 0u);
-                    else mma4_f16(d, wd, xd, idesc, ck ? 1u : 0u);
-                }
-                sfp ^= 1;
-                commit_el(&empty[pipe.s]);
+                commit_el<PAIR>(&empty[pipe.s]);
             }
-            commit_el(&acc_full[ab]);
+            commit_el<PAIR>(&acc_full[ab]);
         }
-    } else if (warp == 3) {
-        // ---------------------------------------------------------------- MXFP4: the input rows' scales
-        // Lane l holds rows l, l + 32, ... of the group, so that it writes 16 consecutive bytes of the layout (row r at
-        // (r % 32) * 16 + (r / 32) * 4, four scales of 128 k). Chunks are fetched kAhead at a time, one batch ahead.
-        if (MX) {
-            constexpr int Q = (NT + 31) / 32, kAhead = 4;
+    } else if (warp < kXWarp0) {
+        // ---------------------------------------------------------------- MXFP4: the sorted rows' scales
+        // Warp 2 the unit's rows 0..127, warp 3 (PAIR) the others; both CTAs of a pair need them all. Lane l holds rows
+        // l, l + 32, ... of the group, so that it writes 16 consecutive bytes of the layout (row r at (r % 32) * 16 +
+        // (r / 32) * 4, four scales of 128 k). Chunks are fetched kAhead at a time, one batch ahead.
+        const int g = warp - 2;
+        if (MX && g < C::SFX_G) {
+            constexpr int Q = NT < 128 ? NT / 32 : 4, kAhead = 4;
             const int nsc = (int)(p.n_in / 32);
             const bool wide = (p.xs_pitch & 7) == 0 && (reinterpret_cast<uintptr_t>(p.x_scales) & 7) == 0;
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
@@ -377,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
                 const uint8_t* src[Q];
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
-                    const int j = lane + 32 * q;
+                    const int j = g * 128 + lane + 32 * q;
                     src[q] = j < u.nr ? p.x_scales + (int64_t)x_row(p, u.r0 + j) * p.xs_pitch : nullptr;
                 }
                 auto fetch = [&](int ck, uint2 v[Q]) {
@@ -399,23 +471,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
                 uint2 cur[kAhead][Q], nxt[kAhead][Q];
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) fetch(a, cur[a]);
-                bool go = true;
-                for (int c0 = 0; c0 < nck && go; c0 += kAhead) {
+                for (int c0 = 0; c0 < nck; c0 += kAhead) {
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) fetch(c0 + kAhead + a, nxt[a]);
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) {
-                        if (c0 + a >= nck || !go) continue;
-                        if (!wait(&empty[pipe.s], pipe.ph ^ 1)) { go = false; continue; }
+                        if (c0 + a >= nck) continue;
+                        wait(&empty[pipe.s], pipe.ph ^ 1);
                         uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
                         lo.x = cur[a][0].x; hi.x = cur[a][0].y;
                         if (Q > 1) { lo.y = cur[a][Q > 1 ? 1 : 0].x; hi.y = cur[a][Q > 1 ? 1 : 0].y; }
                         if (Q > 2) { lo.z = cur[a][Q > 2 ? 2 : 0].x; hi.z = cur[a][Q > 2 ? 2 : 0].y; }
                         if (Q > 3) { lo.w = cur[a][Q > 3 ? 3 : 0].x; hi.w = cur[a][Q > 3 ? 3 : 0].y; }
-                        uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B) + lane;
+                        uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
                         dst[0] = lo;
-                        dst[32] = hi;
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        dst[C::SFX_G * 32] = hi;
+                        proxy_fence();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&full[pipe.s]);
                         pipe.next(ST);
@@ -427,20 +498,56 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
                 }
             }
         }
+    } else if (warp < kEpiWarp0) {
+        // ---------------------------------------------------------------- sorted rows
+        // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's barrier
+        // when they have landed. The MMA warp, which sees that, makes them visible to the asynchronous proxy (a fence by
+        // the loaders would wait for every copy they have in flight).
+        constexpr int RP = (C::NL + 15) / 16;
+        const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
+        const int kb = (int)(MX ? p.n_in / 2 : p.n_in * 2);
+        const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
+        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+            const Unit u = unit_at(i);
+            const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB, r1 = (int)rank * nl;
+            const uint8_t* src[RP];
+            uint32_t live = 0;
+#pragma unroll
+            for (int j = 0; j < RP; ++j) {
+                const int r = rr + 16 * j, at = r1 + r;
+                const bool ok = r < nl && at < u.nr;
+                src[j] = static_cast<const uint8_t*>(p.x) + (ok ? (int64_t)x_row(p, u.r0 + at) * p.x_pitch_bytes + c * 16 : 0);
+                live |= (uint32_t)ok << j;
+            }
+            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+                wait(&empty[pipe.s], pipe.ph ^ 1);
+                const bool in = ck * kRowB + c * 16 < kb;
+                const uint32_t dst = dst0 + pipe.s * C::X_B;
+#pragma unroll
+                for (int j = 0; j < RP; ++j)
+                    if (rr + 16 * j < nl) {
+                        const bool ok = in && (live >> j & 1);
+                        cp16(dst + j * 16 * kRowB, ok ? src[j] + ck * kRowB : src[j], ok ? 16 : 0);
+                    }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[pipe.s])) : "memory");
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ---------------------------------------------------------------- epilogue
-        const int q = warp & 3, ew = warp - kEpiWarp0;
+        const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
         const int es = p.y_dtype == RAD_F32 ? 4 : 2;
         uint8_t* const y = static_cast<uint8_t*>(p.y);
         const bool mx_out = p.y_dtype == EXL3B_MX4;
         // rows no unit writes (outside the runs, dropped slots) are zero: a warp clears a row
         {
+            constexpr int EW = 4 * C::EPI_G;
             int64_t lo = 0, hi = p.n_rows;
             if (p.expert_offset) {
                 lo = p.expert_offset[0];
                 hi = p.expert_offset[p.n_expert];
             }
-            for (int64_t b = ((int64_t)blockIdx.x * kEpiWarps + ew) * 32; b < p.n_rows; b += (int64_t)gridDim.x * kEpiWarps * 32) {
+            for (int64_t b = ((int64_t)blockIdx.x * EW + ew) * 32; b < p.n_rows; b += (int64_t)gridDim.x * EW * 32) {
                 const int64_t i = b + lane;
                 const bool gone = i < p.n_rows && (i < lo || i >= hi || (p.sorted_tok && p.sorted_tok[i] < 0));
                 uint32_t mask = __ballot_sync(0xFFFFFFFFu, gone);
@@ -457,40 +564,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
                 }
             }
         }
-        const int oc = MT * blk_out;                          // outputs a unit: 8 a lane
-        const int lpt = oc / 8, tpw = 32 / lpt;               // lanes a row, rows a warp stores at a time
-        const int c0 = (lane % lpt) * 8;                      // the lane's first output in the unit
-        const int sc = act ? (c0 >> 6) * 128 + (c0 & 63) : c0;   // ... and its column in the staged row
+        float* const st = epi + g * kSlice * kEpiLd;
+        const int lpt = act ? 8 : 16, tpw = 32 / lpt;         // lanes a row (8 outputs a lane), rows a warp stores at a time
+        const int c0 = (lane % lpt) * 8;                      // the lane's first output in the block (and staged column)
         uint32_t ab = 0;
         for (uint32_t i = 0; i < n_mine; ++i, ab ^= 1) {
             const Unit u = unit_at(i);
-            const int64_t n0 = (int64_t)u.blk * blk_out + c0;
+            const int64_t n0 = (int64_t)(u.blk + rank) * blk_out + c0;
             const bool col_ok = n0 < p.n_out;
-            if (epi_any(!wait(&acc_full[ab], (i >> 1) & 1))) break;
+            wait(&acc_full[ab], (i >> 1) & 1);
+            if (epi_any(g, *vdead)) break;
             fence_after();
-            for (int t0 = 0; t0 < u.nr; t0 += kSlice) {
+            for (int t0 = g * kSlice; t0 < u.nr; t0 += C::EPI_G * kSlice) {
+                float a[16];
+                tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    float v[16];
-                    tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * C::ACC + m * NT + t0, v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) epi[j * C::EPI_LD + m * 128 + 32 * q + lane] = v[j];
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-                for (int j = ew * tpw + lane / lpt; j < kSlice; j += kEpiWarps * tpw) {
+                for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = a[j];
+                epi_sync(g);
+                for (int j = q * tpw + lane / lpt; j < kSlice; j += 4 * tpw) {
                     const int64_t r = u.r0 + t0 + j;
                     const bool row_ok = t0 + j < u.nr && !(p.sorted_tok && p.sorted_tok[r] < 0);
-                    float v[8];
-                    {
-                        const float4* s = reinterpret_cast<const float4*>(&epi[j * C::EPI_LD + sc]);
-                        const float4 a = s[0], b = s[1];
-                        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-                    }
+                    const float4* s = reinterpret_cast<const float4*>(&st[j * kEpiLd + c0]);
+                    const float4 s0 = s[0], s1 = s[1];
+                    float v[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
                     if (act) {
-                        const float4* s = reinterpret_cast<const float4*>(&epi[j * C::EPI_LD + sc + 64]);
-                        const float4 a = s[0], b = s[1];
-                        const float up[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+                        const float4 u0 = s[16], u1 = s[17];
+                        const float up[8] = { u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w };
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + __expf(-v[e])) * up[e];
                     }
@@ -507,25 +606,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<MX, MT, NT>::PER_SM)
                         else st8<3>(dst, v);
                     }
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                epi_sync(g);
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[ab]);
-        }
-    }
-    // after a wait that gave up: a producer's copies still in flight land before the CTA's memory goes
-    if (*vdead && (warp == 0 || warp == 1)) {
-        for (uint32_t j = 0; j < ST && j < issued; ++j) {
-            const uint32_t at = issued - 1 - j;
-            mbar_wait_warp(&full[at % ST], (at / ST) & 1, nullptr);
+            if (lane == 0) {
+                if (PAIR) arrive_even(&acc_empty[ab]);
+                else mbar_arrive(&acc_empty[ab]);
+            }
         }
     }
     fence_before();
     __syncthreads();
-    if (warp == 2) {
+    if (PAIR) cluster_sync_all();                             // neither CTA's memory goes while the other uses it
+    if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+        tmem_free<PAIR>(tmem, C::TMEM);
     }
 }
 
@@ -545,57 +641,57 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// Weights: [expert][row][k], boxes of 64 rows; input rows: [row][k], boxes of one row (gather4). 128 bytes of k a box.
-int make_maps(const Exl3bGmmOp* p, CUtensorMap* wmap, CUtensorMap* xmap) {
+// Weights: [expert][row][k], boxes of 128 bytes of k and a block's 128 rows (silu_mul: its 64 gate or 64 up rows).
+int make_map(const Exl3bGmmOp* p, CUtensorMap* map) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return -6;
     const CUtensorMapDataType dt = p->mx4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                           : p->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const cuuint64_t k = (cuuint64_t)(p->mx4 ? p->n_in / 2 : p->n_in);
-    const cuuint32_t kb = p->mx4 ? 128 : 64, one[3] = { 1, 1, 1 };
-    const cuuint64_t wd[3] = { k, (cuuint64_t)p->w_rows, (cuuint64_t)p->n_expert };
-    const cuuint64_t ws[2] = { (cuuint64_t)p->w_pitch_bytes, (cuuint64_t)p->w_expert_bytes };
-    const cuuint32_t wb[3] = { kb, 64, 1 };
-    if (fn(wmap, dt, 3, const_cast<void*>(p->w), wd, ws, wb, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return -6;
-    const cuuint64_t xd[2] = { k, (cuuint64_t)p->x_rows };
-    const cuuint64_t xs[1] = { (cuuint64_t)p->x_pitch_bytes };
-    const cuuint32_t xb[2] = { kb, 1 };
-    if (fn(xmap, dt, 2, const_cast<void*>(p->x), xd, xs, xb, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return -6;
-    return 0;
+    const cuuint64_t dims[3] = { (cuuint64_t)(p->mx4 ? p->n_in / 2 : p->n_in), (cuuint64_t)p->w_rows, (cuuint64_t)p->n_expert };
+    const cuuint64_t strides[2] = { (cuuint64_t)p->w_pitch_bytes, (cuuint64_t)p->w_expert_bytes };
+    const cuuint32_t box[3] = { p->mx4 ? 128u : 64u, p->act ? 64u : 128u, 1u }, one[3] = { 1, 1, 1 };
+    return fn(map, dt, 3, const_cast<void*>(p->w), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0 : -6;
 }
 
-template <bool MX, int MT, int NT>
-int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
-    using C = Cfg<MX, MT, NT>;
-    CUtensorMap wmap, xmap;
-    const int rc = make_maps(p, &wmap, &xmap);
-    if (rc) return rc;
-    const int smem = C::SMEM + (p->n_expert + 4) * 4;
-    auto kern = k_gmm<MX, MT, NT>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -6;
-    // at most this many units: a group a live expert, and one more each NT rows
-    const int64_t blk = (p->act ? 64 : 128) * MT, n_mb = (p->n_out + blk - 1) / blk;
+// An upper bound of the units: a group a live expert and one more each NT rows, times the blocks.
+int64_t most_units(const Exl3bGmmOp* p, int nt, int mb) {
+    const int64_t blk = (p->act ? 64 : 128) * mb;
     const int64_t live = p->n_expert < p->n_rows ? p->n_expert : p->n_rows;
-    const int64_t most = (live + p->n_rows / NT) * n_mb;
-    int64_t grid = (int64_t)sm_count * C::PER_SM;
-    if (most < grid) grid = most;
-    kern<<<(unsigned)grid, kThreads, smem, st>>>(wmap, xmap, *p);
-    return cudaGetLastError() == cudaSuccess ? 0 : -6;
+    return (live + p->n_rows / nt) * ((p->n_out + blk - 1) / blk);
+}
+
+template <bool MX, bool PAIR>
+int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
+    using C = Cfg<MX, PAIR>;
+    CUtensorMap map;
+    const int rc = make_map(p, &map);
+    if (rc) return rc;
+    auto kern = k_gmm<MX, PAIR>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.dynamicSmemBytes = C::SMEM + (p->n_expert + 4) * 4;
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.stream = st;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess) return -6;
+    const int64_t room = PAIR ? sm_count / 2 : (int64_t)sm_count * C::PER_SM, most = most_units(p, C::NT, PAIR ? 2 : 1);
+    cfg.gridDim = dim3((unsigned)((most < room ? most : room) * (PAIR ? 2 : 1)));
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = PAIR ? 2 : 1;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, map, *p) == cudaSuccess ? 0 : -6;
 }
 
 }  // namespace
 
 extern "C" int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // narrow units (128 weight rows, 32 sorted rows, two CTAs an SM) while the experts hold few rows on average: more
-    // units to spread a few experts' weights over the SMs; wide ones (256 weight rows) read each input row half as often
-    const bool narrow = p->n_rows <= 16 * (int64_t)p->n_expert;
-    if (p->mx4) return narrow ? launch<true, 1, 32>(p, sm_count, st) : launch<true, 2, 112>(p, sm_count, st);
-    return narrow ? launch<false, 1, 32>(p, sm_count, st) : launch<false, 2, 128>(p, sm_count, st);
+    const bool pair = p->n_rows > 16 * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4;
+    if (p->mx4) return pair ? launch<true, true>(p, sm_count, st) : launch<true, false>(p, sm_count, st);
+    return pair ? launch<false, true>(p, sm_count, st) : launch<false, false>(p, sm_count, st);
 }
 
 extern "C" int exl3b_gmm_max_expert(void) { return kMaxExpert; }
