@@ -6,7 +6,8 @@
 #include <string.h>
 
 /* exl3b200_norm.cu, exl3b200_gmm.cu, exl3b200_moe.cu */
-int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int vec, void* stream);
+int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int vec, int sm_count,
+                          void* stream);
 int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
                             int64_t q_pitch, uint8_t* qs, int64_t qs_pitch, void* stream);
 int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* qs, int64_t qs_pitch, int64_t rows,
@@ -60,6 +61,9 @@ int exl3b200_block_norm(const Exl3bBlockNorm* d, void* stream) {
         if (d->y_codes_pitch < d->cols / 2 || d->y_scales_pitch < d->cols / 32) return RAD_E_STRIDE;
         if (!vec || mis(d->y_codes, 4) || d->y_codes_pitch % 4) return RAD_E_ALIGN;
     }
+    int sm = 0;
+    int32_t* err = 0;
+    if (exl3b_cuda_device_info(&sm, &err) != 0) return RAD_E_DEVICE;
     Exl3bNormOp p;
     memset(&p, 0, sizeof p);
     p.rows = d->rows;
@@ -84,7 +88,7 @@ int exl3b200_block_norm(const Exl3bBlockNorm* d, void* stream) {
     p.post_eps = d->post_eps;
     p.pre_eps = d->pre_eps;
     p.res_scale = d->res_scale;
-    return rc_of(exl3b_cuda_block_norm(&p, d->dtype, d->branch ? d->branch_dtype : d->dtype, vec, stream));
+    return rc_of(exl3b_cuda_block_norm(&p, d->dtype, d->branch ? d->branch_dtype : d->dtype, vec, sm, stream));
 }
 
 static int check_rows(int64_t rows, int64_t cols) {

@@ -14,33 +14,65 @@ namespace {
 // Row t, all in f32:  n = branch * rsqrt(mean(branch^2) + post_eps) * post_w;  r = res_scale * res + gate * n;
 // y = r * rsqrt(mean(r^2) + pre_eps) * pre_w. HBM bound: every input is read once and every output written once.
 // `tpr` threads hold a row in registers (VPT vectors of eight values each), so the second mean needs no second read;
-// short rows share a block (blockDim.y rows). Rows whose addresses or width rule out 16-byte vectors take the same code
-// over single values, a thread's values blockDim.x apart.
-template <int DT, int BT, int VPT, bool VEC>
-__global__ void __launch_bounds__(1024) k_block_norm(const Exl3bNormOp p) {
+// short rows share a block (blockDim.y rows). A row's fixed cost -- two reductions, its addresses -- is paid by fewer
+// instructions the more values a thread holds (the kernel is near the issue limit: 640 instructions a warp and 256 values
+// with one vector a thread, half of that with four); few short rows take one vector, since there a row's latency counts. Rows whose addresses or width rule out 16-byte vectors take the same code over
+// single values, a thread's values blockDim.x apart.
+// Eight values as they lie in memory.
+template <int DT>
+struct Raw {
+    typedef typename El<DT>::T T;
+    uint4 q[DT == 1 ? 2 : 1];
+    __device__ __forceinline__ void clear() {
+        q[0] = make_uint4(0u, 0u, 0u, 0u);
+        if (DT == 1) q[DT == 1] = q[0];
+    }
+    __device__ __forceinline__ void fetch(const T* p) {
+        q[0] = *reinterpret_cast<const uint4*>(p);
+        if (DT == 1) q[DT == 1] = *(reinterpret_cast<const uint4*>(p) + 1);
+    }
+    __device__ __forceinline__ void set(int e, T v) { reinterpret_cast<T*>(q)[e] = v; }
+    __device__ __forceinline__ void get(float x[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = El<DT>::to(reinterpret_cast<const T*>(q)[e]);
+    }
+};
+
+// 1 / (1 + e^-g) from the special-function unit: relative 2^-20 or so, far inside a 16-bit output's rounding.
+__device__ __forceinline__ float sigmoid(float g) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
+    return r;
+}
+
+template <int DT, int BT, int VPT, int MAXT, bool VEC>
+__global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const Exl3bNormOp p) {
     typedef typename El<DT>::T T;
     typedef typename El<BT>::T B;
-    __shared__ float part[2][32];
-    const int tpr = blockDim.x, tid = threadIdx.x;
-    const int wid = (threadIdx.y * tpr + tid) >> 5, w0 = threadIdx.y * tpr >> 5, nw = tpr >> 5;
-    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    const bool live = row < p.rows;
+    constexpr int NW = MAXT / 32;                       // partial sums a row; those of warps it lacks stay zero
+    __shared__ __align__(16) float part[2][2][MAXT > 512 ? 1 : 4][NW];
+    const int tpr = blockDim.x, tid = threadIdx.x, ty = threadIdx.y;
     const int H = (int)p.cols;
+    const float inv_h = 1.f / (float)H;
+    for (int i = ty * tpr + tid; i < (int)(sizeof part / 4); i += tpr * blockDim.y) (&part[0][0][0][0])[i] = 0.f;
+    __syncthreads();
+    const std::integral_constant<int, DT> stream_dt;
+    const std::integral_constant<int, BT> branch_dt;
     auto at = [&](int v, int e) { return VEC ? (v * tpr + tid) * 8 + e : (v * 8 + e) * tpr + tid; };
-    auto load = [&](auto dt, const void* base, int64_t pitch, int v, float x[8]) {
-        constexpr int D = decltype(dt)::value;
-        typedef typename El<D>::T E;
-        const E* q = static_cast<const E*>(base) + pitch * row;
+    // a row's values (`q` its address), or zeros where there are none
+    auto load = [&](auto dt, const void* row_at, int v, auto& x) {
+        const auto* q = static_cast<const typename El<decltype(dt)::value>::T*>(row_at);
+        x.clear();
+        if (!q) return;
         if (VEC) {
-            if (at(v, 0) < H) ld8<D>(q + at(v, 0), x);
+            if (at(v, 0) < H) x.fetch(q + at(v, 0));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (at(v, e) < H) x[e] = El<D>::to(q[at(v, e)]);
+                if (at(v, e) < H) x.set(e, q[at(v, e)]);
         }
     };
-    auto store = [&](void* base, int64_t pitch, int v, const float x[8]) {
-        T* q = static_cast<T*>(base) + pitch * row;
+    auto store = [&](T* q, int v, const float x[8]) {
         if (VEC) {
             if (at(v, 0) < H) st8<DT>(q + at(v, 0), x);
         } else {
@@ -49,7 +81,8 @@ __global__ void __launch_bounds__(1024) k_block_norm(const Exl3bNormOp p) {
                 if (at(v, e) < H) q[at(v, e)] = El<DT>::from(x[e]);
         }
     };
-    // the row's sum of squares, in every thread of the row, summed in the same order whatever the block's shape
+    // the row's mean square, in every thread of the row; two buffers in turn, so that one barrier a sum does
+    int turn = 0;
     auto mean_square = [&](const float x[VPT][8], int slot) {
         float s = 0.f;
 #pragma unroll
@@ -58,137 +91,237 @@ __global__ void __launch_bounds__(1024) k_block_norm(const Exl3bNormOp p) {
             for (int e = 0; e < 8; ++e) s = fmaf(x[v][e], x[v][e], s);
 #pragma unroll
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-        if ((tid & 31) == 0) part[slot][wid] = s;
+        float* sums = part[slot][turn][ty];
+        if ((tid & 31) == 0) sums[tid >> 5] = s;
         __syncthreads();
-        s = part[slot][w0];
-        for (int w = 1; w < nw; ++w) s += part[slot][w0 + w];
-        return s / (float)H;
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(sums + w);
+            s += (f.x + f.y) + (f.z + f.w);
+        }
+        return s * inv_h;
     };
-    const std::integral_constant<int, DT> stream_dt;
-    const std::integral_constant<int, BT> branch_dt;
-
-    float r[VPT][8], res[VPT][8];
+    const bool gates = p.gate_kind == EXL3B_GATE_ELEMENT || p.gate_kind == EXL3B_GATE_CHANNEL;
+    const int64_t step = (int64_t)gridDim.x * blockDim.y;
+    int64_t row = (int64_t)blockIdx.x * blockDim.y + ty;
+    for (int64_t first = (int64_t)blockIdx.x * blockDim.y; first < p.rows; first += step, row += step, turn ^= 1) {
+        const bool live = row < p.rows;
+        const T* res_at = p.res && live ? static_cast<const T*>(p.res) + row * p.res_pitch : nullptr;
+        const B* branch_at = p.branch && live ? static_cast<const B*>(p.branch) + row * p.branch_pitch : nullptr;
+        const T* gate_at = !gates || !live ? nullptr
+                           : static_cast<const T*>(p.gate) + (p.gate_kind == EXL3B_GATE_ELEMENT ? row * p.gate_pitch : 0);
+        const float token = p.gate_kind == EXL3B_GATE_TOKEN && live ? static_cast<const float*>(p.gate)[row] : 0.f;
+        // the row's loads first (the longest rows have registers for the branch alone)
+        constexpr bool AHEAD = MAXT <= 512;
+        float r[VPT][8];
+        Raw<DT> res[VPT], gate[VPT];
+        {
+            Raw<BT> b[VPT];
 #pragma unroll
-    for (int v = 0; v < VPT; ++v)
+            for (int v = 0; v < VPT; ++v) load(branch_dt, branch_at, v, b[v]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[v][e] = res[v][e] = 0.f;
-    if (live) {
+            for (int v = 0; v < VPT; ++v) {
+                if (AHEAD) load(stream_dt, res_at, v, res[v]);
+                if (AHEAD && VPT == 1) load(stream_dt, gate_at, v, gate[v]);
+            }
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) b[v].get(r[v]);
+        }
+        if (p.post_w) {
+            Raw<DT> w[VPT];
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) load(stream_dt, p.post_w, v, w[v]);
+            const float s = __frsqrt_rn(mean_square(r, 0) + p.post_eps);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                float f[8];
+                w[v].get(f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[v][e] = r[v][e] * s * f[e];
+            }
+        }
+        if (p.gate_kind == EXL3B_GATE_TOKEN) {
+            const float f = sigmoid(token);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[v][e] *= f;
+        } else if (gates) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                float f[8];
+                if (!AHEAD || VPT > 1) load(stream_dt, gate_at, v, gate[v]);
+                gate[v].get(f);
+                if (p.gate_kind == EXL3B_GATE_ELEMENT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = sigmoid(f[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[v][e] *= f[e];
+            }
+        }
+        if (p.res) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                float f[8];
+                if (!AHEAD) load(stream_dt, res_at, v, res[v]);
+                res[v].get(f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[v][e] = fmaf(f[e], p.res_scale, r[v][e]);
+            }
+        }
+        if (p.out && live) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) store(static_cast<T*>(p.out) + row * p.out_pitch, v, r[v]);
+        }
+        if (!p.pre_w) continue;
+        Raw<DT> w[VPT];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) load(stream_dt, p.pre_w, v, w[v]);
+        const float s = __frsqrt_rn(mean_square(r, 1) + p.pre_eps);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            if (p.branch) load(branch_dt, p.branch, p.branch_pitch, v, r[v]);
-            if (p.res) load(stream_dt, p.res, p.res_pitch, v, res[v]);
+            float f[8];
+            w[v].get(f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[v][e] = r[v][e] * s * f[e];
         }
-    }
-    if (p.post_w) {
-        const float s = __frsqrt_rn(mean_square(r, 0) + p.post_eps);
+        if (p.y && live) {
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            float w[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
-            load(stream_dt, p.post_w, 0, v, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[v][e] = r[v][e] * s * w[e];
+            for (int v = 0; v < VPT; ++v) store(static_cast<T*>(p.y) + row * p.y_pitch, v, r[v]);
         }
-    }
-    if (p.gate_kind == EXL3B_GATE_TOKEN) {
-        const float g = live ? 1.f / (1.f + expf(-static_cast<const float*>(p.gate)[row])) : 0.f;
+        if (VEC && p.q) {
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[v][e] *= g;
-    } else if (p.gate_kind != EXL3B_GATE_NONE && live) {
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            float g[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
-            load(stream_dt, p.gate, p.gate_kind == EXL3B_GATE_ELEMENT ? p.gate_pitch : 0, v, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                r[v][e] *= p.gate_kind == EXL3B_GATE_ELEMENT ? 1.f / (1.f + expf(-g[e])) : g[e];
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[v][e] = p.res ? fmaf(res[v][e], p.res_scale, r[v][e]) : r[v][e];
-        if (p.out && live) store(p.out, p.out_pitch, v, r[v]);
-    }
-    if (!p.pre_w) return;
-    const float s = __frsqrt_rn(mean_square(r, 1) + p.pre_eps);
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        float w[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
-        load(stream_dt, p.pre_w, 0, v, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[v][e] = r[v][e] * s * w[e];
-        if (p.y && live) store(p.y, p.y_pitch, v, r[v]);
-        if (VEC && p.q) {      // four neighbouring lanes hold a block of 32
-            const uint32_t code = mx4_quad_code(r[v]);
-            if (live && at(v, 0) < H) {
-                *reinterpret_cast<uint32_t*>(p.q + row * p.q_pitch + at(v, 0) / 2) = mx4_pack8(r[v], code);
-                if ((tid & 3) == 0) p.q_scales[row * p.qs_pitch + at(v, 0) / 32] = (uint8_t)code;
+            for (int v = 0; v < VPT; ++v) {      // four neighbouring lanes hold a block of 32
+                const uint32_t code = mx4_quad_code(r[v]);
+                if (live && at(v, 0) < H) {
+                    *reinterpret_cast<uint32_t*>(p.q + row * p.q_pitch + at(v, 0) / 2) = mx4_pack8(r[v], code);
+                    if ((tid & 3) == 0) p.q_scales[row * p.qs_pitch + at(v, 0) / 32] = (uint8_t)code;
+                }
             }
         }
     }
 }
 
-template <int DT, int BT>
-int launch_norm(const Exl3bNormOp* p, bool vec, cudaStream_t st) {
+template <int DT, int BT, int VPT, int MAXT>
+int launch_norm_t(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st) {
     const int64_t n8 = (p->cols + 7) / 8;
-    const int vpt = n8 <= 1024 ? 1 : n8 <= 2048 ? 2 : 4;
-    const int tpr = (int)(((n8 + vpt - 1) / vpt + 31) / 32 * 32);
-    const int rpb = tpr >= 128 ? 1 : 128 / tpr;
-    const int64_t grid = (p->rows + rpb - 1) / rpb;
+    const int tpr = (int)(((n8 + VPT - 1) / VPT + 31) / 32 * 32);
+    const int rpb = tpr >= 128 || MAXT > 512 ? 1 : 128 / tpr;
+    const int64_t want = (p->rows + rpb - 1) / rpb, room = (int64_t)sm_count * (2048 / (tpr * rpb));
+    const unsigned grid = (unsigned)(want < room ? want : room);
     const dim3 block(tpr, rpb);
-    if (vec) {
-        if (vpt == 1) k_block_norm<DT, BT, 1, true><<<(unsigned)grid, block, 0, st>>>(*p);
-        else if (vpt == 2) k_block_norm<DT, BT, 2, true><<<(unsigned)grid, block, 0, st>>>(*p);
-        else k_block_norm<DT, BT, 4, true><<<(unsigned)grid, block, 0, st>>>(*p);
-    } else {
-        if (vpt == 1) k_block_norm<DT, BT, 1, false><<<(unsigned)grid, block, 0, st>>>(*p);
-        else if (vpt == 2) k_block_norm<DT, BT, 2, false><<<(unsigned)grid, block, 0, st>>>(*p);
-        else k_block_norm<DT, BT, 4, false><<<(unsigned)grid, block, 0, st>>>(*p);
-    }
+    if (vec) k_block_norm<DT, BT, VPT, MAXT, true><<<grid, block, 0, st>>>(*p);
+    else k_block_norm<DT, BT, VPT, MAXT, false><<<grid, block, 0, st>>>(*p);
     return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
 
+template <int DT, int BT>
+int launch_norm(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st) {
+    const int64_t n8 = (p->cols + 7) / 8;
+    // one B200, f32 branch, both norms: 2400 x 2048 in 20.5 / 15.1 / 14.5 us at 1 / 2 / 4 vectors a thread, 9600 x 4096 in
+    // 100 / 80 / 72; an element gate's registers turn the last two round (9600 x 4096, bf16 branch: 111 / 95 / 112); one
+    // row of 2048 in 2.9 / 3.5 / 3.6, of 4096 in 4.1 / 4.2 / 3.5; 9600 rows of 256 in 9.0 / 11.1 / 14.6
+    if (n8 <= 32 || (n8 <= 256 && p->rows < 2 * (int64_t)sm_count)) return launch_norm_t<DT, BT, 1, 256>(p, vec, sm_count, st);
+    if (n8 > 1024) return launch_norm_t<DT, BT, 4, 1024>(p, vec, sm_count, st);
+    if (p->gate_kind == EXL3B_GATE_ELEMENT) return launch_norm_t<DT, BT, 2, 512>(p, vec, sm_count, st);
+    return launch_norm_t<DT, BT, 4, 256>(p, vec, sm_count, st);
+}
+
 // ------------------------------------------------------------------------------------------ MXFP4 rows
-// HBM bound: 16-byte loads, eight values a thread, a block's scale from four neighbouring lanes. blockIdx.y walks the
-// rows (grid-stride), blockIdx.x the row's vectors.
-template <int DT>
-__global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t rows, int cols,
+// HBM bound: a thread takes kUnroll vectors of eight values, 256 vectors apart in the rows laid end to end (whatever the
+// width, every lane has work), all loaded before the first is used; a block's scale comes from four neighbouring lanes.
+constexpr int kUnroll = 4;
+
+// n / d for n < 2^31 by a multiplication (the host computes m and s); BIG: 64-bit division.
+struct RowDiv {
+    uint32_t d, m, s;
+};
+template <bool BIG>
+__device__ __forceinline__ void row_of(int64_t i, const RowDiv& v, int64_t* row, int* vec) {
+    if (BIG) {
+        *row = i / v.d;
+        *vec = (int)(i - *row * v.d);
+    } else {
+        const uint32_t n = (uint32_t)i, q = (__umulhi(n, v.m) + n) >> v.s;
+        *row = q;
+        *vec = (int)(n - q * v.d);
+    }
+}
+RowDiv row_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return RowDiv{ d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s };
+}
+
+template <int DT, bool BIG>
+__global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t n_vec, RowDiv div,
                                                       uint8_t* q, int64_t q_pitch, uint8_t* qs, int64_t qs_pitch) {
     typedef typename El<DT>::T T;
-    const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
-    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        float v[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
-        if (c < cols) ld8<DT>(static_cast<const T*>(x) + row * x_pitch + c, v);
-        const uint32_t code = mx4_quad_code(v);
-        if (c < cols) {
-            *reinterpret_cast<uint32_t*>(q + row * q_pitch + c / 2) = mx4_pack8(v, code);
-            if ((threadIdx.x & 3) == 0) qs[row * qs_pitch + c / 32] = (uint8_t)code;
-        }
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
+    float v[kUnroll][8];
+    int64_t row[kUnroll];
+    int c[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        row_of<BIG>(i0 + 256 * u, div, &row[u], &c[u]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+        if (i0 + 256 * u < n_vec) ld8<DT>(static_cast<const T*>(x) + row[u] * x_pitch + 8 * c[u], v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t code = mx4_quad_code(v[u]);
+        if (i0 + 256 * u >= n_vec) continue;
+        *reinterpret_cast<uint32_t*>(q + row[u] * q_pitch + 4 * c[u]) = mx4_pack8(v[u], code);
+        if ((threadIdx.x & 3) == 0) qs[row[u] * qs_pitch + (c[u] >> 2)] = (uint8_t)code;
     }
 }
 
-// e2m1 code -> f32: the sign bit, then 0 .5 1 1.5 2 3 4 6 from a packed table of halves of those values' doubles.
-__device__ __forceinline__ float e2m1_value(uint32_t n) {
-    const float m = 0.5f * (float)((0xC8643210u >> ((n & 7u) * 4)) & 15u);
-    return n & 8u ? -m : m;
+// Eight e2m1 codes -> f32. As f16 the values 0 .5 1 1.5 2 3 4 6 have zero low bytes: a byte permutation looks four high
+// bytes up at once, another the signs.
+__device__ __forceinline__ void e2m1_unpack8(uint32_t n, float v[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t c = n >> (16 * h);
+        const uint32_t b = __byte_perm(0x3E3C3800u, 0x46444240u, c & 0x7777u) | __byte_perm(0x8000u, 0u, (c >> 3) & 0x1111u);
+        const uint32_t p0 = __byte_perm(b, 0u, 0x1404), p1 = __byte_perm(b, 0u, 0x3424);
+        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
+        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
+        v[4 * h] = f0.x;
+        v[4 * h + 1] = f0.y;
+        v[4 * h + 2] = f1.x;
+        v[4 * h + 3] = f1.y;
+    }
 }
 
-template <int DT>
+template <int DT, bool BIG>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* qs,
-                                                        int64_t qs_pitch, int64_t rows, int cols, void* y,
+                                                        int64_t qs_pitch, int64_t n_vec, RowDiv div, void* y,
                                                         int64_t y_pitch) {
     typedef typename El<DT>::T T;
-    const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
-    if (c >= cols) return;
-    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        const uint32_t n = *reinterpret_cast<const uint32_t*>(q + row * q_pitch + c / 2);
-        const float s = mx4_scale(qs[row * qs_pitch + c / 32]);
-        float v[8];
+    const int64_t i0 = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
+    uint32_t n[kUnroll], s[kUnroll];
+    int64_t row[kUnroll];
+    int c[kUnroll];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = e2m1_value(n >> (4 * i)) * s;
-        st8<DT>(static_cast<T*>(y) + row * y_pitch + c, v);
+    for (int u = 0; u < kUnroll; ++u) {
+        row_of<BIG>(i0 + 256 * u, div, &row[u], &c[u]);
+        n[u] = s[u] = 0;
+        if (i0 + 256 * u >= n_vec) continue;
+        n[u] = *reinterpret_cast<const uint32_t*>(q + row[u] * q_pitch + 4 * c[u]);
+        s[u] = qs[row[u] * qs_pitch + (c[u] >> 2)];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        if (i0 + 256 * u >= n_vec) continue;
+        const float scale = mx4_scale(s[u]);
+        float v[8];
+        e2m1_unpack8(n[u], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= scale;
+        st8<DT>(static_cast<T*>(y) + row[u] * y_pitch + 8 * c[u], v);
     }
 }
 
@@ -217,39 +350,49 @@ __global__ void __launch_bounds__(256) k_mx4_tile(const uint8_t* s, int64_t s_pi
 
 extern "C" {
 
-int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int vec, void* stream) {
+int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int vec, int sm_count, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype * 4 + branch_dtype) {
-    case 1 * 4 + 1: return launch_norm<1, 1>(p, vec, st);
-    case 1 * 4 + 2: return launch_norm<1, 2>(p, vec, st);
-    case 1 * 4 + 3: return launch_norm<1, 3>(p, vec, st);
-    case 2 * 4 + 1: return launch_norm<2, 1>(p, vec, st);
-    case 2 * 4 + 2: return launch_norm<2, 2>(p, vec, st);
-    case 2 * 4 + 3: return launch_norm<2, 3>(p, vec, st);
-    case 3 * 4 + 1: return launch_norm<3, 1>(p, vec, st);
-    case 3 * 4 + 2: return launch_norm<3, 2>(p, vec, st);
-    case 3 * 4 + 3: return launch_norm<3, 3>(p, vec, st);
+    case 1 * 4 + 1: return launch_norm<1, 1>(p, vec, sm_count, st);
+    case 1 * 4 + 2: return launch_norm<1, 2>(p, vec, sm_count, st);
+    case 1 * 4 + 3: return launch_norm<1, 3>(p, vec, sm_count, st);
+    case 2 * 4 + 1: return launch_norm<2, 1>(p, vec, sm_count, st);
+    case 2 * 4 + 2: return launch_norm<2, 2>(p, vec, sm_count, st);
+    case 2 * 4 + 3: return launch_norm<2, 3>(p, vec, sm_count, st);
+    case 3 * 4 + 1: return launch_norm<3, 1>(p, vec, sm_count, st);
+    case 3 * 4 + 2: return launch_norm<3, 2>(p, vec, sm_count, st);
+    case 3 * 4 + 3: return launch_norm<3, 3>(p, vec, sm_count, st);
     default: return -2;
     }
 }
 
+#define EXL3B_MX4_ROWS(KERN, DT, ...)                                                                        \
+    do {                                                                                                     \
+        if (n_vec < (1ll << 31) - 1024) KERN<DT, false><<<grid, 256, 0, st>>>(__VA_ARGS__);                  \
+        else KERN<DT, true><<<grid, 256, 0, st>>>(__VA_ARGS__);                                              \
+    } while (0)
+
 int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
                             int64_t q_pitch, uint8_t* qs, int64_t qs_pitch, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((cols / 8 + 255) / 256), (unsigned)(rows < 65535 ? rows : 65535));
-    if (dtype == 1) k_mx4_quantize<1><<<grid, 256, 0, st>>>(x, x_pitch, rows, (int)cols, q, q_pitch, qs, qs_pitch);
-    else if (dtype == 2) k_mx4_quantize<2><<<grid, 256, 0, st>>>(x, x_pitch, rows, (int)cols, q, q_pitch, qs, qs_pitch);
-    else k_mx4_quantize<3><<<grid, 256, 0, st>>>(x, x_pitch, rows, (int)cols, q, q_pitch, qs, qs_pitch);
+    const int64_t n_vec = rows * (cols / 8);
+    const unsigned grid = (unsigned)((n_vec + 256 * kUnroll - 1) / (256 * kUnroll));
+    const RowDiv div = row_div((uint32_t)(cols / 8));
+    if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_quantize, 1, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
+    else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_quantize, 2, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
+    else EXL3B_MX4_ROWS(k_mx4_quantize, 3, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
     return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
 
 int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* qs, int64_t qs_pitch, int64_t rows,
                               int64_t cols, void* y, int dtype, int64_t y_pitch, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)((cols / 8 + 255) / 256), (unsigned)(rows < 65535 ? rows : 65535));
-    if (dtype == 1) k_mx4_dequantize<1><<<grid, 256, 0, st>>>(q, q_pitch, qs, qs_pitch, rows, (int)cols, y, y_pitch);
-    else if (dtype == 2) k_mx4_dequantize<2><<<grid, 256, 0, st>>>(q, q_pitch, qs, qs_pitch, rows, (int)cols, y, y_pitch);
-    else k_mx4_dequantize<3><<<grid, 256, 0, st>>>(q, q_pitch, qs, qs_pitch, rows, (int)cols, y, y_pitch);
+    const int64_t n_vec = rows * (cols / 8);
+    const unsigned grid = (unsigned)((n_vec + 256 * kUnroll - 1) / (256 * kUnroll));
+    const RowDiv div = row_div((uint32_t)(cols / 8));
+    if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_dequantize, 1, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
+    else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_dequantize, 2, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
+    else EXL3B_MX4_ROWS(k_mx4_dequantize, 3, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
     return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
 
