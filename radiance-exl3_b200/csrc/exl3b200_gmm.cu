@@ -46,6 +46,7 @@ constexpr int kSlice = 16;                       // sorted rows an epilogue grou
 constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
 constexpr int kMaxExpert = 2048;
+constexpr int kMaxSt = 8;                        // stages at most
 
 template <bool MX, bool PAIR>
 struct Cfg {
@@ -63,11 +64,16 @@ struct Cfg {
     static constexpr int COLS = 2 * NT + 2 * SFC;
     static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 512;
     static constexpr int PER_SM = PAIR ? 1 : 2;
-    static constexpr int BUDGET = (PAIR ? 226 : 113) * 1024 - 1024 - EPI_B - 512 - kTab * 16 - 1024 - (kMaxExpert + 4) * 4;
-    static constexpr int ST = BUDGET / STAGE_B > 8 ? 8 : BUDGET / STAGE_B;
-    static constexpr int SMEM = 1024 + ST * STAGE_B + EPI_B + 512;   // the unit prefix follows
-    static_assert(COLS <= 512 && ST >= 4, "tensor or shared memory");
-    static_assert((3 * ST + 4) * 8 + 8 <= 512, "barriers");
+    // shared memory: alignment, staging, barriers, the unit prefix, and as many stages as fit beside the static arrays (the
+    // narrow form: twice an SM)
+    static constexpr int ROOM = (PAIR ? 227 : 113) * 1024 - kTab * 16 - 128;
+    static constexpr int fixed(int n_expert) { return 1024 + EPI_B + 512 + (n_expert + 4) * 4; }
+    static constexpr int stages(int n_expert) {
+        const int n = (ROOM - fixed(n_expert)) / STAGE_B;
+        return n < kMaxSt ? n : kMaxSt;
+    }
+    static_assert(COLS <= 512 && stages(kMaxExpert) >= 4, "tensor or shared memory");
+    static_assert((3 * kMaxSt + 4) * 8 + 8 <= 512, "barriers");
 };
 
 struct Unit {
@@ -202,17 +208,21 @@ __device__ __forceinline__ void tmem_free(uint32_t t, uint32_t cols) {
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float v[16]) {
-    uint32_t r[16];
+// 16 columns of this warp's 32 lanes; tmem_wait before the registers are read.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t r[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
         "%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait(uint32_t r[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -228,6 +238,10 @@ __device__ __forceinline__ void tma_w_el(void* dst, const CUtensorMap* map, int 
 __device__ __forceinline__ void cp16(uint32_t dst, const uint8_t* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// The calling thread's copies so far, landed -> one arrival on bar.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // Shared-memory writes this thread made or has been told of become visible to the asynchronous proxy (tcgen05's reads).
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // One arrival on the even CTA's barrier of the same offset. What it and the waits below order across the CTAs is tensor
@@ -239,13 +253,68 @@ __device__ __forceinline__ void arrive_even(uint64_t* bar) {
                  " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(bar))
                  : "memory");
 }
-// The x row of sorted row i (a dropped slot reads row 0: its outputs are zeroed, not stored), never past x's rows.
-__device__ __forceinline__ int x_row(const Exl3bGmmOp& p, int64_t i) {
-    if (p.top_k == 0) return (int)i;
-    const int32_t f = p.sorted_tok ? p.sorted_tok[i] : (int32_t)i;
-    const int32_t t = f < 0 ? 0 : f / p.top_k;
-    return t < p.x_rows ? t : (int)(p.x_rows - 1);
-}
+// The x rows that a thread loads of a unit: rows first, first + step, ... of it. Their slots are fetched a unit ahead, so a
+// unit's first copies do not wait for them. A dropped slot reads row 0 (its outputs are zeroed, not stored), a row past the
+// unit's its last one; none lies past x's rows.
+template <int N>
+struct RowAhead {
+    const Exl3bGmmOp& p;
+    const int first, step;
+    int32_t slot[N];
+    __device__ __forceinline__ RowAhead(const Exl3bGmmOp& op, int f, int s) : p(op), first(f), step(s) {}
+    __device__ __forceinline__ void fetch(const Unit& u) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = min(u.r0 + max(0, min(first + step * j, u.nr - 1)), (int)(p.n_rows - 1));
+            slot[j] = p.top_k && p.sorted_tok ? p.sorted_tok[i] : i;
+        }
+    }
+    __device__ __forceinline__ void rows(const uint8_t* base, int64_t pitch, const uint8_t* src[N]) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int t = p.top_k ? max(slot[j], 0) / p.top_k : slot[j];
+            src[j] = base + (int64_t)min(t, (int)(p.x_rows - 1)) * pitch;
+        }
+    }
+};
+// 16 scales of an x row from byte `off` on (those past the row's end are zero): one load where rows lie on 16-byte
+// boundaries, else the aligned words around them, shifted; bytes where a word would leave the scales' memory.
+struct RowScales {
+    const uint8_t *lo, *hi;
+    int n;
+    bool whole;
+    __device__ __forceinline__ RowScales(const Exl3bGmmOp& p)
+        : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32), n((int)(p.n_in / 32)),
+          whole(((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0) {}
+    __device__ __forceinline__ uint32_t word(const uint8_t* a) const {
+        if (a >= lo && a + 4 <= hi) return *reinterpret_cast<const uint32_t*>(a);
+        uint32_t w = 0;
+        for (int b = 0; b < 4; ++b)
+            if (a + b >= lo && a + b < hi) w |= (uint32_t)a[b] << (8 * b);
+        return w;
+    }
+    __device__ __forceinline__ uint4 load(const uint8_t* row, int off) const {
+        const uint8_t* a = row + off;
+        // nothing here touches what it loads: the load is waited for where it is used, a batch later
+        if (whole && off + 16 <= n) return *reinterpret_cast<const uint4*>(a);
+        if (off >= n) return make_uint4(0u, 0u, 0u, 0u);
+        uint32_t w[4];
+        const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 3);
+        uint32_t prev = word(a - by);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t next = by || i < 3 ? word(a - by + 4 * i + 4) : 0u;
+            w[i] = __funnelshift_r(prev, next, 8 * by);
+            prev = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int left = n - off - 4 * i;
+            if (left < 4) w[i] = left > 0 ? w[i] & ((1u << (8 * left)) - 1) : 0u;
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
 // Barrier over an epilogue group, and the same with a vote: whether any of its threads has `bad` set (they decide
 // together whether to go on, since they meet at barriers).
 __device__ __forceinline__ void epi_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
@@ -260,9 +329,9 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
 
 template <bool MX, bool PAIR>
 __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
-    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p) {
+    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const int ST) {
     using C = Cfg<MX, PAIR>;
-    constexpr int ST = C::ST, NT = C::NT, THREADS = C::THREADS;
+    constexpr int NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* w_ring = smem;                                   // [ST][128 rows][128 B]
@@ -436,65 +505,57 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         }
     } else if (warp < kXWarp0) {
         // ---------------------------------------------------------------- MXFP4: the sorted rows' scales
-        // Warp 2 the unit's rows 0..127, warp 3 (PAIR) the others; both CTAs of a pair need them all. Lane l holds rows
-        // l, l + 32, ... of the group, so that it writes 16 consecutive bytes of the layout (row r at (r % 32) * 16 +
-        // (r / 32) * 4, four scales of 128 k). Chunks are fetched kAhead at a time, one batch ahead.
+        // Warp 2 the unit's rows 0..127, warp 3 (PAIR) the others; both CTAs of a pair need them all. Row r's four scales of
+        // 128 k go to (r % 32) * 16 + (r / 32) * 4: lane l holds rows l, l + 32, ... and writes 16 consecutive bytes. A lane
+        // reads 32 bytes of each of its rows at a time, four stages' worth, one batch ahead (each row is a line of its own:
+        // 4-byte copies a stage kept the L1 busy, and a batch of two stages is shorter than the loads' latency).
         const int g = warp - 2;
         if (MX && g < C::SFX_G) {
-            constexpr int Q = NT < 128 ? NT / 32 : 4, kAhead = 4;
-            const int nsc = (int)(p.n_in / 32);
-            const bool wide = (p.xs_pitch & 7) == 0 && (reinterpret_cast<uintptr_t>(p.x_scales) & 7) == 0;
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                const Unit u = unit_at(i);
-                const uint8_t* src[Q];
+            constexpr int Q = NT < 128 ? NT / 32 : 4;
+            const RowScales rs(p);
+            RowAhead<Q> ahead(p, lane + g * 128, 32);
+            constexpr int kAhead = 4;                         // stages a batch
+            uint4 nxt[2][Q];
+            const uint8_t* src[Q];
+            if (n_mine) {
+                ahead.fetch(unit_at(0));
+                ahead.rows(p.x_scales, p.xs_pitch, src);
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
-                    const int j = g * 128 + lane + 32 * q;
-                    src[q] = j < u.nr ? p.x_scales + (int64_t)x_row(p, u.r0 + j) * p.xs_pitch : nullptr;
+                    nxt[0][q] = rs.load(src[q], 0);
+                    nxt[1][q] = rs.load(src[q], 16);
                 }
-                auto fetch = [&](int ck, uint2 v[Q]) {
+            }
+            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+                if (i + 1 < n_mine) ahead.fetch(unit_at(i + 1));
+                for (int c0 = 0; c0 < nck; c0 += kAhead) {
+                    uint4 cur[2][Q];
+                    if (c0 + kAhead >= nck && i + 1 < n_mine) ahead.rows(p.x_scales, p.xs_pitch, src);
+                    const int off = c0 + kAhead < nck ? 8 * (c0 + kAhead) : 0;
 #pragma unroll
                     for (int q = 0; q < Q; ++q) {
-                        v[q] = make_uint2(0u, 0u);
-                        if (!src[q] || ck >= nck) continue;
-                        if (wide && ck * 8 + 8 <= nsc) {
-                            v[q] = *reinterpret_cast<const uint2*>(src[q] + ck * 8);
-                        } else {
-                            for (int b = 0; b < 8; ++b)
-                                if (ck * 8 + b < nsc) {
-                                    const uint32_t w = (uint32_t)src[q][ck * 8 + b] << (8 * (b & 3));
-                                    if (b < 4) v[q].x |= w; else v[q].y |= w;
-                                }
-                        }
+                        cur[0][q] = nxt[0][q];
+                        cur[1][q] = nxt[1][q];
+                        nxt[0][q] = rs.load(src[q], off);
+                        nxt[1][q] = rs.load(src[q], off + 16);
                     }
-                };
-                uint2 cur[kAhead][Q], nxt[kAhead][Q];
-#pragma unroll
-                for (int a = 0; a < kAhead; ++a) fetch(a, cur[a]);
-                for (int c0 = 0; c0 < nck; c0 += kAhead) {
-#pragma unroll
-                    for (int a = 0; a < kAhead; ++a) fetch(c0 + kAhead + a, nxt[a]);
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) {
                         if (c0 + a >= nck) continue;
                         wait(&empty[pipe.s], pipe.ph ^ 1);
-                        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-                        lo.x = cur[a][0].x; hi.x = cur[a][0].y;
-                        if (Q > 1) { lo.y = cur[a][Q > 1 ? 1 : 0].x; hi.y = cur[a][Q > 1 ? 1 : 0].y; }
-                        if (Q > 2) { lo.z = cur[a][Q > 2 ? 2 : 0].x; hi.z = cur[a][Q > 2 ? 2 : 0].y; }
-                        if (Q > 3) { lo.w = cur[a][Q > 3 ? 3 : 0].x; hi.w = cur[a][Q > 3 ? 3 : 0].y; }
                         uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
-                        dst[0] = lo;
-                        dst[C::SFX_G * 32] = hi;
-                        proxy_fence();
-                        __syncwarp();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            auto word = [&](int q) {
+                                const uint4 v = cur[a >> 1][q < Q ? q : 0];
+                                return q >= Q ? 0u : a & 1 ? (h ? v.w : v.z) : h ? v.y : v.x;
+                            };
+                            dst[h * (C::SFX_G * 32)] = make_uint4(word(0), word(1), word(2), word(3));
+                        }
+                        __syncwarp();                          // the MMA warp's fence covers these writes too
                         if (lane == 0) mbar_arrive(&full[pipe.s]);
                         pipe.next(ST);
                     }
-#pragma unroll
-                    for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-                        for (int q = 0; q < Q; ++q) cur[a][q] = nxt[a][q];
                 }
             }
         }
@@ -507,29 +568,28 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
         const int kb = (int)(MX ? p.n_in / 2 : p.n_in * 2);
         const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
+        RowAhead<RP> ahead(p, rr, 16);
+        auto mine = [&](uint32_t i) {                         // this CTA's rows of its i-th unit
+            Unit u = unit_at(i);
+            const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
+            u.r0 += (int)rank * nl;
+            u.nr = min(u.nr - (int)rank * nl, nl);
+            return u;
+        };
+        if (n_mine) ahead.fetch(mine(0));
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-            const Unit u = unit_at(i);
-            const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB, r1 = (int)rank * nl;
+            const Unit u = mine(i);
             const uint8_t* src[RP];
-            uint32_t live = 0;
-#pragma unroll
-            for (int j = 0; j < RP; ++j) {
-                const int r = rr + 16 * j, at = r1 + r;
-                const bool ok = r < nl && at < u.nr;
-                src[j] = static_cast<const uint8_t*>(p.x) + (ok ? (int64_t)x_row(p, u.r0 + at) * p.x_pitch_bytes + c * 16 : 0);
-                live |= (uint32_t)ok << j;
-            }
+            ahead.rows(static_cast<const uint8_t*>(p.x) + c * 16, p.x_pitch_bytes, src);
+            if (i + 1 < n_mine) ahead.fetch(mine(i + 1));
             for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                 wait(&empty[pipe.s], pipe.ph ^ 1);
-                const bool in = ck * kRowB + c * 16 < kb;
+                const bool in = ck * kRowB + c * 16 < kb;     // past the row's end: zeros
                 const uint32_t dst = dst0 + pipe.s * C::X_B;
 #pragma unroll
                 for (int j = 0; j < RP; ++j)
-                    if (rr + 16 * j < nl) {
-                        const bool ok = in && (live >> j & 1);
-                        cp16(dst + j * 16 * kRowB, ok ? src[j] + ck * kRowB : src[j], ok ? 16 : 0);
-                    }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[pipe.s])) : "memory");
+                    if (rr + 16 * j < u.nr) cp16(dst + j * 16 * kRowB, in ? src[j] + ck * kRowB : src[j], in ? 16 : 0);
+                cp_arrive(&full[pipe.s]);
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -575,11 +635,14 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             wait(&acc_full[ab], (i >> 1) & 1);
             if (epi_any(g, *vdead)) break;
             fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + ab * NT;
+            uint32_t a[16];
+            if (g * kSlice < u.nr) tmem_ld16(acc + g * kSlice, a);
             for (int t0 = g * kSlice; t0 < u.nr; t0 += C::EPI_G * kSlice) {
-                float a[16];
-                tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
+                tmem_wait(a);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = a[j];
+                for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = __uint_as_float(a[j]);
+                if (t0 + C::EPI_G * kSlice < u.nr) tmem_ld16(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
                 epi_sync(g);
                 for (int j = q * tpw + lane / lpt; j < kSlice; j += 4 * tpw) {
                     const int64_t r = u.r0 + t0 + j;
@@ -591,7 +654,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                         const float4 u0 = s[16], u1 = s[17];
                         const float up[8] = { u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w };
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + __expf(-v[e])) * up[e];
+                        for (int e = 0; e < 8; ++e) v[e] = __fdividef(v[e], 1.f + __expf(-v[e])) * up[e];
                     }
                     if (mx_out) {
                         const uint32_t code = mx4_quad_code(v);          // four lanes: 32 outputs of one row
@@ -670,7 +733,8 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     if (rc) return rc;
     auto kern = k_gmm<MX, PAIR>;
     cudaLaunchConfig_t cfg = {};
-    cfg.dynamicSmemBytes = C::SMEM + (p->n_expert + 4) * 4;
+    const int stages = C::stages(p->n_expert);
+    cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
     cfg.blockDim = dim3(C::THREADS);
     cfg.stream = st;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess) return -6;
@@ -682,7 +746,7 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = PAIR ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, map, *p) == cudaSuccess ? 0 : -6;
+    return cudaLaunchKernelEx(&cfg, kern, map, *p, stages) == cudaSuccess ? 0 : -6;
 }
 
 }  // namespace

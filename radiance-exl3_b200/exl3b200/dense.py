@@ -34,24 +34,24 @@ def _dtype(t):
 
 def _rows(t, name, shape=None, dtype=None):
     """A tensor whose last dimension is dense, on a GPU, of this shape and type: (address, row pitch in elements)."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} is not on a GPU")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}'s last dimension is strided")
-    if t.dim() < 2:
+    have, st = t.shape, t.stride()
+    if not (t.is_cuda and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
+            and (st[-1] == 1 or have[-1] <= 1)):
+        what = ("is not on a GPU" if not t.is_cuda else f"is {t.dtype}, not {dtype}" if dtype not in (None, t.dtype) else
+                f"has shape {tuple(have)}, not {tuple(shape)}" if shape is not None and have != shape else
+                "has a strided last dimension")
+        raise ValueError(f"{name} {what}")
+    if len(st) < 2:
         return t.data_ptr(), 0
-    return t.data_ptr(), t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), t.shape[-1])
+    return t.data_ptr(), st[-2] if have[-2] > 1 else max(st[-2], have[-1])
 
 
 # ------------------------------------------------------------------------------------------------ MXFP4
 def mx4_empty(rows, cols, device="cuda"):
-    """(codes, scales) for `rows` rows of `cols` values."""
+    """(codes, scales) for `rows` rows of `cols` values; the scales' rows 16 bytes apart or a multiple, which GroupedMm
+    reads fastest."""
     return (torch.empty((rows, cols // 2), dtype=torch.uint8, device=device),
-            torch.empty((rows, cols // 32), dtype=torch.uint8, device=device))
+            torch.empty((rows, (cols // 32 + 15) // 16 * 16), dtype=torch.uint8, device=device)[:, :cols // 32])
 
 
 def mx4_quantize(x, codes, scales, stream=0):
