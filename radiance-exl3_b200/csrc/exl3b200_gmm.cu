@@ -632,6 +632,14 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             const Unit u = unit_at(i);
             const int64_t n0 = (int64_t)(u.blk + rank) * blk_out + c0;
             const bool col_ok = n0 < p.n_out;
+            // which of the unit's rows are live, 32 a lane: asked for while the accumulators are still being computed
+            uint32_t live = 0;
+#pragma unroll
+            for (int b = 0; b < (NT + 31) / 32; ++b) {
+                const int j = 32 * b + lane;
+                const uint32_t m = __ballot_sync(0xFFFFFFFFu, j < u.nr && !(p.sorted_tok && p.sorted_tok[u.r0 + j] < 0));
+                if (lane == b) live = m;
+            }
             wait(&acc_full[ab], (i >> 1) & 1);
             if (epi_any(g, *vdead)) break;
             fence_after();
@@ -646,7 +654,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                 epi_sync(g);
                 for (int j = q * tpw + lane / lpt; j < kSlice; j += 4 * tpw) {
                     const int64_t r = u.r0 + t0 + j;
-                    const bool row_ok = t0 + j < u.nr && !(p.sorted_tok && p.sorted_tok[r] < 0);
+                    const bool row_ok = __shfl_sync(0xFFFFFFFFu, live, (t0 + j) >> 5) >> ((t0 + j) & 31) & 1;
                     const float4* s = reinterpret_cast<const float4*>(&st[j * kEpiLd + c0]);
                     const float4 s0 = s[0], s1 = s[1];
                     float v[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
