@@ -40,6 +40,7 @@ typedef struct Exl3bGmmOp {
     int64_t        w_rows;               /* the weight's rows: n_out, or twice that with silu_mul */
     int64_t        x_rows;
     int32_t        n_expert, top_k;      /* top_k 0: sorted row i reads x row i */
+    uint32_t       k_mul, k_shift;       /* slot / top_k = (umulhi(slot, k_mul) + slot) >> k_shift */
     int32_t        act, y_dtype;
     const void*    x;                    /* elements, or MXFP4 codes */
     int64_t        x_pitch_bytes;

@@ -5,8 +5,9 @@
 //   y[i][n] = z[n], or silu(z[n]) * z[n_out + n] (act silu_mul: w[e] holds n_out gate rows, then n_out up rows).
 //
 // The WEIGHT rows are the MMA's M (128 a CTA) and the sorted rows its N: experts hold a few to a few hundred rows, N
-// goes in steps of 16 (PAIR: 32), so a group of 40 rows costs 48 (64) columns where rows as M would cost 128. A block of silu_mul is 64
-// gate rows and their 64 up rows, so the epilogue has both halves of every output.
+// goes in steps of 16 (PAIR: 32), so a group of 40 rows costs 48 (64) columns where rows as M would cost 128. A block of
+// silu_mul is 64 gate rows and their 64 up rows, 16 of each in turn: an epilogue warp, which can read 32 lanes of tensor
+// memory, has both halves of its 16 outputs.
 //
 // Two forms of one kernel, both persistent over units (expert, a group of its sorted rows, a block of weight rows),
 // expert-major, so that the CTAs working at one time share an expert's rows and weights in L2:
@@ -23,8 +24,8 @@
 //   2, 3    MXFP4: the sorted rows' scales, 128 rows a warp, through registers into the layout tcgen05.cp reads
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok into the same swizzle (tile::gather4 copies took ~80 cycles
 //           for four rows: 444 against 205 us at 16 experts, 16384 rows, 1536 -> 4096)
-//   8..     epilogue, groups of four warps: tcgen05.ld, transposed through shared memory so that a row's outputs are
-//           stored contiguously; silu_mul, and the rounding to y's type (MXFP4: with its blocks' scales), happen there
+//   8..     epilogue, groups of four warps: tcgen05.ld, silu_mul, the rounding to y's type, and the transposition through
+//           shared memory by which a row's outputs are stored 16 bytes a thread (MXFP4: with their blocks' scales)
 // Two accumulator buffers in tensor memory: one unit's epilogue runs under the next one's MMAs. Every wait is bounded;
 // one that gives up sets the error word, and every role then drains and leaves.
 #include <cuda.h>
@@ -73,7 +74,7 @@ struct Cfg {
         return n < kMaxSt ? n : kMaxSt;
     }
     static_assert(COLS <= 512 && stages(kMaxExpert) >= 4, "tensor or shared memory");
-    static_assert((3 * kMaxSt + 4) * 8 + 8 <= 512, "barriers");
+    static_assert((2 * kMaxSt + 4) * 8 + 8 <= 512, "barriers");
 };
 
 struct Unit {
@@ -148,37 +149,36 @@ __device__ __forceinline__ void mma4_f16(uint32_t d, uint64_t a, uint64_t b, uin
     if constexpr (PAIR) EXL3B_MMA4_F16("2");
     else EXL3B_MMA4_F16("1");
 }
-// 512 bytes of scales (32 rows of 16) into four tensor-memory columns of all four lane quadrants (PAIR: of both CTAs,
-// each from its own shared memory).
-template <bool PAIR>
-__device__ __forceinline__ void cp_scales(uint32_t t, uint64_t desc) {
+// One MXFP4 stage: its scales into tensor memory (512 bytes, 32 rows of 16, into four columns of all four lane quadrants;
+// PAIR: of both CTAs, each from its own shared memory), then four MMAs of K = 64. Scales: two 128-k halves; the weight
+// rows' 4 columns a half from t on, the sorted rows' 4 G columns a half behind them. Within a half the first MMA takes
+// bytes 0, 1 of each column and the second bytes 2, 3 (id2: the descriptor with both scale ids at 2). sw, sx: the
+// descriptors of the weight rows' and the sorted rows' scales, [half][group][512 B].
+#define EXL3B_CP(G, T, D) " @e tcgen05.cp.cta_group::" G ".32x128b.warpx4 [" T "], " D ";\n"
+#define EXL3B_MX(G, A, B, I, SA, SB, P) \
+    " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], " A ", " B ", " I ", [" SA "], [" SB "], " P ";\n"
+#define EXL3B_STAGE_HEAD                                                                                            \
+    "{\n .reg .pred p, e, t;\n .reg .b64 a, b, w1, x1, x2, x3;\n .reg .b32 u, sb, v, x;\n"                          \
+    " setp.ne.b32 p, %6, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"                                  \
+    " add.u64 w1, %7, 32; add.u64 x1, %8, 32; add.u64 x2, %8, 64; add.u64 x3, %8, 96;\n"                             \
+    " add.u32 u, %5, 4; add.u32 sb, %5, 8; add.u32 x, %5, 12; add.u32 v, sb, %9;\n"
+#define EXL3B_STAGE_MMA(G)                                                                    \
+    EXL3B_MX(G, "%1", "%2", "%3", "%5", "sb", "p")                                            \
+    " add.u64 a, %1, 2; add.u64 b, %2, 2;\n" EXL3B_MX(G, "a", "b", "%4", "%5", "sb", "t")    \
+    " add.u64 a, %1, 4; add.u64 b, %2, 4;\n" EXL3B_MX(G, "a", "b", "%3", "u", "v", "t")      \
+    " add.u64 a, %1, 6; add.u64 b, %2, 6;\n" EXL3B_MX(G, "a", "b", "%4", "u", "v", "t") "}\n"
+template <bool PAIR, int G>
+__device__ __forceinline__ void stage_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t id0, uint32_t id2, uint32_t t,
+                                          uint32_t acc, uint64_t sw, uint64_t sx) {
     if constexpr (PAIR)
-        asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-                     " @e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(t), "l"(desc));
+        asm volatile(EXL3B_STAGE_HEAD EXL3B_CP("2", "%5", "%7") EXL3B_CP("2", "u", "w1") EXL3B_CP("2", "sb", "%8")
+                         EXL3B_CP("2", "x", "x1") EXL3B_CP("2", "v", "x2") " add.u32 x, v, 4;\n" EXL3B_CP("2", "x", "x3")
+                             EXL3B_STAGE_MMA("2") ::"r"(d), "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(t), "r"(acc), "l"(sw),
+                     "l"(sx), "n"(4 * G));
     else
-        asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-                     " @e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(t), "l"(desc));
-}
-// Four MMAs of K = 64 (MXFP4): one stage. Scales: two 128-k halves, sa and sb columns of the first, `hb` columns on for
-// sb's second; within a half the first MMA takes bytes 0, 1 of each column and the second bytes 2, 3 (id2: the
-// descriptor with both scale ids at 2).
-#define EXL3B_MMA4_MX4(G)                                                                                           \
-    asm volatile(                                                                                                   \
-        "{\n .reg .pred p, e, t;\n .reg .b64 a, b;\n .reg .b32 u, v;\n"                                             \
-        " setp.ne.b32 p, %7, 0;\n setp.eq.b32 t, 0, 0;\n elect.sync _|e, 0xffffffff;\n"                             \
-        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"  \
-        " add.u64 a, %1, 2; add.u64 b, %2, 2;\n"                                                                    \
-        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [%5], [%6], t;\n"    \
-        " add.u64 a, %1, 4; add.u64 b, %2, 4; add.u32 u, %5, 4; add.u32 v, %6, %8;\n"                               \
-        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [u], [v], t;\n"      \
-        " add.u64 a, %1, 6; add.u64 b, %2, 6;\n"                                                                    \
-        " @e tcgen05.mma.cta_group::" G ".kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %4, [u], [v], t;\n"      \
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(sa), "r"(sb), "r"(acc), "r"(hb))
-template <bool PAIR>
-__device__ __forceinline__ void mma4_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t id0, uint32_t id2, uint32_t sa,
-                                         uint32_t sb, uint32_t hb, uint32_t acc) {
-    if constexpr (PAIR) EXL3B_MMA4_MX4("2");
-    else EXL3B_MMA4_MX4("1");
+        asm volatile(EXL3B_STAGE_HEAD EXL3B_CP("1", "%5", "%7") EXL3B_CP("1", "u", "w1") EXL3B_CP("1", "sb", "%8")
+                         EXL3B_CP("1", "v", "x1") EXL3B_STAGE_MMA("1") ::"r"(d), "l"(a), "l"(b), "r"(id0), "r"(id2), "r"(t),
+                     "r"(acc), "l"(sw), "l"(sx), "n"(4 * G));
 }
 // The MMAs issued so far done -> one arrival on bar (PAIR: on both CTAs' bar of that offset).
 template <bool PAIR>
@@ -234,9 +234,19 @@ __device__ __forceinline__ void tma_w_el(void* dst, const CUtensorMap* map, int 
                      "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
 }
-// 16 bytes global -> shared, or 16 zero bytes (`bytes` 0: nothing is read).
-__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// A block of silu_mul in one copy: box z = groups of 16 rows from `group` on, in each its gate rows and then its up rows.
+__device__ __forceinline__ void tma_w5_el(void* dst, const CUtensorMap* map, int x, int group, int e, uint64_t* bar) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, %5}], [%6];\n}\n" ::
+                     "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(0), "r"(group), "r"(e), "r"(smem_u32(bar))
+                 : "memory");
+}
+// 16 bytes global -> shared; or 16 zero bytes, nothing read.
+__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const uint8_t* src, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
 // The calling thread's copies so far, landed -> one arrival on bar.
 __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
@@ -272,8 +282,9 @@ struct RowAhead {
     __device__ __forceinline__ void rows(const uint8_t* base, int64_t pitch, const uint8_t* src[N]) const {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int t = p.top_k ? max(slot[j], 0) / p.top_k : slot[j];
-            src[j] = base + (int64_t)min(t, (int)(p.x_rows - 1)) * pitch;
+            // slot / top_k by a multiplication (top_k 0: 1): exact for slots below 2^31
+            const uint32_t f = (uint32_t)max(slot[j], 0), t = (__umulhi(f, p.k_mul) + f) >> p.k_shift;
+            src[j] = base + (int64_t)min(t, (uint32_t)p.x_rows - 1) * pitch;
         }
     }
 };
@@ -315,6 +326,18 @@ struct RowScales {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
+// z / (1 + e^-z), from the special-function unit.
+__device__ __forceinline__ float silu(float z) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-z)));
+    return z * r;
+}
+__device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
+    uint32_t r;
+    if (dtype == RAD_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 // Barrier over an epilogue group, and the same with a vote: whether any of its threads has `bad` set (they decide
 // together whether to go on, since they meet at barriers).
 __device__ __forceinline__ void epi_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
@@ -340,10 +363,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     uint8_t* sfx_ring = sfw_ring + ST * C::SFW_B;             // [ST][2 halves][SFX_G][512 B]
     float* epi = reinterpret_cast<float*>(sfx_ring + ST * C::SFX_B);
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(epi) + C::EPI_B);
-    uint64_t* full = bars;                                    // this CTA's producers -> its MMA warp
+    uint64_t* full = bars;                                    // producers (PAIR: and the odd CTA's MMA warp) -> MMA warp
     uint64_t* empty = full + ST;                              // MMA commit -> producers
-    uint64_t* peer = empty + ST;                              // PAIR, even CTA: the odd one's stage is full
-    uint64_t* acc_full = peer + ST;                           // MMA commit -> epilogue [2]
+    uint64_t* acc_full = empty + ST;                          // MMA commit -> epilogue [2]
     uint64_t* acc_empty = acc_full + 2;                       // epilogue (PAIR: of both CTAs) -> MMA [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
@@ -359,9 +381,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     const uint32_t n_mb = (uint32_t)((p.n_out + blk_out * MB - 1) / (blk_out * MB));
     if (tid == 0) {
         for (int s = 0; s < ST; ++s) {
-            mbar_init(&full[s], 1 + 32 * kXWarps + C::SFX_G);
+            mbar_init(&full[s], 1 + 32 * kXWarps + C::SFX_G + (PAIR && rank == 0 ? 1 : 0));
             mbar_init(&empty[s], 1);
-            mbar_init(&peer[s], 1);
         }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * C::EPI_G * MB); }
         *dead = 0;
@@ -443,8 +464,17 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                 mbar_expect_tx_el(&full[pipe.s], kW_B + C::SFW_B);
                 uint8_t* dst = w_ring + pipe.s * kW_B;
                 const int k = ck * (MX ? 128 : 64);
-                tma_w_el(dst, &wmap, k, b * blk_out, u.e, &full[pipe.s]);
-                if (act) tma_w_el(dst + kW_B / 2, &wmap, k, (int)p.n_out + b * 64, u.e, &full[pipe.s]);
+                if (!act) {
+                    tma_w_el(dst, &wmap, k, b * 128, u.e, &full[pipe.s]);
+                } else if (p.n_out % 16 == 0) {
+                    tma_w5_el(dst, &wmap, k, b * 4, u.e, &full[pipe.s]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        tma_w_el(dst + q * 4096, &wmap, k, b * 64 + 16 * q, u.e, &full[pipe.s]);
+                        tma_w_el(dst + q * 4096 + 2048, &wmap, k, (int)p.n_out + b * 64 + 16 * q, u.e, &full[pipe.s]);
+                    }
+                }
                 if (MX)
                     tma_bulk_g2s_el(sfw_ring + pipe.s * C::SFW_B,
                                     p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes + ck * 1024, 1024,
@@ -460,7 +490,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                 wait(&full[pipe.s], pipe.ph);
                 proxy_fence();
-                if (lane == 0) arrive_even(&peer[pipe.s]);
+                if (lane == 0) arrive_even(&full[pipe.s]);
                 __syncwarp();
             }
         }
@@ -480,21 +510,13 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             const uint32_t d = tmem + ab * NT;
             for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                 wait(&full[pipe.s], pipe.ph);
-                if (PAIR) wait(&peer[pipe.s], pipe.ph);
                 proxy_fence();
                 fence_after();
                 const uint64_t wd = wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd = xd0 + (uint64_t)(pipe.s * C::X_B >> 4);
                 if constexpr (MX) {
-                    const uint32_t sa = tmem + 2 * NT + sfp * C::SFC, sb = sa + 8;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        cp_scales<PAIR>(sa + 4 * h, swd0 + (uint64_t)((pipe.s * C::SFW_B + h * 512) >> 4));
-#pragma unroll
-                        for (int g = 0; g < C::SFX_G; ++g)
-                            cp_scales<PAIR>(sb + 4 * (h * C::SFX_G + g),
-                                            sxd0 + (uint64_t)((pipe.s * C::SFX_B + (h * C::SFX_G + g) * 512) >> 4));
-                    }
-                    mma4_mx4<PAIR>(d, wd, xd, idesc, idesc | 2u << 4 | 2u << 29, sa, sb, 4 * C::SFX_G, ck ? 1u : 0u);
+                    stage_mx4<PAIR, C::SFX_G>(d, wd, xd, idesc, idesc | 2u << 4 | 2u << 29, tmem + 2 * NT + sfp * C::SFC,
+                                              ck ? 1u : 0u, swd0 + (uint64_t)(pipe.s * C::SFW_B >> 4),
+                                              sxd0 + (uint64_t)(pipe.s * C::SFX_B >> 4));
                     sfp ^= 1;
                 } else {
                     mma4_f16<PAIR>(d, wd, xd, idesc, ck ? 1u : 0u);
@@ -564,32 +586,50 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's barrier
         // when they have landed. The MMA warp, which sees that, makes them visible to the asynchronous proxy (a fence by
         // the loaders would wait for every copy they have in flight).
-        constexpr int RP = (C::NL + 15) / 16;
+        constexpr int RP = (C::NL + 15) / 16, kStep = 4;      // passes a stage; stages a step of the row pointers
         const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
         const int kb = (int)(MX ? p.n_in / 2 : p.n_in * 2);
         const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
         RowAhead<RP> ahead(p, rr, 16);
-        auto mine = [&](uint32_t i) {                         // this CTA's rows of its i-th unit
+        auto mine = [&](uint32_t i) {                         // this CTA's rows of its i-th unit; blk: rows of its tile
             Unit u = unit_at(i);
             const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
             u.r0 += (int)rank * nl;
             u.nr = min(u.nr - (int)rank * nl, nl);
+            u.blk = nl;
             return u;
         };
-        if (n_mine) ahead.fetch(mine(0));
+        Unit u = n_mine ? mine(0) : Unit{};
+        if (n_mine) ahead.fetch(u);
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-            const Unit u = mine(i);
+            const int nl = u.blk;
             const uint8_t* src[RP];
             ahead.rows(static_cast<const uint8_t*>(p.x) + c * 16, p.x_pitch_bytes, src);
-            if (i + 1 < n_mine) ahead.fetch(mine(i + 1));
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
-                wait(&empty[pipe.s], pipe.ph ^ 1);
-                const bool in = ck * kRowB + c * 16 < kb;     // past the row's end: zeros
-                const uint32_t dst = dst0 + pipe.s * C::X_B;
+            if (i + 1 < n_mine) {
+                u = mine(i + 1);
+                ahead.fetch(u);
+            }
+            for (int c0 = 0; c0 < nck; c0 += kStep) {
 #pragma unroll
-                for (int j = 0; j < RP; ++j)
-                    if (rr + 16 * j < u.nr) cp16(dst + j * 16 * kRowB, in ? src[j] + ck * kRowB : src[j], in ? 16 : 0);
-                cp_arrive(&full[pipe.s]);
+                for (int a = 0; a < kStep; ++a) {
+                    if (c0 + a >= nck) break;
+                    wait(&empty[pipe.s], pipe.ph ^ 1);
+                    const uint32_t dst = dst0 + pipe.s * C::X_B;
+                    if ((c0 + a + 1) * kRowB <= kb) {
+#pragma unroll
+                        for (int j = 0; j < RP; ++j)
+                            if (16 * j < nl) cp16(dst + j * 16 * kRowB, src[j] + a * kRowB);
+                    } else {                                  // the row ends in this stage: zeros behind it
+                        const bool in = (c0 + a) * kRowB + c * 16 < kb;
+#pragma unroll
+                        for (int j = 0; j < RP; ++j)
+                            if (16 * j < nl) cp16_or_zero(dst + j * 16 * kRowB, in ? src[j] + a * kRowB : src[j], in);
+                    }
+                    cp_arrive(&full[pipe.s]);
+                    pipe.next(ST);
+                }
+#pragma unroll
+                for (int j = 0; j < RP; ++j) src[j] += kStep * kRowB;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -625,13 +665,11 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             }
         }
         float* const st = epi + g * kSlice * kEpiLd;
-        const int lpt = act ? 8 : 16, tpw = 32 / lpt;         // lanes a row (8 outputs a lane), rows a warp stores at a time
-        const int c0 = (lane % lpt) * 8;                      // the lane's first output in the block (and staged column)
+        const int64_t row_b = p.y_pitch * es;
         uint32_t ab = 0;
         for (uint32_t i = 0; i < n_mine; ++i, ab ^= 1) {
             const Unit u = unit_at(i);
-            const int64_t n0 = (int64_t)(u.blk + rank) * blk_out + c0;
-            const bool col_ok = n0 < p.n_out;
+            const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
             // which of the unit's rows are live, 32 a lane: asked for while the accumulators are still being computed
             uint32_t live = 0;
 #pragma unroll
@@ -642,39 +680,101 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             }
             wait(&acc_full[ab], (i >> 1) & 1);
             if (epi_any(g, *vdead)) break;
+            int turn = 0;
             fence_after();
+            // silu_mul: lanes 0..15 hold 16 gate rows, 16..31 their up rows; the lower half takes the even rows' outputs of
+            // a slice, the upper the odd ones'
+            const bool up = lane >= 16;
+            const int64_t n = b0 + (act ? 16 * q + (lane & 15) : 32 * q + lane);
             const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + ab * NT;
             uint32_t a[16];
             if (g * kSlice < u.nr) tmem_ld16(acc + g * kSlice, a);
             for (int t0 = g * kSlice; t0 < u.nr; t0 += C::EPI_G * kSlice) {
                 tmem_wait(a);
+                float v[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = __uint_as_float(a[j]);
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(a[j]);
                 if (t0 + C::EPI_G * kSlice < u.nr) tmem_ld16(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
+                uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
+                if (act) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float other = __shfl_xor_sync(0xFFFFFFFFu, up ? v[2 * j] : v[2 * j + 1], 16);
+                        const float z = up ? other : v[2 * j];
+                        v[j] = silu(z) * (up ? v[2 * j + 1] : other);
+                    }
+                }
+                if (p.y_dtype == RAD_F32) {
+                    // straight from the registers: a warp's store is 32 outputs of a row (silu_mul: 16 of two rows)
+                    uint8_t* d = y + (u.r0 + t0 + (act && up ? 1 : 0)) * row_b + n * 4;
+                    here = n < p.n_out ? act && up ? here >> 1 : here : 0u;
+                    if (act) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j, d += 2 * row_b)
+                            if (here >> (2 * j) & 1) *reinterpret_cast<float*>(d) = v[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, d += row_b)
+                            if (here >> j & 1) *reinterpret_cast<float*>(d) = v[j];
+                    }
+                    continue;
+                }
+                if (!mx_out) {
+                    // Two rows of an output a word, lines of words in shared memory (two buffers in turn, so one barrier a
+                    // slice does), then 16 (silu_mul: 8) bytes of two rows a thread. Two-byte stores straight from the
+                    // registers took 12 cycles each: 218 against 177 us at 16 experts, 16067 rows, 1536 -> 4096.
+                    uint32_t* sw = reinterpret_cast<uint32_t*>(st) + turn * 1024;
+                    turn ^= 1;
+                    if (act) {
+#pragma unroll
+                        for (int m = 0; m < 4; ++m)
+                            sw[(2 * m + (lane >> 4)) * 80 + 16 * q + (lane & 15)] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
+                        epi_sync(g);
+                        const int line = 2 * q + (lane >> 4), c = 4 * (lane & 15), j = (line >> 1) * 4 + (line & 1);
+                        const uint4 w = *reinterpret_cast<const uint4*>(sw + line * 80 + c);
+                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + (b0 + c) * 2;
+                        if (b0 + c < p.n_out) {
+                            if (here >> j & 1) *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
+                            if (here >> (j + 2) & 1)
+                                *reinterpret_cast<uint2*>(d + 2 * row_b) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
+                        }
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) sw[m * 128 + 32 * q + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
+                        epi_sync(g);
+                        const int line = 2 * q + (lane >> 4), c = 8 * (lane & 15), j = 2 * line;
+                        const uint4 w0 = *reinterpret_cast<const uint4*>(sw + line * 128 + c);
+                        const uint4 w1 = *reinterpret_cast<const uint4*>(sw + line * 128 + c + 4);
+                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + (b0 + c) * 2;
+                        if (b0 + c < p.n_out) {
+                            if (here >> j & 1)
+                                *reinterpret_cast<uint4*>(d) = make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
+                                                                          __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
+                            if (here >> (j + 1) & 1)
+                                *reinterpret_cast<uint4*>(d + row_b) = make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
+                                                                                  __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
+                        }
+                    }
+                    continue;
+                }
+                // MXFP4: staged, since a block's 32 outputs lie in two warps (silu_mul); eight outputs of a row a thread
+                const int lpt = blk_out / 8, tpw = 32 / lpt, c0 = (lane % lpt) * 8;
+                if (act) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) st[(2 * j + (lane >> 4)) * kEpiLd + 16 * q + (lane & 15)] = v[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = v[j];
+                }
                 epi_sync(g);
                 for (int j = q * tpw + lane / lpt; j < kSlice; j += 4 * tpw) {
-                    const int64_t r = u.r0 + t0 + j;
-                    const bool row_ok = __shfl_sync(0xFFFFFFFFu, live, (t0 + j) >> 5) >> ((t0 + j) & 31) & 1;
-                    const float4* s = reinterpret_cast<const float4*>(&st[j * kEpiLd + c0]);
-                    const float4 s0 = s[0], s1 = s[1];
-                    float v[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
-                    if (act) {
-                        const float4 u0 = s[16], u1 = s[17];
-                        const float up[8] = { u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w };
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = __fdividef(v[e], 1.f + __expf(-v[e])) * up[e];
-                    }
-                    if (mx_out) {
-                        const uint32_t code = mx4_quad_code(v);          // four lanes: 32 outputs of one row
-                        if (row_ok && col_ok) {
-                            *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(v, code);
-                            if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
-                        }
-                    } else if (row_ok && col_ok) {
-                        uint8_t* dst = y + (r * p.y_pitch + n0) * es;
-                        if (p.y_dtype == RAD_F32) st8<1>(dst, v);
-                        else if (p.y_dtype == RAD_F16) st8<2>(dst, v);
-                        else st8<3>(dst, v);
+                    const int64_t r = u.r0 + t0 + j, n0 = b0 + c0;
+                    float f[8];
+                    ld8<1>(&st[j * kEpiLd + c0], f);
+                    const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
+                    if (here >> j & 1 && n0 < p.n_out) {
+                        *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);
+                        if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
                     }
                 }
                 epi_sync(g);
@@ -712,17 +812,26 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// Weights: [expert][row][k], boxes of 128 bytes of k and a block's 128 rows (silu_mul: its 64 gate or 64 up rows).
+// Weights, boxes of 128 bytes of k: [expert][row][k] and a block's 128 rows; for silu_mul [expert][group of 16 rows]
+// [gate, up][16][k] and a block's four groups, in one box (eight boxes of 16 rows a stage kept the issuing warp busy, 550
+// cycles a stage) unless the last group is half a one and the box would leave the weight: then a box a half group.
 int make_map(const Exl3bGmmOp* p, CUtensorMap* map) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return -6;
     const CUtensorMapDataType dt = p->mx4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                           : p->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const cuuint64_t dims[3] = { (cuuint64_t)(p->mx4 ? p->n_in / 2 : p->n_in), (cuuint64_t)p->w_rows, (cuuint64_t)p->n_expert };
-    const cuuint64_t strides[2] = { (cuuint64_t)p->w_pitch_bytes, (cuuint64_t)p->w_expert_bytes };
-    const cuuint32_t box[3] = { p->mx4 ? 128u : 64u, p->act ? 64u : 128u, 1u }, one[3] = { 1, 1, 1 };
-    return fn(map, dt, 3, const_cast<void*>(p->w), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+    const cuuint64_t k = (cuuint64_t)(p->mx4 ? p->n_in / 2 : p->n_in), pitch = (cuuint64_t)p->w_pitch_bytes;
+    const cuuint32_t kb = p->mx4 ? 128u : 64u, one[5] = { 1, 1, 1, 1, 1 };
+    const bool whole = p->act && p->n_out % 16 == 0;
+    const cuuint64_t dims3[3] = { k, (cuuint64_t)p->w_rows, (cuuint64_t)p->n_expert };
+    const cuuint64_t strides3[2] = { pitch, (cuuint64_t)p->w_expert_bytes };
+    const cuuint32_t box3[3] = { kb, p->act ? 16u : 128u, 1u };
+    const cuuint64_t dims5[5] = { k, 16, 2, (cuuint64_t)(p->n_out / 16), (cuuint64_t)p->n_expert };
+    const cuuint64_t strides5[4] = { pitch, (cuuint64_t)p->n_out * pitch, 16 * pitch, (cuuint64_t)p->w_expert_bytes };
+    const cuuint32_t box5[5] = { kb, 16, 2, 4, 1 };
+    return fn(map, dt, whole ? 5 : 3, const_cast<void*>(p->w), whole ? dims5 : dims3, whole ? strides5 : strides3,
+              whole ? box5 : box3, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? 0 : -6;
 }
 

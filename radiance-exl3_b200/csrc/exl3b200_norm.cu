@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* q, int64_
 
 // A weight's row-major scales [E][rows][cols / 32] -> the tiles the product's kernel copies whole: per expert, per block
 // of 128 weight rows, per 128 input columns 512 bytes, row r's four scales at (r % 32) * 16 + (r / 32) * 4. With
-// silu_mul a block is 64 gate rows then their 64 up rows. Rows and columns past the weight's get code 0.
+// silu_mul a block is 64 gate rows and their 64 up rows, 16 of each in turn. Rows and columns past the weight's get code 0.
 __global__ void __launch_bounds__(256) k_mx4_tile(const uint8_t* s, int64_t s_pitch, int64_t e_pitch, int64_t rows,
                                                   int64_t cols, int act, int64_t n_blk, int64_t n_k, int64_t total,
                                                   uint32_t* out) {
@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(256) k_mx4_tile(const uint8_t* s, int64_t s_pi
         const int64_t tile = i >> 7;
         const int w = (int)(i & 127), r = (w >> 2) + 32 * (w & 3);       // word w: row r's four scales
         const int64_t kb = tile % n_k, blk = tile / n_k % n_blk, e = tile / n_k / n_blk;
-        const int64_t half = rows / 2, j = blk * 64 + (r & 63);
-        const int64_t row = act ? (j < half ? (r < 64 ? j : half + j) : rows) : blk * 128 + r;
+        const int64_t half = rows / 2, j = blk * 64 + (r >> 5) * 16 + (r & 15);
+        const int64_t row = act ? (j < half ? (r & 16 ? half + j : j) : rows) : blk * 128 + r;
         uint32_t v = 0;
         for (int b = 0; b < 4; ++b) {
             const int64_t c = kb * 4 + b;
