@@ -47,7 +47,7 @@ constexpr int kSlice = 16;                       // sorted rows an epilogue grou
 constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
 constexpr int kMaxExpert = 2048;
-constexpr int kMaxSt = 8;                        // stages at most
+constexpr int kMaxSt = 10;                       // stages at most
 
 template <bool MX, bool PAIR>
 struct Cfg {
@@ -67,13 +67,12 @@ struct Cfg {
     static constexpr int PER_SM = PAIR ? 1 : 2;
     // shared memory: alignment, staging, barriers, the unit prefix, and as many stages as fit beside the static arrays (the
     // narrow form: twice an SM)
-    static constexpr int ROOM = (PAIR ? 227 : 113) * 1024 - kTab * 16 - 128;
     static constexpr int fixed(int n_expert) { return 1024 + EPI_B + 512 + (n_expert + 4) * 4; }
-    static constexpr int stages(int n_expert) {
-        const int n = (ROOM - fixed(n_expert)) / STAGE_B;
+    static constexpr int stages(int n_expert, int per_sm) {
+        const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kTab * 16 - 128 - fixed(n_expert)) / STAGE_B;
         return n < kMaxSt ? n : kMaxSt;
     }
-    static_assert(COLS <= 512 && stages(kMaxExpert) >= 4, "tensor or shared memory");
+    static_assert(COLS <= 512 && stages(kMaxExpert, PER_SM) >= 4, "tensor or shared memory");
     static_assert((2 * kMaxSt + 4) * 8 + 8 <= 512, "barriers");
 };
 
@@ -850,12 +849,15 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     if (rc) return rc;
     auto kern = k_gmm<MX, PAIR>;
     cudaLaunchConfig_t cfg = {};
-    const int stages = C::stages(p->n_expert);
+    const int64_t most = most_units(p, C::NT, PAIR ? 2 : 1);
+    // few units: one CTA an SM, with the whole of its shared memory for stages in flight
+    const int per_sm = !PAIR && most <= sm_count ? 1 : C::PER_SM;
+    const int64_t room = PAIR ? sm_count / 2 : (int64_t)sm_count * per_sm;
+    const int stages = C::stages(p->n_expert, per_sm);
     cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
     cfg.blockDim = dim3(C::THREADS);
     cfg.stream = st;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess) return -6;
-    const int64_t room = PAIR ? sm_count / 2 : (int64_t)sm_count * C::PER_SM, most = most_units(p, C::NT, PAIR ? 2 : 1);
     cfg.gridDim = dim3((unsigned)((most < room ? most : room) * (PAIR ? 2 : 1)));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
