@@ -43,9 +43,11 @@ namespace {
 constexpr int kXWarp0 = 4, kXWarps = 4, kEpiWarp0 = 8;
 constexpr int kRowB = 128;                       // bytes of k a stage: one swizzle row
 constexpr int kW_B = 128 * kRowB;                // a CTA's weight rows of a stage
-constexpr int kSlice = 16;                       // sorted rows an epilogue group stages at a time
+constexpr int kSlice = 16;                       // sorted rows an epilogue group takes at a time
+constexpr int kStage = 8;                        // ... and stages (in f32; in 16 bits all 16)
 constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
+constexpr int kStatic = 3072;                    // the static shared arrays, up to the ring's alignment
 constexpr int kMaxExpert = 2048;
 constexpr int kMaxSt = 10;                       // stages at most
 
@@ -60,7 +62,7 @@ struct Cfg {
     static constexpr int SFX_G = MX ? (NT + 127) / 128 : 0;      // 128-row groups of the sorted rows' scales
     static constexpr int SFX_B = SFX_G * 1024;
     static constexpr int STAGE_B = kW_B + X_B + SFW_B + SFX_B;
-    static constexpr int EPI_B = EPI_G * kSlice * kEpiLd * 4;
+    static constexpr int EPI_B = EPI_G * kStage * kEpiLd * 4;
     static constexpr int SFC = MX ? 8 + 8 * SFX_G : 0;           // TMEM columns of a stage's scales
     static constexpr int COLS = 2 * NT + 2 * SFC;
     static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 512;
@@ -69,7 +71,7 @@ struct Cfg {
     // narrow form: twice an SM)
     static constexpr int fixed(int n_expert) { return 1024 + EPI_B + 512 + (n_expert + 4) * 4; }
     static constexpr int stages(int n_expert, int per_sm) {
-        const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kTab * 16 - 128 - fixed(n_expert)) / STAGE_B;
+        const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kStatic - fixed(n_expert)) / STAGE_B;
         return n < kMaxSt ? n : kMaxSt;
     }
     static_assert(COLS <= 512 && stages(kMaxExpert, PER_SM) >= 4, "tensor or shared memory");
@@ -82,40 +84,40 @@ struct Unit {
     int32_t nr;          // sorted rows
 };
 
-template <int NT>
-__device__ __forceinline__ uint32_t groups(const Exl3bGmmOp& p, int e, int64_t* r0, int64_t* r1) {
-    if (p.expert_offset) {
-        *r0 = p.expert_offset[e];
-        *r1 = p.expert_offset[e + 1];
-        if (*r0 < 0) *r0 = 0;
-        if (*r1 > p.n_rows) *r1 = p.n_rows;
-    } else {
-        *r0 = 0;
-        *r1 = p.n_rows;
-    }
-    return *r1 > *r0 ? (uint32_t)((*r1 - *r0 + NT - 1) / NT) : 0u;
+// The sorted rows of expert e, and into how many groups of at most NT they fall.
+struct Run {
+    int32_t r0, rows;
+};
+__device__ __forceinline__ Run run_of(const Exl3bGmmOp& p, int e) {
+    if (!p.expert_offset) return Run{ 0, (int32_t)p.n_rows };
+    const int32_t a = max(p.expert_offset[e], 0), b = min(p.expert_offset[e + 1], (int32_t)p.n_rows);
+    return Run{ a, max(b - a, 0) };
 }
-
 template <int NT>
-__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, uint32_t n_mb,
-                                          int mt) {
+__device__ __forceinline__ uint32_t groups(const Run& r) { return (uint32_t)(r.rows + NT - 1) / NT; }
+
+// Unit `local` of expert e: block by block, then group by group. An expert's rows are split evenly over its groups, in
+// steps of the MMA's N, so that no group is left with a sliver.
+template <int NT, int MB>
+__device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, uint32_t n_mb) {
+    const uint32_t g = local / n_mb, ng = groups<NT>(r), step = 16 * MB;
+    const uint32_t per = (((uint32_t)r.rows + ng - 1) / ng + step - 1) / step * step;
+    Unit u;
+    u.e = e;
+    u.blk = (int32_t)(local - g * n_mb) * MB;
+    u.r0 = r.r0 + (int32_t)(g * per);
+    u.nr = min((int32_t)per, r.rows - (int32_t)(g * per));
+    return u;
+}
+// ... found by its number among all units.
+template <int NT, int MB>
+__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, uint32_t n_mb) {
     int lo = 0, hi = p.n_expert;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid] <= unit) lo = mid; else hi = mid;
     }
-    const uint32_t local = unit - prefix[lo], g = local / n_mb;
-    int64_t r0, r1;
-    const uint32_t ng = groups<NT>(p, lo, &r0, &r1);
-    // the expert's rows split evenly over its groups, in steps of the MMA's N: no group is left with a sliver
-    const int64_t step = 16 * mt, per = ((r1 - r0 + ng - 1) / ng + step - 1) / step * step;
-    Unit u;
-    u.e = lo;
-    u.blk = (int32_t)(local % n_mb) * mt;
-    const int64_t a = r0 + g * per, left = r1 - a;
-    u.r0 = (int32_t)a;
-    u.nr = (int32_t)(left < per ? left : per);
-    return u;
+    return make_unit<NT, MB>(lo, run_of(p, lo), unit - prefix[lo], n_mb);
 }
 
 struct Pipe {
@@ -328,7 +330,8 @@ struct RowScales {
 // z / (1 + e^-z), from the special-function unit.
 __device__ __forceinline__ float silu(float z) {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-z)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + r));
     return z * r;
 }
 __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
@@ -388,14 +391,14 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
-    // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts)
+    // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts); this CTA's units
+    // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
         __shared__ uint32_t wsum[THREADS / 32];
         const int per = (p.n_expert + THREADS - 1) / THREADS;
         const int e0 = min(tid * per, p.n_expert), e1 = min(e0 + per, p.n_expert);
-        int64_t a, b;
         uint32_t sum = 0;
-        for (int e = e0; e < e1; ++e) sum += groups<NT>(p, e, &a, &b) * n_mb;
+        for (int e = e0; e < e1; ++e) sum += groups<NT>(run_of(p, e)) * n_mb;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -407,23 +410,27 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         uint32_t acc = incl - sum;
         for (int w = 0; w < warp; ++w) acc += wsum[w];
         for (int e = e0; e < e1; ++e) {
+            const Run r = run_of(p, e);
+            const uint32_t n = groups<NT>(r) * n_mb;
             prefix[e] = acc;
-            acc += groups<NT>(p, e, &a, &b) * n_mb;
+            if (n) {
+                uint32_t i = acc > first ? (acc - first + stride - 1) / stride : 0u;
+                for (; i < kTab && first + i * stride < acc + n; ++i)
+                    utab[i] = make_unit<NT, MB>(e, r, first + i * stride - acc, n_mb);
+            }
+            acc += n;
         }
         if (tid == THREADS - 1) prefix[p.n_expert] = acc;
     }
-    __syncthreads();
-    const uint32_t n_units = prefix[p.n_expert];
-    const uint32_t n_mine = n_units > first ? (n_units - first + stride - 1) / stride : 0;
-    for (uint32_t i = tid; i < n_mine && i < kTab; i += THREADS)
-        utab[i] = find_unit<NT>(p, prefix, first + i * stride, n_mb, MB);
     fence_before();
     __syncthreads();
     if (PAIR) cluster_sync_all();                             // both CTAs' barriers and tensor memory are set up
     fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    const uint32_t n_units = prefix[p.n_expert];
+    const uint32_t n_mine = n_units > first ? (n_units - first + stride - 1) / stride : 0;
     auto unit_at = [&](uint32_t i) {
-        return i < kTab ? utab[i] : find_unit<NT>(p, prefix, first + i * stride, n_mb, MB);
+        return i < kTab ? utab[i] : find_unit<NT, MB>(p, prefix, first + i * stride, n_mb);
     };
     const int nck = (int)((p.n_in + (MX ? 255 : 63)) / (MX ? 256 : 64));
     volatile uint32_t* vdead = dead;
@@ -528,56 +535,60 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         // ---------------------------------------------------------------- MXFP4: the sorted rows' scales
         // Warp 2 the unit's rows 0..127, warp 3 (PAIR) the others; both CTAs of a pair need them all. Row r's four scales of
         // 128 k go to (r % 32) * 16 + (r / 32) * 4: lane l holds rows l, l + 32, ... and writes 16 consecutive bytes. A lane
-        // reads 32 bytes of each of its rows at a time, four stages' worth, one batch ahead (each row is a line of its own:
-        // 4-byte copies a stage kept the L1 busy, and a batch of two stages is shorter than the loads' latency).
+        // reads 16 bytes of each of its rows at a time, two stages' worth (each row is a line of its own: 4-byte copies a
+        // stage kept the L1 busy), into two register sets in turn, one on its way while the other is used, across units.
         const int g = warp - 2;
-        if (MX && g < C::SFX_G) {
+        if (MX && g < C::SFX_G && n_mine) {
             constexpr int Q = NT < 128 ? NT / 32 : 4;
             const RowScales rs(p);
             RowAhead<Q> ahead(p, lane + g * 128, 32);
-            constexpr int kAhead = 4;                         // stages a batch
-            uint4 nxt[2][Q];
             const uint8_t* src[Q];
-            if (n_mine) {
-                ahead.fetch(unit_at(0));
-                ahead.rows(p.x_scales, p.xs_pitch, src);
+            uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
+            int lc = 0, cc = 0;                               // ... and their first stages
+            ahead.fetch(unit_at(0));
+            ahead.rows(p.x_scales, p.xs_pitch, src);
+            if (n_mine > 1) ahead.fetch(unit_at(1));
+            auto load = [&](uint4 v[Q]) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    nxt[0][q] = rs.load(src[q], 0);
-                    nxt[1][q] = rs.load(src[q], 16);
+                for (int q = 0; q < Q; ++q) v[q] = rs.load(src[q], 8 * lc);
+                if ((lc += 2) >= nck && ++lu < n_mine) {
+                    lc = 0;
+                    ahead.rows(p.x_scales, p.xs_pitch, src);
+                    if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
                 }
-            }
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                if (i + 1 < n_mine) ahead.fetch(unit_at(i + 1));
-                for (int c0 = 0; c0 < nck; c0 += kAhead) {
-                    uint4 cur[2][Q];
-                    if (c0 + kAhead >= nck && i + 1 < n_mine) ahead.rows(p.x_scales, p.xs_pitch, src);
-                    const int off = c0 + kAhead < nck ? 8 * (c0 + kAhead) : 0;
+            };
+            auto use = [&](const uint4 v[Q]) {
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) {
-                        cur[0][q] = nxt[0][q];
-                        cur[1][q] = nxt[1][q];
-                        nxt[0][q] = rs.load(src[q], off);
-                        nxt[1][q] = rs.load(src[q], off + 16);
+                for (int a = 0; a < 2; ++a) {
+                    if (cc + a >= nck) break;
+                    wait(&empty[pipe.s], pipe.ph ^ 1);
+                    uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        auto word = [&](int q) {
+                            const uint4 x = v[q < Q ? q : 0];
+                            return q >= Q ? 0u : a ? (h ? x.w : x.z) : h ? x.y : x.x;
+                        };
+                        dst[h * (C::SFX_G * 32)] = make_uint4(word(0), word(1), word(2), word(3));
                     }
-#pragma unroll
-                    for (int a = 0; a < kAhead; ++a) {
-                        if (c0 + a >= nck) continue;
-                        wait(&empty[pipe.s], pipe.ph ^ 1);
-                        uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            auto word = [&](int q) {
-                                const uint4 v = cur[a >> 1][q < Q ? q : 0];
-                                return q >= Q ? 0u : a & 1 ? (h ? v.w : v.z) : h ? v.y : v.x;
-                            };
-                            dst[h * (C::SFX_G * 32)] = make_uint4(word(0), word(1), word(2), word(3));
-                        }
-                        __syncwarp();                          // the MMA warp's fence covers these writes too
-                        if (lane == 0) mbar_arrive(&full[pipe.s]);
-                        pipe.next(ST);
-                    }
+                    __syncwarp();                              // the MMA warp's fence covers these writes too
+                    if (lane == 0) mbar_arrive(&full[pipe.s]);
+                    pipe.next(ST);
                 }
+                if ((cc += 2) >= nck) {
+                    cc = 0;
+                    ++cu;
+                }
+            };
+            uint4 even[Q], odd[Q];
+            load(even);
+            load(odd);
+            while (cu < n_mine && !*vdead) {
+                use(even);
+                load(even);
+                if (cu >= n_mine) break;
+                use(odd);
+                load(odd);
             }
         }
     } else if (warp < kEpiWarp0) {
@@ -663,7 +674,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                 }
             }
         }
-        float* const st = epi + g * kSlice * kEpiLd;
+        float* const st = epi + g * kStage * kEpiLd;
         const int64_t row_b = p.y_pitch * es;
         uint32_t ab = 0;
         for (uint32_t i = 0; i < n_mine; ++i, ab ^= 1) {
@@ -678,8 +689,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                 if (lane == b) live = m;
             }
             wait(&acc_full[ab], (i >> 1) & 1);
-            if (epi_any(g, *vdead)) break;
-            int turn = 0;
+            if (mx_out ? epi_any(g, *vdead) : __any_sync(0xFFFFFFFFu, *vdead)) break;
+
             fence_after();
             // silu_mul: lanes 0..15 hold 16 gate rows, 16..31 their up rows; the lower half takes the even rows' outputs of
             // a slice, the upper the odd ones'
@@ -719,64 +730,61 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                     continue;
                 }
                 if (!mx_out) {
-                    // Two rows of an output a word, lines of words in shared memory (two buffers in turn, so one barrier a
-                    // slice does), then 16 (silu_mul: 8) bytes of two rows a thread. Two-byte stores straight from the
-                    // registers took 12 cycles each: 218 against 177 us at 16 experts, 16067 rows, 1536 -> 4096.
-                    uint32_t* sw = reinterpret_cast<uint32_t*>(st) + turn * 1024;
-                    turn ^= 1;
+                    // Two rows of an output a word, lines of words in the warp's own 1 KB of shared memory, then four outputs
+                    // of two rows a thread: whole 32-byte sectors, and no warp waits for another. Two-byte stores straight
+                    // from the registers took 12 cycles each: 218 against 177 us at 16 experts, 16067 rows, 1536 -> 4096.
+                    uint32_t* sw = reinterpret_cast<uint32_t*>(epi) + ew * 256;
                     if (act) {
 #pragma unroll
-                        for (int m = 0; m < 4; ++m)
-                            sw[(2 * m + (lane >> 4)) * 80 + 16 * q + (lane & 15)] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
-                        epi_sync(g);
-                        const int line = 2 * q + (lane >> 4), c = 4 * (lane & 15), j = (line >> 1) * 4 + (line & 1);
-                        const uint4 w = *reinterpret_cast<const uint4*>(sw + line * 80 + c);
-                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + (b0 + c) * 2;
-                        if (b0 + c < p.n_out) {
-                            if (here >> j & 1) *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
-                            if (here >> (j + 2) & 1)
-                                *reinterpret_cast<uint2*>(d + 2 * row_b) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
-                        }
+                        for (int m = 0; m < 4; ++m) sw[32 * m + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
                     } else {
 #pragma unroll
-                        for (int m = 0; m < 8; ++m) sw[m * 128 + 32 * q + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
-                        epi_sync(g);
-                        const int line = 2 * q + (lane >> 4), c = 8 * (lane & 15), j = 2 * line;
-                        const uint4 w0 = *reinterpret_cast<const uint4*>(sw + line * 128 + c);
-                        const uint4 w1 = *reinterpret_cast<const uint4*>(sw + line * 128 + c + 4);
-                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + (b0 + c) * 2;
-                        if (b0 + c < p.n_out) {
-                            if (here >> j & 1)
-                                *reinterpret_cast<uint4*>(d) = make_uint4(__byte_perm(w0.x, w0.y, 0x5410), __byte_perm(w0.z, w0.w, 0x5410),
-                                                                          __byte_perm(w1.x, w1.y, 0x5410), __byte_perm(w1.z, w1.w, 0x5410));
-                            if (here >> (j + 1) & 1)
-                                *reinterpret_cast<uint4*>(d + row_b) = make_uint4(__byte_perm(w0.x, w0.y, 0x7632), __byte_perm(w0.z, w0.w, 0x7632),
-                                                                                  __byte_perm(w1.x, w1.y, 0x7632), __byte_perm(w1.z, w1.w, 0x7632));
+                        for (int m = 0; m < 8; ++m) sw[32 * m + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (k && act) break;
+                        const uint4 w = *reinterpret_cast<const uint4*>(sw + 128 * k + 4 * lane);
+                        // act: line 2m + odd holds rows 4m + odd and 4m + odd + 2; else line m rows 2m and 2m + 1
+                        const int line = act ? lane >> 2 : 4 * k + (lane >> 3), dj = act ? 2 : 1;
+                        const int j = act ? (line >> 1) * 4 + (line & 1) : 2 * line;
+                        const int64_t n0 = b0 + (act ? 16 * q + 4 * (lane & 3) : 32 * q + 4 * (lane & 7));
+                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + n0 * 2;
+                        if (n0 < p.n_out) {
+                            if (here >> j & 1) *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
+                            if (here >> (j + dj) & 1)
+                                *reinterpret_cast<uint2*>(d + dj * row_b) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
                         }
                     }
+                    __syncwarp();
                     continue;
                 }
                 // MXFP4: staged, since a block's 32 outputs lie in two warps (silu_mul); eight outputs of a row a thread
                 const int lpt = blk_out / 8, tpw = 32 / lpt, c0 = (lane % lpt) * 8;
-                if (act) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) st[(2 * j + (lane >> 4)) * kEpiLd + 16 * q + (lane & 15)] = v[j];
-                } else {
+                for (int h = 0; h < 2; ++h) {
+                    if (act) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) st[j * kEpiLd + 32 * q + lane] = v[j];
-                }
-                epi_sync(g);
-                for (int j = q * tpw + lane / lpt; j < kSlice; j += 4 * tpw) {
-                    const int64_t r = u.r0 + t0 + j, n0 = b0 + c0;
-                    float f[8];
-                    ld8<1>(&st[j * kEpiLd + c0], f);
-                    const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
-                    if (here >> j & 1 && n0 < p.n_out) {
-                        *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);
-                        if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
+                        for (int j = 0; j < 4; ++j) st[(2 * j + (lane >> 4)) * kEpiLd + 16 * q + (lane & 15)] = v[4 * h + j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) st[j * kEpiLd + 32 * q + lane] = v[8 * h + j];
                     }
+                    epi_sync(g);
+                    if (q * tpw < kStage) {                                  // whole warps: the quads vote
+                        const int j = q * tpw + lane / lpt;
+                        const int64_t r = u.r0 + t0 + 8 * h + j, n0 = b0 + c0;
+                        float f[8];
+                        ld8<1>(&st[j * kEpiLd + c0], f);
+                        const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
+                        if (here >> (8 * h + j) & 1 && n0 < p.n_out) {
+                            *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);
+                            if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
+                        }
+                    }
+                    epi_sync(g);
                 }
-                epi_sync(g);
             }
             fence_before();
             __syncwarp();
@@ -857,7 +865,13 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
     cfg.blockDim = dim3(C::THREADS);
     cfg.stream = st;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess) return -6;
+    static bool allowed[64];                                  // the most shared memory, once a device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
+    if (!allowed[dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
+        allowed[dev] = true;
+    }
     cfg.gridDim = dim3((unsigned)((most < room ? most : room) * (PAIR ? 2 : 1)));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
