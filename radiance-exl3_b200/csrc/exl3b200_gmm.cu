@@ -381,24 +381,33 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
     constexpr int MB = PAIR ? 2 : 1;
     const uint32_t n_mb = (uint32_t)((p.n_out + blk_out * MB - 1) / (blk_out * MB));
-    if (tid == 0) {
-        for (int s = 0; s < ST; ++s) {
-            mbar_init(&full[s], 1 + 32 * kXWarps + C::SFX_G + (PAIR && rank == 0 ? 1 : 0));
-            mbar_init(&empty[s], 1);
-        }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * C::EPI_G * MB); }
+    // the runs of this thread's experts first: their latency covers the barriers' set-up
+    constexpr int kPer = (kMaxExpert + THREADS - 1) / THREADS;
+    const int per = (p.n_expert + THREADS - 1) / THREADS, e0 = tid * per;
+    Run run[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) run[i] = i < per && e0 + i < p.n_expert ? run_of(p, e0 + i) : Run{ 0, 0 };
+    if (tid < ST) {
+        mbar_init(&full[tid], 1 + 32 * kXWarps + C::SFX_G + (PAIR && rank == 0 ? 1 : 0));
+        mbar_init(&empty[tid], 1);
+    } else if (tid < ST + 2) {
+        mbar_init(&acc_full[tid - ST], 1);
+        mbar_init(&acc_empty[tid - ST], 4 * C::EPI_G * MB);
+    } else if (tid == ST + 2) {
         *dead = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
     }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
     if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
+    if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts); this CTA's units
     // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
         __shared__ uint32_t wsum[THREADS / 32];
-        const int per = (p.n_expert + THREADS - 1) / THREADS;
-        const int e0 = min(tid * per, p.n_expert), e1 = min(e0 + per, p.n_expert);
         uint32_t sum = 0;
-        for (int e = e0; e < e1; ++e) sum += groups<NT>(run_of(p, e)) * n_mb;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += groups<NT>(run[i]) * n_mb;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -409,14 +418,15 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         __syncthreads();
         uint32_t acc = incl - sum;
         for (int w = 0; w < warp; ++w) acc += wsum[w];
-        for (int e = e0; e < e1; ++e) {
-            const Run r = run_of(p, e);
-            const uint32_t n = groups<NT>(r) * n_mb;
-            prefix[e] = acc;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (j >= per || e0 + j >= p.n_expert) break;
+            const uint32_t n = groups<NT>(run[j]) * n_mb;
+            prefix[e0 + j] = acc;
             if (n) {
                 uint32_t i = acc > first ? (acc - first + stride - 1) / stride : 0u;
                 for (; i < kTab && first + i * stride < acc + n; ++i)
-                    utab[i] = make_unit<NT, MB>(e, r, first + i * stride - acc, n_mb);
+                    utab[i] = make_unit<NT, MB>(e0 + j, run[j], first + i * stride - acc, n_mb);
             }
             acc += n;
         }
@@ -424,7 +434,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     }
     fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();                             // both CTAs' barriers and tensor memory are set up
+    if (PAIR) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // both CTAs' barriers and tensor memory are set up
     fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
