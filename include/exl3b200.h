@@ -499,6 +499,53 @@ typedef struct Exl3bBlockNorm {
 } Exl3bBlockNorm;
 int     exl3b200_block_norm(const Exl3bBlockNorm* norm, void* stream);
 
+/* A residual MoE block over such experts, the sequence an engine issues for it, driven from C:
+ *   xn = rmsnorm(x) * pre_w -> logits = xn . router_w (f32) -> router_scatter -> h = silu_mul(gate, up) -> down ->
+ *   moe_gather (softmax weights) -> out = res_scale * x + gate * rmsnorm(gathered) * post_w; next = rmsnorm(out) * next_w
+ * over block_norm, grouped_mm and the routing entries above. x, out and next are [T][hidden] of `dtype` (RAD_F16 or
+ * RAD_BF16), as are router_w [n_expert][hidden] and the norms' and the gate's [hidden] (post_w, gate, next_w may be NULL).
+ * weights: `dtype`, or EXL3B_MX4 (gu_w [n_expert][2 width][hidden] and dn_w [n_expert][hidden][width] as codes, the
+ * scales tiled: gu_scales for SILU_MUL; xn is then also quantised for them, and h is MXFP4). `out` may be x; `next` is
+ * optional. n_expert a multiple of 8, at most 2048; hidden and width multiples of 8 (MXFP4: 32).
+ * exl3b200_expert_block_work_bytes sizes one device block for up to max_tokens tokens a pass (-1: refused),
+ * exl3b200_expert_block_carve cuts it, and a forward only enqueues (it can be captured in a CUDA graph). */
+typedef struct Exl3bExpertBlockDesc {
+    int64_t     n_expert, hidden, width, top_k;
+    int32_t     dtype, weights;
+    float       eps, res_scale;
+    const void* router_w;
+    const void* gu_w;
+    const void* gu_scales;
+    const void* dn_w;
+    const void* dn_scales;
+    const void* pre_w;
+    const void* post_w;
+    const void* gate;
+    const void* next_w;
+} Exl3bExpertBlockDesc;
+typedef struct Exl3bExpertBlockBufs {
+    int64_t   max_tokens;
+    void*     xn;             /* [max_tokens][hidden] */
+    uint8_t*  x_codes;        /* MXFP4: [max_tokens][hidden / 2] */
+    uint8_t*  x_scales;
+    float*    logits;         /* [max_tokens][n_expert] */
+    int32_t*  ids;            /* [max_tokens][top_k] */
+    float*    w;
+    int32_t*  sorted_tok;     /* [max_tokens * top_k] */
+    int32_t*  expert_offset;  /* [n_expert + 1] */
+    void*     scatter_work;
+    void*     h;              /* [max_tokens * top_k][width], elements or codes */
+    uint8_t*  h_scales;
+    uint16_t* y_rows;         /* bf16 [max_tokens * top_k][hidden] */
+    float*    branch;         /* [max_tokens][hidden] */
+    void*     gather_work;
+} Exl3bExpertBlockBufs;
+int64_t exl3b200_expert_block_work_bytes(const Exl3bExpertBlockDesc* desc, int64_t max_tokens);
+int     exl3b200_expert_block_carve(const Exl3bExpertBlockDesc* desc, int64_t max_tokens, void* work, int64_t work_bytes,
+                                    Exl3bExpertBlockBufs* bufs);
+int     exl3b200_expert_block_forward(const Exl3bExpertBlockDesc* desc, const Exl3bExpertBlockBufs* bufs, const void* x,
+                                      int64_t n_tok, void* out, void* next, void* stream);
+
 /* How long a kernel that waits on another rank's flag (p2p_wait_dispatch, p2p_wait_combine, tp_reduce, tp_pull)
  * waits before it gives up, sets its status and the error word, and returns: `ns` nanoseconds, or the default 5 s
  * for ns <= 0 (more than 600 s is refused, RAD_E_INVAL). Process-wide; each launch reads it when it is enqueued

@@ -9,7 +9,7 @@ import ctypes as C
 
 import torch
 
-from .native import BlockNormDesc, GroupedMmDesc, Native
+from .native import BlockNormDesc, ExpertBlockDesc, GroupedMmDesc, Native
 
 MX4 = 1024 + 0x3B4                      # EXL3B_MX4
 DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
@@ -179,3 +179,53 @@ class BlockNorm(_Plan):
         if y_scales is not None:
             d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", (rows, cols // 32), torch.uint8)
         self._finish(d, branch, post_w, gate, res, out, pre_w, y, y_codes, y_scales)
+
+
+# ------------------------------------------------------------------------------------------------ the block
+class ExpertBlock:
+    """A residual MoE block over such experts (exl3b200_expert_block_forward): norm, router, the experts' gate / up and down
+    products, the gather, and the norm, gate and residual behind it, and the next block's norm.
+
+    router_w [experts, hidden] in f16 or bf16 sets the stream's type, which pre_w, post_w, gate (a scale a channel) and
+    next_w [hidden] share. gu_w [experts, 2 width, hidden] and dn_w [experts, hidden, width] are of that type, or uint8
+    MXFP4 codes with gu_scales and dn_scales [experts, rows, cols / 32] (tiled here, once)."""
+
+    def __init__(self, *, router_w, gu_w, dn_w, pre_w, post_w=None, gate=None, next_w=None, gu_scales=None, dn_scales=None,
+                 top_k, eps=1e-6, res_scale=1.0, max_tokens=2048):
+        E, H = router_w.shape
+        mx = gu_w.dtype == torch.uint8
+        per, dt = 2 if mx else 1, router_w.dtype
+        W = dn_w.shape[2] * per
+        d = self.desc = ExpertBlockDesc()
+        d.n_expert, d.hidden, d.width, d.top_k, d.eps, d.res_scale = E, H, W, top_k, eps, res_scale
+        d.dtype, d.weights = _dtype(router_w), MX4 if mx else _dtype(gu_w)
+        want = torch.uint8 if mx else dt
+        keep = [router_w, gu_w, dn_w, pre_w, post_w, gate, next_w]
+        for name, t, shape, kind in (("router_w", router_w, (E, H), dt), ("gu_w", gu_w, (E, 2 * W, H // per), want),
+                                     ("dn_w", dn_w, (E, H, W // per), want), ("pre_w", pre_w, (H,), dt),
+                                     ("post_w", post_w, (H,), dt), ("gate", gate, (H,), dt), ("next_w", next_w, (H,), dt)):
+            if t is not None:
+                if not t.is_contiguous():
+                    raise ValueError(f"{name} is strided")
+                setattr(d, name, _rows(t, name, shape, kind)[0])
+        if mx:
+            _rows(gu_scales, "gu_scales", (E, 2 * W, H // 32), torch.uint8)
+            _rows(dn_scales, "dn_scales", (E, H, W // 32), torch.uint8)
+            keep += [mx4_tile_scales(gu_scales, "silu_mul"), mx4_tile_scales(dn_scales)]
+            d.gu_scales, d.dn_scales = keep[-2].data_ptr(), keep[-1].data_ptr()
+        self._keep, self.dtype, self.hidden, self.max_tokens = keep, dt, H, max_tokens
+        n = native().expert_block_work_bytes(d, max_tokens)
+        self.work = torch.empty(n, dtype=torch.uint8, device=router_w.device)
+        self.bufs = native().expert_block_carve(d, max_tokens, self.work.data_ptr(), n)
+
+    def forward(self, x, out, next_out=None, stream=0):
+        """x [T, hidden] through the block into out (which may be x); next_out: the next block's normed input."""
+        T = x.shape[0]
+        for name, t in (("x", x), ("out", out), ("next_out", next_out)):
+            if t is not None:
+                _rows(t, name, (T, self.hidden), self.dtype)
+                if not t.is_contiguous():
+                    raise ValueError(f"{name} is strided")
+        native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
+                                      next_out.data_ptr() if next_out is not None else None, stream)
+        return out

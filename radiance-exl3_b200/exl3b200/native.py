@@ -74,6 +74,20 @@ class BlockNormDesc(C.Structure):
         ("y_codes", _VP), ("y_codes_pitch", _I64), ("y_scales", _VP), ("y_scales_pitch", _I64)]
 
 
+class ExpertBlockDesc(C.Structure):
+    """Exl3bExpertBlockDesc (include/exl3b200.h)."""
+    _fields_ = [(n, _I64) for n in ("n_expert", "hidden", "width", "top_k")] + [
+        ("dtype", C.c_int32), ("weights", C.c_int32), ("eps", C.c_float), ("res_scale", C.c_float)] + [
+        (n, _VP) for n in ("router_w", "gu_w", "gu_scales", "dn_w", "dn_scales", "pre_w", "post_w", "gate", "next_w")]
+
+
+class ExpertBlockBufs(C.Structure):
+    """Exl3bExpertBlockBufs (include/exl3b200.h): device addresses inside the caller's work block."""
+    _fields_ = [("max_tokens", _I64)] + [(n, _VP) for n in (
+        "xn", "x_codes", "x_scales", "logits", "ids", "w", "sorted_tok", "expert_offset", "scatter_work", "h", "h_scales",
+        "y_rows", "branch", "gather_work")]
+
+
 def marks_array(events):
     """A C array of cudaEvent_t from torch.cuda.Event objects (None entries stay NULL), or None. torch creates an
     event's handle at its first record, so each is recorded once here before its handle is taken."""
@@ -166,6 +180,11 @@ class Native:
         L.exl3b200_mx4_tiled_bytes.restype = _I64
         L.exl3b200_mx4_tiled_bytes.argtypes = [_I64, _I64, _I64, _I]
         L.exl3b200_mx4_tile_scales.argtypes = [_VP, _I64, _I64, _I64, _I64, _I64, _I, _VP, _VP]
+        L.exl3b200_expert_block_work_bytes.restype = _I64
+        L.exl3b200_expert_block_work_bytes.argtypes = [C.POINTER(ExpertBlockDesc), _I64]
+        L.exl3b200_expert_block_carve.argtypes = [C.POINTER(ExpertBlockDesc), _I64, _VP, _I64, C.POINTER(ExpertBlockBufs)]
+        L.exl3b200_expert_block_forward.argtypes = [C.POINTER(ExpertBlockDesc), C.POINTER(ExpertBlockBufs), _VP, _I64, _VP,
+                                                    _VP, _VP]
         # descriptors by address: a plan takes its own once (ctypes.addressof), not a byref a call
         L.exl3b200_grouped_mm.argtypes = [_VP, _VP]
         L.exl3b200_block_norm.argtypes = [_VP, _VP]
@@ -439,3 +458,19 @@ class Native:
 
     def block_norm(self, desc, stream=0):
         self._check(self.lib.exl3b200_block_norm(C.addressof(desc), stream), "exl3b200_block_norm")
+
+    def expert_block_work_bytes(self, desc, max_tokens):
+        n = int(self.lib.exl3b200_expert_block_work_bytes(C.byref(desc), max_tokens))
+        if n < 0:
+            raise RuntimeError("exl3b200_expert_block_work_bytes: the block description was refused")
+        return n
+
+    def expert_block_carve(self, desc, max_tokens, work, work_bytes):
+        b = ExpertBlockBufs()
+        self._check(self.lib.exl3b200_expert_block_carve(C.byref(desc), max_tokens, work, work_bytes, C.byref(b)),
+                    "exl3b200_expert_block_carve")
+        return b
+
+    def expert_block_forward(self, desc, bufs, x, n_tok, out, next_, stream=0):
+        self._check(self.lib.exl3b200_expert_block_forward(C.byref(desc), C.byref(bufs), x, n_tok, out, next_, stream),
+                    "exl3b200_expert_block_forward")
