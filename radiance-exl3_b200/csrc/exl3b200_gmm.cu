@@ -289,40 +289,40 @@ struct RowAhead {
         }
     }
 };
-// 16 scales of an x row from byte `off` on (those past the row's end are zero): one load where rows lie on 16-byte
-// boundaries, else the aligned words around them, shifted; bytes where a word would leave the scales' memory.
+// 16 scales of an x row from byte `off` on; what lies past the row's end is some byte or other. One load where rows lie on
+// 16-byte boundaries: nothing here touches what it loads, so it is waited for where it is used. Else the two aligned 16
+// bytes around them, shifted; and byte by byte where either would leave the scales' memory.
 struct RowScales {
     const uint8_t *lo, *hi;
-    int n;
     bool whole;
     __device__ __forceinline__ RowScales(const Exl3bGmmOp& p)
-        : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32), n((int)(p.n_in / 32)),
+        : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32),
           whole(((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0) {}
-    __device__ __forceinline__ uint32_t word(const uint8_t* a) const {
-        if (a >= lo && a + 4 <= hi) return *reinterpret_cast<const uint32_t*>(a);
-        uint32_t w = 0;
-        for (int b = 0; b < 4; ++b)
-            if (a + b >= lo && a + b < hi) w |= (uint32_t)a[b] << (8 * b);
-        return w;
-    }
     __device__ __forceinline__ uint4 load(const uint8_t* row, int off) const {
         const uint8_t* a = row + off;
-        // nothing here touches what it loads: the load is waited for where it is used, a batch later
-        if (whole && off + 16 <= n) return *reinterpret_cast<const uint4*>(a);
-        if (off >= n) return make_uint4(0u, 0u, 0u, 0u);
-        uint32_t w[4];
-        const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 3);
-        uint32_t prev = word(a - by);
+        if (whole && a + 16 <= hi) return *reinterpret_cast<const uint4*>(a);
+        const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 15);
+        const uint8_t* b = a - by;
+        uint32_t w[8];
+        if (b >= lo && b + 32 <= hi) {
+            const uint4 x = *reinterpret_cast<const uint4*>(b), y = *reinterpret_cast<const uint4*>(b + 16);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+            // words from `by` / 4 on, then bytes
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t next = by || i < 3 ? word(a - by + 4 * i + 4) : 0u;
-            w[i] = __funnelshift_r(prev, next, 8 * by);
-            prev = next;
-        }
+            for (int i = 0; i < 6; ++i) w[i] = by & 8 ? w[i + 2] : w[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int left = n - off - 4 * i;
-            if (left < 4) w[i] = left > 0 ? w[i] & ((1u << (8 * left)) - 1) : 0u;
+            for (int i = 0; i < 5; ++i) w[i] = by & 4 ? w[i + 1] : w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (by & 3));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (a + 4 * i + j < hi) w[i] |= (uint32_t)a[4 * i + j] << (8 * j);
+            }
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         if (MX && g < C::SFX_G && n_mine) {
             constexpr int Q = NT < 128 ? NT / 32 : 4;
             const RowScales rs(p);
+            const int nsc = (int)(p.n_in / 32);
             RowAhead<Q> ahead(p, lane + g * 128, 32);
             const uint8_t* src[Q];
             uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             if (n_mine > 1) ahead.fetch(unit_at(1));
             auto load = [&](uint4 v[Q]) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) v[q] = rs.load(src[q], 8 * lc);
+                for (int q = 0; q < Q; ++q) v[q] = lc < nck ? rs.load(src[q], 8 * lc) : make_uint4(0u, 0u, 0u, 0u);
                 if ((lc += 2) >= nck && ++lu < n_mine) {
                     lc = 0;
                     ahead.rows(p.x_scales, p.xs_pitch, src);
@@ -575,9 +576,12 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                     uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        // scales past the row's end are those of zero codes: any that is not a NaN
+                        const int left = nsc - 8 * (cc + a) - 4 * h;
+                        const uint32_t mask = left >= 4 ? 0xFFFFFFFFu : left > 0 ? (1u << (8 * left)) - 1 : 0u;
                         auto word = [&](int q) {
                             const uint4 x = v[q < Q ? q : 0];
-                            return q >= Q ? 0u : a ? (h ? x.w : x.z) : h ? x.y : x.x;
+                            return q >= Q ? 0u : (a ? (h ? x.w : x.z) : h ? x.y : x.x) & mask;
                         };
                         dst[h * (C::SFX_G * 32)] = make_uint4(word(0), word(1), word(2), word(3));
                     }
@@ -896,7 +900,12 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
 
 extern "C" int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool pair = p->n_rows > 16 * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4;
+    // The pair form from 16 rows an expert on average (512 -> 2240 over 479 experts of 15 rows, MXFP4: narrow 47 us, pair
+    // 67; 792 -> 1648 over 112 experts of 33 rows, f16: 72 and 52), or 96 where a weight has so few rows that its last pair
+    // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 27 and 33); and where its units keep half
+    // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
+    const int64_t few = p->w_rows < 512 ? 96 : 16;
+    const bool pair = p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4;
     if (p->mx4) return pair ? launch<true, true>(p, sm_count, st) : launch<true, false>(p, sm_count, st);
     return pair ? launch<false, true>(p, sm_count, st) : launch<false, false>(p, sm_count, st);
 }
