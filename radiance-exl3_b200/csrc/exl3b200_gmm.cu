@@ -9,10 +9,12 @@
 // silu_mul is 64 gate rows and their 64 up rows, 16 of each in turn: an epilogue warp, which can read 32 lanes of tensor
 // memory, has both halves of its 16 outputs.
 //
-// Two forms of one kernel, both persistent over units (expert, a group of its sorted rows, a block of weight rows),
+// Three forms of one kernel, all persistent over units (expert, a group of its sorted rows, a block of weight rows),
 // expert-major, so that the CTAs working at one time share an expert's rows and weights in L2:
 //   narrow  a CTA a unit of 128 weight rows and up to 32 sorted rows, two CTAs an SM: a few rows an expert, where the
 //           weights' bytes count and units are needed to spread them over the SMs
+//   SPLIT   the narrow form with few units: a cluster a unit, each CTA a part of its k, the parts summed through
+//           distributed shared memory in the CTAs' order
 //   PAIR    two CTAs (a cluster) a unit of 256 weight rows and up to 256 sorted rows (MXFP4: 224, the scales take
 //           tensor memory), tcgen05 cta_group::2: each CTA brings its 128 weight rows and HALF of the sorted rows, and
 //           both multiply by all of them, 32 KB a CTA for 4.2 MFLOP against 48 KB for a CTA alone
@@ -51,7 +53,7 @@ constexpr int kStatic = 3072;                    // the static shared arrays, up
 constexpr int kMaxExpert = 2048;
 constexpr int kMaxSt = 10;                       // stages at most
 
-template <bool MX, bool PAIR>
+template <bool MX, bool PAIR, bool SPLIT>
 struct Cfg {
     static constexpr int NT = !PAIR ? 32 : MX ? 224 : 256;       // sorted rows a unit at most
     static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
@@ -62,7 +64,7 @@ struct Cfg {
     static constexpr int SFX_G = MX ? (NT + 127) / 128 : 0;      // 128-row groups of the sorted rows' scales
     static constexpr int SFX_B = SFX_G * 1024;
     static constexpr int STAGE_B = kW_B + X_B + SFW_B + SFX_B;
-    static constexpr int EPI_B = EPI_G * kStage * kEpiLd * 4;
+    static constexpr int EPI_B = (SPLIT ? NT : EPI_G * kStage) * kEpiLd * 4;
     static constexpr int SFC = MX ? 8 + 8 * SFX_G : 0;           // TMEM columns of a stage's scales
     static constexpr int COLS = 2 * NT + 2 * SFC;
     static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 512;
@@ -74,8 +76,8 @@ struct Cfg {
         const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kStatic - fixed(n_expert)) / STAGE_B;
         return n < kMaxSt ? n : kMaxSt;
     }
-    static_assert(COLS <= 512 && stages(kMaxExpert, PER_SM) >= 4, "tensor or shared memory");
-    static_assert((2 * kMaxSt + 4) * 8 + 8 <= 512, "barriers");
+    static_assert(COLS <= 512 && stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4), "tensor or shared memory");
+    static_assert((2 * kMaxSt + 6) * 8 + 8 <= 512, "barriers");
 };
 
 struct Unit {
@@ -264,6 +266,19 @@ __device__ __forceinline__ void arrive_even(uint64_t* bar) {
                  " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(bar))
                  : "memory");
 }
+// One arrival on the barrier of the same offset in the cluster's CTA `rank`, publishing what this thread has seen written.
+__device__ __forceinline__ void arrive_at(uint64_t* bar, uint32_t rank) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
+                 " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(bar)), "r"(rank)
+                 : "memory");
+}
+// Four floats at the same offset in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ void ld_cluster(const float* p, uint32_t rank, float v[4]) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}\n"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                 : "r"(smem_u32(p)), "r"(rank)
+                 : "memory");
+}
 // The x rows that a thread loads of a unit: rows first, first + step, ... of it. Their slots are fetched a unit ahead, so a
 // unit's first copies do not wait for them. A dropped slot reads row 0 (its outputs are zeroed, not stored), a row past the
 // unit's its last one; none lies past x's rows.
@@ -352,10 +367,10 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
     return r != 0;
 }
 
-template <bool MX, bool PAIR>
-__global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
-    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const int ST) {
-    using C = Cfg<MX, PAIR>;
+template <bool MX, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, SPLIT>::PER_SM)
+    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const int ST, const int split) {
+    using C = Cfg<MX, PAIR, SPLIT>;
     constexpr int NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -369,14 +384,18 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     uint64_t* empty = full + ST;                              // MMA commit -> producers
     uint64_t* acc_full = empty + ST;                          // MMA commit -> epilogue [2]
     uint64_t* acc_empty = acc_full + 2;                       // epilogue (PAIR: of both CTAs) -> MMA [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* part_full = acc_empty + 2;                      // SPLIT: every CTA's partial sums are in its shared memory
+    uint64_t* part_empty = part_full + 1;                     // ... and have been read by every CTA
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 1);
     uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
     uint32_t* prefix = reinterpret_cast<uint32_t*>(bars) + 128;   // [n_expert + 1]
     __shared__ Unit utab[kTab];
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;
-    const uint32_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;        // which half of the unit's weight rows
+    const uint32_t part = SPLIT ? blockIdx.x % split : 0u;    // which part of its k
+    const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / split : blockIdx.x;
+    const uint32_t stride = PAIR ? gridDim.x >> 1 : SPLIT ? gridDim.x / split : gridDim.x;
     const int act = p.act;
     const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
     constexpr int MB = PAIR ? 2 : 1;
@@ -395,12 +414,16 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         mbar_init(&acc_empty[tid - ST], 4 * C::EPI_G * MB);
     } else if (tid == ST + 2) {
         *dead = 0;
+        if (SPLIT) {
+            mbar_init(part_full, 4 * split);
+            mbar_init(part_empty, 4 * split);
+        }
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
     if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
-    if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (PAIR || SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts); this CTA's units
     // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
@@ -434,7 +457,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     }
     fence_before();
     __syncthreads();
-    if (PAIR) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // both CTAs' barriers and tensor memory are set up
+    if (PAIR || SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs' barriers and tensor memory are set up
     fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
@@ -443,6 +466,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         return i < kTab ? utab[i] : find_unit<NT, MB>(p, prefix, first + i * stride, n_mb);
     };
     const int nck = (int)((p.n_in + (MX ? 255 : 63)) / (MX ? 256 : 64));
+    // this CTA's stages of a unit
+    static_assert(!(MX && SPLIT), "scales are read from even stages on");
+    const int k0 = SPLIT ? (int)((int64_t)part * nck / split) : 0, k1 = SPLIT ? (int)((int64_t)(part + 1) * nck / split) : nck;
     volatile uint32_t* vdead = dead;
     // A bounded wait by a whole warp, which reports nothing: one that gives up marks the CTA dead, every other wait of the
     // CTA then gives up at its next try, and the roles leave at their next unit. (A result tested each stage cost up to
@@ -468,6 +494,11 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         }
         __syncwarp();
     };
+    // ... for arrivals that publish what the cluster's other CTAs wrote
+    auto wait_cluster = [&](uint64_t* bar, uint32_t parity) {
+        wait(bar, parity);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    };
     Pipe pipe;
 
     if (warp == 0) {
@@ -475,7 +506,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
             const Unit u = unit_at(i);
             const int b = u.blk + (int)rank;
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+            for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
                 wait(&empty[pipe.s], pipe.ph ^ 1);
                 mbar_expect_tx_el(&full[pipe.s], kW_B + C::SFW_B);
                 uint8_t* dst = w_ring + pipe.s * kW_B;
@@ -503,7 +534,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     } else if (warp == 1 && rank == 1) {
         // ---------------------------------------------------------------- PAIR, odd CTA: its filled stages, reported
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+            for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
                 wait(&full[pipe.s], pipe.ph);
                 proxy_fence();
                 if (lane == 0) arrive_even(&full[pipe.s]);
@@ -524,18 +555,18 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             wait(&acc_empty[ab], ((i >> 1) & 1) ^ 1);
             fence_after();
             const uint32_t d = tmem + ab * NT;
-            for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
+            for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
                 wait(&full[pipe.s], pipe.ph);
                 proxy_fence();
                 fence_after();
                 const uint64_t wd = wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd = xd0 + (uint64_t)(pipe.s * C::X_B >> 4);
                 if constexpr (MX) {
                     stage_mx4<PAIR, C::SFX_G>(d, wd, xd, idesc, idesc | 2u << 4 | 2u << 29, tmem + 2 * NT + sfp * C::SFC,
-                                              ck ? 1u : 0u, swd0 + (uint64_t)(pipe.s * C::SFW_B >> 4),
+                                              ck > k0 ? 1u : 0u, swd0 + (uint64_t)(pipe.s * C::SFW_B >> 4),
                                               sxd0 + (uint64_t)(pipe.s * C::SFX_B >> 4));
                     sfp ^= 1;
                 } else {
-                    mma4_f16<PAIR>(d, wd, xd, idesc, ck ? 1u : 0u);
+                    mma4_f16<PAIR>(d, wd, xd, idesc, ck > k0 ? 1u : 0u);
                 }
                 commit_el<PAIR>(&empty[pipe.s]);
             }
@@ -555,15 +586,15 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             RowAhead<Q> ahead(p, lane + g * 128, 32);
             const uint8_t* src[Q];
             uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
-            int lc = 0, cc = 0;                               // ... and their first stages
+            int lc = k0, cc = k0;                             // ... and their first stages
             ahead.fetch(unit_at(0));
             ahead.rows(p.x_scales, p.xs_pitch, src);
             if (n_mine > 1) ahead.fetch(unit_at(1));
             auto load = [&](uint4 v[Q]) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) v[q] = lc < nck ? rs.load(src[q], 8 * lc) : make_uint4(0u, 0u, 0u, 0u);
-                if ((lc += 2) >= nck && ++lu < n_mine) {
-                    lc = 0;
+                for (int q = 0; q < Q; ++q) v[q] = lc < k1 ? rs.load(src[q], 8 * lc) : make_uint4(0u, 0u, 0u, 0u);
+                if ((lc += 2) >= k1 && ++lu < n_mine) {
+                    lc = k0;
                     ahead.rows(p.x_scales, p.xs_pitch, src);
                     if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
                 }
@@ -571,7 +602,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
             auto use = [&](const uint4 v[Q]) {
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
-                    if (cc + a >= nck) break;
+                    if (cc + a >= k1) break;
                     wait(&empty[pipe.s], pipe.ph ^ 1);
                     uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
 #pragma unroll
@@ -589,8 +620,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                     if (lane == 0) mbar_arrive(&full[pipe.s]);
                     pipe.next(ST);
                 }
-                if ((cc += 2) >= nck) {
-                    cc = 0;
+                if ((cc += 2) >= k1) {
+                    cc = k0;
                     ++cu;
                 }
             };
@@ -628,15 +659,15 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
         for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
             const int nl = u.blk;
             const uint8_t* src[RP];
-            ahead.rows(static_cast<const uint8_t*>(p.x) + c * 16, p.x_pitch_bytes, src);
+            ahead.rows(static_cast<const uint8_t*>(p.x) + k0 * kRowB + c * 16, p.x_pitch_bytes, src);
             if (i + 1 < n_mine) {
                 u = mine(i + 1);
                 ahead.fetch(u);
             }
-            for (int c0 = 0; c0 < nck; c0 += kStep) {
+            for (int c0 = k0; c0 < k1; c0 += kStep) {
 #pragma unroll
                 for (int a = 0; a < kStep; ++a) {
-                    if (c0 + a >= nck) break;
+                    if (c0 + a >= k1) break;
                     wait(&empty[pipe.s], pipe.ph ^ 1);
                     const uint32_t dst = dst0 + pipe.s * C::X_B;
                     if ((c0 + a + 1) * kRowB <= kb) {
@@ -703,9 +734,67 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
                 if (lane == b) live = m;
             }
             wait(&acc_full[ab], (i >> 1) & 1);
-            if (mx_out ? epi_any(g, *vdead) : __any_sync(0xFFFFFFFFu, *vdead)) break;
-
+            if (mx_out && !SPLIT ? epi_any(g, *vdead) : __any_sync(0xFFFFFFFFu, *vdead)) break;
             fence_after();
+            if constexpr (SPLIT) {
+                // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
+                // then sums every split-th row over the CTAs, in their order, and stores it.
+                wait_cluster(part_empty, (i & 1) ^ 1);
+                for (int t0 = 0; t0 < u.nr; t0 += kSlice) {
+                    uint32_t a[16];
+                    tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
+                    tmem_wait(a);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) st[(t0 + j) * kEpiLd + 32 * q + lane] = __uint_as_float(a[j]);
+                }
+                fence_before();
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[ab]);
+                if (lane < split) arrive_at(part_full, lane);
+                __syncwarp();
+                wait_cluster(part_full, i & 1);
+                const bool out_lane = !act || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
+                const int64_t n0 = b0 + (act ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
+                for (int j = part + split * q; j < u.nr; j += split * 4) {
+                    float v[4] = { 0.f, 0.f, 0.f, 0.f };
+                    for (int s = 0; s < split; ++s) {
+                        float f[4];
+                        ld_cluster(&st[j * kEpiLd + 4 * lane], s, f);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += f[e];
+                    }
+                    if (act) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float up = __shfl_xor_sync(0xFFFFFFFFu, v[e], 4);
+                            v[e] = silu(v[e]) * up;
+                        }
+                    }
+                    const int64_t r = u.r0 + j;
+                    const uint32_t rows_live = __shfl_sync(0xFFFFFFFFu, live, 0);      // by every lane
+                    const bool ok = out_lane && n0 < p.n_out && (rows_live >> j & 1);
+                    if (mx_out) {
+                        uint32_t m = max(max(mx4_mag(v[0]), mx4_mag(v[1])), max(mx4_mag(v[2]), mx4_mag(v[3])));
+                        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+                        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+                        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, act ? 8 : 4));      // the eight lanes of a block of 32
+                        const uint32_t code = mx4_scale_code(m);
+                        const float f[8] = { v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f };
+                        if (ok) {
+                            *reinterpret_cast<uint16_t*>(y + r * p.y_pitch + n0 / 2) = (uint16_t)mx4_pack8(f, code);
+                            if ((n0 & 31) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
+                        }
+                    } else if (ok) {
+                        uint8_t* d = y + r * row_b + n0 * es;
+                        if (p.y_dtype == RAD_F32) *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2*>(d) = make_uint2(pack2(p.y_dtype, v[0], v[1]), pack2(p.y_dtype, v[2], v[3]));
+                    }
+                }
+                __syncwarp();
+                if (lane < split) arrive_at(part_empty, lane);
+                continue;
+            }
             // silu_mul: lanes 0..15 hold 16 gate rows, 16..31 their up rows; the lower half takes the even rows' outputs of
             // a slice, the upper the odd ones'
             const bool up = lane >= 16;
@@ -810,7 +899,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR>::THREADS, Cfg<MX, PAIR>::PER_SM)
     }
     fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();                             // neither CTA's memory goes while the other uses it
+    if (PAIR || SPLIT) cluster_sync_all();                    // no CTA's memory goes while another uses it
     if (warp == 1) {
         fence_after();
         tmem_free<PAIR>(tmem, C::TMEM);
@@ -863,22 +952,14 @@ int64_t most_units(const Exl3bGmmOp* p, int nt, int mb) {
     return (live + p->n_rows / nt) * ((p->n_out + blk - 1) / blk);
 }
 
-template <bool MX, bool PAIR>
-int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
-    using C = Cfg<MX, PAIR>;
+// split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
+template <bool MX, bool PAIR, bool SPLIT>
+int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
+    using C = Cfg<MX, PAIR, SPLIT>;
     CUtensorMap map;
     const int rc = make_map(p, &map);
     if (rc) return rc;
-    auto kern = k_gmm<MX, PAIR>;
-    cudaLaunchConfig_t cfg = {};
-    const int64_t most = most_units(p, C::NT, PAIR ? 2 : 1);
-    // few units: one CTA an SM, with the whole of its shared memory for stages in flight
-    const int per_sm = !PAIR && most <= sm_count ? 1 : C::PER_SM;
-    const int64_t room = PAIR ? sm_count / 2 : (int64_t)sm_count * per_sm;
-    const int stages = C::stages(p->n_expert, per_sm);
-    cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.stream = st;
+    auto kern = k_gmm<MX, PAIR, SPLIT>;
     static bool allowed[64];                                  // the most shared memory, once a device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
@@ -886,28 +967,54 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
         allowed[dev] = true;
     }
-    cfg.gridDim = dim3((unsigned)((most < room ? most : room) * (PAIR ? 2 : 1)));
+    const int ctas = PAIR ? 2 : split;                        // of a cluster
+    const int64_t most = most_units(p, C::NT, PAIR ? 2 : 1);
+    // few units: one CTA an SM, with the whole of its shared memory for stages in flight
+    const int per_sm = !PAIR && most * ctas <= sm_count ? 1 : C::PER_SM;
+    const int64_t room = (int64_t)sm_count * per_sm / ctas;
+    const int stages = C::stages(p->n_expert, per_sm);
+    cudaLaunchConfig_t cfg = {};
+    cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.gridDim = dim3((unsigned)((most < room ? most : room) * ctas));
+    cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = PAIR ? 2 : 1;
+    attr.val.clusterDim.x = ctas;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, map, *p, stages) == cudaSuccess ? 0 : -6;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, map, *p, stages, split) == cudaSuccess ? 0 : -6;
+}
+
+template <bool MX>
+int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
+    // The pair form from 16 rows an expert on average (512 -> 2240 over 479 experts of 15 rows, MXFP4: narrow 47 us, pair
+    // 67; 792 -> 1648 over 112 experts of 33 rows, f16: 72 and 52), or 96 where a weight has so few rows that its last pair
+    // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 27 and 33); and where its units keep half
+    // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
+    const int64_t few = p->w_rows < 512 ? 96 : 16;
+    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4)
+        return launch<MX, true, false>(p, sm_count, 1, st);
+    // Few narrow units over a long k: up to four CTAs a unit while each has an SM, four stages a part at least (one token,
+    // two experts, 2048 -> 512 silu_mul: 11.1 us, in four parts 8.9; 16 rows, 4096 -> 4096: 16.3 and 12.6; ten experts make
+    // 80 units: 13.7, in three parts 15.1; clusters of eight do not always fit at once: 15.1 for 8.9). MXFP4 has a quarter
+    // of the stages and gains nothing (two experts 8.9 and 10.3).
+    if (!MX) {
+        const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 63) / 64;
+        int64_t split = sm_count / most;
+        if (split > nck / 4) split = nck / 4;
+        if (split > 4) split = 4;
+        if (split >= 2) return launch<false, false, true>(p, sm_count, (int)split, st);
+    }
+    return launch<MX, false, false>(p, sm_count, 1, st);
 }
 
 }  // namespace
 
 extern "C" int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // The pair form from 16 rows an expert on average (512 -> 2240 over 479 experts of 15 rows, MXFP4: narrow 47 us, pair
-    // 67; 792 -> 1648 over 112 experts of 33 rows, f16: 72 and 52), or 96 where a weight has so few rows that its last pair
-    // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 27 and 33); and where its units keep half
-    // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
-    const int64_t few = p->w_rows < 512 ? 96 : 16;
-    const bool pair = p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4;
-    if (p->mx4) return pair ? launch<true, true>(p, sm_count, st) : launch<true, false>(p, sm_count, st);
-    return pair ? launch<false, true>(p, sm_count, st) : launch<false, false>(p, sm_count, st);
+    return p->mx4 ? launch_form<true>(p, sm_count, st) : launch_form<false>(p, sm_count, st);
 }
 
 extern "C" int exl3b_gmm_max_expert(void) { return kMaxExpert; }
