@@ -304,18 +304,17 @@ struct RowAhead {
         }
     }
 };
-// 16 scales of an x row from byte `off` on; what lies past the row's end is some byte or other. One load where rows lie on
-// 16-byte boundaries: nothing here touches what it loads, so it is waited for where it is used. Else the two aligned 16
-// bytes around them, shifted; and byte by byte where either would leave the scales' memory.
+// 16 scales of an x row from byte `off` on; what lies past the row's end is some byte or other. Rows on 16-byte boundaries
+// are one load (`whole`; of the last row only where the row has them). Else the two aligned 16 bytes around them, shifted;
+// and byte by byte where either would leave the scales' memory.
 struct RowScales {
-    const uint8_t *lo, *hi;
+    const uint8_t *lo, *hi, *last;
     bool whole;
     __device__ __forceinline__ RowScales(const Exl3bGmmOp& p)
-        : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32),
+        : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32), last(hi - p.n_in / 32),
           whole(((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0) {}
     __device__ __forceinline__ uint4 load(const uint8_t* row, int off) const {
         const uint8_t* a = row + off;
-        if (whole && a + 16 <= hi) return *reinterpret_cast<const uint4*>(a);
         const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 15);
         const uint8_t* b = a - by;
         uint32_t w[8];
@@ -587,15 +586,31 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             const uint8_t* src[Q];
             uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
             int lc = k0, cc = k0;                             // ... and their first stages
+            bool edge;                                        // one of the warp's rows is x's last
+            auto rows = [&]() {
+                ahead.rows(p.x_scales, p.xs_pitch, src);
+                bool mine = false;
+#pragma unroll
+                for (int q = 0; q < Q; ++q) mine |= src[q] == rs.last;
+                edge = __any_sync(0xFFFFFFFFu, mine);
+            };
             ahead.fetch(unit_at(0));
-            ahead.rows(p.x_scales, p.xs_pitch, src);
+            rows();
             if (n_mine > 1) ahead.fetch(unit_at(1));
             auto load = [&](uint4 v[Q]) {
+                const int off = 8 * lc;
+                if (lc >= k1) return;
+                if (rs.whole && (off + 16 <= nsc || !edge)) {
+                    // nothing here touches what it loads: it is waited for where it is used
 #pragma unroll
-                for (int q = 0; q < Q; ++q) v[q] = lc < k1 ? rs.load(src[q], 8 * lc) : make_uint4(0u, 0u, 0u, 0u);
+                    for (int q = 0; q < Q; ++q) v[q] = *reinterpret_cast<const uint4*>(src[q] + off);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) v[q] = rs.load(src[q], off);
+                }
                 if ((lc += 2) >= k1 && ++lu < n_mine) {
                     lc = k0;
-                    ahead.rows(p.x_scales, p.xs_pitch, src);
+                    rows();
                     if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
                 }
             };
@@ -605,16 +620,19 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     if (cc + a >= k1) break;
                     wait(&empty[pipe.s], pipe.ph ^ 1);
                     uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        // scales past the row's end are those of zero codes: any that is not a NaN
-                        const int left = nsc - 8 * (cc + a) - 4 * h;
-                        const uint32_t mask = left >= 4 ? 0xFFFFFFFFu : left > 0 ? (1u << (8 * left)) - 1 : 0u;
-                        auto word = [&](int q) {
+                    auto put = [&](uint32_t m0, uint32_t m1) {
+                        auto word = [&](int q, int h) {
                             const uint4 x = v[q < Q ? q : 0];
-                            return q >= Q ? 0u : (a ? (h ? x.w : x.z) : h ? x.y : x.x) & mask;
+                            return q >= Q ? 0u : a ? (h ? x.w : x.z) : h ? x.y : x.x;
                         };
-                        dst[h * (C::SFX_G * 32)] = make_uint4(word(0), word(1), word(2), word(3));
+                        dst[0] = make_uint4(word(0, 0) & m0, word(1, 0) & m0, word(2, 0) & m0, word(3, 0) & m0);
+                        dst[C::SFX_G * 32] = make_uint4(word(0, 1) & m1, word(1, 1) & m1, word(2, 1) & m1, word(3, 1) & m1);
+                    };
+                    const int left = nsc - 8 * (cc + a);
+                    if (left >= 8) {
+                        put(~0u, ~0u);
+                    } else {                                   // past the row's end the scales of zero codes: any but a NaN
+                        put(left >= 4 ? ~0u : (1u << (8 * left)) - 1, left > 4 ? (1u << (8 * (left - 4))) - 1 : 0u);
                     }
                     __syncwarp();                              // the MMA warp's fence covers these writes too
                     if (lane == 0) mbar_arrive(&full[pipe.s]);
