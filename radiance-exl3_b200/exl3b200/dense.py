@@ -27,9 +27,10 @@ def native():
 
 
 def _dtype(t):
-    if t.dtype not in DTYPES:
+    dt = DTYPES.get(t.dtype)
+    if dt is None:
         raise ValueError(f"f32, f16 or bf16, not {t.dtype}")
-    return DTYPES[t.dtype]
+    return dt
 
 
 def _rows(t, name, shape=None, dtype=None):
@@ -60,7 +61,9 @@ def mx4_quantize(x, codes, scales, stream=0):
     xp, pitch = _rows(x, "x")
     cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
-    native().mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch, stream)
+    rc = native().lib.exl3b200_mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch, stream)
+    if rc:
+        raise RuntimeError(f"exl3b200_mx4_quantize: status {rc}")
     return codes, scales
 
 
@@ -70,7 +73,9 @@ def mx4_dequantize(codes, scales, y, stream=0):
     yp, pitch = _rows(y, "y")
     cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
-    native().mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch, stream)
+    rc = native().lib.exl3b200_mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch, stream)
+    if rc:
+        raise RuntimeError(f"exl3b200_mx4_dequantize: status {rc}")
     return y
 
 

@@ -435,14 +435,6 @@ class Native:
                                                         stream), "exl3b200_moe_block_forward")
 
     # ---- experts not kept as EXL3 records, and the norms around a block (exl3b200_dense.c)
-    def mx4_quantize(self, x, x_dtype, x_pitch, rows, cols, codes, codes_pitch, scales, scales_pitch, stream=0):
-        self._check(self.lib.exl3b200_mx4_quantize(x, x_dtype, x_pitch, rows, cols, codes, codes_pitch, scales,
-                                                   scales_pitch, stream), "exl3b200_mx4_quantize")
-
-    def mx4_dequantize(self, codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype, y_pitch, stream=0):
-        self._check(self.lib.exl3b200_mx4_dequantize(codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype,
-                                                     y_pitch, stream), "exl3b200_mx4_dequantize")
-
     def mx4_tiled_bytes(self, n_expert, rows, cols, act):
         n = int(self.lib.exl3b200_mx4_tiled_bytes(n_expert, rows, cols, act))
         if n < 0:
@@ -452,12 +444,6 @@ class Native:
     def mx4_tile_scales(self, scales, scales_pitch, expert_pitch, n_expert, rows, cols, act, tiled, stream=0):
         self._check(self.lib.exl3b200_mx4_tile_scales(scales, scales_pitch, expert_pitch, n_expert, rows, cols, act,
                                                       tiled, stream), "exl3b200_mx4_tile_scales")
-
-    def grouped_mm(self, desc, stream=0):
-        self._check(self.lib.exl3b200_grouped_mm(C.addressof(desc), stream), "exl3b200_grouped_mm")
-
-    def block_norm(self, desc, stream=0):
-        self._check(self.lib.exl3b200_block_norm(C.addressof(desc), stream), "exl3b200_block_norm")
 
     def expert_block_work_bytes(self, desc, max_tokens):
         n = int(self.lib.exl3b200_expert_block_work_bytes(C.byref(desc), max_tokens))
