@@ -255,26 +255,50 @@ RowDiv row_div(uint32_t d) {
     return RowDiv{ d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s };
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// The scale code of a block whose 32 values four neighbouring lanes hold. 16-bit types: the magnitudes two a word, which
+// order as integers too.
+template <int DT>
+__device__ __forceinline__ uint32_t quad_code(const Raw<DT>& x) {
+    if constexpr (DT == 1) {
+        float v[8];
+        x.get(v);
+        return mx4_quad_code(v);
+    } else {
+        const uint32_t k = 0x7FFF7FFFu;
+        uint32_t m = max_u16x2(max_u16x2(x.q[0].x & k, x.q[0].y & k), max_u16x2(x.q[0].z & k, x.q[0].w & k));
+        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+        m = max(m & 0xFFFFu, m >> 16);
+        return mx4_scale_code(DT == 3 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))));
+    }
+}
+
 template <int DT, bool BIG>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t n_vec, RowDiv div,
                                                       uint8_t* q, int64_t q_pitch, uint8_t* qs, int64_t qs_pitch) {
     typedef typename El<DT>::T T;
     const int64_t i0 = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
-    float v[kUnroll][8];
+    Raw<DT> v[kUnroll];
     int64_t row[kUnroll];
     int c[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         row_of<BIG>(i0 + 256 * u, div, &row[u], &c[u]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-        if (i0 + 256 * u < n_vec) ld8<DT>(static_cast<const T*>(x) + row[u] * x_pitch + 8 * c[u], v[u]);
+        v[u].clear();
+        if (i0 + 256 * u < n_vec) v[u].fetch(static_cast<const T*>(x) + row[u] * x_pitch + 8 * c[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const uint32_t code = mx4_quad_code(v[u]);
+        const uint32_t code = quad_code<DT>(v[u]);
         if (i0 + 256 * u >= n_vec) continue;
-        *reinterpret_cast<uint32_t*>(q + row[u] * q_pitch + 4 * c[u]) = mx4_pack8(v[u], code);
+        float f[8];
+        v[u].get(f);
+        *reinterpret_cast<uint32_t*>(q + row[u] * q_pitch + 4 * c[u]) = mx4_pack8(f, code);
         if ((threadIdx.x & 3) == 0) qs[row[u] * qs_pitch + (c[u] >> 2)] = (uint8_t)code;
     }
 }
@@ -294,6 +318,28 @@ __device__ __forceinline__ void e2m1_unpack8(uint32_t n, float v[8]) {
         v[4 * h + 2] = f1.x;
         v[4 * h + 3] = f1.y;
     }
+}
+
+// Eight e2m1 codes times 2^(code - 127) in bf16: both bytes of a value looked up, then one product of pairs, which rounds
+// (below the normal range) as the f32 product would.
+__device__ __forceinline__ uint4 e2m1_bf16x8(uint32_t n, uint32_t code) {
+    const uint32_t bits = code == kMx4Nan ? 0x7FFFu : code ? code << 7 : 0x40u;
+    const __nv_bfloat162 s = __halves2bfloat162(__ushort_as_bfloat16((unsigned short)bits), __ushort_as_bfloat16((unsigned short)bits));
+    uint32_t w[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t c = n >> (16 * h), m = c & 0x7777u;
+        const uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, m) | __byte_perm(0x8000u, 0u, (c >> 3) & 0x1111u);
+        const uint32_t lo = __byte_perm(0xC0800000u, 0xC0804000u, m);
+        w[2 * h] = __byte_perm(lo, hi, 0x5140);
+        w[2 * h + 1] = __byte_perm(lo, hi, 0x7362);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), s);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int DT, bool BIG>
@@ -316,12 +362,17 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* q, int64_
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
         if (i0 + 256 * u >= n_vec) continue;
+        T* d = static_cast<T*>(y) + row[u] * y_pitch + 8 * c[u];
+        if (DT == 3) {
+            *reinterpret_cast<uint4*>(d) = e2m1_bf16x8(n[u], s[u]);
+            continue;
+        }
         const float scale = mx4_scale(s[u]);
         float v[8];
         e2m1_unpack8(n[u], v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= scale;
-        st8<DT>(static_cast<T*>(y) + row[u] * y_pitch + 8 * c[u], v);
+        st8<DT>(d, v);
     }
 }
 

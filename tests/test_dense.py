@@ -131,6 +131,17 @@ def test_dequantize_every_code_and_scale():
     assert np.array_equal(y.double().cpu().numpy(), want.astype(np.float32).astype(np.float64), equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_dequantize_every_code_and_scale_rounds_once(dtype):
+    """Below the type's range the values round (to nearest, ties to even), above it they are infinite. A code has two
+    significant bits: 64 bits, then 32, then the type round no differently from 64 bits to the type at once."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").reshape(16, 16).repeat(16, 1)
+    scales = torch.arange(256, dtype=torch.uint8, device="cuda").reshape(256, 1)
+    y = dense.mx4_dequantize(codes, scales, torch.empty((256, 32), dtype=dtype, device="cuda"), stream())
+    want = torch.from_numpy(decode(codes, scales)).cuda().to(F32).to(dtype)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y), torch.nan_to_num(want))
+
+
 def test_quantize_of_no_rows_and_refusals():
     n, u8 = dense.native(), torch.uint8
     x = torch.zeros((4, 64), device="cuda")
