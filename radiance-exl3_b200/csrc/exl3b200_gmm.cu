@@ -51,6 +51,7 @@ constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
 constexpr int kStatic = 3072;                    // the static shared arrays, up to the ring's alignment
 constexpr int kMaxExpert = 2048;
+constexpr int kMaxSplit = 4;                     // CTAs a unit at most (SPLIT)
 constexpr int kMaxSt = 10;                       // stages at most
 
 template <bool MX, bool PAIR, bool SPLIT>
@@ -80,6 +81,22 @@ struct Cfg {
     static_assert((2 * kMaxSt + 6) * 8 + 8 <= 512, "barriers");
 };
 
+// n / d for n < 2^31 by a multiplication; the host computes mul and shift.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+FastDiv fast_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return FastDiv{ d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s };
+}
+// What the host works out of a launch, so that no CTA divides for it.
+struct Shape {
+    FastDiv n_mb, stride;   // weight-row blocks (PAIR: pairs) an output row; CTAs (PAIR, SPLIT: clusters) of the grid
+    int32_t nck, st, split; // stages of a unit's k, of the ring; CTAs a unit (SPLIT)
+};
+
 struct Unit {
     int32_t r0;          // first sorted row
     int32_t e, blk;      // expert, first 128-row block
@@ -101,19 +118,19 @@ __device__ __forceinline__ uint32_t groups(const Run& r) { return (uint32_t)(r.r
 // Unit `local` of expert e: block by block, then group by group. An expert's rows are split evenly over its groups, in
 // steps of the MMA's N, so that no group is left with a sliver.
 template <int NT, int MB>
-__device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, uint32_t n_mb) {
-    const uint32_t g = local / n_mb, ng = groups<NT>(r), step = 16 * MB;
-    const uint32_t per = (((uint32_t)r.rows + ng - 1) / ng + step - 1) / step * step;
+__device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, const FastDiv& n_mb) {
+    const uint32_t g = n_mb(local), ng = groups<NT>(r), step = 16 * MB;
+    const uint32_t even = ng > 1 ? ((uint32_t)r.rows + ng - 1) / ng : (uint32_t)r.rows, per = (even + step - 1) / step * step;
     Unit u;
     u.e = e;
-    u.blk = (int32_t)(local - g * n_mb) * MB;
+    u.blk = (int32_t)(local - g * n_mb.d) * MB;
     u.r0 = r.r0 + (int32_t)(g * per);
     u.nr = min((int32_t)per, r.rows - (int32_t)(g * per));
     return u;
 }
 // ... found by its number among all units.
 template <int NT, int MB>
-__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, uint32_t n_mb) {
+__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, const FastDiv& n_mb) {
     int lo = 0, hi = p.n_expert;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -368,7 +385,8 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
 
 template <bool MX, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, SPLIT>::PER_SM)
-    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const int ST, const int split) {
+    k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
+    const int ST = sh.st, split = sh.split;
     using C = Cfg<MX, PAIR, SPLIT>;
     constexpr int NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -394,17 +412,14 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;        // which half of the unit's weight rows
     const uint32_t part = SPLIT ? blockIdx.x % split : 0u;    // which part of its k
     const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / split : blockIdx.x;
-    const uint32_t stride = PAIR ? gridDim.x >> 1 : SPLIT ? gridDim.x / split : gridDim.x;
+    const uint32_t stride = sh.stride.d;
     const int act = p.act;
     const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
     constexpr int MB = PAIR ? 2 : 1;
-    const uint32_t n_mb = (uint32_t)((p.n_out + blk_out * MB - 1) / (blk_out * MB));
-    // the runs of this thread's experts first: their latency covers the barriers' set-up
-    constexpr int kPer = (kMaxExpert + THREADS - 1) / THREADS;
-    const int per = (p.n_expert + THREADS - 1) / THREADS, e0 = tid * per;
-    Run run[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) run[i] = i < per && e0 + i < p.n_expert ? run_of(p, e0 + i) : Run{ 0, 0 };
+    const uint32_t n_mb = sh.n_mb.d;
+    // the run of this thread's first expert before all else: its latency covers the barriers' set-up
+    const int per = (p.n_expert + THREADS - 1) / THREADS, e0 = tid * per, e1 = min(e0 + per, p.n_expert);
+    const Run run0 = e0 < e1 ? run_of(p, e0) : Run{ 0, 0 };
     if (tid < ST) {
         mbar_init(&full[tid], 1 + 32 * kXWarps + C::SFX_G + (PAIR && rank == 0 ? 1 : 0));
         mbar_init(&empty[tid], 1);
@@ -427,9 +442,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
         __shared__ uint32_t wsum[THREADS / 32];
-        uint32_t sum = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += groups<NT>(run[i]) * n_mb;
+        uint32_t sum = groups<NT>(run0) * n_mb;
+#pragma unroll 1
+        for (int e = e0 + 1; e < e1; ++e) sum += groups<NT>(run_of(p, e)) * n_mb;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -440,15 +455,16 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
         __syncthreads();
         uint32_t acc = incl - sum;
         for (int w = 0; w < warp; ++w) acc += wsum[w];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (j >= per || e0 + j >= p.n_expert) break;
-            const uint32_t n = groups<NT>(run[j]) * n_mb;
-            prefix[e0 + j] = acc;
+#pragma unroll 1
+        for (int e = e0; e < e1; ++e) {
+            const Run r = e == e0 ? run0 : run_of(p, e);
+            const uint32_t n = groups<NT>(r) * n_mb;
+            prefix[e] = acc;
             if (n) {
-                uint32_t i = acc > first ? (acc - first + stride - 1) / stride : 0u;
+                uint32_t i = acc > first ? sh.stride(acc - first + stride - 1) : 0u;
+#pragma unroll 1
                 for (; i < kTab && first + i * stride < acc + n; ++i)
-                    utab[i] = make_unit<NT, MB>(e0 + j, run[j], first + i * stride - acc, n_mb);
+                    utab[i] = make_unit<NT, MB>(e, r, first + i * stride - acc, sh.n_mb);
             }
             acc += n;
         }
@@ -460,14 +476,15 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
-    const uint32_t n_mine = n_units > first ? (n_units - first + stride - 1) / stride : 0;
+    const uint32_t n_mine = n_units > first ? sh.stride(n_units - first + stride - 1) : 0;
     auto unit_at = [&](uint32_t i) {
-        return i < kTab ? utab[i] : find_unit<NT, MB>(p, prefix, first + i * stride, n_mb);
+        return i < kTab ? utab[i] : find_unit<NT, MB>(p, prefix, first + i * stride, sh.n_mb);
     };
-    const int nck = (int)((p.n_in + (MX ? 255 : 63)) / (MX ? 256 : 64));
+    const int nck = sh.nck;
     // this CTA's stages of a unit
     static_assert(!(MX && SPLIT), "scales are read from even stages on");
-    const int k0 = SPLIT ? (int)((int64_t)part * nck / split) : 0, k1 = SPLIT ? (int)((int64_t)(part + 1) * nck / split) : nck;
+    const int k0 = SPLIT ? (int)(part * (uint32_t)nck / (uint32_t)split) : 0;
+    const int k1 = SPLIT ? (int)((part + 1) * (uint32_t)nck / (uint32_t)split) : nck;
     volatile uint32_t* vdead = dead;
     // A bounded wait by a whole warp, which reports nothing: one that gives up marks the CTA dead, every other wait of the
     // CTA then gives up at its next try, and the roles leave at their next unit. (A result tested each stage cost up to
@@ -757,7 +774,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             if constexpr (SPLIT) {
                 // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
                 // then sums every split-th row over the CTAs, in their order, and stores it.
-                wait_cluster(part_empty, (i & 1) ^ 1);
+                if (i) wait_cluster(part_empty, (i & 1) ^ 1);
                 for (int t0 = 0; t0 < u.nr; t0 += kSlice) {
                     uint32_t a[16];
                     tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
@@ -766,21 +783,24 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     for (int j = 0; j < 16; ++j) st[(t0 + j) * kEpiLd + 32 * q + lane] = __uint_as_float(a[j]);
                 }
                 fence_before();
-                asm volatile("fence.acq_rel.cluster;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[ab]);
+                __syncwarp();                                  // the arrivals publish the whole warp's sums
                 if (lane < split) arrive_at(part_full, lane);
+                if (lane == 0) mbar_arrive(&acc_empty[ab]);
                 __syncwarp();
                 wait_cluster(part_full, i & 1);
                 const bool out_lane = !act || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
                 const int64_t n0 = b0 + (act ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
                 for (int j = part + split * q; j < u.nr; j += split * 4) {
-                    float v[4] = { 0.f, 0.f, 0.f, 0.f };
-                    for (int s = 0; s < split; ++s) {
-                        float f[4];
-                        ld_cluster(&st[j * kEpiLd + 4 * lane], s, f);
+                    float f[kMaxSplit][4], v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += f[e];
+                    for (int s = 0; s < kMaxSplit; ++s)       // all on their way before the first is added
+                        if (s < split) ld_cluster(&st[j * kEpiLd + 4 * lane], s, f[s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = f[0][e];
+#pragma unroll
+                        for (int s = 1; s < kMaxSplit; ++s)
+                            if (s < split) v[e] += f[s][e];
                     }
                     if (act) {
 #pragma unroll
@@ -810,7 +830,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     }
                 }
                 __syncwarp();
-                if (lane < split) arrive_at(part_empty, lane);
+                if (i + 1 < n_mine && lane < split) arrive_at(part_empty, lane);
                 continue;
             }
             // silu_mul: lanes 0..15 hold 16 gate rows, 16..31 their up rows; the lower half takes the even rows' outputs of
@@ -994,7 +1014,10 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
     cfg.blockDim = dim3(C::THREADS);
-    cfg.gridDim = dim3((unsigned)((most < room ? most : room) * ctas));
+    const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
+    cfg.gridDim = dim3((unsigned)(units * ctas));
+    const Shape sh = { fast_div((uint32_t)((p->n_out + blk - 1) / blk)), fast_div((uint32_t)units),
+                       (int32_t)((p->n_in + (MX ? 255 : 63)) / (MX ? 256 : 64)), stages, split };
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1002,7 +1025,7 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = ctas > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, map, *p, stages, split) == cudaSuccess ? 0 : -6;
+    return cudaLaunchKernelEx(&cfg, kern, map, *p, sh) == cudaSuccess ? 0 : -6;
 }
 
 template <bool MX>
@@ -1022,7 +1045,7 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 63) / 64;
         int64_t split = sm_count / most;
         if (split > nck / 4) split = nck / 4;
-        if (split > 4) split = 4;
+        if (split > kMaxSplit) split = kMaxSplit;
         if (split >= 2) return launch<false, false, true>(p, sm_count, (int)split, st);
     }
     return launch<MX, false, false>(p, sm_count, 1, st);
