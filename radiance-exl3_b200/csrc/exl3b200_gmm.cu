@@ -54,11 +54,12 @@ constexpr int kMaxExpert = 2048;
 constexpr int kMaxSplit = 4;                     // CTAs a unit at most (SPLIT)
 constexpr int kMaxSt = 10;                       // stages at most
 
-template <bool MX, bool PAIR, bool SPLIT>
+// EG: epilogue groups of four warps.
+template <bool MX, bool PAIR, bool SPLIT, int EG>
 struct Cfg {
     static constexpr int NT = !PAIR ? 32 : MX ? 224 : 256;       // sorted rows a unit at most
     static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
-    static constexpr int EPI_G = PAIR ? 2 : 1;                   // epilogue groups of four warps
+    static constexpr int EPI_G = EG;
     static constexpr int THREADS = (kEpiWarp0 + 4 * EPI_G) * 32;
     static constexpr int X_B = NL * kRowB;
     static constexpr int SFW_B = MX ? 1024 : 0;                  // two 128-k halves of 512 bytes
@@ -383,11 +384,11 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
     return r != 0;
 }
 
-template <bool MX, bool PAIR, bool SPLIT>
-__global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, SPLIT>::PER_SM)
+template <bool MX, bool PAIR, bool SPLIT, int EG>
+__global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAIR, SPLIT, EG>::PER_SM)
     k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
     const int ST = sh.st, split = sh.split;
-    using C = Cfg<MX, PAIR, SPLIT>;
+    using C = Cfg<MX, PAIR, SPLIT, EG>;
     constexpr int NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -991,13 +992,13 @@ int64_t most_units(const Exl3bGmmOp* p, int nt, int mb) {
 }
 
 // split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
-template <bool MX, bool PAIR, bool SPLIT>
+template <bool MX, bool PAIR, bool SPLIT, int EG>
 int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
-    using C = Cfg<MX, PAIR, SPLIT>;
+    using C = Cfg<MX, PAIR, SPLIT, EG>;
     CUtensorMap map;
     const int rc = make_map(p, &map);
     if (rc) return rc;
-    auto kern = k_gmm<MX, PAIR, SPLIT>;
+    auto kern = k_gmm<MX, PAIR, SPLIT, EG>;
     static bool allowed[64];                                  // the most shared memory, once a device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
@@ -1035,8 +1036,13 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 27 and 33); and where its units keep half
     // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
     const int64_t few = p->w_rows < 512 ? 96 : 16;
-    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4)
-        return launch<MX, true, false>(p, sm_count, 1, st);
+    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4) {
+        // A third group of epilogue warps where the epilogue is the longer part, silu_mul's and that of a short k (16 experts,
+        // 16067 rows, bf16: 512 -> 1024 silu_mul 50 us with two groups, 43 with three; 512 -> 4096 102 and 97); over a long
+        // k its warps only get in the others' way (MXFP4 4096 -> 1536: 60 and 62; 1536 -> 4096: 173 and 175).
+        return p->act || p->n_in <= (MX ? 1024 : 512) ? launch<MX, true, false, 3>(p, sm_count, 1, st)
+                                                      : launch<MX, true, false, 2>(p, sm_count, 1, st);
+    }
     // Few narrow units over a long k: up to four CTAs a unit while each has an SM, four stages a part at least (one token,
     // two experts, 2048 -> 512 silu_mul: 11.1 us, in four parts 8.9; 16 rows, 4096 -> 4096: 16.3 and 12.6; ten experts make
     // 80 units: 13.7, in three parts 15.1; clusters of eight do not always fit at once: 15.1 for 8.9). MXFP4 has a quarter
@@ -1046,9 +1052,9 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         int64_t split = sm_count / most;
         if (split > nck / 4) split = nck / 4;
         if (split > kMaxSplit) split = kMaxSplit;
-        if (split >= 2) return launch<false, false, true>(p, sm_count, (int)split, st);
+        if (split >= 2) return launch<false, false, true, 1>(p, sm_count, (int)split, st);
     }
-    return launch<MX, false, false>(p, sm_count, 1, st);
+    return launch<MX, false, false, 1>(p, sm_count, 1, st);
 }
 
 }  // namespace
