@@ -58,6 +58,7 @@ constexpr int kXWarp0 = 4, kXWarps = 4, kEpiWarp0 = 8;
 constexpr int kRowB = 128;                       // bytes of k a stage: one swizzle row
 constexpr int kW_B = 128 * kRowB;                // a CTA's weight rows of a stage
 constexpr int kSlice = 16;                       // sorted rows an epilogue group takes at a time
+constexpr int kMaxTurn = 16;                      // slices a unit at most
 constexpr int kStage = 8;                        // ... and stages at once, where it stages in f32
 constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
@@ -774,17 +775,28 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
         }
         float* const st = epi + g * kStage * kEpiLd;
         const int64_t row_b = p.y_pitch * es;
-        uint32_t ab = 0;
-        for (uint32_t i = 0; i < n_mine; ++i, ab ^= 1) {
-            const Unit u = unit_at(i);
-            const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
-            // which of the unit's rows are live, 32 a lane: asked for while the accumulators are still being computed
-            uint32_t live = 0;
+        // a unit's slots, row 32 b + lane in slot[b]: fetched a unit ahead
+        constexpr int LB = (NT + 31) / 32;
+        int32_t slot[LB];
+        auto fetch = [&](const Unit& n) {
 #pragma unroll
-            for (int b = 0; b < (NT + 31) / 32; ++b) {
-                const int j = 32 * b + lane;
-                const uint32_t m = __ballot_sync(0xFFFFFFFFu, j < u.nr && !(p.sorted_tok && p.sorted_tok[u.r0 + j] < 0));
+            for (int b = 0; b < LB; ++b) slot[b] = p.sorted_tok && 32 * b + lane < n.nr ? p.sorted_tok[n.r0 + 32 * b + lane] : 0;
+        };
+        uint32_t ab = 0, turn = g;                            // turn: this group's first slice of the unit
+        Unit u = n_mine ? unit_at(0) : Unit{};
+        if (n_mine) fetch(u);
+        for (uint32_t i = 0; i < n_mine; ++i, ab ^= 1) {
+            const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
+            uint32_t live = 0;                                               // which of its rows are, 32 a lane
+#pragma unroll
+            for (int b = 0; b < LB; ++b) {
+                const uint32_t m = __ballot_sync(0xFFFFFFFFu, slot[b] >= 0);
                 if (lane == b) live = m;
+            }
+            const Unit now = u;
+            if (i + 1 < n_mine) {
+                u = unit_at(i + 1);
+                fetch(u);
             }
             wait(&acc_full[ab], (i >> 1) & 1);
             if (mx_out && !SPLIT ? epi_any(g, *vdead) : __any_sync(0xFFFFFFFFu, *vdead)) break;
@@ -793,7 +805,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                 // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
                 // then sums every split-th row over the CTAs, in their order, and stores it.
                 if (i) wait_cluster(part_empty, (i & 1) ^ 1);
-                for (int t0 = 0; t0 < u.nr; t0 += kSlice) {
+                for (int t0 = 0; t0 < now.nr; t0 += kSlice) {
                     uint32_t a[16];
                     tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
                     tmem_wait(a);
@@ -809,7 +821,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                 const bool out_lane = !act || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
                 const int64_t n0 = b0 + (act ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
                 const uint32_t rows_live = __shfl_sync(0xFFFFFFFFu, live, 0);
-                for (int j = part + split * q; j < u.nr; j += split * 4) {
+                for (int j = part + split * q; j < now.nr; j += split * 4) {
                     float f[kMaxSplit][4], v[4];
 #pragma unroll
                     for (int s = 0; s < kMaxSplit; ++s)       // all on their way before the first is added
@@ -828,7 +840,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                             v[e] = silu(v[e]) * up;
                         }
                     }
-                    const int64_t r = u.r0 + j;
+                    const int64_t r = now.r0 + j;
                     const bool ok = out_lane && n0 < p.n_out;
                     if (!(rows_live >> j & 1)) v[0] = v[1] = v[2] = v[3] = 0.f;        // a dropped slot
                     if (mx_out) {
@@ -858,14 +870,17 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
             const int64_t n = b0 + (act ? 16 * q + (lane & 15) : 32 * q + lane);
             const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + ab * NT;
             uint32_t a[16];
-            if (g * kSlice < u.nr) tmem_ld16(acc + g * kSlice, a);
-            for (int t0 = g * kSlice; t0 < u.nr; t0 += C::EPI_G * kSlice) {
+            // the groups take turns at slices, on from where the last unit's ended
+            const int t1 = (int)turn * kSlice;
+            if (t1 < now.nr) tmem_ld16(acc + t1, a);
+            turn = (turn + C::EPI_G * kMaxTurn - (uint32_t)(now.nr + kSlice - 1) / kSlice) % C::EPI_G;
+            for (int t0 = t1; t0 < now.nr; t0 += C::EPI_G * kSlice) {
                 tmem_wait(a);
                 float v[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(a[j]);
-                if (t0 + C::EPI_G * kSlice < u.nr) tmem_ld16(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
-                uint32_t here = (1u << min(u.nr - t0, kSlice)) - 1;              // the slice's rows
+                if (t0 + C::EPI_G * kSlice < now.nr) tmem_ld16(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
+                uint32_t here = (1u << min(now.nr - t0, kSlice)) - 1;              // the slice's rows
                 const uint32_t drop = here & ~(__shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31));
                 if (drop) {                                                       // dropped slots are zero
 #pragma unroll
@@ -881,7 +896,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                 }
                 if (p.y_dtype == RAD_F32) {
                     // straight from the registers: a warp's store is 32 outputs of a row (silu_mul: 16 of two rows)
-                    uint8_t* d = y + (u.r0 + t0 + (act && up ? 1 : 0)) * row_b + n * 4;
+                    uint8_t* d = y + (now.r0 + t0 + (act && up ? 1 : 0)) * row_b + n * 4;
                     here = n < p.n_out ? act && up ? here >> 1 : here : 0u;
                     if (act) {
 #pragma unroll
@@ -915,7 +930,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                         const int line = act ? lane >> 2 : 4 * k + (lane >> 3), dj = act ? 2 : 1;
                         const int j = act ? (line >> 1) * 4 + (line & 1) : 2 * line;
                         const int64_t n0 = b0 + (act ? 16 * q + 4 * (lane & 3) : 32 * q + 4 * (lane & 7));
-                        uint8_t* d = y + (u.r0 + t0 + j) * row_b + n0 * 2;
+                        uint8_t* d = y + (now.r0 + t0 + j) * row_b + n0 * 2;
                         if (n0 < p.n_out) {
                             if (here >> j & 1) *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
                             if (here >> (j + dj) & 1)
@@ -939,7 +954,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                     epi_sync(g);
                     if (q * tpw < kStage) {                                  // whole warps: the quads vote
                         const int j = q * tpw + lane / lpt;
-                        const int64_t r = u.r0 + t0 + 8 * h + j, n0 = b0 + c0;
+                        const int64_t r = now.r0 + t0 + 8 * h + j, n0 = b0 + c0;
                         float f[8];
                         ld8<1>(&st[j * kEpiLd + c0], f);
                         const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
