@@ -242,7 +242,7 @@ __device__ __forceinline__ void tmem_free(uint32_t t, uint32_t cols) {
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(t), "r"(cols) : "memory");
 }
-// 16 columns of this warp's 32 lanes; tmem_wait before the registers are read.
+// 16 columns of this warp's 32 lanes; tmem_wait before the registers are read. tmem_ld16: lane l's 16 in thread l.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t r[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -250,6 +250,23 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t r[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+// ... and in 8 x 8 pieces: r[8 s + 4 h + 2 g + e] is lane 16 s + 8 g + t / 4, column 8 h + 2 (t % 4) + e in thread t, so
+// that lanes 0..15 (silu_mul's gates) and 16..31 (its ups) meet in the same thread.
+__device__ __forceinline__ void tmem_ld8x8(uint32_t taddr, uint32_t r[16]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[8 * s]), "=r"(r[8 * s + 1]), "=r"(r[8 * s + 2]), "=r"(r[8 * s + 3]), "=r"(r[8 * s + 4]),
+                       "=r"(r[8 * s + 5]), "=r"(r[8 * s + 6]), "=r"(r[8 * s + 7])
+                     : "r"(taddr + ((16u * s) << 16)));
+}
+// Four 8 x 8 pieces of 16-bit pairs (columns 2 c and 2 c + 1 of lane t / 4 a word), transposed into shared memory: thread
+// t's address is that of column t % 8 of piece t / 8, 16 bytes of eight lanes' values.
+__device__ __forceinline__ void st8x8t(uint32_t dst, const uint32_t w[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait(uint32_t r[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -379,9 +396,10 @@ __device__ __forceinline__ float silu(float z) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + r));
     return z * r;
 }
-__device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi) {
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
-    if (dtype == RAD_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    if constexpr (DT == RAD_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
@@ -397,7 +415,8 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
     return r != 0;
 }
 
-template <bool MX, bool PAIR, bool SPLIT, int EG>
+// OUT: y_dtype; ACT: silu_mul.
+template <bool MX, bool PAIR, bool SPLIT, int EG, int OUT, bool ACT>
 __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAIR, SPLIT, EG>::PER_SM)
     k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
     const int ST = sh.st, split = sh.split;
@@ -427,7 +446,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
     const uint32_t part = SPLIT ? blockIdx.x % split : 0u;    // which part of its k
     const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / split : blockIdx.x;
     const uint32_t stride = sh.stride.d;
-    const int act = p.act;
+    constexpr bool act = ACT;
     const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
     constexpr int MB = PAIR ? 2 : 1;
     const uint32_t n_mb = sh.n_mb.d;
@@ -740,9 +759,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
     } else {
         // ---------------------------------------------------------------- epilogue
         const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
-        const int es = p.y_dtype == RAD_F32 ? 4 : 2;
+        constexpr int es = OUT == RAD_F32 ? 4 : 2;
         uint8_t* const y = static_cast<uint8_t*>(p.y);
-        const bool mx_out = p.y_dtype == EXL3B_MX4;
+        constexpr bool mx_out = OUT == (int)EXL3B_MX4;
         // Rows outside the runs are zero: 512 bytes (MXFP4: 128 and their scales) of a row a warp, spread over the whole grid.
         // (A row a warp, 32 rows at a time, left the last rows to one pair: 172 us for 137 at 16 experts, 16067 of 16384
         // rows, 1536 -> 4096.)
@@ -856,114 +875,93 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAI
                         }
                     } else if (ok) {
                         uint8_t* d = y + r * row_b + n0 * es;
-                        if (p.y_dtype == RAD_F32) *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
-                        else *reinterpret_cast<uint2*>(d) = make_uint2(pack2(p.y_dtype, v[0], v[1]), pack2(p.y_dtype, v[2], v[3]));
+                        if constexpr (OUT == RAD_F32) *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2*>(d) = make_uint2(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]));
                     }
                 }
                 __syncwarp();
                 if (i + 1 < n_mine && lane < split) arrive_at(part_empty, lane);
                 continue;
             }
-            // silu_mul: lanes 0..15 hold 16 gate rows, 16..31 their up rows; the lower half takes the even rows' outputs of
-            // a slice, the upper the odd ones'
-            const bool up = lane >= 16;
-            const int64_t n = b0 + (act ? 16 * q + (lane & 15) : 32 * q + lane);
+            // Thread t has outputs o and o + 8 (act NONE: and 16 more) of rows c2, c2 + 1, 8 + c2, 9 + c2 of a slice
+            constexpr int NV = ACT ? 8 : 16;
+            const int o = lane >> 2, c2 = 2 * (lane & 3);
+            const int64_t n_warp = b0 + (act ? 16 : 32) * q;                 // the warp's first output
             const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16) + ab * NT;
             uint32_t a[16];
             // the groups take turns at slices, on from where the last unit's ended
             const int t1 = (int)turn * kSlice;
-            if (t1 < now.nr) tmem_ld16(acc + t1, a);
+            if (t1 < now.nr) tmem_ld8x8(acc + t1, a);
             turn = (turn + C::EPI_G * kMaxTurn - (uint32_t)(now.nr + kSlice - 1) / kSlice) % C::EPI_G;
             for (int t0 = t1; t0 < now.nr; t0 += C::EPI_G * kSlice) {
                 tmem_wait(a);
-                float v[16];
+                float v[NV];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(a[j]);
-                if (t0 + C::EPI_G * kSlice < now.nr) tmem_ld16(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
-                uint32_t here = (1u << min(now.nr - t0, kSlice)) - 1;              // the slice's rows
-                const uint32_t drop = here & ~(__shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31));
-                if (drop) {                                                       // dropped slots are zero
+                for (int k = 0; k < NV; ++k) v[k] = act ? silu(__uint_as_float(a[k])) * __uint_as_float(a[(8 + k) & 15]) : __uint_as_float(a[k]);
+                if (t0 + C::EPI_G * kSlice < now.nr) tmem_ld8x8(acc + t0 + C::EPI_G * kSlice, a);   // the next slice, meanwhile
+                const int left = now.nr - t0;                                     // rows of the slice, if less than 16
+                const uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
+                if ((here & 0xFFFFu) != 0xFFFFu) {                                // dropped slots are zero
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = drop >> j & 1 ? 0.f : v[j];
+                    for (int k = 0; k < NV; ++k)
+                        if (!(here >> (8 * (k >> 2 & 1) + c2 + (k & 1)) & 1)) v[k] = 0.f;
                 }
-                if (act) {
+                if constexpr (OUT == RAD_F32) {
+                    // straight from the registers: a warp's store is 32 bytes each of four rows
+                    const int64_t n = n_warp + o;
+                    uint8_t* d = y + (now.r0 + t0 + c2) * row_b + n * 4;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float other = __shfl_xor_sync(0xFFFFFFFFu, up ? v[2 * j] : v[2 * j + 1], 16);
-                        const float z = up ? other : v[2 * j];
-                        v[j] = silu(z) * (up ? v[2 * j + 1] : other);
+                    for (int k = 0; k < NV; ++k) {
+                        const int j = 8 * (k >> 2 & 1) + (k & 1), m = 16 * (k >> 3) + 8 * (k >> 1 & 1);
+                        if (c2 + j < left && n + m < p.n_out) *reinterpret_cast<float*>(d + j * row_b + 4 * m) = v[k];
                     }
-                }
-                if (p.y_dtype == RAD_F32) {
-                    // straight from the registers: a warp's store is 32 outputs of a row (silu_mul: 16 of two rows)
-                    uint8_t* d = y + (now.r0 + t0 + (act && up ? 1 : 0)) * row_b + n * 4;
-                    here = n < p.n_out ? act && up ? here >> 1 : here : 0u;
-                    if (act) {
+                } else if constexpr (!mx_out) {
+                    // Transposed through the warp's own 1 KB of shared memory -- a row's outputs, 16-byte pieces swizzled
+                    // against bank conflicts -- then 16 bytes a thread: whole 32-byte sectors, and no warp waits for another.
+                    // (Two-byte stores straight from the registers: 218 against 177 us at 16 experts, 16067 rows, 1536 ->
+                    // 4096.)
+                    constexpr int P = NV / 4, SH = ACT ? 2 : 1;                   // 16-byte pieces a row; rows that share banks
+                    uint8_t* const sw = reinterpret_cast<uint8_t*>(epi) + ew * 1024;
+                    auto at = [](int row, int piece) { return (row * P + (piece ^ (row >> SH & (P - 1)))) * 16; };
 #pragma unroll
-                        for (int j = 0; j < 8; ++j, d += 2 * row_b)
-                            if (here >> (2 * j) & 1) *reinterpret_cast<float*>(d) = v[j];
-                    } else {
+                    for (int s = 0; s < NV / 8; ++s) {
+                        uint32_t w[4];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j, d += row_b)
-                            if (here >> j & 1) *reinterpret_cast<float*>(d) = v[j];
-                    }
-                    continue;
-                }
-                if (!mx_out) {
-                    // Two rows of an output a word, lines of words in the warp's own 1 KB of shared memory, then four outputs
-                    // of two rows a thread: whole 32-byte sectors, and no warp waits for another. Two-byte stores straight
-                    // from the registers took 12 cycles each: 218 against 177 us at 16 experts, 16067 rows, 1536 -> 4096.
-                    uint32_t* sw = reinterpret_cast<uint32_t*>(epi) + ew * 256;
-                    if (act) {
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) sw[32 * m + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
-                    } else {
-#pragma unroll
-                        for (int m = 0; m < 8; ++m) sw[32 * m + lane] = pack2(p.y_dtype, v[2 * m], v[2 * m + 1]);
+                        for (int m = 0; m < 4; ++m) w[m] = pack2<OUT>(v[8 * s + 2 * m], v[8 * s + 2 * m + 1]);
+                        st8x8t(smem_u32(sw) + at(8 * (lane >> 4) + (lane & 7), 2 * s + (lane >> 3 & 1)), w);
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        if (k && act) break;
-                        const uint4 w = *reinterpret_cast<const uint4*>(sw + 128 * k + 4 * lane);
-                        // act: line 2m + odd holds rows 4m + odd and 4m + odd + 2; else line m rows 2m and 2m + 1
-                        const int line = act ? lane >> 2 : 4 * k + (lane >> 3), dj = act ? 2 : 1;
-                        const int j = act ? (line >> 1) * 4 + (line & 1) : 2 * line;
-                        const int64_t n0 = b0 + (act ? 16 * q + 4 * (lane & 3) : 32 * q + 4 * (lane & 7));
-                        uint8_t* d = y + (now.r0 + t0 + j) * row_b + n0 * 2;
-                        if (n0 < p.n_out) {
-                            if (here >> j & 1) *reinterpret_cast<uint2*>(d) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
-                            if (here >> (j + dj) & 1)
-                                *reinterpret_cast<uint2*>(d + dj * row_b) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
-                        }
+                    for (int s = 0; s < NV / 8; ++s) {
+                        const int row = (32 * s + lane) / P, piece = lane % P;
+                        const uint4 w = *reinterpret_cast<const uint4*>(sw + at(row, piece));
+                        const int64_t n = n_warp + 8 * piece;
+                        if (row < left && n < p.n_out) *reinterpret_cast<uint4*>(y + (now.r0 + t0 + row) * row_b + n * 2) = w;
                     }
                     __syncwarp();
-                    continue;
-                }
-                // MXFP4: staged, since a block's 32 outputs lie in two warps (silu_mul); eight outputs of a row a thread
-                const int lpt = blk_out / 8, tpw = 32 / lpt, c0 = (lane % lpt) * 8;
+                } else {
+                    // MXFP4: staged in f32, since a block's 32 outputs lie in two warps (silu_mul); eight of a row a thread
+                    const int lpt = blk_out / 8, tpw = 32 / lpt, c0 = (lane % lpt) * 8;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (act) {
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) st[(2 * j + (lane >> 4)) * kEpiLd + 16 * q + (lane & 15)] = v[4 * h + j];
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) st[j * kEpiLd + 32 * q + lane] = v[8 * h + j];
-                    }
-                    epi_sync(g);
-                    if (q * tpw < kStage) {                                  // whole warps: the quads vote
-                        const int j = q * tpw + lane / lpt;
-                        const int64_t r = now.r0 + t0 + 8 * h + j, n0 = b0 + c0;
-                        float f[8];
-                        ld8<1>(&st[j * kEpiLd + c0], f);
-                        const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
-                        if (here >> (8 * h + j) & 1 && n0 < p.n_out) {
-                            *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);
-                            if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
+                        for (int k = 0; k < NV; ++k)
+                            if ((k >> 2 & 1) == h)
+                                st[(c2 + (k & 1)) * kEpiLd + (act ? 16 : 32) * q + 16 * (k >> 3) + 8 * (k >> 1 & 1) + o] = v[k];
+                        epi_sync(g);
+                        if (q * tpw < kStage) {                                  // whole warps: the quads vote
+                            const int j = q * tpw + lane / lpt;
+                            const int64_t r = now.r0 + t0 + 8 * h + j, n0 = b0 + c0;
+                            float f[8];
+                            ld8<1>(&st[j * kEpiLd + c0], f);
+                            const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
+                            if (8 * h + j < left && n0 < p.n_out) {
+                                *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);
+                                if ((lane & 3) == 0) p.y_scales[r * p.ys_pitch + n0 / 32] = (uint8_t)code;
+                            }
                         }
+                        epi_sync(g);
                     }
-                    epi_sync(g);
                 }
             }
             fence_before();
@@ -1029,6 +1027,9 @@ int64_t most_units(const Exl3bGmmOp* p, int nt, int mb) {
     return (live + p->n_rows / nt) * ((p->n_out + blk - 1) / blk);
 }
 
+typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
+int out_kind(int dt) { return dt == RAD_F32 ? 0 : dt == RAD_F16 ? 1 : dt == RAD_BF16 ? 2 : 3; }
+
 // split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
 template <bool MX, bool PAIR, bool SPLIT, int EG>
 int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
@@ -1036,13 +1037,18 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     CUtensorMap map;
     const int rc = make_map(p, &map);
     if (rc) return rc;
-    auto kern = k_gmm<MX, PAIR, SPLIT, EG>;
-    static bool allowed[64];                                  // the most shared memory, once a device
+    static const Kern kerns[8] = { k_gmm<MX, PAIR, SPLIT, EG, RAD_F32, false>, k_gmm<MX, PAIR, SPLIT, EG, RAD_F16, false>,
+                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_BF16, false>, k_gmm<MX, PAIR, SPLIT, EG, EXL3B_MX4, false>,
+                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_F32, true>, k_gmm<MX, PAIR, SPLIT, EG, RAD_F16, true>,
+                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_BF16, true>, k_gmm<MX, PAIR, SPLIT, EG, EXL3B_MX4, true> };
+    static bool allowed[64][8];                               // the most shared memory, once a device
+    const int which = out_kind(p->y_dtype) + (p->act ? 4 : 0);
+    const Kern kern = kerns[which];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
-    if (!allowed[dev]) {
+    if (!allowed[dev][which]) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
-        allowed[dev] = true;
+        allowed[dev][which] = true;
     }
     const int ctas = PAIR ? 2 : split;                        // of a cluster
     const int64_t most = most_units(p, C::NT, PAIR ? 2 : 1);
