@@ -67,12 +67,13 @@ constexpr int kMaxExpert = 2048;
 constexpr int kMaxSplit = 4;                     // CTAs a unit at most (SPLIT)
 constexpr int kMaxSt = 10;                       // stages at most
 
-// EG: epilogue groups of four warps.
-template <bool MX, bool PAIR, bool SPLIT, int EG>
+template <bool MX, bool PAIR, bool SPLIT>
 struct Cfg {
     static constexpr int NT = !PAIR ? 32 : MX ? 224 : 256;       // sorted rows a unit at most
     static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
-    static constexpr int EPI_G = EG;
+    // epilogue groups of four warps; PAIR: the third counts where the epilogue is the longer part, 16 experts of 16060 rows,
+    // bf16 256 -> 1024 silu_mul in 28 us with two and 26 with three, and costs nothing elsewhere
+    static constexpr int EPI_G = PAIR ? 3 : 1;
     static constexpr int THREADS = (kEpiWarp0 + 4 * EPI_G) * 32;
     static constexpr int X_B = NL * kRowB;
     static constexpr int SFW_B = MX ? 1024 : 0;                  // two 128-k halves of 512 bytes
@@ -416,11 +417,11 @@ __device__ __forceinline__ bool epi_any(int g, bool bad) {
 }
 
 // OUT: y_dtype; ACT: silu_mul.
-template <bool MX, bool PAIR, bool SPLIT, int EG, int OUT, bool ACT>
-__global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT, EG>::THREADS, Cfg<MX, PAIR, SPLIT, EG>::PER_SM)
+template <bool MX, bool PAIR, bool SPLIT, int OUT, bool ACT>
+__global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, SPLIT>::PER_SM)
     k_gmm(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
     const int ST = sh.st, split = sh.split;
-    using C = Cfg<MX, PAIR, SPLIT, EG>;
+    using C = Cfg<MX, PAIR, SPLIT>;
     constexpr int NT = C::NT, THREADS = C::THREADS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -1031,16 +1032,16 @@ typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
 int out_kind(int dt) { return dt == RAD_F32 ? 0 : dt == RAD_F16 ? 1 : dt == RAD_BF16 ? 2 : 3; }
 
 // split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
-template <bool MX, bool PAIR, bool SPLIT, int EG>
+template <bool MX, bool PAIR, bool SPLIT>
 int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
-    using C = Cfg<MX, PAIR, SPLIT, EG>;
+    using C = Cfg<MX, PAIR, SPLIT>;
     CUtensorMap map;
     const int rc = make_map(p, &map);
     if (rc) return rc;
-    static const Kern kerns[8] = { k_gmm<MX, PAIR, SPLIT, EG, RAD_F32, false>, k_gmm<MX, PAIR, SPLIT, EG, RAD_F16, false>,
-                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_BF16, false>, k_gmm<MX, PAIR, SPLIT, EG, EXL3B_MX4, false>,
-                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_F32, true>, k_gmm<MX, PAIR, SPLIT, EG, RAD_F16, true>,
-                                    k_gmm<MX, PAIR, SPLIT, EG, RAD_BF16, true>, k_gmm<MX, PAIR, SPLIT, EG, EXL3B_MX4, true> };
+    static const Kern kerns[8] = { k_gmm<MX, PAIR, SPLIT, RAD_F32, false>, k_gmm<MX, PAIR, SPLIT, RAD_F16, false>,
+                                    k_gmm<MX, PAIR, SPLIT, RAD_BF16, false>, k_gmm<MX, PAIR, SPLIT, EXL3B_MX4, false>,
+                                    k_gmm<MX, PAIR, SPLIT, RAD_F32, true>, k_gmm<MX, PAIR, SPLIT, RAD_F16, true>,
+                                    k_gmm<MX, PAIR, SPLIT, RAD_BF16, true>, k_gmm<MX, PAIR, SPLIT, EXL3B_MX4, true> };
     static bool allowed[64][8];                               // the most shared memory, once a device
     const int which = out_kind(p->y_dtype) + (p->act ? 4 : 0);
     const Kern kern = kerns[which];
@@ -1081,11 +1082,7 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
     const int64_t few = p->w_rows < 512 ? 96 : 16;
     if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4) {
-        // A third group of epilogue warps where the epilogue is the longer part, silu_mul's and that of a short k (16 experts,
-        // 16067 rows, bf16: 512 -> 1024 silu_mul 50 us with two groups, 43 with three; 512 -> 4096 102 and 97); over a long
-        // k its warps only get in the others' way (MXFP4 4096 -> 1536: 60 and 62; 1536 -> 4096: 173 and 175).
-        return p->act || p->n_in <= (MX ? 1024 : 512) ? launch<MX, true, false, 3>(p, sm_count, 1, st)
-                                                      : launch<MX, true, false, 2>(p, sm_count, 1, st);
+        return launch<MX, true, false>(p, sm_count, 1, st);
     }
     // Few narrow units over a long k: up to four CTAs a unit while each has an SM, four stages a part at least (one token,
     // two experts, 2048 -> 512 silu_mul: 11.1 us, in four parts 8.9; 16 rows, 4096 -> 4096: 16.3 and 12.6; ten experts make
@@ -1096,9 +1093,9 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         int64_t split = sm_count / most;
         if (split > nck / 4) split = nck / 4;
         if (split > kMaxSplit) split = kMaxSplit;
-        if (split >= 2) return launch<false, false, true, 1>(p, sm_count, (int)split, st);
+        if (split >= 2) return launch<false, false, true>(p, sm_count, (int)split, st);
     }
-    return launch<MX, false, false, 1>(p, sm_count, 1, st);
+    return launch<MX, false, false>(p, sm_count, 1, st);
 }
 
 }  // namespace
