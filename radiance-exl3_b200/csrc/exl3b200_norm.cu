@@ -49,6 +49,8 @@ __device__ __forceinline__ float sigmoid(float g) {
     return r;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 template <int DT, int BT, int VPT, int MAXT, bool VEC>
 __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const Exl3bNormOp p) {
     typedef typename El<DT>::T T;
@@ -116,6 +118,20 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
         const T* gate_at = !gates || !live ? nullptr
                            : static_cast<const T*>(p.gate) + (p.gate_kind == EXL3B_GATE_ELEMENT ? row * p.gate_pitch : 0);
         const float token = p.gate_kind == EXL3B_GATE_TOKEN && live ? static_cast<const float*>(p.gate)[row] : 0.f;
+        // An element gate's registers leave few rows in flight: the next row's lines are asked into L2 meanwhile (9600 x 4096
+        // 77.8 and 73.7 us, 2048 x 2560 15.5 and 15.0; not for 128 threads a row, 4096 x 2048 19.7 and 20.6; the other gates
+        // gain nothing)
+        if (VEC && p.gate_kind == EXL3B_GATE_ELEMENT && tpr > 128 && row + step < p.rows) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = at(v, 0);
+                if (c < H && c % (128 / (int)sizeof(T)) == 0) {
+                    prefetch_l2(gate_at + step * p.gate_pitch + c);
+                    if (p.res) prefetch_l2(res_at + step * p.res_pitch + c);
+                }
+                if (p.branch && c < H && c % (128 / (int)sizeof(B)) == 0) prefetch_l2(branch_at + step * p.branch_pitch + c);
+            }
+        }
         // the row's loads first (the longest rows have registers for the branch alone)
         constexpr bool AHEAD = MAXT <= 512;
         float r[VPT][8];
@@ -127,7 +143,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 if (AHEAD) load(stream_dt, res_at, v, res[v]);
-                if (AHEAD && VPT == 1) load(stream_dt, gate_at, v, gate[v]);
+                if (AHEAD && VPT <= 2) load(stream_dt, gate_at, v, gate[v]);
             }
 #pragma unroll
             for (int v = 0; v < VPT; ++v) b[v].get(r[v]);
@@ -155,7 +171,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 float f[8];
-                if (!AHEAD || VPT > 1) load(stream_dt, gate_at, v, gate[v]);
+                if (!AHEAD || VPT > 2) load(stream_dt, gate_at, v, gate[v]);
                 gate[v].get(f);
                 if (p.gate_kind == EXL3B_GATE_ELEMENT) {
 #pragma unroll
