@@ -46,6 +46,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "exl3b200_chain.cuh"
 #include "exl3b200_decode.cuh"
 #include "exl3b200_dense.h"
 #include "exl3b200_mx4.cuh"
@@ -451,9 +452,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     const int blk_out = act ? 64 : 128;                       // outputs a block (a CTA's part of a unit)
     constexpr int MB = PAIR ? 2 : 1;
     const uint32_t n_mb = sh.n_mb.d;
-    // the run of this thread's first expert before all else: its latency covers the barriers' set-up
     const int per = (p.n_expert + THREADS - 1) / THREADS, e0 = tid * per, e1 = min(e0 + per, p.n_expert);
-    const Run run0 = e0 < e1 ? run_of(p, e0) : Run{ 0, 0 };
     if (tid < ST) {
         mbar_init(&full[tid], 1 + 32 * kXWarps + C::SFX_G + (PAIR && rank == 0 ? 1 : 0));
         mbar_init(&empty[tid], 1);
@@ -472,6 +471,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     __syncwarp();
     if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
     if (PAIR || SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    chain_wait();                                             // all above needs no memory but the CTA's own
+    const Run run0 = e0 < e1 ? run_of(p, e0) : Run{ 0, 0 };
     // prefix[e]: the first unit of expert e (block-wide exclusive scan, a thread a run of experts); this CTA's units
     // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     __syncthreads();
     if (PAIR || SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs' barriers and tensor memory are set up
     fence_after();
+    chain_next();                                             // every CTA has its tensor memory: a later kernel may ask for its own
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
     const uint32_t n_mine = n_units > first ? sh.stride(n_units - first + stride - 1) : 0;
@@ -1057,21 +1059,11 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     const int per_sm = !PAIR && most * ctas <= sm_count ? 1 : C::PER_SM;
     const int64_t room = (int64_t)sm_count * per_sm / ctas;
     const int stages = C::stages(p->n_expert, per_sm);
-    cudaLaunchConfig_t cfg = {};
-    cfg.dynamicSmemBytes = C::fixed(p->n_expert) + stages * C::STAGE_B;
-    cfg.blockDim = dim3(C::THREADS);
     const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
-    cfg.gridDim = dim3((unsigned)(units * ctas));
     const Shape sh = { fast_div((uint32_t)((p->n_out + blk - 1) / blk)), fast_div((uint32_t)units),
                        (int32_t)((p->n_in + (MX ? 255 : 63)) / (MX ? 256 : 64)), stages, split };
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = ctas > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, map, *p, sh) == cudaSuccess ? 0 : -6;
+    return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
+                        ctas, st, map, *p, sh);
 }
 
 template <bool MX>

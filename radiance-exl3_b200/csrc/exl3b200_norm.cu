@@ -1,6 +1,7 @@
 // exl3b200_norm.cu -- the row-wise operators around an expert block: block_norm (the norm behind a block with its gate
 // and residual scale, and the norm before the next, one pass over the row), MXFP4 quantisation and its reverse, and the
 // one-time layout of a weight's scales. sm_100a.
+#include "exl3b200_chain.cuh"
 #include "exl3b200_dense.h"
 #include "exl3b200_mx4.cuh"
 
@@ -61,6 +62,8 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
     const int H = (int)p.cols;
     const float inv_h = 1.f / (float)H;
     for (int i = ty * tpr + tid; i < (int)(sizeof part / 4); i += tpr * blockDim.y) (&part[0][0][0][0])[i] = 0.f;
+    chain_wait();
+    chain_next();
     __syncthreads();
     const std::integral_constant<int, DT> stream_dt;
     const std::integral_constant<int, BT> branch_dt;
@@ -232,9 +235,8 @@ int launch_norm_t(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st)
     const int64_t want = (p->rows + rpb - 1) / rpb, room = (int64_t)sm_count * (2048 / (tpr * rpb));
     const unsigned grid = (unsigned)(want < room ? want : room);
     const dim3 block(tpr, rpb);
-    if (vec) k_block_norm<DT, BT, VPT, MAXT, true><<<grid, block, 0, st>>>(*p);
-    else k_block_norm<DT, BT, VPT, MAXT, false><<<grid, block, 0, st>>>(*p);
-    return cudaGetLastError() == cudaSuccess ? 0 : -6;
+    return vec ? chain_launch(k_block_norm<DT, BT, VPT, MAXT, true>, dim3(grid), block, 0, 1, st, *p)
+               : chain_launch(k_block_norm<DT, BT, VPT, MAXT, false>, dim3(grid), block, 0, 1, st, *p);
 }
 
 template <int DT, int BT>
@@ -304,6 +306,8 @@ template <int DT, bool BIG>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t n_vec, RowDiv div,
                                                       uint8_t* q, int64_t q_pitch, uint8_t* qs, int64_t qs_pitch) {
     typedef typename El<DT>::T T;
+    chain_wait();
+    chain_next();
     const int64_t i0 = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
     Raw<DT> v[kUnroll];
     int64_t row[kUnroll];
@@ -369,6 +373,8 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* q, int64_
                                                         int64_t qs_pitch, int64_t n_vec, RowDiv div, void* y,
                                                         int64_t y_pitch) {
     typedef typename El<DT>::T T;
+    chain_wait();
+    chain_next();
     const int64_t i0 = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
     uint32_t n[kUnroll], s[kUnroll];
     int64_t row[kUnroll];
@@ -441,8 +447,8 @@ int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int
 
 #define EXL3B_MX4_ROWS(KERN, DT, ...)                                                                        \
     do {                                                                                                     \
-        if (n_vec < (1ll << 31) - 1024) KERN<DT, false><<<grid, 256, 0, st>>>(__VA_ARGS__);                  \
-        else KERN<DT, true><<<grid, 256, 0, st>>>(__VA_ARGS__);                                              \
+        if (n_vec < (1ll << 31) - 1024) return chain_launch(KERN<DT, false>, dim3(grid), dim3(256), 0, 1, st, __VA_ARGS__); \
+        return chain_launch(KERN<DT, true>, dim3(grid), dim3(256), 0, 1, st, __VA_ARGS__);                   \
     } while (0)
 
 int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
@@ -454,7 +460,6 @@ int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t r
     if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_quantize, 1, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
     else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_quantize, 2, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
     else EXL3B_MX4_ROWS(k_mx4_quantize, 3, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
-    return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
 
 int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* qs, int64_t qs_pitch, int64_t rows,
@@ -466,7 +471,6 @@ int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* 
     if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_dequantize, 1, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
     else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_dequantize, 2, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
     else EXL3B_MX4_ROWS(k_mx4_dequantize, 3, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
-    return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
 
 int exl3b_cuda_mx4_tile(const uint8_t* s, int64_t s_pitch, int64_t e_pitch, int64_t n_expert, int64_t rows, int64_t cols,
