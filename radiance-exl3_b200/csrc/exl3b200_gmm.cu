@@ -46,6 +46,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "exl3b200_chain.cuh"
 #include "exl3b200_decode.cuh"
 #include "exl3b200_dense.h"
@@ -355,42 +357,26 @@ struct RowAhead {
     }
 };
 // 16 scales of an x row from byte `off` on; what lies past the row's end is some byte or other. Rows on 16-byte boundaries
-// are one load (`whole`; of the last row only where the row has them). Else the two aligned 16 bytes around them, shifted;
-// and byte by byte where either would leave the scales' memory.
+// are one load (`whole`; of the last row only where the row has them). Else the five words that hold them, shifted when they
+// are used, not when they are loaded (85 and 55 us at 174 experts of 118 rows, 3808 -> 320); and byte by byte a word that
+// would leave the scales' memory.
 struct RowScales {
     const uint8_t *lo, *hi, *last;
     bool whole;
     __device__ __forceinline__ RowScales(const Exl3bGmmOp& p)
         : lo(p.x_scales), hi(p.x_scales + (p.x_rows - 1) * p.xs_pitch + p.n_in / 32), last(hi - p.n_in / 32),
           whole(((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0) {}
-    __device__ __forceinline__ uint4 load(const uint8_t* row, int off) const {
-        const uint8_t* a = row + off;
-        const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(a) & 15);
-        const uint8_t* b = a - by;
-        uint32_t w[8];
-        if (b >= lo && b + 32 <= hi) {
-            const uint4 x = *reinterpret_cast<const uint4*>(b), y = *reinterpret_cast<const uint4*>(b + 16);
-            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-            w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
-            // words from `by` / 4 on, then bytes
-#pragma unroll
-            for (int i = 0; i < 6; ++i) w[i] = by & 8 ? w[i + 2] : w[i];
-#pragma unroll
-            for (int i = 0; i < 5; ++i) w[i] = by & 4 ? w[i + 1] : w[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (by & 3));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (a + 4 * i + j < hi) w[i] |= (uint32_t)a[4 * i + j] << (8 * j);
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+    template <int U>
+    __device__ __forceinline__ uint32_t word(const uint8_t* b) const {
+        if (b >= lo && b + 4 <= hi) return *reinterpret_cast<const uint32_t*>(b);
+        uint32_t w = 0;
+#pragma unroll U
+        for (int j = 0; j < 4; ++j)
+            if (b + j >= lo && b + j < hi) w |= (uint32_t)b[j] << (8 * j);
+        return w;
     }
 };
+
 // z / (1 + e^-z), from the special-function unit.
 __device__ __forceinline__ float silu(float z) {
     float r;
@@ -631,9 +617,12 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
         // reads 16 bytes of each of its rows at a time, two stages' worth (each row is a line of its own: 4-byte copies a
         // stage kept the L1 busy), into two register sets in turn, one on its way while the other is used, across units.
         const int g = warp - 2;
-        if (MX && g < C::SFX_G && n_mine) {
+        auto run = [&](auto whole, const RowScales& rs) {                          // whole: RowScales'
+            constexpr bool WHOLE = decltype(whole)::value;
             constexpr int Q = NT < 128 ? NT / 32 : 4;
-            const RowScales rs(p);
+            struct Set {
+                uint32_t w[Q][WHOLE ? 4 : 5], sh;
+            };
             const int nsc = (int)(p.n_in / 32);
             RowAhead<Q> ahead(p, lane + g * 128, 32);
             const uint8_t* src[Q];
@@ -650,16 +639,39 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             ahead.fetch(unit_at(0));
             rows();
             if (n_mine > 1) ahead.fetch(unit_at(1));
-            auto load = [&](uint4 v[Q]) {
+            // nothing here touches what it loads: it is waited for where it is used. x.sh: each row's shift, a byte a row
+            auto load = [&](Set& x) {
                 const int off = 8 * lc;
                 if (lc >= k1) return;
-                if (rs.whole && (off + 16 <= nsc || !edge)) {
-                    // nothing here touches what it loads: it is waited for where it is used
+                x.sh = 0;
+                if (WHOLE && (off + 16 <= nsc || !edge)) {
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) v[q] = *reinterpret_cast<const uint4*>(src[q] + off);
+                    for (int q = 0; q < Q; ++q) {
+                        const uint4 t = *reinterpret_cast<const uint4*>(src[q] + off);
+                        x.w[q][0] = t.x; x.w[q][1] = t.y; x.w[q][2] = t.z; x.w[q][3] = t.w;
+                    }
                 } else {
+                    const uint8_t* b[Q];
+                    bool in = true;
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) v[q] = rs.load(src[q], off);
+                    for (int q = 0; q < Q; ++q) {
+                        const uint32_t by = (uint32_t)(reinterpret_cast<uintptr_t>(src[q] + off) & 3);
+                        b[q] = src[q] + off - by;
+                        x.sh |= by << (8 * q + 3);
+                        in = in && b[q] >= rs.lo && b[q] + 20 <= rs.hi;
+                    }
+                    constexpr int W = WHOLE ? 4 : 5;
+                    if (!WHOLE && __all_sync(0xFFFFFFFFu, in)) {
+#pragma unroll
+                        for (int q = 0; q < Q; ++q)
+#pragma unroll
+                            for (int i = 0; i < W; ++i) x.w[q][i] = *reinterpret_cast<const uint32_t*>(b[q] + 4 * i);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < Q; ++q)
+#pragma unroll
+                            for (int i = 0; i < W; ++i) x.w[q][i] = rs.word<WHOLE ? 4 : 1>(b[q] + 4 * i);
+                    }
                 }
                 if ((lc += 2) >= k1 && ++lu < n_mine) {
                     lc = k0;
@@ -667,7 +679,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
                 }
             };
-            auto use = [&](const uint4 v[Q]) {
+            auto use = [&](const Set& x) {
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
                     if (cc + a >= k1) break;
@@ -675,8 +687,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     uint4* dst = reinterpret_cast<uint4*>(sfx_ring + pipe.s * C::SFX_B + g * 512) + lane;
                     auto put = [&](uint32_t m0, uint32_t m1) {
                         auto word = [&](int q, int h) {
-                            const uint4 x = v[q < Q ? q : 0];
-                            return q >= Q ? 0u : a ? (h ? x.w : x.z) : h ? x.y : x.x;
+                            const int r = q < Q ? q : 0, i = 2 * a + h;
+                            return q >= Q ? 0u : WHOLE ? x.w[r][i] : __funnelshift_r(x.w[r][i], x.w[r][(i + 1) % 5], x.sh >> (8 * r));
                         };
                         dst[0] = make_uint4(word(0, 0) & m0, word(1, 0) & m0, word(2, 0) & m0, word(3, 0) & m0);
                         dst[C::SFX_G * 32] = make_uint4(word(0, 1) & m1, word(1, 1) & m1, word(2, 1) & m1, word(3, 1) & m1);
@@ -696,7 +708,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                     ++cu;
                 }
             };
-            uint4 even[Q], odd[Q];
+            Set even = {}, odd = {};
             load(even);
             load(odd);
             while (cu < n_mine && !*vdead) {
@@ -705,6 +717,13 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                 if (cu >= n_mine) break;
                 use(odd);
                 load(odd);
+            }
+        };
+        if constexpr (MX) {
+            const RowScales rs(p);
+            if (g < C::SFX_G && n_mine) {
+                if (rs.whole) run(std::true_type(), rs);
+                else run(std::false_type(), rs);
             }
         }
     } else if (warp < kEpiWarp0) {
