@@ -112,6 +112,7 @@ FastDiv fast_div(uint32_t d) {
 // What the host works out of a launch, so that no CTA divides for it.
 struct Shape {
     FastDiv n_mb, stride;   // weight-row blocks (PAIR: pairs) an output row; CTAs (PAIR, SPLIT: clusters) of the grid
+    FastDiv nt;             // sorted rows a unit at most
     int32_t nck, st, split; // stages of a unit's k, of the ring; CTAs a unit (SPLIT)
 };
 
@@ -121,7 +122,7 @@ struct Unit {
     int32_t nr;          // sorted rows
 };
 
-// The sorted rows of expert e, and into how many groups of at most NT they fall.
+// The sorted rows of expert e, and into how many groups of at most nt they fall.
 struct Run {
     int32_t r0, rows;
 };
@@ -130,14 +131,14 @@ __device__ __forceinline__ Run run_of(const Exl3bGmmOp& p, int e) {
     const int32_t a = max(p.expert_offset[e], 0), b = min(p.expert_offset[e + 1], (int32_t)p.n_rows);
     return Run{ a, max(b - a, 0) };
 }
-template <int NT>
-__device__ __forceinline__ uint32_t groups(const Run& r) { return (uint32_t)(r.rows + NT - 1) / NT; }
+__device__ __forceinline__ uint32_t groups(const Run& r, const FastDiv& nt) { return nt((uint32_t)r.rows + nt.d - 1); }
 
 // Unit `local` of expert e: block by block, then group by group. An expert's rows are split evenly over its groups, in
 // steps of the MMA's N, so that no group is left with a sliver.
-template <int NT, int MB>
-__device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, const FastDiv& n_mb) {
-    const uint32_t g = n_mb(local), ng = groups<NT>(r), step = 16 * MB;
+template <int MB>
+__device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, const Shape& sh) {
+    const FastDiv& n_mb = sh.n_mb;
+    const uint32_t g = n_mb(local), ng = groups(r, sh.nt), step = 16 * MB;
     const uint32_t even = ng > 1 ? ((uint32_t)r.rows + ng - 1) / ng : (uint32_t)r.rows, per = (even + step - 1) / step * step;
     Unit u;
     u.e = e;
@@ -147,14 +148,14 @@ __device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, c
     return u;
 }
 // ... found by its number among all units.
-template <int NT, int MB>
-__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, const FastDiv& n_mb) {
+template <int MB>
+__device__ __forceinline__ Unit find_unit(const Exl3bGmmOp& p, const uint32_t* prefix, uint32_t unit, const Shape& sh) {
     int lo = 0, hi = p.n_expert;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid] <= unit) lo = mid; else hi = mid;
     }
-    return make_unit<NT, MB>(lo, run_of(p, lo), unit - prefix[lo], n_mb);
+    return make_unit<MB>(lo, run_of(p, lo), unit - prefix[lo], sh);
 }
 
 struct Pipe {
@@ -463,9 +464,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     // (first, first + stride, ...) go into the table by the threads that pass over their experts
     {
         __shared__ uint32_t wsum[THREADS / 32];
-        uint32_t sum = groups<NT>(run0) * n_mb;
+        uint32_t sum = groups(run0, sh.nt) * n_mb;
 #pragma unroll 1
-        for (int e = e0 + 1; e < e1; ++e) sum += groups<NT>(run_of(p, e)) * n_mb;
+        for (int e = e0 + 1; e < e1; ++e) sum += groups(run_of(p, e), sh.nt) * n_mb;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -479,13 +480,13 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
 #pragma unroll 1
         for (int e = e0; e < e1; ++e) {
             const Run r = e == e0 ? run0 : run_of(p, e);
-            const uint32_t n = groups<NT>(r) * n_mb;
+            const uint32_t n = groups(r, sh.nt) * n_mb;
             prefix[e] = acc;
             if (n) {
                 uint32_t i = acc > first ? sh.stride(acc - first + stride - 1) : 0u;
 #pragma unroll 1
                 for (; i < kTab && first + i * stride < acc + n; ++i)
-                    utab[i] = make_unit<NT, MB>(e, r, first + i * stride - acc, sh.n_mb);
+                    utab[i] = make_unit<MB>(e, r, first + i * stride - acc, sh);
             }
             acc += n;
         }
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     const uint32_t n_units = prefix[p.n_expert];
     const uint32_t n_mine = n_units > first ? sh.stride(n_units - first + stride - 1) : 0;
     auto unit_at = [&](uint32_t i) {
-        return i < kTab ? utab[i] : find_unit<NT, MB>(p, prefix, first + i * stride, sh.n_mb);
+        return i < kTab ? utab[i] : find_unit<MB>(p, prefix, first + i * stride, sh);
     };
     const int nck = sh.nck;
     // this CTA's stages of a unit
@@ -1049,6 +1050,14 @@ int64_t most_units(const Exl3bGmmOp* p, int nt, int mb) {
     return (live + p->n_rows / nt) * ((p->n_out + blk - 1) / blk);
 }
 
+// Sorted rows a unit of the pair form: where units of `most` leave pairs of SMs without one, as few as still give every
+// pair at most one (one expert of 1024 rows, 2048 -> 2048, bf16: 16.3 us with units of 256 rows, 12.3 with these).
+int pair_rows(const Exl3bGmmOp* p, int most, int sm_count) {
+    int nt = most;
+    while (nt > 64 && most_units(p, nt - 32, 2) <= sm_count / 2) nt -= 32;
+    return nt;
+}
+
 typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
 int out_kind(int dt) { return dt == RAD_F32 ? 0 : dt == RAD_F16 ? 1 : dt == RAD_BF16 ? 2 : 3; }
 
@@ -1073,13 +1082,14 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
         allowed[dev][which] = true;
     }
     const int ctas = PAIR ? 2 : split;                        // of a cluster
-    const int64_t most = most_units(p, C::NT, PAIR ? 2 : 1);
+    const int nt = PAIR ? pair_rows(p, C::NT, sm_count) : C::NT;
+    const int64_t most = most_units(p, nt, PAIR ? 2 : 1);
     // few units: one CTA an SM, with the whole of its shared memory for stages in flight
     const int per_sm = !PAIR && most * ctas <= sm_count ? 1 : C::PER_SM;
     const int64_t room = (int64_t)sm_count * per_sm / ctas;
     const int stages = C::stages(p->n_expert, per_sm);
     const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
-    const Shape sh = { fast_div((uint32_t)((p->n_out + blk - 1) / blk)), fast_div((uint32_t)units),
+    const Shape sh = { fast_div((uint32_t)((p->n_out + blk - 1) / blk)), fast_div((uint32_t)units), fast_div((uint32_t)nt),
                        (int32_t)((p->n_in + (MX ? 255 : 63)) / (MX ? 256 : 64)), stages, split };
     return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
                         ctas, st, map, *p, sh);
@@ -1087,18 +1097,19 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
 
 template <bool MX>
 int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
-    // The pair form from 16 rows an expert on average (512 -> 2240 over 479 experts of 15 rows, MXFP4: narrow 47 us, pair
-    // 67; 792 -> 1648 over 112 experts of 33 rows, f16: 72 and 52), or 96 where a weight has so few rows that its last pair
-    // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 27 and 33); and where its units keep half
-    // the pairs busy (one expert of 306 rows, 3064 -> 328: 17 and 22; two of 908, 1568 -> 1728 MXFP4: 20 and 17).
+    // The pair form from 16 rows an expert on average (512 -> 2240 over 479 experts of 15 rows, MXFP4: narrow 39 us, pair
+    // 43; 792 -> 1648 over 112 experts of 33 rows, bf16: 68 and 50), or 96 where a weight has so few rows that its last pair
+    // of blocks is mostly empty (448 -> 320 over 298 experts of 84 rows, MXFP4: 17 and 24); and where its units, as short as
+    // 96 rows, keep half the pairs busy (one expert, bf16: 4096 rows, 2048 -> 512: 18.7 and 12.6; 306 rows, 3064 -> 328: 8.9
+    // and 16.5).
     const int64_t few = p->w_rows < 512 ? 96 : 16;
-    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 256, 2) >= sm_count / 4) {
+    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4) {
         return launch<MX, true, false>(p, sm_count, 1, st);
     }
     // Few narrow units over a long k: up to four CTAs a unit while each has an SM, four stages a part at least (one token,
-    // two experts, 2048 -> 512 silu_mul: 11.1 us, in four parts 8.9; 16 rows, 4096 -> 4096: 16.3 and 12.6; ten experts make
-    // 80 units: 13.7, in three parts 15.1; clusters of eight do not always fit at once: 15.1 for 8.9). MXFP4 has a quarter
-    // of the stages and gains nothing (two experts 8.9 and 10.3).
+    // two experts, 2048 -> 512 silu_mul: 9.6 us, in four parts 7.0; 16 rows, 4096 -> 4096: 14.8 and 10.4; ten experts make
+    // 80 units: in three parts, more CTAs than SMs, 13.7 and 15.1; clusters of eight do not always fit at once: 15.1 for
+    // 8.9). MXFP4 has a quarter of the stages and gains nothing (two experts 8.9 and 10.3).
     if (!MX) {
         const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 63) / 64;
         int64_t split = sm_count / most;
