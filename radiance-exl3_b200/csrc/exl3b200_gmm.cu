@@ -33,15 +33,16 @@
 //
 // Measured on one B200 that copies 6539 GB/s and reaches 1650 TFLOP/s of bf16 in its library product; a launch's time in a
 // CUDA graph, and what bounds it:
-//   512 experts, 191 live of 624 rows, 640 -> 2560, bf16 (narrow)           96 us  6.5 TB/s: the weights' bytes
-//   512 experts, 418 live of 20072 rows, 2048 -> 512 silu_mul, f16 (PAIR)  282 us  6.3 TB/s: the weights' bytes
-//   16 experts of 16060 rows, 1536 -> 4096, bf16 (PAIR)                    171 us  1182 TFLOP/s: the stages' latency out of
-//     L2, 32 KB a CTA in the ~500 cycles of a stage (tensor pipe busy 63 % of the time)
-//   16 experts of 16060 rows, 4096 -> 1536, MXFP4 (PAIR)                    62 us  3239 TFLOP/s: the same, and the epilogue
-//   64 experts of 20072 rows, 2048 -> 512 silu_mul, MXFP4 (PAIR)            42 us  1996 TFLOP/s: the epilogue, whose
-//     shared-memory traffic competes with the MMAs' operands (tensor pipe 24 %)
-//   one token's ten experts, 2048 -> 512 silu_mul, f16 (narrow)             14 us  42 MB, 6.4 us at the copy rate; the rest
-//     is the launch, the set-up and the first stage's latency. The same in MXFP4 (narrow): 9 us, of them 1.7 for bytes
+//   512 experts, 191 live of 624 rows, 640 -> 2560, bf16 (narrow)           96 us  6.6 TB/s: the weights' bytes
+//   512 experts, 418 live of 20072 rows, 2048 -> 512 silu_mul, f16 (PAIR)  278 us  6.4 TB/s: the weights' bytes
+//   16 experts of 16060 rows, 1536 -> 4096, bf16 (PAIR)                    153 us  1323 TFLOP/s: a stage of 256 x 256 x 64 in
+//     490 to 500 cycles, the MMA's own 512 at full rate, at a clock that power brings down to 1.2 .. 1.5 GHz
+//   16 experts of 16060 rows, 4096 -> 1536, MXFP4 (PAIR)                    54 us  3743 TFLOP/s: a stage of 33 KB a CTA in
+//     ~650 cycles where its MMAs take ~450: L2's rate, 13 TB/s over the GPU; seven units a pair at most where 6.5 would do
+//   64 experts of 20072 rows, 2048 -> 512 silu_mul, MXFP4 (PAIR)            31 us  2735 TFLOP/s: the same, 29 KB in ~560
+//     cycles, and five of the 31 us before the first stage is there (launch, set-up, the first loads)
+//   one token's ten experts, 2048 -> 512 silu_mul, f16 (narrow)             13 us  42 MB, 6.4 us at the copy rate; the rest
+//     is the launch, the set-up and the first stage's latency. The same in MXFP4 (narrow): 8 us, of them 1.7 for bytes
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -21,8 +21,8 @@ namespace {
 // Rows whose addresses or width rule out 16-byte vectors take the same code over single values, a thread's values
 // blockDim.x apart.
 // Measured on one B200 (copies at 6.5 TB/s): 16384 rows of 4096, f32 branch, token gate, both norms, bf16 and MXFP4 out:
-// 133 us, 5.3 TB/s. 2048 rows of 2560 in f16 with an element gate: 15.6 us, 3.4 TB/s, a row's chain of load, two
-// reductions and store each with few rows a CTA. One row of 2048: 2.8 us, a launch.
+// 126 us, 5.6 TB/s. 2048 rows of 2560 in f16 with an element gate: 14.5 us, 3.6 TB/s: 14 rows an SM, too few rounds of
+// load, two reductions and store to hide one another. One row of 2048: 2.8 us, a launch.
 // Eight values as they lie in memory.
 template <int DT>
 struct Raw {
@@ -254,7 +254,7 @@ int launch_norm(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st) {
 // ------------------------------------------------------------------------------------------ MXFP4 rows
 // HBM bound: a thread takes kUnroll vectors of eight values, 256 vectors apart in the rows laid end to end (whatever the
 // width, every lane has work), all loaded before the first is used; a block's scale comes from four neighbouring lanes.
-// Measured on one B200, 20480 x 4096 in bf16: quantised in 38 us (5.6 TB/s), back in 35 us (6.1 TB/s): HBM's bytes; 64 x
+// Measured on one B200, 20480 x 4096 in bf16: quantised in 37 us (5.7 TB/s), back in 34 us (6.2 TB/s): HBM's bytes; 64 x
 // 2048: 2.8 us each, a launch.
 constexpr int kUnroll = 4;
 
