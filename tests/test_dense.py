@@ -588,3 +588,144 @@ def test_block_norm_refusals():
         dense.BlockNorm(branch=x, res=x[:1], out=x)
     with pytest.raises(KeyError):
         dense.BlockNorm(branch=x, gate=w, gate_kind="row", out=x)
+
+
+# ------------------------------------------------------------------------------------------------ forms, chains
+# (counts, K, N): few units over a long k; a few rows an expert; hundreds of rows an expert in pairs of CTAs, in units cut
+# short to fill the SMs and, over more outputs, in whole ones
+FORMS = {"split": ([3, 0, 2], 1024, 96), "narrow": ([5, 0, 33, 1, 17, 12, 0, 0, 0, 0, 0, 0] * 9, 320, 352),
+         "pair": ([600, 0, 715, 257], 320, 544), "wide": ([600, 0, 715, 257], 64, 4128)}
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("act", ["none", "silu_mul"])
+@pytest.mark.parametrize("dtype", [F16, BF16, "mx4"])
+def test_every_form_and_output_with_dropped_slots(form, act, dtype):
+    """Rows outside the runs on both sides, single dropped slots, a whole slice of them and an expert's all."""
+    counts, K, N = FORMS[form]
+    before, after = 70, 333
+    g = gen(N)
+    n = before + sum(counts) + after
+    dropped = sorted({before, before + 3, n - after - 1} | set(range(before + 48, min(before + 70, n - after)))
+                     | set(range(n - after - counts[-1], n - after)))
+    tok, off, n = routing(counts, before, after, dropped, g=g)
+    x, w = randn(g, n, K), randn(g, len(counts), N * (2 if act == "silu_mul" else 1), K) * K ** -0.5
+    kw = dict(expert_offset=off, sorted_tok=tok, top_k=1, act=act)
+    if dtype == "mx4":
+        (xq, xs, xv), (wq, ws, wv) = mx4_of(x), mx4_of(w)
+        kw |= dict(x=xq, x_scales=xs, w=wq, w_scales=dense.mx4_tile_scales(ws, act))
+    else:
+        xv, wv = x.to(dtype), w.to(dtype)
+        kw |= dict(x=xv, w=wv)
+    want, tol = plain(xv, wv, tok, off, 1, act, N)
+    y32 = torch.full((n, N), float("nan"), device="cuda")
+    dense.GroupedMm(y=y32, **kw).run(stream())
+    close(y32, want, tol, F32)
+    gone = (tok < 0) | (torch.arange(n, device="cuda") < before) | (torch.arange(n, device="cuda") >= n - after)
+    assert not y32[gone].any()
+    for yd in (F16, BF16):
+        y = torch.full((n, N), float("nan"), dtype=yd, device="cuda")
+        dense.GroupedMm(y=y, **kw).run(stream())
+        assert torch.equal(y, y32.to(yd))
+    want_q, want_s = dense.mx4_empty(n, N)
+    dense.mx4_quantize(y32, want_q, want_s, stream())
+    q, s = torch.full_like(want_q, 0x11), torch.full((n, N // 32), 0x11, dtype=torch.uint8, device="cuda")
+    dense.GroupedMm(y=q, y_scales=s, **kw).run(stream())
+    assert torch.equal(s, want_s) and np.array_equal(decode(q, s), decode(want_q, want_s))
+
+
+@pytest.mark.parametrize("rows", [1, 63, 97, 1024, 2869, 4100])
+@pytest.mark.parametrize("N,act", [(248, "silu_mul"), (512, "none"), (1064, "none")])
+@pytest.mark.parametrize("dtype", [BF16, "mx4"])
+def test_one_expert_of_many_rows(rows, N, act, dtype):
+    """Where one expert's units would leave SMs without one, they are cut shorter."""
+    g, K = gen(rows), 416
+    x, w = randn(g, rows, K), randn(g, 1, N * (2 if act == "silu_mul" else 1), K) * K ** -0.5
+    if dtype == "mx4":
+        (x, xs, xv), (w, ws, wv) = mx4_of(x), mx4_of(w)
+        kw = dict(x_scales=xs, w_scales=dense.mx4_tile_scales(ws, act))
+    else:
+        x, w = x.to(BF16), w.to(BF16)
+        xv, wv, kw = x, w, {}
+    y = torch.full((rows, N), float("nan"), dtype=BF16, device="cuda")
+    dense.GroupedMm(x=x, w=w, y=y, act=act, **kw).run(stream())
+    every = torch.arange(rows, device="cuda", dtype=torch.int32)
+    want, tol = plain(xv, wv, every, torch.tensor([0, rows]), 0, act, N)
+    close(y, want, tol, BF16)
+
+
+@pytest.mark.parametrize("K", [32, 288, 544, 3808])
+@pytest.mark.parametrize("form", ["narrow", "pair"])
+@pytest.mark.parametrize("shift,extra", [(0, 0), (1, 0), (3, 2), (4, 4), (8, 8), (16, 5)])
+def test_scales_at_any_alignment(K, form, shift, extra):
+    """Row scales `shift` bytes behind a 16-byte boundary, `extra` between the rows, nothing behind the last: the same
+    bits as scales on 16-byte rows."""
+    counts, _, N = FORMS[form]
+    g = gen(K)
+    tok, off, n = routing(counts, g=g)
+    xq, xs, _ = mx4_of(randn(g, n, K))
+    wq, ws, _ = mx4_of(randn(g, len(counts), N, K))
+    kw = dict(x=xq, w=wq, w_scales=dense.mx4_tile_scales(ws), expert_offset=off, sorted_tok=tok, top_k=1)
+    want, y = (torch.full((n, N), float("nan"), dtype=BF16, device="cuda") for _ in range(2))
+    dense.GroupedMm(y=want, x_scales=xs, **kw).run(stream())
+    pitch = K // 32 + extra
+    flat = torch.full((shift + (n - 1) * pitch + K // 32,), 255, dtype=torch.uint8, device="cuda")
+    at = flat[shift:].as_strided((n, K // 32), (pitch, 1))
+    at.copy_(xs)
+    dense.GroupedMm(y=y, x_scales=at, **kw).run(stream())
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("form", ["split", "narrow", "pair"])
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_chain_waits_for_each_predecessor(form, graph):
+    """Norm, quantisation, two products and the way back, each reading what the last one wrote and the first overwriting
+    what the last reads, many times without a pause: the same bits as with a synchronisation after every call."""
+    counts, K, _ = FORMS[form]
+    H, W = K, 2 * K
+    g = gen(K)
+    tok, off, n = routing(counts, 3, 20, (5,), g=g)
+    w1, w2 = randn(g, len(counts), 2 * W, H) * H ** -0.5, randn(g, len(counts), H, W) * W ** -0.5
+    (q1, s1, _), w2 = mx4_of(w1), w2.to(BF16)
+    start, norm_w = randn(g, n, H, dtype=BF16), randn(g, H, dtype=BF16)
+    route = dict(expert_offset=off, sorted_tok=tok, top_k=1)
+    x, xn, h, branch = (torch.empty((n, c), dtype=BF16, device="cuda") for c in (H, H, W, H))
+    xq, xs = dense.mx4_empty(n, H)
+    pre = dense.BlockNorm(res=x, pre_w=norm_w, y=xn)
+    up = dense.GroupedMm(x=xq, x_scales=xs, w=q1, w_scales=dense.mx4_tile_scales(s1, "silu_mul"), y=h, act="silu_mul", **route)
+    down = dense.GroupedMm(x=h, w=w2, y=branch, expert_offset=off, sorted_tok=tok, top_k=0)
+    post = dense.BlockNorm(branch=branch, post_w=norm_w, res=x, res_scale=0.5, out=x)
+
+    def steps(st):
+        yield lambda: pre.run(st)
+        yield lambda: dense.mx4_quantize(xn, xq, xs, st)
+        yield lambda: up.run(st)
+        yield lambda: down.run(st)
+        yield lambda: dense.mx4_dequantize(xq, xs, xn, st)
+        yield lambda: post.run(st)
+
+    x.copy_(start)
+    for _ in range(12):
+        for call in steps(stream()):
+            call()
+            torch.cuda.synchronize()
+    want = [t.clone() for t in (x, xn, h, branch)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            x.copy_(start)
+            if graph:
+                captured = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(captured, stream=side):
+                    for _ in range(12):
+                        for call in steps(torch.cuda.current_stream().cuda_stream):
+                            call()
+                x.copy_(start)
+                captured.replay()
+            else:
+                for _ in range(12):
+                    for call in steps(side.cuda_stream):
+                        call()
+            side.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip((x, xn, h, branch), want))
