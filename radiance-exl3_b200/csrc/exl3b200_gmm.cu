@@ -1085,8 +1085,11 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     const int ctas = PAIR ? 2 : split;                        // of a cluster
     const int nt = PAIR ? pair_rows(p, C::NT, sm_count) : C::NT;
     const int64_t most = most_units(p, nt, PAIR ? 2 : 1);
-    // few units: one CTA an SM, with the whole of its shared memory for stages in flight
-    const int per_sm = !PAIR && most * ctas <= sm_count ? 1 : C::PER_SM;
+    // few units: one CTA an SM, with the whole of its shared memory for stages in flight; clusters of three or four do not
+    // fill the SMs of every processing cluster, and such that found no room would wait for the others (48 units in three
+    // parts: 15.8 us with one CTA an SM, 9.7 with two)
+    const int64_t alone = ctas > 2 ? sm_count - sm_count / 8 : sm_count;
+    const int per_sm = !PAIR && most * ctas <= alone ? 1 : C::PER_SM;
     const int64_t room = (int64_t)sm_count * per_sm / ctas;
     const int stages = C::stages(p->n_expert, per_sm);
     const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
