@@ -36,7 +36,7 @@
 //   512 experts, 191 live of 624 rows, 640 -> 2560, bf16 (narrow)           96 us  6.6 TB/s: the weights' bytes
 //   512 experts, 418 live of 20072 rows, 2048 -> 512 silu_mul, f16 (PAIR)  278 us  6.4 TB/s: the weights' bytes
 //   16 experts of 16060 rows, 1536 -> 4096, bf16 (PAIR)                    153 us  1323 TFLOP/s: a stage of 256 x 256 x 64 in
-//     490 to 500 cycles, the MMA's own 512 at full rate, at a clock that power brings down to 1.2 .. 1.5 GHz
+//     about 510 cycles, the MMAs' own time at full rate, at a clock that power brings down to 1.2 .. 1.5 GHz
 //   16 experts of 16060 rows, 4096 -> 1536, MXFP4 (PAIR)                    54 us  3743 TFLOP/s: a stage of 33 KB a CTA in
 //     ~650 cycles where its MMAs take ~450: L2's rate, 13 TB/s over the GPU; seven units a pair at most where 6.5 would do
 //   64 experts of 20072 rows, 2048 -> 512 silu_mul, MXFP4 (PAIR)            31 us  2735 TFLOP/s: the same, 29 KB in ~560
