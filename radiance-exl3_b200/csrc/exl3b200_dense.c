@@ -21,6 +21,9 @@ int exl3b_cuda_device_info(int* sm_count, int32_t** err_word);
 /* Largest sizes taken: rows and columns that 32-bit coordinates hold, norm rows that a block holds in registers. */
 static const int64_t kMaxDim = (int64_t)1 << 30;
 static const int64_t kMaxNormCols = 32768;
+/* A product's n_in: its byte offsets along k, and those of the scales' tiles (1 KB each 256 columns), stay in 32 bits, and
+ * the stages of one unit's k (a million at 16 bits) inside the 2 s after which a wait for its sums gives up. */
+static const int64_t kMaxIn = (int64_t)1 << 26;
 
 static int is_float(int dt) { return dt == RAD_F32 || dt == RAD_F16 || dt == RAD_BF16; }
 static int64_t size_of(int dt) { return dt == RAD_F32 ? 4 : 2; }
@@ -153,7 +156,7 @@ int exl3b200_grouped_mm(const Exl3bGroupedMm* d, void* stream) {
     if (d->act != EXL3B_ACT_NONE && d->act != EXL3B_ACT_SILU_MUL) return RAD_E_INVAL;
     if (d->n_expert < 1 || d->n_expert > exl3b_gmm_max_expert() || d->n_rows < 0 || d->n_rows > kMaxDim ||
         d->x_rows < 0 || d->x_rows > kMaxDim || d->top_k < 0 || d->top_k > 4096 || d->n_out < 8 || d->n_out % 8 ||
-        d->n_out > kMaxDim / 2 || d->n_in < 8 || d->n_in > kMaxDim || d->n_in % (mx ? 32 : 8) ||
+        d->n_out > kMaxDim / 2 || d->n_in < 8 || d->n_in > kMaxIn || d->n_in % (mx ? 32 : 8) ||
         (mx_out && d->n_out % 32))
         return RAD_E_SHAPE;
     if (d->n_rows == 0) return RAD_OK;

@@ -1,0 +1,58 @@
+"""The dense and MXFP4 expert operators where they can go wrong at their edges: the longest k."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from exl3b200 import dense  # noqa: E402
+from test_dense import gen, stream  # noqa: E402
+
+F16 = torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.set_device(0)
+    yield
+    torch.cuda.synchronize()
+    assert dense.native().read_error() == 0
+
+
+def places(K):
+    """Columns at the first and last stages of k, around the middle, and at the row's two ends."""
+    at = [0, 1, 255, 256, K // 2 - 1, K // 2, K - 257, K - 256, K - 65, K - 64, K - 1]
+    return torch.tensor(sorted(set(at)), device="cuda")
+
+
+@pytest.mark.parametrize("K", [1 << 26, (1 << 26) - 8, (1 << 26) - 200])
+def test_the_longest_k_16_bit(K):
+    """A row of zeros but for a few small whole numbers, times small whole numbers: the sum is exact in f32."""
+    g, at = gen(1), places(K)
+    w = torch.randint(-8, 9, (1, 8, K), generator=g, device="cuda", dtype=torch.int8).to(F16)
+    x = torch.zeros((1, K), dtype=F16, device="cuda")
+    x[0, at] = torch.arange(1, len(at) + 1, device="cuda").to(F16)
+    y = torch.empty((1, 8), device="cuda")
+    dense.GroupedMm(x=x, w=w, y=y).run(stream())
+    assert torch.equal(y[0].double(), w[0][:, at].double() @ x[0, at].double())
+
+
+@pytest.mark.parametrize("K", [1 << 26, (1 << 26) - 32])
+def test_the_longest_k_mxfp4(K):
+    """The same in MXFP4, every block with a scale of its own: values of two bits times powers of two within 2^8 of one
+    another, a dozen of them, are exact in f32."""
+    g, at = gen(2), places(K)
+    wq = torch.randint(0, 256, (1, 8, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    ws = torch.randint(124, 129, (1, 8, K // 32), generator=g, device="cuda", dtype=torch.uint8)
+    xq, xs = dense.mx4_empty(1, K)
+    xq.zero_()
+    xs.copy_(torch.randint(125, 130, (1, K // 32), generator=g, device="cuda", dtype=torch.uint8))
+    for c in at.tolist():
+        xq[0, c // 2] |= 2 << (4 * (c & 1))                  # the code of 1
+    y = torch.empty((1, 8), device="cuda")
+    dense.GroupedMm(x=xq, x_scales=xs, w=wq, w_scales=dense.mx4_tile_scales(ws, stream=stream()), y=y).run(stream())
+    grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64, device="cuda")
+    codes = (wq[0][:, at // 2].int() >> (4 * (at & 1))) & 15
+    e = ws[0][:, at // 32].double() - 127 + xs[0, at // 32].double() - 127
+    assert torch.equal(y[0].double(), (grid[codes] * torch.exp2(e)).sum(1))
