@@ -1,13 +1,15 @@
-"""The dense and MXFP4 expert operators where they can go wrong at their edges: the longest k."""
+"""The dense and MXFP4 expert operators where they can go wrong at their edges: the longest k, calls in which no expert has
+a row."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from exl3b200 import dense  # noqa: E402
-from test_dense import gen, stream  # noqa: E402
+from test_dense import decode, gen, mx4_of, randn, stream  # noqa: E402
 
-F16 = torch.float16
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -56,3 +58,29 @@ def test_the_longest_k_mxfp4(K):
     codes = (wq[0][:, at // 2].int() >> (4 * (at & 1))) & 15
     e = ws[0][:, at // 32].double() - 127 + xs[0, at // 32].double() - 127
     assert torch.equal(y[0].double(), (grid[codes] * torch.exp2(e)).sum(1))
+
+
+@pytest.mark.parametrize("dtype", [BF16, "mx4"])
+@pytest.mark.parametrize("E,n,N", [(5, 1, 264), (5, 40, 264), (3, 900, 1056)])
+@pytest.mark.parametrize("start", [0, 1])
+def test_no_expert_has_a_row(dtype, E, n, N, start):
+    """Every offset the same (nothing routed here), in the split, narrow and pair forms: all rows are zero."""
+    g, K = gen(E + n), 512
+    x, w = randn(g, n, K), randn(g, E, N, K)
+    off = torch.full((E + 1,), start, dtype=torch.int32, device="cuda")
+    tok = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    kw = dict(expert_offset=off, sorted_tok=tok, top_k=1)
+    if dtype == "mx4":
+        (x, xs, _), (w, ws, _) = mx4_of(x), mx4_of(w)
+        kw |= dict(x_scales=xs, w_scales=dense.mx4_tile_scales(ws, stream=stream()))
+    else:
+        x, w = x.to(dtype), w.to(dtype)
+    y = torch.full((n, N), float("nan"), dtype=BF16, device="cuda")
+    dense.GroupedMm(x=x, w=w, y=y, **kw).run(stream())
+    assert torch.equal(y, torch.zeros_like(y))
+    if N % 32 == 0:
+        q, s = dense.mx4_empty(n, N)
+        q.fill_(0x11)
+        s.fill_(0x11)
+        dense.GroupedMm(x=x, w=w, y=q, y_scales=s, **kw).run(stream())
+        assert not q.any() and not s.any() and not np.any(decode(q, s))
