@@ -3,7 +3,8 @@ tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (inc
 
 A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
 `run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). The tensors' contents may
-change between runs, their addresses may not. torch only holds memory here; every refusal is the library's own status,
+change between runs, their addresses may not. A call's tensors share one GPU, which is the current device when it runs.
+torch only holds memory here; every refusal is the library's own status,
 raised. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
 import ctypes as C
 
@@ -33,12 +34,27 @@ def _dtype(t):
     return dt
 
 
-def _rows(t, name, shape=None, dtype=None):
-    """A tensor whose last dimension is dense, on a GPU, of this shape and type: (address, row pitch in elements)."""
+def _gpu(t, name):
+    """The GPU that a call's first tensor is on; the others have to share it."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name} is not on a GPU")
+    return dev
+
+
+def _check_current(dev):
+    """The library launches on the current device: a call's tensors have to be there."""
+    if torch.cuda.current_device() != dev:
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _rows(t, name, dev, shape=None, dtype=None):
+    """A tensor whose last dimension is dense, on GPU dev, of this shape and type: (address, row pitch in elements)."""
     have, st = t.shape, t.stride()
-    if not (t.is_cuda and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
+    if not (t.get_device() == dev and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
             and (st[-1] == 1 or have[-1] <= 1)):
-        what = ("is not on a GPU" if not t.is_cuda else f"is {t.dtype}, not {dtype}" if dtype not in (None, t.dtype) else
+        what = (f"is on {t.device}, not cuda:{dev}" if t.get_device() != dev else
+                f"is {t.dtype}, not {dtype}" if dtype not in (None, t.dtype) else
                 f"has shape {tuple(have)}, not {tuple(shape)}" if shape is not None and have != shape else
                 "has a strided last dimension")
         raise ValueError(f"{name} {what}")
@@ -58,9 +74,11 @@ def mx4_empty(rows, cols, device="cuda"):
 def mx4_quantize(x, codes, scales, stream=0):
     """x [rows, cols] in f32, f16 or bf16 -> its MXFP4 codes and scales."""
     rows, cols = x.shape
-    xp, pitch = _rows(x, "x")
-    cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
-    sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
+    dev = _gpu(x, "x")
+    xp, pitch = _rows(x, "x", dev)
+    cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
+    sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
+    _check_current(dev)
     rc = native().lib.exl3b200_mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch, stream)
     if rc:
         raise RuntimeError(f"exl3b200_mx4_quantize: status {rc}")
@@ -70,9 +88,11 @@ def mx4_quantize(x, codes, scales, stream=0):
 def mx4_dequantize(codes, scales, y, stream=0):
     """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
     rows, cols = y.shape
-    yp, pitch = _rows(y, "y")
-    cp, c_pitch = _rows(codes, "codes", (rows, cols // 2), torch.uint8)
-    sp, s_pitch = _rows(scales, "scales", (rows, cols // 32), torch.uint8)
+    dev = _gpu(y, "y")
+    yp, pitch = _rows(y, "y", dev)
+    cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
+    sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
+    _check_current(dev)
     rc = native().lib.exl3b200_mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch, stream)
     if rc:
         raise RuntimeError(f"exl3b200_mx4_dequantize: status {rc}")
@@ -83,7 +103,9 @@ def mx4_tile_scales(scales, act="none", stream=None):
     """A weight's scales [experts, rows, cols / 32] in the form GroupedMm reads; once, when the weight is loaded. On the
     current stream unless another is given."""
     n_expert, rows, blocks = scales.shape
-    sp, pitch = _rows(scales, "scales", dtype=torch.uint8)
+    dev = _gpu(scales, "scales")
+    sp, pitch = _rows(scales, "scales", dev, dtype=torch.uint8)
+    _check_current(dev)
     out = torch.empty(native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act]), dtype=torch.uint8,
                       device=scales.device)
     if stream is None:
@@ -96,11 +118,12 @@ def mx4_tile_scales(scales, act="none", stream=None):
 class _Plan:
     _entry = None
 
-    def _finish(self, desc, *tensors):
-        self.desc, self._keep = desc, tensors
+    def _finish(self, desc, dev, *tensors):
+        self.desc, self._dev, self._keep = desc, dev, tensors
         self._addr, self._call = C.addressof(desc), getattr(native().lib, self._entry)
 
     def run(self, stream=0):
+        _check_current(self._dev)
         rc = self._call(self._addr, stream)
         if rc:
             raise RuntimeError(f"{self._entry}: status {rc}")
@@ -123,27 +146,28 @@ class GroupedMm(_Plan):
         per, per_out = 2 if mx else 1, 2 if mx_out else 1
         if x.dtype != w.dtype:
             raise ValueError(f"x is {x.dtype}, w {w.dtype}")
+        dev = _gpu(x, "x")
         d.n_expert, d.n_rows, d.x_rows, d.top_k = w.shape[0], y.shape[0], x.shape[0], top_k
         d.n_out, d.n_in, d.act = y.shape[1] * per_out, x.shape[1] * per, ACTS[act]
         d.dtype, d.y_dtype = MX4 if mx else _dtype(x), MX4 if mx_out else _dtype(y)
-        _rows(w, "w", (d.n_expert, d.n_out * (2 if d.act else 1), x.shape[1]))
-        d.x, pitch = _rows(x, "x")
+        _rows(w, "w", dev, (d.n_expert, d.n_out * (2 if d.act else 1), x.shape[1]))
+        d.x, pitch = _rows(x, "x", dev)
         d.x_pitch = pitch * per
-        d.w, pitch = _rows(w, "w")
+        d.w, pitch = _rows(w, "w", dev)
         d.w_pitch, d.w_expert_pitch = pitch * per, w.stride(0) * per
-        d.y, pitch = _rows(y, "y")
+        d.y, pitch = _rows(y, "y", dev)
         d.y_pitch = pitch * per_out
         if mx:
-            d.x_scales, d.x_scales_pitch = _rows(x_scales, "x_scales", (d.x_rows, d.n_in // 32), torch.uint8)
+            d.x_scales, d.x_scales_pitch = _rows(x_scales, "x_scales", dev, (d.x_rows, d.n_in // 32), torch.uint8)
             want = native().mx4_tiled_bytes(d.n_expert, w.shape[1], d.n_in, d.act)
-            d.w_scales, _ = _rows(w_scales, "w_scales", (want,), torch.uint8)
+            d.w_scales, _ = _rows(w_scales, "w_scales", dev, (want,), torch.uint8)
         if mx_out:
-            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", (d.n_rows, d.n_out // 32), torch.uint8)
+            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", dev, (d.n_rows, d.n_out // 32), torch.uint8)
         if expert_offset is not None:
-            d.expert_offset, _ = _rows(expert_offset, "expert_offset", (d.n_expert + 1,), torch.int32)
+            d.expert_offset, _ = _rows(expert_offset, "expert_offset", dev, (d.n_expert + 1,), torch.int32)
         if sorted_tok is not None:
-            d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", (d.n_rows,), torch.int32)
-        self._finish(d, x, w, y, expert_offset, sorted_tok, x_scales, w_scales, y_scales)
+            d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", dev, (d.n_rows,), torch.int32)
+        self._finish(d, dev, x, w, y, expert_offset, sorted_tok, x_scales, w_scales, y_scales)
 
 
 class BlockNorm(_Plan):
@@ -160,30 +184,31 @@ class BlockNorm(_Plan):
         if lead is None:
             raise ValueError("neither branch nor res")
         rows, cols = d.rows, d.cols = lead.shape
+        dev = _gpu(lead, "branch" if branch is not None else "res")
         typed = next((t for t in (res, out, y, post_w, pre_w) if t is not None), lead)
         dt = typed.dtype
         d.dtype, d.gate_kind = _dtype(typed), GATES[gate_kind]
         d.res_scale, d.post_eps, d.pre_eps = res_scale, post_eps, pre_eps
         if branch is not None:
-            d.branch, d.branch_pitch = _rows(branch, "branch", (rows, cols))
+            d.branch, d.branch_pitch = _rows(branch, "branch", dev, (rows, cols))
             d.branch_dtype = _dtype(branch)
         for name, t in (("res", res), ("out", out), ("y", y)):
             if t is not None:
-                p, pitch = _rows(t, name, (rows, cols), dt)
+                p, pitch = _rows(t, name, dev, (rows, cols), dt)
                 setattr(d, name, p)
                 setattr(d, name + "_pitch", pitch)
         for name, t in (("post_w", post_w), ("pre_w", pre_w)):
             if t is not None:
-                setattr(d, name, _rows(t, name, (cols,), dt)[0])
+                setattr(d, name, _rows(t, name, dev, (cols,), dt)[0])
         if gate is not None:
             shape, want = {"token": ((rows,), torch.float32), "channel": ((cols,), dt),
                            "element": ((rows, cols), dt)}.get(gate_kind, (None, None))
-            d.gate, d.gate_pitch = _rows(gate, "gate", shape, want)
+            d.gate, d.gate_pitch = _rows(gate, "gate", dev, shape, want)
         if y_codes is not None:
-            d.y_codes, d.y_codes_pitch = _rows(y_codes, "y_codes", (rows, cols // 2), torch.uint8)
+            d.y_codes, d.y_codes_pitch = _rows(y_codes, "y_codes", dev, (rows, cols // 2), torch.uint8)
         if y_scales is not None:
-            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", (rows, cols // 32), torch.uint8)
-        self._finish(d, branch, post_w, gate, res, out, pre_w, y, y_codes, y_scales)
+            d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", dev, (rows, cols // 32), torch.uint8)
+        self._finish(d, dev, branch, post_w, gate, res, out, pre_w, y, y_codes, y_scales)
 
 
 # ------------------------------------------------------------------------------------------------ the block
@@ -198,6 +223,7 @@ class ExpertBlock:
     def __init__(self, *, router_w, gu_w, dn_w, pre_w, post_w=None, gate=None, next_w=None, gu_scales=None, dn_scales=None,
                  top_k, eps=1e-6, res_scale=1.0, max_tokens=2048):
         E, H = router_w.shape
+        dev = self._dev = _gpu(router_w, "router_w")
         mx = gu_w.dtype == torch.uint8
         per, dt = 2 if mx else 1, router_w.dtype
         W = dn_w.shape[2] * per
@@ -212,10 +238,10 @@ class ExpertBlock:
             if t is not None:
                 if not t.is_contiguous():
                     raise ValueError(f"{name} is strided")
-                setattr(d, name, _rows(t, name, shape, kind)[0])
+                setattr(d, name, _rows(t, name, dev, shape, kind)[0])
         if mx:
-            _rows(gu_scales, "gu_scales", (E, 2 * W, H // 32), torch.uint8)
-            _rows(dn_scales, "dn_scales", (E, H, W // 32), torch.uint8)
+            _rows(gu_scales, "gu_scales", dev, (E, 2 * W, H // 32), torch.uint8)
+            _rows(dn_scales, "dn_scales", dev, (E, H, W // 32), torch.uint8)
             keep += [mx4_tile_scales(gu_scales, "silu_mul"), mx4_tile_scales(dn_scales)]
             d.gu_scales, d.dn_scales = keep[-2].data_ptr(), keep[-1].data_ptr()
         self._keep, self.dtype, self.hidden, self.max_tokens = keep, dt, H, max_tokens
@@ -228,9 +254,10 @@ class ExpertBlock:
         T = x.shape[0]
         for name, t in (("x", x), ("out", out), ("next_out", next_out)):
             if t is not None:
-                _rows(t, name, (T, self.hidden), self.dtype)
+                _rows(t, name, self._dev, (T, self.hidden), self.dtype)
                 if not t.is_contiguous():
                     raise ValueError(f"{name} is strided")
+        _check_current(self._dev)
         native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
                                       next_out.data_ptr() if next_out is not None else None, stream)
         return out

@@ -1,0 +1,123 @@
+"""What exl3b200/dense.py refuses before it calls the library, over stand-ins for tensors: no GPU, none of them is read."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from exl3b200 import dense  # noqa: E402
+
+F32, F16, BF16, U8, I32 = torch.float32, torch.float16, torch.bfloat16, torch.uint8, torch.int32
+
+
+class Fake:
+    """As much of a dense tensor on GPU `dev` (-1: on the CPU) as a plan asks for."""
+
+    def __init__(self, *shape, dtype=BF16, dev=0):
+        self.shape, self.dtype, self.dev = torch.Size(shape), dtype, dev
+        self.is_cuda, self.device = dev >= 0, torch.device("cuda", dev) if dev >= 0 else torch.device("cpu")
+
+    def get_device(self):
+        return self.dev
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, d=None):
+        st, n = [], 1
+        for s in reversed(self.shape):
+            st.insert(0, n)
+            n *= s
+        return tuple(st) if d is None else st[d]
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 4096
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The calls that reach the library, which is not called; the current device is GPU 0."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a[-1])) or 0
+
+    class Host:
+        lib = Lib()
+
+        def mx4_tiled_bytes(self, *a):
+            return 4096
+
+    monkeypatch.setattr(dense, "_native", Host())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    return calls
+
+
+def grouped(**k):
+    t = dict(x=Fake(4, 64), w=Fake(2, 32, 64), y=Fake(4, 32), expert_offset=Fake(3, dtype=I32), sorted_tok=Fake(4, dtype=I32),
+             top_k=1)
+    return dense.GroupedMm(**dict(t, **k))
+
+
+def grouped_mx4(**k):
+    t = dict(x=Fake(4, 32, dtype=U8), x_scales=Fake(4, 2, dtype=U8), w=Fake(2, 32, 32, dtype=U8), w_scales=Fake(4096, dtype=U8),
+             y=Fake(4, 16, dtype=U8), y_scales=Fake(4, 1, dtype=U8), expert_offset=Fake(3, dtype=I32))
+    return dense.GroupedMm(**dict(t, **k))
+
+
+def norm(**k):
+    t = dict(branch=Fake(4, 64), post_w=Fake(64), gate=Fake(64), gate_kind="channel", res=Fake(4, 64), out=Fake(4, 64),
+             pre_w=Fake(64), y=Fake(4, 64), y_codes=Fake(4, 32, dtype=U8), y_scales=Fake(4, 2, dtype=U8))
+    return dense.BlockNorm(**dict(t, **k))
+
+
+OTHER = {grouped: ("x", "w", "y", "expert_offset", "sorted_tok"), grouped_mx4: ("x_scales", "w_scales", "y_scales"),
+         norm: ("branch", "post_w", "gate", "res", "out", "pre_w", "y", "y_codes", "y_scales")}
+
+
+@pytest.mark.parametrize("make,name", [(m, n) for m, names in OTHER.items() for n in names])
+@pytest.mark.parametrize("dev", [-1, 1])
+def test_a_plans_tensors_share_a_gpu(launched, make, name, dev):
+    base = {"x": Fake(4, 64), "w": Fake(2, 32, 64), "y": Fake(4, 32), "expert_offset": Fake(3, dtype=I32),
+            "sorted_tok": Fake(4, dtype=I32)}
+    if make is grouped_mx4:
+        base = {"x_scales": Fake(4, 2, dtype=U8), "w_scales": Fake(4096, dtype=U8), "y_scales": Fake(4, 1, dtype=U8)}
+    if make is norm:
+        base = {n: Fake(4, 64) for n in ("branch", "res", "out", "y")} | {n: Fake(64) for n in ("post_w", "gate", "pre_w")} | {
+            "y_codes": Fake(4, 32, dtype=U8), "y_scales": Fake(4, 2, dtype=U8)}
+    t = base[name]
+    make(**{name: t}).run(0)
+    assert len(launched) == 1
+    with pytest.raises(ValueError, match="GPU|cuda"):
+        make(**{name: Fake(*t.shape, dtype=t.dtype, dev=dev)}).run(0)
+    assert len(launched) == 1
+
+
+@pytest.mark.parametrize("make", [grouped, grouped_mx4, norm])
+def test_a_plan_runs_on_its_own_gpu_only(launched, monkeypatch, make):
+    plan = make()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ValueError, match="cuda:0"):
+        plan.run(0)
+    assert not launched
+
+
+def test_the_conversions_tensors_share_the_current_gpu(launched, monkeypatch):
+    x, codes, scales = Fake(4, 64), Fake(4, 32, dtype=U8), Fake(4, 2, dtype=U8)
+    dense.mx4_quantize(x, codes, scales, 0)
+    dense.mx4_dequantize(codes, scales, x, 0)
+    assert len(launched) == 2
+    for bad in ((Fake(4, 64, dev=1), codes, scales), (x, Fake(4, 32, dtype=U8, dev=1), scales),
+                (x, codes, Fake(4, 2, dtype=U8, dev=1)), (x, codes, Fake(4, 2, dtype=U8, dev=-1))):
+        with pytest.raises(ValueError):
+            dense.mx4_quantize(*bad, 0)
+        with pytest.raises(ValueError):
+            dense.mx4_dequantize(bad[1], bad[2], bad[0], 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: dense.mx4_quantize(x, codes, scales, 0), lambda: dense.mx4_dequantize(codes, scales, x, 0),
+                 lambda: dense.mx4_tile_scales(Fake(2, 32, 2, dtype=U8), stream=0)):
+        with pytest.raises(ValueError):
+            call()
+    assert len(launched) == 2
