@@ -4,8 +4,8 @@ tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (inc
 A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
 `run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). The tensors' contents may
 change between runs, their addresses may not. A call's tensors share one GPU, which is the current device when it runs.
-torch only holds memory here; every refusal is the library's own status,
-raised. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
+torch only holds memory here. Tensors that do not fit one another are a ValueError; what the library refuses is a
+RuntimeError with its status. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
 import ctypes as C
 
 import torch
@@ -50,6 +50,8 @@ def _check_current(dev):
 
 def _rows(t, name, dev, shape=None, dtype=None):
     """A tensor whose last dimension is dense, on GPU dev, of this shape and type: (address, row pitch in elements)."""
+    if t is None:
+        raise ValueError(f"{name} is missing")
     have, st = t.shape, t.stride()
     if not (t.get_device() == dev and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
             and (st[-1] == 1 or have[-1] <= 1)):

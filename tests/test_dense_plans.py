@@ -121,3 +121,17 @@ def test_the_conversions_tensors_share_the_current_gpu(launched, monkeypatch):
         with pytest.raises(ValueError):
             call()
     assert len(launched) == 2
+
+
+@pytest.mark.parametrize("make,missing", [(grouped_mx4, "x_scales"), (grouped_mx4, "w_scales"), (grouped_mx4, "y_scales")])
+def test_mxfp4_without_its_scales(launched, make, missing):
+    with pytest.raises(ValueError, match=missing):
+        make(**{missing: None})
+
+
+@pytest.mark.parametrize("gu,dn", [(False, True), (True, False)])
+def test_an_mxfp4_block_without_its_scales(launched, gu, dn):
+    U = lambda *s: Fake(*s, dtype=U8)  # noqa: E731
+    with pytest.raises(ValueError, match="dn_scales" if gu else "gu_scales"):
+        dense.ExpertBlock(router_w=Fake(8, 64), gu_w=U(8, 128, 32), dn_w=U(8, 64, 32), pre_w=Fake(64), top_k=2,
+                          gu_scales=U(8, 128, 2) if gu else None, dn_scales=U(8, 64, 2) if dn else None)
