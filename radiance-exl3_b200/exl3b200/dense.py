@@ -148,6 +148,8 @@ class GroupedMm(_Plan):
         per, per_out = 2 if mx else 1, 2 if mx_out else 1
         if x.dtype != w.dtype:
             raise ValueError(f"x is {x.dtype}, w {w.dtype}")
+        if (x.dim(), w.dim(), y.dim()) != (2, 3, 2):
+            raise ValueError(f"x, w and y have {x.dim()}, {w.dim()} and {y.dim()} dimensions, not 2, 3 and 2")
         dev = _gpu(x, "x")
         d.n_expert, d.n_rows, d.x_rows, d.top_k = w.shape[0], y.shape[0], x.shape[0], top_k
         d.n_out, d.n_in, d.act = y.shape[1] * per_out, x.shape[1] * per, ACTS[act]

@@ -135,3 +135,20 @@ def test_an_mxfp4_block_without_its_scales(launched, gu, dn):
     with pytest.raises(ValueError, match="dn_scales" if gu else "gu_scales"):
         dense.ExpertBlock(router_w=Fake(8, 64), gu_w=U(8, 128, 32), dn_w=U(8, 64, 32), pre_w=Fake(64), top_k=2,
                           gu_scales=U(8, 128, 2) if gu else None, dn_scales=U(8, 64, 2) if dn else None)
+
+
+@pytest.mark.parametrize("name,shape", [("x", (4, 64, 72)), ("x", (64,)), ("y", (4, 32, 40)), ("y", (32,)), ("w", (32, 64)),
+                                        ("w", (2, 32, 64, 8))])
+def test_grouped_mm_wants_matrices(launched, name, shape):
+    """Rows of a third dimension were taken for rows of the second one's length."""
+    with pytest.raises(ValueError):
+        grouped(**{name: Fake(*shape)})
+
+
+@pytest.mark.parametrize("shape", [(4, 64, 72), (64,)])
+def test_norms_and_conversions_want_matrices(launched, shape):
+    with pytest.raises(ValueError):
+        norm(branch=Fake(*shape))
+    with pytest.raises(ValueError):
+        dense.mx4_quantize(Fake(*shape), Fake(4, 32, dtype=U8), Fake(4, 2, dtype=U8), 0)
+    assert not launched
