@@ -2,8 +2,9 @@
 tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (include/exl3b200.h).
 
 A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
-`run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). The tensors' contents may
-change between runs, their addresses may not. A call's tensors share one GPU, which is the current device when it runs.
+`run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). Every entry's default is torch's
+current stream. The tensors' contents may change between runs, their addresses may not. A call's tensors share one GPU, which
+is the current device when it runs.
 torch only holds memory here. Tensors that do not fit one another are a ValueError; what the library refuses is a
 RuntimeError with its status. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
 import ctypes as C
@@ -48,6 +49,10 @@ def _check_current(dev):
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _stream(stream, dev):
+    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+
+
 def _rows(t, name, dev, shape=None, dtype=None):
     """A tensor whose last dimension is dense, on GPU dev, of this shape and type: (address, row pitch in elements)."""
     if t is None:
@@ -73,7 +78,7 @@ def mx4_empty(rows, cols, device="cuda"):
             torch.empty((rows, (cols // 32 + 15) // 16 * 16), dtype=torch.uint8, device=device)[:, :cols // 32])
 
 
-def mx4_quantize(x, codes, scales, stream=0):
+def mx4_quantize(x, codes, scales, stream=None):
     """x [rows, cols] in f32, f16 or bf16 -> its MXFP4 codes and scales."""
     rows, cols = x.shape
     dev = _gpu(x, "x")
@@ -81,13 +86,14 @@ def mx4_quantize(x, codes, scales, stream=0):
     cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
     _check_current(dev)
-    rc = native().lib.exl3b200_mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch, stream)
+    rc = native().lib.exl3b200_mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch,
+                                           _stream(stream, dev))
     if rc:
         raise RuntimeError(f"exl3b200_mx4_quantize: status {rc}")
     return codes, scales
 
 
-def mx4_dequantize(codes, scales, y, stream=0):
+def mx4_dequantize(codes, scales, y, stream=None):
     """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
     rows, cols = y.shape
     dev = _gpu(y, "y")
@@ -95,24 +101,23 @@ def mx4_dequantize(codes, scales, y, stream=0):
     cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
     _check_current(dev)
-    rc = native().lib.exl3b200_mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch, stream)
+    rc = native().lib.exl3b200_mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch,
+                                             _stream(stream, dev))
     if rc:
         raise RuntimeError(f"exl3b200_mx4_dequantize: status {rc}")
     return y
 
 
 def mx4_tile_scales(scales, act="none", stream=None):
-    """A weight's scales [experts, rows, cols / 32] in the form GroupedMm reads; once, when the weight is loaded. On the
-    current stream unless another is given."""
+    """A weight's scales [experts, rows, cols / 32] in the form GroupedMm reads; once, when the weight is loaded."""
     n_expert, rows, blocks = scales.shape
     dev = _gpu(scales, "scales")
     sp, pitch = _rows(scales, "scales", dev, dtype=torch.uint8)
     _check_current(dev)
     out = torch.empty(native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act]), dtype=torch.uint8,
                       device=scales.device)
-    if stream is None:
-        stream = torch.cuda.current_stream(scales.device).cuda_stream
-    native().mx4_tile_scales(sp, pitch, scales.stride(0), n_expert, rows, blocks * 32, ACTS[act], out.data_ptr(), stream)
+    native().mx4_tile_scales(sp, pitch, scales.stride(0), n_expert, rows, blocks * 32, ACTS[act], out.data_ptr(),
+                             _stream(stream, dev))
     return out
 
 
@@ -124,9 +129,9 @@ class _Plan:
         self.desc, self._dev, self._keep = desc, dev, tensors
         self._addr, self._call = C.addressof(desc), getattr(native().lib, self._entry)
 
-    def run(self, stream=0):
+    def run(self, stream=None):
         _check_current(self._dev)
-        rc = self._call(self._addr, stream)
+        rc = self._call(self._addr, _stream(stream, self._dev))
         if rc:
             raise RuntimeError(f"{self._entry}: status {rc}")
 
@@ -222,7 +227,10 @@ class ExpertBlock:
 
     router_w [experts, hidden] in f16 or bf16 sets the stream's type, which pre_w, post_w, gate (a scale a channel) and
     next_w [hidden] share. gu_w [experts, 2 width, hidden] and dn_w [experts, hidden, width] are of that type, or uint8
-    MXFP4 codes with gu_scales and dn_scales [experts, rows, cols / 32] (tiled here, once)."""
+    MXFP4 codes with gu_scales and dn_scales [experts, rows, cols / 32] (tiled here, once).
+
+    A block has one work buffer: its forwards run one after another, on one stream or on streams that wait for each other,
+    and it is kept until they are done."""
 
     def __init__(self, *, router_w, gu_w, dn_w, pre_w, post_w=None, gate=None, next_w=None, gu_scales=None, dn_scales=None,
                  top_k, eps=1e-6, res_scale=1.0, max_tokens=2048):
@@ -252,8 +260,10 @@ class ExpertBlock:
         n = native().expert_block_work_bytes(d, max_tokens)
         self.work = torch.empty(n, dtype=torch.uint8, device=router_w.device)
         self.bufs = native().expert_block_carve(d, max_tokens, self.work.data_ptr(), n)
+        # a forward may come on any stream: the tiling is done by then, and whatever used the work buffer's memory before
+        torch.cuda.current_stream(dev).synchronize()
 
-    def forward(self, x, out, next_out=None, stream=0):
+    def forward(self, x, out, next_out=None, stream=None):
         """x [T, hidden] through the block into out (which may be x); next_out: the next block's normed input."""
         T = x.shape[0]
         for name, t in (("x", x), ("out", out), ("next_out", next_out)):
@@ -263,5 +273,5 @@ class ExpertBlock:
                     raise ValueError(f"{name} is strided")
         _check_current(self._dev)
         native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
-                                      next_out.data_ptr() if next_out is not None else None, stream)
+                                      next_out.data_ptr() if next_out is not None else None, _stream(stream, self._dev))
         return out

@@ -37,21 +37,36 @@ class Fake:
 
 @pytest.fixture
 def launched(monkeypatch):
-    """The calls that reach the library, which is not called; the current device is GPU 0."""
+    """The calls that reach the library, which is not called, and their streams; the current device is GPU 0, its current
+    stream 77."""
     calls = []
 
     class Lib:
         def __getattr__(self, name):
             return lambda *a: calls.append((name, a[-1])) or 0
 
-    class Host:
+    class Host(Lib):
         lib = Lib()
 
         def mx4_tiled_bytes(self, *a):
             return 4096
 
+        def expert_block_work_bytes(self, *a):
+            return 4096
+
+        def expert_block_carve(self, *a):
+            pass
+
+    class Stream:
+        cuda_stream = 77
+
+        def synchronize(self):
+            calls.append(("synchronize", 77))
+
     monkeypatch.setattr(dense, "_native", Host())
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: Stream())
+    monkeypatch.setattr(torch, "empty", lambda n, dtype=None, device=None: Fake(n, dtype=dtype))
     return calls
 
 
@@ -152,3 +167,33 @@ def test_norms_and_conversions_want_matrices(launched, shape):
     with pytest.raises(ValueError):
         dense.mx4_quantize(Fake(*shape), Fake(4, 32, dtype=U8), Fake(4, 2, dtype=U8), 0)
     assert not launched
+
+
+def block():
+    U = lambda *s: Fake(*s, dtype=U8)  # noqa: E731
+    return dense.ExpertBlock(router_w=Fake(8, 64), gu_w=U(8, 128, 32), dn_w=U(8, 64, 32), pre_w=Fake(64), top_k=2,
+                             gu_scales=U(8, 128, 2), dn_scales=U(8, 64, 2))
+
+
+@pytest.mark.parametrize("given", [None, 0, 5])
+def test_every_call_takes_the_same_default_stream(launched, given):
+    """torch's current stream, where the tensors were written; its side streams do not wait for the legacy one."""
+    kw, want = ({}, 77) if given is None else (dict(stream=given), given)
+    x, codes, scales = Fake(4, 64), Fake(4, 32, dtype=U8), Fake(4, 2, dtype=U8)
+    b = block()
+    launched.clear()
+    dense.mx4_quantize(x, codes, scales, **kw)
+    dense.mx4_dequantize(codes, scales, x, **kw)
+    grouped().run(**kw)
+    norm().run(**kw)
+    b.forward(x, x, **kw)
+    assert [s for _, s in launched] == [want] * 5
+    if given is None:
+        dense.mx4_tile_scales(Fake(2, 32, 2, dtype=U8))
+        assert launched[-1][1] == 77
+
+
+def test_a_block_is_ready_on_any_stream(launched):
+    """Its scales are tiled, and its work block's earlier uses over, before the constructor returns."""
+    block()
+    assert [n for n, _ in launched] == ["mx4_tile_scales", "mx4_tile_scales", "synchronize"]
