@@ -114,10 +114,14 @@ def mx4_tile_scales(scales, act="none", stream=None):
     dev = _gpu(scales, "scales")
     sp, pitch = _rows(scales, "scales", dev, dtype=torch.uint8)
     _check_current(dev)
-    out = torch.empty(native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act]), dtype=torch.uint8,
-                      device=scales.device)
-    native().mx4_tile_scales(sp, pitch, scales.stride(0), n_expert, rows, blocks * 32, ACTS[act], out.data_ptr(),
-                             _stream(stream, dev))
+    n = native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act])
+    here = torch.cuda.current_stream(dev).cuda_stream
+    if stream is None or stream == here:
+        stream, out = here, torch.empty(n, dtype=torch.uint8, device=scales.device)
+    else:                               # memory of that stream's: this one's pool may hand out what is still in use here
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, dev) if stream else torch.cuda.default_stream(dev)):
+            out = torch.empty(n, dtype=torch.uint8, device=scales.device)
+    native().mx4_tile_scales(sp, pitch, scales.stride(0), n_expert, rows, blocks * 32, ACTS[act], out.data_ptr(), stream)
     return out
 
 

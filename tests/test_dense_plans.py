@@ -197,3 +197,27 @@ def test_a_block_is_ready_on_any_stream(launched):
     """Its scales are tiled, and its work block's earlier uses over, before the constructor returns."""
     block()
     assert [n for n, _ in launched] == ["mx4_tile_scales", "mx4_tile_scales", "synchronize"]
+
+
+@pytest.mark.parametrize("given,want", [(None, None), (77, None), (5, 5), (0, 0)])
+def test_tiled_scales_lie_in_their_streams_memory(launched, monkeypatch, given, want):
+    """What is written on a stream is allocated there: memory of the current one's pool may still be in use on it."""
+    inside, got = [], []
+
+    class On:
+        def __init__(self, s):
+            self.s = s
+
+        def __enter__(self):
+            inside.append(self.s)
+
+        def __exit__(self, *a):
+            inside.pop()
+
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda s, device=None: s)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda dev=None: 0)
+    monkeypatch.setattr(torch, "empty", lambda n, dtype=None, device=None: got.append(inside[-1] if inside else None)
+                        or Fake(n, dtype=dtype))
+    dense.mx4_tile_scales(Fake(2, 32, 2, dtype=U8), stream=given)
+    assert got == [want] and launched[-1][1] == (77 if given is None else given)

@@ -81,3 +81,20 @@ def test_a_block_built_on_one_stream_runs_on_another(mx):
             again.forward(x, out.fill_(float("nan")))
         st.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("legacy", [False, True])
+def test_scales_tiled_on_another_stream_keep_their_memory(legacy):
+    """A block of the current stream's memory, freed while it is still being written there, is not what they lie in."""
+    ws = torch.randint(0, 255, (4, 256, 16), generator=gen(2), device="cuda", dtype=torch.uint8)
+    want = dense.mx4_tile_scales(ws, "silu_mul")
+    torch.cuda.synchronize()
+    other = torch.cuda.default_stream() if legacy else torch.cuda.Stream()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        junk = torch.empty_like(want)
+        torch.cuda._sleep(PAUSE)
+        junk.fill_(0xAA)
+        del junk
+        out = dense.mx4_tile_scales(ws, "silu_mul", stream=other.cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
