@@ -6,6 +6,7 @@
 
 #include <string.h>
 
+static int mis(const void* p, int64_t a) { return (int)((uintptr_t)p % (uintptr_t)a); }
 static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
 static int check(const Exl3bExpertBlockDesc* d) {
@@ -89,6 +90,10 @@ int exl3b200_expert_block_forward(const Exl3bExpertBlockDesc* d, const Exl3bExpe
     if (T == 0) return RAD_OK;
     if (!x || !out || (next && !d->next_w)) return RAD_E_INVAL;
     const int mx = d->weights == EXL3B_MX4;
+    /* what the later steps would refuse is refused before the first is enqueued */
+    if (mis(out, 2) || mis(next, 2) || mis(d->post_w, 2) || mis(d->gate, 2) || mis(d->next_w, 2) || mis(d->router_w, 16) ||
+        mis(d->gu_w, 16) || mis(d->dn_w, 16) || (mx && (mis(d->gu_scales, 16) || mis(d->dn_scales, 16))))
+        return RAD_E_ALIGN;
     const int64_t H = d->hidden, W = d->width, P = T * d->top_k;
     const int64_t xs_pitch = (H / 32 + 15) / 16 * 16, hs_pitch = (W / 32 + 15) / 16 * 16;
 

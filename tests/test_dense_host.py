@@ -1,14 +1,16 @@
-"""The dense and MXFP4 expert operators' refusals that need no GPU: nothing is enqueued, so the addresses are made up."""
+"""The dense and MXFP4 expert operators' refusals that need no GPU: nothing is enqueued, so the addresses are made up (and
+the tests are for machines without a GPU, where a call that is not refused ends with no device)."""
 import ctypes as C
 
 import pytest
 
-pytest.importorskip("torch")
+torch = pytest.importorskip("torch")
 
 from exl3b200 import dense  # noqa: E402
-from exl3b200.native import GroupedMmDesc, Native  # noqa: E402
+from exl3b200.native import ExpertBlockBufs, ExpertBlockDesc, GroupedMmDesc, Native  # noqa: E402
 
-E_SHAPE = -1
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses")
+E_SHAPE, E_ALIGN, E_DEVICE = -1, -3, -6
 LIMIT = 1 << 26                         # grouped_mm's n_in
 
 
@@ -29,3 +31,18 @@ def test_grouped_mm_refuses_a_k_past_its_indices(dtype, step):
         assert lib.exl3b200_grouped_mm(C.addressof(d), None) == E_SHAPE, n_in
     for n in (LIMIT, 2 * LIMIT):        # what the limit is for: the last stage's offsets
         assert (n // 256 - 1) * 1024 < 1 << 31 and n * 2 < 1 << 31
+
+
+@pytest.mark.parametrize("weights", [3, dense.MX4])
+@pytest.mark.parametrize("name", ["out", "next", "router_w", "gu_w", "dn_w", "gu_scales", "dn_scales", "post_w", "gate", "next_w"])
+def test_the_expert_block_refuses_misaligned_operands_before_its_first_step(weights, name):
+    """Not when the step that reads them is reached, with the others enqueued."""
+    nat = Native()
+    at = {n: 4096 for n in ("router_w", "gu_w", "dn_w", "gu_scales", "dn_scales", "pre_w", "post_w", "gate", "next_w")}
+    io = {"out": 4096, "next": 4096}
+    odd = 4097 if name in ("out", "next", "post_w", "gate", "next_w") else 4096 + 8
+    (io if name in io else at)[name] = odd
+    d = ExpertBlockDesc(n_expert=64, hidden=2048, width=512, top_k=10, dtype=3, weights=weights, eps=1e-6, res_scale=1.0, **at)
+    b = nat.expert_block_carve(d, 8, 4096, nat.expert_block_work_bytes(d, 8))
+    rc = nat.lib.exl3b200_expert_block_forward(d, b, 4096, 4, io["out"], io["next"], None)
+    assert rc == (E_DEVICE if weights == 3 and name in ("gu_scales", "dn_scales") else E_ALIGN)      # unread: 16-bit weights
