@@ -43,11 +43,19 @@ struct Raw {
     }
 };
 
-// 1 / (1 + e^-g) from the special-function unit: relative 2^-20 or so, far inside a 16-bit output's rounding.
+// r / (1 + e^-g), within 2^-19 of the value down to the bottom of f32's range. From kGateLow up both functions are the
+// special-function unit's; below it, rare enough for a branch, the rounding of the exponential's argument would pass that
+// bound, and below -60, where 1 + e^-g is e^-g to every bit, r e^(g/2) e^(g/2) stays in range while the value does.
+constexpr float kGateLow = -16.f;
 __device__ __forceinline__ float sigmoid(float g) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
     return r;
+}
+__device__ __forceinline__ float gated(float r, float g) {
+    if (!(g < kGateLow)) return r * sigmoid(g);
+    const float e = expf(g < -60.f ? 0.5f * g : -g);
+    return g < -60.f ? r * e * e : r / (1.f + e);
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
@@ -165,11 +173,12 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
             }
         }
         if (p.gate_kind == EXL3B_GATE_TOKEN) {
-            const float f = sigmoid(token);
+            const bool far = token < -60.f;                  // as gated: e^(g/2) twice
+            const float f = gated(1.f, far ? 0.5f * token : token);
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) r[v][e] *= f;
+                for (int e = 0; e < 8; ++e) r[v][e] = far ? r[v][e] * f * f : r[v][e] * f;
         } else if (gates) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
@@ -177,6 +186,14 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
                 if (!AHEAD || VPT > 2) load(stream_dt, gate_at, v, gate[v]);
                 gate[v].get(f);
                 if (p.gate_kind == EXL3B_GATE_ELEMENT) {
+                    float least = f[0];
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) least = fminf(least, f[e]);
+                    if (least < kGateLow) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) r[v][e] = gated(r[v][e], f[e]);
+                        continue;
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = sigmoid(f[e]);
                 }

@@ -68,3 +68,23 @@ def test_silu_mul_of_infinities_and_nan(form):
     dense.GroupedMm(x=x, w=w, y=y, act="silu_mul").run(stream())
     y = y.reshape(rows, 200, 4)
     assert torch.isposinf(y[..., 0]).all() and torch.isnan(y[..., 1]).all() and torch.isfinite(y[..., 2:]).all()
+
+
+@pytest.mark.parametrize("kind", ["token", "element"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("H", [2048, 2047, 12000])
+@pytest.mark.parametrize("n", [1.0, -(2.0 ** 15)])
+def test_sigmoid_gates_over_the_whole_range(kind, dtype, H, n):
+    """sigmoid(g) * branch alone: the same bound."""
+    T = 420 if kind == "token" else 2
+    size = T if kind == "token" else T * H
+    g = ((torch.arange(size, device="cuda") % 1680).double() / (4 if kind == "token" else 8) - 105)
+    g[:6] = torch.tensor([0.0, -0.0, 300.0, -300.0, float("inf"), float("-inf")], device="cuda")
+    g = g.to(F32) if kind == "token" else g.to(dtype).reshape(T, H)
+    branch = torch.full((T, H), n, dtype=dtype, device="cuda")
+    out = torch.empty((T, H), dtype=dtype, device="cuda")
+    dense.BlockNorm(branch=branch, gate=g, gate_kind=kind, out=out).run(stream())
+    want = torch.sigmoid(g.double()) * n
+    want = want[:, None].expand(T, H) if kind == "token" else want
+    err = (out.double() - want).abs()
+    assert bool((err <= (2.0 ** -19 + ULP[dtype]) * want.abs() * (1 + 2.0 ** -18) + TINY[dtype]).all())
