@@ -13,8 +13,8 @@
 // expert-major, so that the CTAs working at one time share an expert's rows and weights in L2:
 //   narrow  a CTA a unit of 128 weight rows and up to 32 sorted rows, two CTAs an SM: a few rows an expert, where the
 //           weights' bytes count and units are needed to spread them over the SMs
-//   SPLIT   the narrow form with few units: a cluster a unit, each CTA a part of its k, the parts summed through
-//           distributed shared memory in the CTAs' order
+//   SPLIT   the narrow form with few units: a cluster for each of them, every CTA a part of its k, the parts summed
+//           through distributed shared memory in the CTAs' order
 //   PAIR    two CTAs (a cluster) a unit of 256 weight rows and up to 256 sorted rows (MXFP4: 224, the scales take
 //           tensor memory), tcgen05 cta_group::2: each CTA brings its 128 weight rows and HALF of the sorted rows, and
 //           both multiply by all of them: 64 KB brought in a stage of 256 x 256 where two CTAs alone would bring 96 KB
@@ -97,7 +97,7 @@ struct Cfg {
         return n < kMaxSt ? n : kMaxSt;
     }
     static_assert(COLS <= 512 && stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4), "tensor or shared memory");
-    static_assert((2 * kMaxSt + 6) * 8 + 8 <= 512, "barriers");
+    static_assert((2 * kMaxSt + 5) * 8 + 8 <= 512, "barriers");
 };
 
 // n / d for n < 2^31 by a multiplication; the host computes mul and shift.
@@ -435,8 +435,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     uint64_t* acc_full = empty + ST;                          // MMA commit -> epilogue [2]
     uint64_t* acc_empty = acc_full + 2;                       // epilogue (PAIR: of both CTAs) -> MMA [2]
     uint64_t* part_full = acc_empty + 2;                      // SPLIT: every CTA's partial sums are in its shared memory
-    uint64_t* part_empty = part_full + 1;                     // ... and have been read by every CTA
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_full + 1);
     uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
     uint32_t* prefix = reinterpret_cast<uint32_t*>(bars) + 128;   // [n_expert + 1]
     __shared__ Unit utab[kTab];
@@ -459,10 +458,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
         mbar_init(&acc_empty[tid - ST], 4 * C::EPI_G * MB);
     } else if (tid == ST + 2) {
         *dead = 0;
-        if (SPLIT) {
-            mbar_init(part_full, 4 * split);
-            mbar_init(part_empty, 4 * split);
-        }
+        if (SPLIT) mbar_init(part_full, 4 * split);
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -510,7 +506,8 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     chain_next();                                             // every CTA has its tensor memory: a later kernel may ask for its own
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
-    const uint32_t n_mine = n_units > first ? sh.stride(n_units - first + stride - 1) : 0;
+    // SPLIT: the grid has a cluster for every unit that offsets in ascending order can make, so one at most
+    const uint32_t n_mine = n_units > first ? SPLIT ? 1u : sh.stride(n_units - first + stride - 1) : 0u;
     auto unit_at = [&](uint32_t i) {
         return i < kTab ? utab[i] : find_unit<MB>(p, prefix, first + i * stride, sh);
     };
@@ -543,11 +540,6 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             }
         }
         __syncwarp();
-    };
-    // ... for arrivals that publish what the cluster's other CTAs wrote
-    auto wait_cluster = [&](uint64_t* bar, uint32_t parity) {
-        wait(bar, parity);
-        asm volatile("fence.acq_rel.cluster;" ::: "memory");
     };
     Pipe pipe;
 
@@ -857,7 +849,6 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             if constexpr (SPLIT) {
                 // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
                 // then sums every split-th row over the CTAs, in their order, and stores it.
-                if (i) wait_cluster(part_empty, (i & 1) ^ 1);
                 for (int t0 = 0; t0 < now.nr; t0 += kSlice) {
                     uint32_t a[16];
                     tmem_ld16(tmem + ((uint32_t)(32 * q) << 16) + ab * NT + t0, a);
@@ -868,9 +859,9 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                 fence_before();
                 __syncwarp();                                  // the arrivals publish the whole warp's sums
                 if (lane < split) arrive_at(part_full, lane);
-                if (lane == 0) mbar_arrive(&acc_empty[ab]);
                 __syncwarp();
-                wait_cluster(part_full, i & 1);
+                wait(part_full, 0);
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 const bool out_lane = !act || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
                 const int64_t n0 = b0 + (act ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
                 const uint32_t rows_live = __shfl_sync(0xFFFFFFFFu, live, 0);
@@ -913,9 +904,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                         else *reinterpret_cast<uint2*>(d) = make_uint2(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]));
                     }
                 }
-                __syncwarp();
-                if (i + 1 < n_mine && lane < split) arrive_at(part_empty, lane);
-                continue;
+                break;
             }
             // Thread t has outputs o and o + 8 (act NONE: and 16 more) of rows c2, c2 + 1, 8 + c2, 9 + c2 of a slice
             constexpr int NV = ACT ? 8 : 16;
@@ -1136,7 +1125,7 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     // 8.9). MXFP4 has a quarter of the stages and gains nothing (two experts 8.9 and 10.3).
     if (!MX) {
         const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 63) / 64;
-        int64_t split = sm_count / most;
+        int64_t split = sm_count / most;                      // so the grid has room for a cluster a unit: the kernel counts on it
         if (split > nck / 4) split = nck / 4;
         if (split > kMaxSplit) split = kMaxSplit;
         if (split >= 2) return launch<false, false, true>(p, sm_count, (int)split, st);
