@@ -190,9 +190,7 @@ int exl3b200_grouped_mm(const Exl3bGroupedMm* d, void* stream) {
     p.x_rows = d->x_rows;
     p.n_expert = (int32_t)d->n_expert;
     p.top_k = (int32_t)d->top_k;
-    const uint64_t k = d->top_k > 1 ? (uint64_t)d->top_k : 1;
-    while (((uint64_t)1 << p.k_shift) < k) ++p.k_shift;
-    p.k_mul = (uint32_t)(((((uint64_t)1 << p.k_shift) - k) << 32) / k + 1);
+    p.slots = exl3b_div(d->top_k > 1 ? (uint32_t)d->top_k : 1);
     p.act = d->act;
     p.y_dtype = d->y_dtype;
     p.x = d->x;

@@ -11,6 +11,24 @@
 extern "C" {
 #endif
 
+/* n / d for n < 2^31 as (umulhi(n, mul) + n) >> shift, with 2^shift the least power of two from d on and
+ * mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery, "Division by Invariant Integers using
+ * Multiplication", 1994). */
+typedef struct Exl3bDiv {
+    uint32_t d, mul, shift;
+} Exl3bDiv;
+static inline Exl3bDiv exl3b_div(uint32_t d) {
+    Exl3bDiv v = { d, 0, 0 };
+    while (((uint64_t)1 << v.shift) < d) ++v.shift;
+    v.mul = (uint32_t)(((((uint64_t)1 << v.shift) - d) << 32) / d + 1);
+    return v;
+}
+#ifdef __CUDACC__
+static __device__ __forceinline__ uint32_t exl3b_div_of(uint32_t n, const Exl3bDiv& v) {
+    return (__umulhi(n, v.mul) + n) >> v.shift;
+}
+#endif
+
 /* block_norm (exl3b200_norm.cu); pitches in elements, q_pitch and qs_pitch in bytes. */
 typedef struct Exl3bNormOp {
     int64_t     rows, cols;
@@ -40,7 +58,7 @@ typedef struct Exl3bGmmOp {
     int64_t        w_rows;               /* the weight's rows: n_out, or twice that with silu_mul */
     int64_t        x_rows;
     int32_t        n_expert, top_k;      /* top_k 0: sorted row i reads x row i */
-    uint32_t       k_mul, k_shift;       /* slot / top_k = (umulhi(slot, k_mul) + slot) >> k_shift */
+    Exl3bDiv       slots;                /* of a token: top_k (0: 1) */
     int32_t        act, y_dtype;
     const void*    x;                    /* elements, or MXFP4 codes */
     int64_t        x_pitch_bytes;

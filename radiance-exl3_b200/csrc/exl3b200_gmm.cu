@@ -100,20 +100,10 @@ struct Cfg {
     static_assert((2 * kMaxSt + 5) * 8 + 8 <= 512, "barriers");
 };
 
-// n / d for n < 2^31 by a multiplication; the host computes mul and shift.
-struct FastDiv {
-    uint32_t d, mul, shift;
-    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-FastDiv fast_div(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    return FastDiv{ d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s };
-}
 // What the host works out of a launch, so that no CTA divides for it.
 struct Shape {
-    FastDiv n_mb, stride;   // weight-row blocks (PAIR: pairs) an output row; CTAs (PAIR, SPLIT: clusters) of the grid
-    FastDiv nt;             // sorted rows a unit at most
+    Exl3bDiv n_mb, stride;   // weight-row blocks (PAIR: pairs) an output row; CTAs (PAIR, SPLIT: clusters) of the grid
+    Exl3bDiv nt;            // sorted rows a unit at most
     int32_t nck, st, split; // stages of a unit's k, of the ring; CTAs a unit (SPLIT)
 };
 
@@ -132,14 +122,16 @@ __device__ __forceinline__ Run run_of(const Exl3bGmmOp& p, int e) {
     const int32_t a = max(p.expert_offset[e], 0), b = min(p.expert_offset[e + 1], (int32_t)p.n_rows);
     return Run{ a, max(b - a, 0) };
 }
-__device__ __forceinline__ uint32_t groups(const Run& r, const FastDiv& nt) { return nt((uint32_t)r.rows + nt.d - 1); }
+__device__ __forceinline__ uint32_t groups(const Run& r, const Exl3bDiv& nt) {
+    return exl3b_div_of((uint32_t)r.rows + nt.d - 1, nt);
+}
 
 // Unit `local` of expert e: block by block, then group by group. An expert's rows are split evenly over its groups, in
 // steps of the MMA's N, so that no group is left with a sliver.
 template <int MB>
 __device__ __forceinline__ Unit make_unit(int e, const Run& r, uint32_t local, const Shape& sh) {
-    const FastDiv& n_mb = sh.n_mb;
-    const uint32_t g = n_mb(local), ng = groups(r, sh.nt), step = 16 * MB;
+    const Exl3bDiv& n_mb = sh.n_mb;
+    const uint32_t g = exl3b_div_of(local, n_mb), ng = groups(r, sh.nt), step = 16 * MB;
     const uint32_t even = ng > 1 ? ((uint32_t)r.rows + ng - 1) / ng : (uint32_t)r.rows, per = (even + step - 1) / step * step;
     Unit u;
     u.e = e;
@@ -352,8 +344,7 @@ struct RowAhead {
     __device__ __forceinline__ void rows(const uint8_t* base, int64_t pitch, const uint8_t* src[N]) const {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            // slot / top_k by a multiplication (top_k 0: 1): exact for slots below 2^31
-            const uint32_t f = (uint32_t)max(slot[j], 0), t = (__umulhi(f, p.k_mul) + f) >> p.k_shift;
+            const uint32_t t = exl3b_div_of((uint32_t)max(slot[j], 0), p.slots);
             src[j] = base + (int64_t)min(t, (uint32_t)p.x_rows - 1) * pitch;
         }
     }
@@ -490,7 +481,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
             const uint32_t n = groups(r, sh.nt) * n_mb;
             prefix[e] = acc;
             if (n) {
-                uint32_t i = acc > first ? sh.stride(acc - first + stride - 1) : 0u;
+                uint32_t i = acc > first ? exl3b_div_of(acc - first + stride - 1, sh.stride) : 0u;
 #pragma unroll 1
                 for (; i < kTab && first + i * stride < acc + n; ++i)
                     utab[i] = make_unit<MB>(e, r, first + i * stride - acc, sh);
@@ -507,7 +498,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t n_units = prefix[p.n_expert];
     // SPLIT: the grid has a cluster for every unit that offsets in ascending order can make, so one at most
-    const uint32_t n_mine = n_units > first ? SPLIT ? 1u : sh.stride(n_units - first + stride - 1) : 0u;
+    const uint32_t n_mine = n_units > first ? SPLIT ? 1u : exl3b_div_of(n_units - first + stride - 1, sh.stride) : 0u;
     auto unit_at = [&](uint32_t i) {
         return i < kTab ? utab[i] : find_unit<MB>(p, prefix, first + i * stride, sh);
     };
@@ -1102,7 +1093,7 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
     const int64_t room = (int64_t)sm_count * per_sm / ctas;
     const int stages = C::stages(p->n_expert, per_sm);
     const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
-    const Shape sh = { fast_div((uint32_t)((p->n_out + blk - 1) / blk)), fast_div((uint32_t)units), fast_div((uint32_t)nt),
+    const Shape sh = { exl3b_div((uint32_t)((p->n_out + blk - 1) / blk)), exl3b_div((uint32_t)units), exl3b_div((uint32_t)nt),
                        (int32_t)((p->n_in + (MX ? 255 : 63)) / (MX ? 256 : 64)), stages, split };
     return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
                         ctas, st, map, *p, sh);

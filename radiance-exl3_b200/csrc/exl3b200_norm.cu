@@ -275,25 +275,17 @@ int launch_norm(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st) {
 // 2048: 2.8 us each, a launch.
 constexpr int kUnroll = 4;
 
-// n / d for n < 2^31 by a multiplication (the host computes m and s); BIG: 64-bit division.
-struct RowDiv {
-    uint32_t d, m, s;
-};
+// Vector i's row and place in it; BIG: vectors past 2^31, a 64-bit division.
 template <bool BIG>
-__device__ __forceinline__ void row_of(int64_t i, const RowDiv& v, int64_t* row, int* vec) {
+__device__ __forceinline__ void row_of(int64_t i, const Exl3bDiv& v, int64_t* row, int* vec) {
     if (BIG) {
         *row = i / v.d;
         *vec = (int)(i - *row * v.d);
     } else {
-        const uint32_t n = (uint32_t)i, q = (__umulhi(n, v.m) + n) >> v.s;
+        const uint32_t n = (uint32_t)i, q = exl3b_div_of(n, v);
         *row = q;
         *vec = (int)(n - q * v.d);
     }
-}
-RowDiv row_div(uint32_t d) {
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    return RowDiv{ d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s };
 }
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
@@ -320,7 +312,7 @@ __device__ __forceinline__ uint32_t quad_code(const Raw<DT>& x) {
 }
 
 template <int DT, bool BIG>
-__global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t n_vec, RowDiv div,
+__global__ void __launch_bounds__(256) k_mx4_quantize(const void* x, int64_t x_pitch, int64_t n_vec, Exl3bDiv div,
                                                       uint8_t* q, int64_t q_pitch, uint8_t* qs, int64_t qs_pitch) {
     typedef typename El<DT>::T T;
     chain_wait();
@@ -387,7 +379,7 @@ __device__ __forceinline__ uint4 e2m1_bf16x8(uint32_t n, uint32_t code) {
 
 template <int DT, bool BIG>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* qs,
-                                                        int64_t qs_pitch, int64_t n_vec, RowDiv div, void* y,
+                                                        int64_t qs_pitch, int64_t n_vec, Exl3bDiv div, void* y,
                                                         int64_t y_pitch) {
     typedef typename El<DT>::T T;
     chain_wait();
@@ -473,7 +465,7 @@ int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t r
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t n_vec = rows * (cols / 8);
     const unsigned grid = (unsigned)((n_vec + 256 * kUnroll - 1) / (256 * kUnroll));
-    const RowDiv div = row_div((uint32_t)(cols / 8));
+    const Exl3bDiv div = exl3b_div((uint32_t)(cols / 8));
     if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_quantize, 1, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
     else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_quantize, 2, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
     else EXL3B_MX4_ROWS(k_mx4_quantize, 3, x, x_pitch, n_vec, div, q, q_pitch, qs, qs_pitch);
@@ -484,7 +476,7 @@ int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t n_vec = rows * (cols / 8);
     const unsigned grid = (unsigned)((n_vec + 256 * kUnroll - 1) / (256 * kUnroll));
-    const RowDiv div = row_div((uint32_t)(cols / 8));
+    const Exl3bDiv div = exl3b_div((uint32_t)(cols / 8));
     if (dtype == 1) EXL3B_MX4_ROWS(k_mx4_dequantize, 1, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
     else if (dtype == 2) EXL3B_MX4_ROWS(k_mx4_dequantize, 2, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
     else EXL3B_MX4_ROWS(k_mx4_dequantize, 3, q, q_pitch, qs, qs_pitch, n_vec, div, y, y_pitch);
