@@ -977,7 +977,7 @@ __global__ void __launch_bounds__(Cfg<MX, PAIR, SPLIT>::THREADS, Cfg<MX, PAIR, S
                             const int j = q * tpw + lane / lpt;
                             const int64_t r = now.r0 + t0 + 8 * h + j, n0 = b0 + c0;
                             float f[8];
-                            ld8<1>(&st[j * kEpiLd + c0], f);
+                            ld8(&st[j * kEpiLd + c0], f);
                             const uint32_t code = mx4_quad_code(f);              // four lanes: 32 outputs of one row
                             if (8 * h + j < left && n0 < p.n_out) {
                                 *reinterpret_cast<uint32_t*>(y + r * p.y_pitch + n0 / 2) = mx4_pack8(f, code);

@@ -75,19 +75,10 @@ struct El<3> {
 };
 
 // Eight consecutive values at a 16-byte aligned address.
-template <int DT>
-__device__ __forceinline__ void ld8(const void* p, float v[8]) {
-    if constexpr (DT == 1) {
-        const float4 a = *static_cast<const float4*>(p), b = *(static_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        typedef typename El<DT>::T T;
-        const uint4 a = *static_cast<const uint4*>(p);
-        const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = El<DT>::to(e[i]);
-    }
+__device__ __forceinline__ void ld8(const float* p, float v[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 template <int DT>
 __device__ __forceinline__ void st8(void* p, const float v[8]) {
