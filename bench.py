@@ -286,6 +286,19 @@ def reference_op_seconds(op, reps=3, **case_kw):
     return float(np.median(times))
 
 
+def beside_reference(line, us, rows, op, note="", **case_kw):
+    """Adds the reference's time of one op over `rows` rows to a line of ours of `us` microseconds, or why there is none."""
+    try:
+        t = reference_op_seconds(op, **case_kw)
+    except Exception as exc:             # the reference's library is absent on this machine
+        line["cpu_reference"] = {"unavailable": str(exc)}
+        return
+    line["cpu_reference"] = {"us": round(t * 1e6, 1), "tokens_per_s": round(rows / t, 1), "cores": 1, "kind": "reference"}
+    if note:
+        line["cpu_reference"]["op"] = note
+    line["speedup_vs_cpu"] = round(t * 1e6 / us, 1)
+
+
 def single_expert_configs(plugin, hbm, with_cpu):
     """Config 1 (one EXL3 linear, 16 rows of 2048 -> 512, K=4 mul1, f16 out: exl3b200_moe_down_f16) and config 2
     (one expert MLP, gate/up [512, 2048] and down [2048, 512] at K=4, M = 1, 4, 8, 32 rows: the moe_exl3_gate_up_down
@@ -302,11 +315,8 @@ def single_expert_configs(plugin, hbm, with_cpu):
           "frac_hbm": round(lin.bytes_per_call() / (us / 1e6) / 1e9 / hbm, 3), "bytes_per_call": lin.bytes_per_call(),
           "tokens_per_s": round(16 / (us / 1e6), 1), "copies": n1, "out": "f16", "entry": "exl3b200_moe_down_f16"}
     if with_cpu:
-        t = reference_op_seconds("moe_exl3_down", M=16, top_k=1, n_expert=1, geom=[(512, 2048)], bits=4,
-                                 codebook="mul1")
-        c1["cpu_reference"] = {"us": round(t * 1e6, 1), "tokens_per_s": round(16 / t, 1), "cores": 1,
-                               "kind": "reference", "op": "moe_exl3_down (bf16 rows)"}
-        c1["speedup_vs_cpu"] = round(t * 1e6 / us, 1)
+        beside_reference(c1, us, 16, "moe_exl3_down", "moe_exl3_down (bf16 rows)", M=16, top_k=1, n_expert=1,
+                         geom=[(512, 2048)], bits=4, codebook="mul1")
     del lin
     res["config1_linear_16x2048_to_512"] = c1
     c2 = {}
@@ -318,11 +328,8 @@ def single_expert_configs(plugin, hbm, with_cpu):
              "frac_hbm": round(mlp.bytes_per_call() / (us / 1e6) / 1e9 / hbm, 3),
              "tokens_per_s": round(M / (us / 1e6), 1), "copies": n2}
         if with_cpu:
-            t = reference_op_seconds("moe_exl3_gate_up_down", M=M, top_k=1, n_expert=1, geom=[(1024, 2048)], bits=4,
-                                     codebook="mul1")
-            e["cpu_reference"] = {"us": round(t * 1e6, 1), "tokens_per_s": round(M / t, 1), "cores": 1,
-                                  "kind": "reference"}
-            e["speedup_vs_cpu"] = round(t * 1e6 / us, 1)
+            beside_reference(e, us, M, "moe_exl3_gate_up_down", M=M, top_k=1, n_expert=1, geom=[(1024, 2048)], bits=4,
+                             codebook="mul1")
         c2[f"M{M}"] = e
         del mlp
     res["config2_expert_mlp_2048x512_K4"] = c2
@@ -846,7 +853,11 @@ def main():
         if rank != 0:
             return 0
         threads = max(1, min(os.cpu_count() or 1, 64))
-        v, step, sample = time_reference(threads, args.steps, args.warmup, n_experts=2)
+        try:
+            v, step, sample = time_reference(threads, args.steps, args.warmup, n_experts=2)
+        except OSError as exc:           # the reference's library is absent on this machine
+            print(json.dumps({"impl": "reference", "unavailable": " ".join(str(exc).split())}), flush=True)
+            return 0
         line = {"metric": METRIC, "impl": "reference", "value": round(v, 3), "unit": "tokens/s", "n_gpus": args.gpus,
                 "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(step * 1e3, 2),
                 "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "f32 host",
