@@ -19,12 +19,13 @@ ACTS = {"none": 0, "silu_mul": 1}
 GATES = {"none": 0, "token": 1, "channel": 2, "element": 3}
 
 _native = None
+_several = True                         # more than one GPU here: with one there is no other that could be current
 
 
 def native():
-    global _native
+    global _native, _several
     if _native is None:
-        _native = Native()
+        _native, _several = Native(), torch.cuda.device_count() != 1
     return _native
 
 
@@ -35,32 +36,25 @@ def _dtype(t):
     return dt
 
 
-def _gpu(t, name):
-    """The GPU that a call's first tensor is on; the others have to share it."""
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{name} is not on a GPU")
-    return dev
-
-
 def _check_current(dev):
     """The library launches on the current device: a call's tensors have to be there."""
     if torch.cuda.current_device() != dev:
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def _stream(stream, dev):
-    return torch.cuda.current_stream(dev).cuda_stream if stream is None else stream
+def _current_stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def _rows(t, name, dev, shape=None, dtype=None):
-    """A tensor whose last dimension is dense, on GPU dev, of this shape and type: (address, row pitch in elements)."""
+    """A tensor whose last dimension is dense, on GPU dev (that of the call's first tensor), of this shape and type:
+    (address, row pitch in elements)."""
     if t is None:
         raise ValueError(f"{name} is missing")
     have, st = t.shape, t.stride()
-    if not (t.get_device() == dev and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
+    if not (t.get_device() == dev >= 0 and (dtype is None or t.dtype is dtype) and (shape is None or have == shape)
             and (st[-1] == 1 or have[-1] <= 1)):
-        what = (f"is on {t.device}, not cuda:{dev}" if t.get_device() != dev else
+        what = ("is not on a GPU" if t.get_device() < 0 else f"is on {t.device}, not cuda:{dev}" if t.get_device() != dev else
                 f"is {t.dtype}, not {dtype}" if dtype not in (None, t.dtype) else
                 f"has shape {tuple(have)}, not {tuple(shape)}" if shape is not None and have != shape else
                 "has a strided last dimension")
@@ -81,13 +75,14 @@ def mx4_empty(rows, cols, device="cuda"):
 def mx4_quantize(x, codes, scales, stream=None):
     """x [rows, cols] in f32, f16 or bf16 -> its MXFP4 codes and scales."""
     rows, cols = x.shape
-    dev = _gpu(x, "x")
+    dev = x.get_device()
     xp, pitch = _rows(x, "x", dev)
     cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
-    _check_current(dev)
+    if _several:
+        _check_current(dev)
     rc = native().lib.exl3b200_mx4_quantize(xp, _dtype(x), pitch, rows, cols, cp, c_pitch, sp, s_pitch,
-                                           _stream(stream, dev))
+                                           _current_stream(dev) if stream is None else stream)
     if rc:
         raise RuntimeError(f"exl3b200_mx4_quantize: status {rc}")
     return codes, scales
@@ -96,13 +91,14 @@ def mx4_quantize(x, codes, scales, stream=None):
 def mx4_dequantize(codes, scales, y, stream=None):
     """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
     rows, cols = y.shape
-    dev = _gpu(y, "y")
+    dev = y.get_device()
     yp, pitch = _rows(y, "y", dev)
     cp, c_pitch = _rows(codes, "codes", dev, (rows, cols // 2), torch.uint8)
     sp, s_pitch = _rows(scales, "scales", dev, (rows, cols // 32), torch.uint8)
-    _check_current(dev)
+    if _several:
+        _check_current(dev)
     rc = native().lib.exl3b200_mx4_dequantize(cp, c_pitch, sp, s_pitch, rows, cols, yp, _dtype(y), pitch,
-                                             _stream(stream, dev))
+                                             _current_stream(dev) if stream is None else stream)
     if rc:
         raise RuntimeError(f"exl3b200_mx4_dequantize: status {rc}")
     return y
@@ -111,11 +107,12 @@ def mx4_dequantize(codes, scales, y, stream=None):
 def mx4_tile_scales(scales, act="none", stream=None):
     """A weight's scales [experts, rows, cols / 32] in the form GroupedMm reads; once, when the weight is loaded."""
     n_expert, rows, blocks = scales.shape
-    dev = _gpu(scales, "scales")
+    dev = scales.get_device()
     sp, pitch = _rows(scales, "scales", dev, dtype=torch.uint8)
-    _check_current(dev)
+    if _several:
+        _check_current(dev)
     n = native().mx4_tiled_bytes(n_expert, rows, blocks * 32, ACTS[act])
-    here = torch.cuda.current_stream(dev).cuda_stream
+    here = _current_stream(dev)
     if stream is None or stream == here:
         stream, out = here, torch.empty(n, dtype=torch.uint8, device=scales.device)
     else:                               # memory of that stream's: this one's pool may hand out what is still in use here
@@ -134,8 +131,9 @@ class _Plan:
         self._addr, self._call = C.addressof(desc), getattr(native().lib, self._entry)
 
     def run(self, stream=None):
-        _check_current(self._dev)
-        rc = self._call(self._addr, _stream(stream, self._dev))
+        if _several:
+            _check_current(self._dev)
+        rc = self._call(self._addr, _current_stream(self._dev) if stream is None else stream)
         if rc:
             raise RuntimeError(f"{self._entry}: status {rc}")
 
@@ -159,7 +157,7 @@ class GroupedMm(_Plan):
             raise ValueError(f"x is {x.dtype}, w {w.dtype}")
         if (x.dim(), w.dim(), y.dim()) != (2, 3, 2):
             raise ValueError(f"x, w and y have {x.dim()}, {w.dim()} and {y.dim()} dimensions, not 2, 3 and 2")
-        dev = _gpu(x, "x")
+        dev = x.get_device()
         d.n_expert, d.n_rows, d.x_rows, d.top_k = w.shape[0], y.shape[0], x.shape[0], top_k
         d.n_out, d.n_in, d.act = y.shape[1] * per_out, x.shape[1] * per, ACTS[act]
         d.dtype, d.y_dtype = MX4 if mx else _dtype(x), MX4 if mx_out else _dtype(y)
@@ -197,7 +195,7 @@ class BlockNorm(_Plan):
         if lead is None:
             raise ValueError("neither branch nor res")
         rows, cols = d.rows, d.cols = lead.shape
-        dev = _gpu(lead, "branch" if branch is not None else "res")
+        dev = lead.get_device()
         typed = next((t for t in (res, out, y, post_w, pre_w) if t is not None), lead)
         dt = typed.dtype
         d.dtype, d.gate_kind = _dtype(typed), GATES[gate_kind]
@@ -239,7 +237,7 @@ class ExpertBlock:
     def __init__(self, *, router_w, gu_w, dn_w, pre_w, post_w=None, gate=None, next_w=None, gu_scales=None, dn_scales=None,
                  top_k, eps=1e-6, res_scale=1.0, max_tokens=2048):
         E, H = router_w.shape
-        dev = self._dev = _gpu(router_w, "router_w")
+        dev = self._dev = router_w.get_device()
         mx = gu_w.dtype == torch.uint8
         per, dt = 2 if mx else 1, router_w.dtype
         W = dn_w.shape[2] * per
@@ -275,7 +273,9 @@ class ExpertBlock:
                 _rows(t, name, self._dev, (T, self.hidden), self.dtype)
                 if not t.is_contiguous():
                     raise ValueError(f"{name} is strided")
-        _check_current(self._dev)
+        if _several:
+            _check_current(self._dev)
         native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
-                                      next_out.data_ptr() if next_out is not None else None, _stream(stream, self._dev))
+                                      next_out.data_ptr() if next_out is not None else None,
+                                      _current_stream(self._dev) if stream is None else stream)
         return out

@@ -64,6 +64,7 @@ def launched(monkeypatch):
             calls.append(("synchronize", 77))
 
     monkeypatch.setattr(dense, "_native", Host())
+    monkeypatch.setattr(dense, "_several", True)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: Stream())
     monkeypatch.setattr(torch, "empty", lambda n, dtype=None, device=None: Fake(n, dtype=dtype))
