@@ -1,5 +1,5 @@
 """The dense and MXFP4 expert operators where they can go wrong at their edges: the longest k, calls in which no expert has
-a row."""
+a row, rows beside those of EXL3 experts."""
 import numpy as np
 import pytest
 
@@ -84,3 +84,29 @@ def test_no_expert_has_a_row(dtype, E, n, N, start):
         s.fill_(0x11)
         dense.GroupedMm(x=x, w=w, y=q, y_scales=s, **kw).run(stream())
         assert not q.any() and not s.any() and not np.any(decode(q, s))
+
+
+@pytest.mark.parametrize("T,pad", [(3, 3), (128, 96)])
+def test_beside_exl3_experts_in_one_buffer(T, pad):
+    """Trailing experts in bf16 behind a layer's EXL3 ones: grouped_mm over their part of the offsets, which clears the rows
+    before them, then the EXL3 ops over their live rows alone, which leave the others."""
+    from exl3b200 import load_plugin
+    from exl3b200.layer import MoeLayer
+    lay = MoeLayer(load_plugin(), n_expert=16, hidden=2048, width=512, top_k=4, bits_gu=3, bits_dn=4, max_tokens=T, seed=3,
+                   max_rows=T * 4 + pad)
+    g, R, K = gen(4), T * lay.k, 256
+    lay.x.copy_(randn(g, *lay.x.shape, dtype=F16))
+    lay.logits.copy_(randn(g, *lay.logits.shape))
+    lay.forward(T, stream())
+    torch.cuda.synchronize()
+    want = lay.y_rows[:R].view(torch.int16).clone()
+    n = R + pad
+    off = torch.tensor([R, R + pad // 3, n], dtype=torch.int32, device="cuda")
+    y = lay.y_rows[:n].view(BF16)
+    x, w = randn(g, n, K, dtype=BF16), randn(g, 2, lay.H, K, dtype=BF16)
+    dense.GroupedMm(x=x, w=w, y=y, expert_offset=off).run(stream())
+    alone = y[R:].clone()
+    assert alone.any() and not y[:R].any()
+    lay.experts(T, n, stream(), live=True)
+    torch.cuda.synchronize()
+    assert torch.equal(y[R:], alone) and torch.equal(lay.y_rows[:R].view(torch.int16), want)
