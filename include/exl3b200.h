@@ -441,7 +441,8 @@ int     exl3b200_mx4_tile_scales(const uint8_t* scales, int64_t scales_pitch, in
  *   act SILU_MUL: y[i][n] = silu(z[n]) * z[n_out + n], w[e] holding n_out gate rows and then n_out up rows.
  * Each output is rounded once to y_dtype (RAD_F32, RAD_F16, RAD_BF16, or EXL3B_MX4: codes and scales as mx4_quantize
  * makes them of the f32 values). Rows outside [expert_offset[0], expert_offset[n_expert]) and dropped slots
- * (sorted_tok < 0) are zero. expert_offset NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and
+ * (sorted_tok < 0) are zero, as the EXL3 rows leave them: beside EXL3 experts in one buffer it is called first, over its
+ * part of the offsets, and exl3b200_moe_op_live then, which leaves the rows outside its own runs. expert_offset NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and
  * slot i is i. dtype: RAD_F16, RAD_BF16, or EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form).
  * Pitches in elements (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32), at most
  * 2^26, n_out of 8 (MXFP4 out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048. */
@@ -500,8 +501,9 @@ typedef struct Exl3bBlockNorm {
 int     exl3b200_block_norm(const Exl3bBlockNorm* norm, void* stream);
 
 /* A residual MoE block over such experts, the sequence an engine issues for it, driven from C:
- *   xn = rmsnorm(x) * pre_w -> logits = xn . router_w (f32) -> router_scatter -> h = silu_mul(gate, up) -> down ->
- *   moe_gather (softmax weights) -> out = res_scale * x + gate * rmsnorm(gathered) * post_w; next = rmsnorm(out) * next_w
+ *   xn = rmsnorm(x) * pre_w -> logits = xn . router_w (f32) -> router_scatter -> h = silu_mul(gate, up) -> down, its rows
+ *   rounded to bf16 whatever `dtype`, as moe_gather reads them -> moe_gather (softmax weights) ->
+ *   out = res_scale * x + gate * rmsnorm(gathered) * post_w; next = rmsnorm(out) * next_w
  * over block_norm, grouped_mm and the routing entries above. x, out and next are [T][hidden] of `dtype` (RAD_F16 or
  * RAD_BF16), as are router_w [n_expert][hidden] and the norms' and the gate's [hidden] (post_w, gate, next_w may be NULL).
  * weights: `dtype`, or EXL3B_MX4 (gu_w [n_expert][2 width][hidden] and dn_w [n_expert][hidden][width] as codes, the

@@ -166,7 +166,7 @@ int exl3b200_expert_block_forward(const Exl3bExpertBlockDesc* d, const Exl3bExpe
     m.n_in = W;
     m.x_rows = P;
     m.top_k = 0;
-    m.y_dtype = RAD_BF16;
+    m.y_dtype = RAD_BF16;             /* what moe_gather reads, an f16 block's rows too: f16's range and more, three bits less */
     m.act = EXL3B_ACT_NONE;
     m.x = b->h;
     m.x_pitch = m.w_pitch = W;

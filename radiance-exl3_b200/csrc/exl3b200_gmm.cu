@@ -33,12 +33,13 @@
 //
 // Measured on one B200 that copies 6539 GB/s and reaches 1650 TFLOP/s of bf16 in its library product; a launch's time in a
 // CUDA graph, and what bounds it:
-//   512 experts, 191 live of 624 rows, 640 -> 2560, bf16 (narrow)           96 us  6.6 TB/s: the weights' bytes
-//   512 experts, 418 live of 20072 rows, 2048 -> 512 silu_mul, f16 (PAIR)  278 us  6.4 TB/s: the weights' bytes
-//   16 experts of 16060 rows, 1536 -> 4096, bf16 (PAIR)                    153 us  1323 TFLOP/s: a stage of 256 x 256 x 64 in
+//   512 experts, 191 live of 624 rows, 640 -> 2560, bf16 (narrow)           95 us  6.6 TB/s: the weights' bytes
+//   512 experts, 418 live of 20072 rows, 2048 -> 512 silu_mul, f16 (PAIR)  279 us  6.4 TB/s: the weights' bytes
+//   16 experts of 16060 rows, 1536 -> 4096, bf16 (PAIR)                    151 us  1338 TFLOP/s: a stage of 256 x 256 x 64 in
 //     about 510 cycles, the MMAs' own time at full rate, at a clock that power brings down to 1.2 .. 1.5 GHz
 //   16 experts of 16060 rows, 4096 -> 1536, MXFP4 (PAIR)                    54 us  3743 TFLOP/s: a stage of 33 KB a CTA in
-//     ~650 cycles where its MMAs take ~450: L2's rate, 13 TB/s over the GPU; seven units a pair at most where 6.5 would do
+//     ~650 cycles where its MMAs take ~450: 51 bytes a cycle into an SM, in both MXFP4 cases, while L2 is at 29 % of its
+//     peak (64 experts): the way into the SM, by inference, no counter; seven units a pair at most where 6.5 would do
 //   64 experts of 20072 rows, 2048 -> 512 silu_mul, MXFP4 (PAIR)            31 us  2735 TFLOP/s: the same, 29 KB in ~560
 //     cycles, and five of the 31 us before the first stage is there (launch, set-up, the first loads)
 //   one token's ten experts, 2048 -> 512 silu_mul, f16 (narrow)             13 us  42 MB, 6.4 us at the copy rate; the rest
@@ -1111,7 +1112,7 @@ int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         return launch<MX, true, false>(p, sm_count, 1, st);
     }
     // Few narrow units over a long k: up to four CTAs a unit while each has an SM, four stages a part at least (one token,
-    // two experts, 2048 -> 512 silu_mul: 9.6 us, in four parts 7.0; 16 rows, 4096 -> 4096: 14.8 and 10.4; ten experts make
+    // two experts, 2048 -> 512 silu_mul: 8.2 us, in four parts 5.7; 16 rows, 4096 -> 4096: 13.8 and 9.5; ten experts make
     // 80 units: in three parts, more CTAs than SMs, 13.7 and 15.1; clusters of eight do not always fit at once: 15.1 for
     // 8.9). MXFP4 has a quarter of the stages and gains nothing (two experts 8.9 and 10.3).
     if (!MX) {

@@ -14,15 +14,20 @@ namespace {
 // ------------------------------------------------------------------------------------------ block_norm
 // Row t, all in f32:  n = branch * rsqrt(mean(branch^2) + post_eps) * post_w;  r = res_scale * res + gate * n;
 // y = r * rsqrt(mean(r^2) + pre_eps) * pre_w. HBM bound: every input is read once and every output written once.
-// `tpr` threads hold a row in registers (VPT vectors of eight values each), so the second mean needs no second read;
-// short rows share a block (blockDim.y rows). A row's fixed cost -- two reductions, its addresses -- is paid by fewer
+// `tpr` threads hold a row (VPT vectors of eight values each), so the second mean needs no second read of HBM; short rows
+// share a block (blockDim.y rows). A row's fixed cost -- two reductions, its addresses -- is paid by fewer
 // instructions the more values a thread holds (the kernel is near the issue limit: 640 instructions a warp and 256 values
 // with one vector a thread, half of that with four); few short rows take one vector, since there a row's latency counts.
 // Rows whose addresses or width rule out 16-byte vectors take the same code over single values, a thread's values
 // blockDim.x apart.
+// What a thread holds is in registers for 16-byte rows of up to 8192 values (an f32 row with an element gate: but for 100
+// bytes). Not so for longer rows, whose 1024 threads have 64 registers each (24 bytes of a thread's values go through local
+// memory in f16, 200 to 310 in bf16 and f32), and for single values, put into their words one by one (280 to 570 bytes, f32
+// 680 to 1020; over 8192 values 1000 to 1490).
 // Measured on one B200 (copies at 6.5 TB/s): 16384 rows of 4096, f32 branch, token gate, both norms, bf16 and MXFP4 out:
-// 126 us, 5.6 TB/s. 2048 rows of 2560 in f16 with an element gate: 14.5 us, 3.6 TB/s: 14 rows an SM, too few rounds of
-// load, two reductions and store to hide one another. One row of 2048: 2.8 us, a launch.
+// 126 us, 5.6 TB/s. 2048 rows of 2560 in f16 with an element gate: 14.6 us, 3.6 TB/s: 14 rows an SM, too few rounds of
+// load, two reductions and store to hide one another. One row of 2048: 2.8 us, a launch. f32 branch, both norms, bf16:
+// 4096 rows of 2048 in 19 us, of 2047 in 103 (local memory); 2048 of 8192 in 34 us, 5.0 TB/s; 1024 of 16384 in 51 (f16: 35).
 // Eight values as they lie in memory.
 template <int DT>
 struct Raw {
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 512 ? 2 : 1) k_block_norm(const 
                            : static_cast<const T*>(p.gate) + (p.gate_kind == EXL3B_GATE_ELEMENT ? row * p.gate_pitch : 0);
         const float token = p.gate_kind == EXL3B_GATE_TOKEN && live ? static_cast<const float*>(p.gate)[row] : 0.f;
         // An element gate's registers leave few rows in flight: the next row's lines are asked into L2 meanwhile (9600 x 4096
-        // 77.8 and 73.7 us, 2048 x 2560 15.5 and 15.0; not for 128 threads a row, 4096 x 2048 19.7 and 20.6; the other gates
+        // 77.8 and 73.7 us, 2048 x 2560 15.5 without; not for 128 threads a row, 4096 x 2048 19.7 and 20.6; the other gates
         // gain nothing)
         if (VEC && p.gate_kind == EXL3B_GATE_ELEMENT && tpr > 128 && row + step < p.rows) {
 #pragma unroll
