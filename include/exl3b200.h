@@ -442,10 +442,11 @@ int     exl3b200_mx4_tile_scales(const uint8_t* scales, int64_t scales_pitch, in
  * Each output is rounded once to y_dtype (RAD_F32, RAD_F16, RAD_BF16, or EXL3B_MX4: codes and scales as mx4_quantize
  * makes them of the f32 values). Rows outside [expert_offset[0], expert_offset[n_expert]) and dropped slots
  * (sorted_tok < 0) are zero, as the EXL3 rows leave them: beside EXL3 experts in one buffer it is called first, over its
- * part of the offsets, and exl3b200_moe_op_live then, which leaves the rows outside its own runs. expert_offset NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and
- * slot i is i. dtype: RAD_F16, RAD_BF16, or EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form).
- * Pitches in elements (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32), at most
- * 2^26, n_out of 8 (MXFP4 out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048. */
+ * part of the offsets, and exl3b200_moe_op_live then, which leaves the rows outside its own runs. expert_offset, in
+ * ascending order, NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and slot i is i. dtype:
+ * RAD_F16, RAD_BF16, or EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form). Pitches in elements
+ * (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32), at most 2^26, n_out of 8 (MXFP4
+ * out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048. */
 enum { EXL3B_ACT_NONE = 0, EXL3B_ACT_SILU_MUL = 1 };
 typedef struct Exl3bGroupedMm {
     int64_t        n_expert, n_rows, n_out, n_in;

@@ -4,9 +4,9 @@ tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (inc
 A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
 `run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). Every entry's default is torch's
 current stream. The tensors' contents may change between runs, their addresses may not. A call's tensors share one GPU, which
-is the current device when it runs.
-torch only holds memory here. Tensors that do not fit one another are a ValueError; what the library refuses is a
-RuntimeError with its status. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales [rows, cols / 32]."""
+is the current device when it runs. torch only holds memory here. Tensors that do not fit one another are a ValueError; what
+the library refuses is a RuntimeError with its status. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales
+[rows, cols / 32]."""
 import ctypes as C
 
 import torch
