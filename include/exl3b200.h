@@ -435,6 +435,53 @@ int64_t exl3b200_mx4_tiled_bytes(int64_t n_expert, int64_t rows, int64_t cols, i
 int     exl3b200_mx4_tile_scales(const uint8_t* scales, int64_t scales_pitch, int64_t expert_pitch, int64_t n_expert,
                                  int64_t rows, int64_t cols, int act, void* tiled, void* stream);
 
+/* FP8 rows (dtype EXL3B_F8): e4m3 bytes [rows][cols] with an f32 scale for each 128 values of a row, scales
+ * [rows][ceil(cols / 128)]; a value is its code times its block's scale.
+ *   f8_quantize:   x (f32 / f16 / bf16) -> codes, scales. With m = max(max |x| of the block, 2^-110), in f32 with one rounding
+ *                  an operation: scale = m / 448, code = e4m3(x * (448 / m)), to nearest, ties to even; pow2 != 0: scale = the
+ *                  least power of two from m / 448 on, code = e4m3(x / scale). A block with a NaN or an infinity: scale NaN,
+ *                  codes 0.
+ *   f8_dequantize: code * scale in f32, rounded to y's type.
+ * Pitches in elements of their array. cols a multiple of 8; rows of x and y on 16-byte boundaries, codes on 8-byte ones
+ * (grouped_mm: 16). */
+enum { EXL3B_F8 = RAD_DT_PLUGIN_BASE + 0x3B8 };
+int     exl3b200_f8_quantize(const void* x, int x_dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* codes,
+                             int64_t codes_pitch, float* scales, int64_t scales_pitch, int pow2, void* stream);
+int     exl3b200_f8_dequantize(const uint8_t* codes, int64_t codes_pitch, const float* scales, int64_t scales_pitch,
+                               int64_t rows, int64_t cols, void* y, int y_dtype, int64_t y_pitch, void* stream);
+
+/* router: which experts a token goes to, beside router_topk (softmax over all, the top_k) for models that route otherwise:
+ *   s[e] = exp(l[e]) / sum_j exp(l[j])  or  1 / (1 + exp(-l[e]));  c[e] = s[e] + bias[e]  (bias f32 [n_expert], or NULL)
+ *   of n_group groups of n_expert / n_group neighbouring experts the group_keep stay whose group_top (1 or 2) largest c have
+ *   the largest sum; of their experts the top_k with the largest c are chosen, in descending order -> ids i32 [n_tok][top_k]
+ *   w f32 [n_tok][top_k] = scale * s of each, divided first by their sum over the chosen ones (renorm)
+ * Ties go to the lower group and the lower expert, and scores compare as the real numbers do: by the logits, or in 64 bits
+ * where a bias or a sum of two needs it. Masked experts, never chosen: a logit or a c that is -inf or NaN (their logits add
+ * nothing to the softmax); +inf logits count as the largest f32. A slot for which no expert is left: id -1, w 0.
+ * sorted_tok i32 [n_tok * top_k] and expert_offset i32 [n_local + 1], if given: moe_scatter of the ids over
+ * [expert_base, expert_base + n_local), `work` as moe_scatter's (with up to 2048 pairs it may be NULL); one launch for up to 32
+ * tokens and 1024 local experts. logits f32 / f16 / bf16, their row pitch in elements. n_expert <= 2048, a multiple of n_group
+ * <= 32 (no power of two of them: up to 1024 experts always, more while 64 a lane hold a group); top_k <= 32 and no more than
+ * the kept groups hold. */
+enum { EXL3B_SCORE_SOFTMAX = 0, EXL3B_SCORE_SIGMOID = 1 };
+typedef struct Exl3bRouter {
+    int64_t      n_tok, n_expert, top_k;
+    int32_t      dtype, score;
+    int32_t      n_group, group_keep, group_top, renorm;
+    float        scale;
+    int32_t      pad0;
+    const void*  logits;
+    int64_t      logits_pitch;
+    const float* bias;
+    int32_t*     ids;
+    float*       w;
+    int64_t      n_local, expert_base;
+    int32_t*     sorted_tok;
+    int32_t*     expert_offset;
+    void*        work;
+} Exl3bRouter;
+int     exl3b200_router(const Exl3bRouter* router, void* stream);
+
 /* grouped_mm: the routing contract's rows (moe_scatter's sorted_tok and expert_offset) times their expert's weight.
  * Sorted row i of expert e, t = sorted_tok[i] / top_k (top_k 0: the row of x is i itself):
  *   z[n] = sum over k of x[t][k] * w[e][n][k]  in f32;  act NONE: y[i][n] = z[n] for n < n_out;

@@ -16,6 +16,13 @@ int exl3b_cuda_mx4_tile(const uint8_t* s, int64_t s_pitch, int64_t e_pitch, int6
                         int act, int64_t n_blk, int64_t n_k, void* out, void* stream);
 int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream);
 int exl3b_gmm_max_expert(void);
+/* exl3b200_route.cu, exl3b200_f8.cu */
+int exl3b_route_fuses(int64_t n_tok, int64_t n_local);
+int exl3b_cuda_route(const Exl3bRouteOp* p, int dtype, int fused, void* stream);
+int exl3b_cuda_f8_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
+                           int64_t q_pitch, float* s, int64_t s_pitch, int pow2, void* stream);
+int exl3b_cuda_f8_dequantize(const uint8_t* q, int64_t q_pitch, const float* s, int64_t s_pitch, int64_t rows, int64_t cols,
+                             void* y, int dtype, int64_t y_pitch, void* stream);
 int exl3b_cuda_device_info(int* sm_count, int32_t** err_word);
 
 /* Largest sizes taken: rows and columns that 32-bit coordinates hold, norm rows that a block holds in registers. */
@@ -122,6 +129,95 @@ int exl3b200_mx4_dequantize(const uint8_t* codes, int64_t codes_pitch, const uin
     if (mis(y, 16) || y_pitch * size_of(y_dtype) % 16 || mis(codes, 4) || codes_pitch % 4) return RAD_E_ALIGN;
     return rc_of(exl3b_cuda_mx4_dequantize(codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype, y_pitch,
                                            stream));
+}
+
+/* FP8 rows: eight values a lane, 1024 lanes a block of the grid. */
+static int check_f8(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 8 || cols % 8 || rows > kMaxDim || cols > kMaxDim) return RAD_E_SHAPE;
+    return rows * ((cols + 127) / 128 * 16) > (int64_t)INT32_MAX * 1024 ? RAD_E_SHAPE : RAD_OK;
+}
+
+int exl3b200_f8_quantize(const void* x, int x_dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* codes,
+                         int64_t codes_pitch, float* scales, int64_t scales_pitch, int pow2, void* stream) {
+    const int rc = check_f8(rows, cols);
+    if (rc) return rc;
+    if (!is_float(x_dtype)) return RAD_E_DTYPE;
+    if (rows == 0) return RAD_OK;
+    if (!x || !codes || !scales) return RAD_E_INVAL;
+    if (x_pitch < cols || codes_pitch < cols || scales_pitch < (cols + 127) / 128) return RAD_E_STRIDE;
+    if (mis(x, 16) || x_pitch * size_of(x_dtype) % 16 || mis(codes, 8) || codes_pitch % 8 || mis(scales, 4))
+        return RAD_E_ALIGN;
+    return rc_of(exl3b_cuda_f8_quantize(x, x_dtype, x_pitch, rows, cols, codes, codes_pitch, scales, scales_pitch, pow2 != 0,
+                                        stream));
+}
+
+int exl3b200_f8_dequantize(const uint8_t* codes, int64_t codes_pitch, const float* scales, int64_t scales_pitch,
+                           int64_t rows, int64_t cols, void* y, int y_dtype, int64_t y_pitch, void* stream) {
+    const int rc = check_f8(rows, cols);
+    if (rc) return rc;
+    if (!is_float(y_dtype)) return RAD_E_DTYPE;
+    if (rows == 0) return RAD_OK;
+    if (!y || !codes || !scales) return RAD_E_INVAL;
+    if (y_pitch < cols || codes_pitch < cols || scales_pitch < (cols + 127) / 128) return RAD_E_STRIDE;
+    if (mis(y, 16) || y_pitch * size_of(y_dtype) % 16 || mis(codes, 8) || codes_pitch % 8 || mis(scales, 4))
+        return RAD_E_ALIGN;
+    return rc_of(exl3b_cuda_f8_dequantize(codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype, y_pitch, stream));
+}
+
+int exl3b200_router(const Exl3bRouter* d, void* stream) {
+    if (!d) return RAD_E_INVAL;
+    if (!is_float(d->dtype)) return RAD_E_DTYPE;
+    if ((d->score != EXL3B_SCORE_SOFTMAX && d->score != EXL3B_SCORE_SIGMOID) || !(d->scale - d->scale == 0.f)) return RAD_E_INVAL;
+    const int64_t E = d->n_expert, G = d->n_group;
+    if (d->n_tok < 0 || E < 1 || E > 2048 || d->top_k < 1 || d->top_k > 32 || d->n_tok > INT32_MAX / d->top_k || G < 1 ||
+        G > 32 || E % G || d->group_keep < 1 || d->group_keep > G || d->group_top < 1 || d->group_top > 2 ||
+        d->top_k > E / G * d->group_keep)
+        return RAD_E_SHAPE;
+    int lanes = 32;                      /* of a group */
+    while (lanes * G > 32) lanes /= 2;
+    const int64_t per = (E / G + lanes - 1) / lanes;
+    if (per > 64) return RAD_E_SHAPE;
+    const int sort = d->expert_offset != 0;
+    if (d->n_tok > 0 && sort != (d->sorted_tok != 0)) return RAD_E_INVAL;
+    if (sort && (d->n_local < 1 || d->n_local > 16384)) return RAD_E_SHAPE;
+    if (sort && d->n_tok * d->top_k > 2048 && !d->work) return RAD_E_INVAL;
+    if (d->n_tok > 0 && (!d->logits || !d->ids || !d->w)) return RAD_E_INVAL;
+    if (d->n_tok > 0 && d->logits_pitch < E) return RAD_E_STRIDE;
+    if (mis(d->logits, size_of(d->dtype)) || mis(d->bias, 4) || mis(d->ids, 4) || mis(d->w, 4) || mis(d->sorted_tok, 4) ||
+        mis(d->expert_offset, 4) || (sort && mis(d->work, 4)))
+        return RAD_E_ALIGN;
+    if (d->n_tok > 0) {
+        const int fused = sort && exl3b_route_fuses(d->n_tok, d->n_local);
+        Exl3bRouteOp p;
+        memset(&p, 0, sizeof p);
+        p.n_tok = d->n_tok;
+        p.logits = d->logits;
+        p.logits_pitch = d->logits_pitch;
+        p.bias = d->bias;
+        p.score = d->score;
+        p.top_k = (int32_t)d->top_k;
+        p.renorm = d->renorm != 0;
+        p.n_group = d->n_group;
+        p.group_keep = d->group_keep;
+        p.group_top = d->group_top;
+        p.group_size = (int32_t)(E / G);
+        p.group_lanes = lanes;
+        p.lane_experts = (int32_t)per;
+        p.scale = d->scale;
+        p.ids = d->ids;
+        p.w = d->w;
+        p.sorted_tok = d->sorted_tok;
+        p.expert_offset = d->expert_offset;
+        p.expert_base = d->expert_base;
+        p.n_local = (int32_t)d->n_local;
+        const int rc = exl3b_cuda_route(&p, d->dtype, fused, stream);
+        if (rc || fused) return rc_of(rc);
+    }
+    if (!sort) return RAD_OK;
+    if (d->n_tok == 0)                   /* no pairs: neither array is looked at */
+        return exl3b200_moe_scatter(d->expert_offset, 0, d->n_local, 0, d->expert_offset, d->expert_offset, 0, stream);
+    return exl3b200_moe_scatter(d->ids, d->n_tok * d->top_k, d->n_local, d->expert_base, d->sorted_tok, d->expert_offset,
+                                d->work, stream);
 }
 
 /* Blocks of 128 weight rows (silu_mul: 64 gate + 64 up), padded to pairs; 128-column tiles, padded to pairs. */

@@ -78,6 +78,23 @@ typedef struct Exl3bGmmOp {
     int32_t*       err;                  /* device word: set nonzero when a bounded wait gives up */
 } Exl3bGmmOp;
 
+/* router (exl3b200_route.cu). A group has group_lanes lanes of a warp, each lane_experts neighbouring experts of it. */
+typedef struct Exl3bRouteOp {
+    int64_t      n_tok;
+    const void*  logits;
+    int64_t      logits_pitch;           /* elements */
+    const float* bias;
+    int32_t      score, top_k, renorm;
+    int32_t      n_group, group_keep, group_top, group_size, group_lanes, lane_experts;
+    float        scale;
+    int32_t*     ids;
+    float*       w;
+    int32_t*     sorted_tok;             /* the sort in the same launch */
+    int32_t*     expert_offset;
+    int64_t      expert_base;
+    int32_t      n_local;
+} Exl3bRouteOp;
+
 #ifdef __cplusplus
 }
 #endif

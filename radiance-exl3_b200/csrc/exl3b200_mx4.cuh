@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "exl3b200_rows.cuh"
+
 namespace exl3b {
 
 constexpr uint32_t kMx4Nan = 255;
@@ -49,50 +51,6 @@ __device__ __forceinline__ uint32_t mx4_quad_code(const float v[8]) {
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
     return mx4_scale_code(m);
-}
-
-// ------------------------------------------------------------------------------------------ rows of 8 values
-// dtype codes: RAD_F32 1, RAD_F16 2, RAD_BF16 3 (include/rad_types.h).
-template <int DT>
-struct El;
-template <>
-struct El<1> {
-    typedef float T;
-    static __device__ __forceinline__ float to(float v) { return v; }
-    static __device__ __forceinline__ float from(float v) { return v; }
-};
-template <>
-struct El<2> {
-    typedef __half T;
-    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
-};
-template <>
-struct El<3> {
-    typedef __nv_bfloat16 T;
-    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
-};
-
-// Eight consecutive values at a 16-byte aligned address.
-__device__ __forceinline__ void ld8(const float* p, float v[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <int DT>
-__device__ __forceinline__ void st8(void* p, const float v[8]) {
-    if constexpr (DT == 1) {
-        *static_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *(static_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        typedef typename El<DT>::T T;
-        uint4 a;
-        T* e = reinterpret_cast<T*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = El<DT>::from(v[i]);
-        *static_cast<uint4*>(p) = a;
-    }
 }
 
 }  // namespace exl3b

@@ -28,26 +28,6 @@ namespace {
 // 126 us, 5.6 TB/s. 2048 rows of 2560 in f16 with an element gate: 14.6 us, 3.6 TB/s: 14 rows an SM, too few rounds of
 // load, two reductions and store to hide one another. One row of 2048: 2.8 us, a launch. f32 branch, both norms, bf16:
 // 4096 rows of 2048 in 19 us, of 2047 in 103 (local memory); 2048 of 8192 in 34 us, 5.0 TB/s; 1024 of 16384 in 51 (f16: 35).
-// Eight values as they lie in memory.
-template <int DT>
-struct Raw {
-    typedef typename El<DT>::T T;
-    uint4 q[DT == 1 ? 2 : 1];
-    __device__ __forceinline__ void clear() {
-        q[0] = make_uint4(0u, 0u, 0u, 0u);
-        if (DT == 1) q[DT == 1] = q[0];
-    }
-    __device__ __forceinline__ void fetch(const T* p) {
-        q[0] = *reinterpret_cast<const uint4*>(p);
-        if (DT == 1) q[DT == 1] = *(reinterpret_cast<const uint4*>(p) + 1);
-    }
-    __device__ __forceinline__ void set(int e, T v) { reinterpret_cast<T*>(q)[e] = v; }
-    __device__ __forceinline__ void get(float x[8]) const {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = El<DT>::to(reinterpret_cast<const T*>(q)[e]);
-    }
-};
-
 // r / (1 + e^-g), within 2^-19 of the value down to the bottom of f32's range. From kGateLow up both functions are the
 // special-function unit's; below it, rare enough for a branch, the rounding of the exponential's argument would pass that
 // bound, and below -60, where 1 + e^-g is e^-g to every bit, r e^(g/2) e^(g/2) stays in range while the value does.
@@ -280,24 +260,6 @@ int launch_norm(const Exl3bNormOp* p, bool vec, int sm_count, cudaStream_t st) {
 // 2048: 2.8 us each, a launch.
 constexpr int kUnroll = 4;
 
-// Vector i's row and place in it; BIG: vectors past 2^31, a 64-bit division.
-template <bool BIG>
-__device__ __forceinline__ void row_of(int64_t i, const Exl3bDiv& v, int64_t* row, int* vec) {
-    if (BIG) {
-        *row = i / v.d;
-        *vec = (int)(i - *row * v.d);
-    } else {
-        const uint32_t n = (uint32_t)i, q = exl3b_div_of(n, v);
-        *row = q;
-        *vec = (int)(n - q * v.d);
-    }
-}
-
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 // The scale code of a block whose 32 values four neighbouring lanes hold. 16-bit types: the magnitudes two a word, which
 // order as integers too.
 template <int DT>

@@ -1,21 +1,24 @@
-"""dense.py -- experts whose weights are not EXL3 records (f16, bf16 or MXFP4) and the norms around a block, over torch
-tensors: grouped_mm, block_norm and the MXFP4 conversions of libexl3b200.so (include/exl3b200.h).
+"""dense.py -- experts whose weights are not EXL3 records (f16, bf16, FP8 or MXFP4), the router before them and the norms
+around a block, over torch tensors: grouped_mm, router, block_norm and the FP8 and MXFP4 conversions of libexl3b200.so
+(include/exl3b200.h).
 
-A GroupedMm or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
+A GroupedMm, Router or BlockNorm is a plan: it reads its tensors' addresses, shapes and strides once, keeps the tensors alive, and
 `run(stream)` enqueues the call on a cudaStream_t (an integer; 0 the legacy default stream). Every entry's default is torch's
 current stream. The tensors' contents may change between runs, their addresses may not. A call's tensors share one GPU, which
 is the current device when it runs. torch only holds memory here. Tensors that do not fit one another are a ValueError; what
 the library refuses is a RuntimeError with its status. MXFP4 rows are two uint8 tensors: codes [rows, cols / 2] and scales
-[rows, cols / 32]."""
+[rows, cols / 32]. FP8 rows: codes of float8_e4m3fn [rows, cols] and f32 scales [rows, ceil(cols / 128)]."""
 import ctypes as C
 
 import torch
 
-from .native import BlockNormDesc, ExpertBlockDesc, GroupedMmDesc, Native
+from .native import BlockNormDesc, ExpertBlockDesc, GroupedMmDesc, Native, RouterDesc
 
 MX4 = 1024 + 0x3B4                      # EXL3B_MX4
+F8 = 1024 + 0x3B8                       # EXL3B_F8
 DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 ACTS = {"none": 0, "silu_mul": 1}
+SCORES = {"softmax": 0, "sigmoid": 1}
 GATES = {"none": 0, "token": 1, "channel": 2, "element": 3}
 
 _native = None
@@ -122,6 +125,47 @@ def mx4_tile_scales(scales, act="none", stream=None):
     return out
 
 
+# ------------------------------------------------------------------------------------------------ FP8
+def f8_empty(rows, cols, device="cuda"):
+    """(codes, scales) for `rows` rows of `cols` values; the scales' rows 16 bytes apart or a multiple, which GroupedMm
+    reads fastest."""
+    blocks = (cols + 127) // 128
+    return (torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.float32, device=device)[:, :blocks])
+
+
+def _f8_rows(x, codes, scales, name):
+    """Both conversions' checks: (address, type, pitch) of x, (address, pitch) of the codes and of the scales."""
+    if x.dim() != 2:
+        raise ValueError(f"{name} has {x.dim()} dimensions, not 2")
+    rows, cols = x.shape
+    dev = x.get_device()
+    xp, pitch = _rows(x, name, dev)
+    at = _rows(codes, "codes", dev, (rows, cols), torch.float8_e4m3fn)
+    at += _rows(scales, "scales", dev, (rows, (cols + 127) // 128), torch.float32)
+    if _several:
+        _check_current(dev)
+    return dev, (xp, _dtype(x), pitch), at
+
+
+def f8_quantize(x, codes, scales, pow2=False, stream=None):
+    """x [rows, cols] in f32, f16 or bf16 -> its e4m3 codes and their scales (pow2: powers of two)."""
+    dev, (xp, dt, pitch), at = _f8_rows(x, codes, scales, "x")
+    rc = native().lib.exl3b200_f8_quantize(xp, dt, pitch, *x.shape, *at, pow2, _current_stream(dev) if stream is None else stream)
+    if rc:
+        raise RuntimeError(f"exl3b200_f8_quantize: status {rc}")
+    return codes, scales
+
+
+def f8_dequantize(codes, scales, y, stream=None):
+    """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
+    dev, (yp, dt, pitch), at = _f8_rows(y, codes, scales, "y")
+    rc = native().lib.exl3b200_f8_dequantize(*at, *y.shape, yp, dt, pitch, _current_stream(dev) if stream is None else stream)
+    if rc:
+        raise RuntimeError(f"exl3b200_f8_dequantize: status {rc}")
+    return y
+
+
 # ------------------------------------------------------------------------------------------------ plans
 class _Plan:
     _entry = None
@@ -179,6 +223,48 @@ class GroupedMm(_Plan):
         if sorted_tok is not None:
             d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", dev, (d.n_rows,), torch.int32)
         self._finish(d, dev, x, w, y, expert_offset, sorted_tok, x_scales, w_scales, y_scales)
+
+
+class Router(_Plan):
+    """Which experts a token goes to: scores ("softmax" or "sigmoid" of logits [tokens, experts]), compared with bias [experts]
+    f32 added, the keep_groups best of `groups` groups (by the sum of their group_top best), the top_k best of those ->
+    ids [tokens, top_k] i32 (-1 where none is left) and w [tokens, top_k] f32: the scores without the bias, divided by their sum
+    (renorm), times scale. logits in f32, f16 or bf16.
+
+    sorted_tok [tokens * top_k] and expert_offset [local experts + 1] i32 (both or neither): the pairs sorted over the experts
+    from expert_base on, as GroupedMm reads them. A plan that sorts has a work buffer: its runs come one after another."""
+    _entry = "exl3b200_router"
+
+    def __init__(self, *, logits, top_k, ids, w, score="softmax", bias=None, groups=1, keep_groups=1, group_top=1, renorm=False,
+                 scale=1.0, sorted_tok=None, expert_offset=None, expert_base=0):
+        d = RouterDesc()
+        if logits.dim() != 2:
+            raise ValueError(f"logits have {logits.dim()} dimensions, not 2")
+        dev = logits.get_device()
+        d.n_tok, d.n_expert = logits.shape
+        d.top_k, d.score, d.renorm, d.scale = top_k, SCORES[score], renorm, scale
+        d.n_group, d.group_keep, d.group_top = groups, keep_groups, group_top
+        d.logits, d.logits_pitch = _rows(logits, "logits", dev)
+        d.dtype = _dtype(logits)
+        if bias is not None:
+            d.bias, _ = _rows(bias, "bias", dev, (d.n_expert,), torch.float32)
+        for name, t, kind in (("ids", ids, torch.int32), ("w", w, torch.float32)):
+            p, _ = _rows(t, name, dev, (d.n_tok, top_k), kind)
+            if not t.is_contiguous():
+                raise ValueError(f"{name} is strided")
+            setattr(d, name, p)
+        work = None
+        if sorted_tok is not None or expert_offset is not None:
+            d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", dev, (d.n_tok * top_k,), torch.int32)
+            d.expert_offset, _ = _rows(expert_offset, "expert_offset", dev, dtype=torch.int32)
+            if expert_offset.dim() != 1 or len(expert_offset) < 2:
+                raise ValueError(f"expert_offset has shape {tuple(expert_offset.shape)}, not (local experts + 1,)")
+            d.n_local, d.expert_base = len(expert_offset) - 1, expert_base
+            work = torch.empty(native().scatter_work_bytes(d.n_tok * top_k, d.n_local), dtype=torch.uint8, device=logits.device)
+            d.work = work.data_ptr()
+            # a run may come on any stream: whatever used the buffer's memory before is done by then
+            torch.cuda.current_stream(dev).synchronize()
+        self._finish(d, dev, logits, bias, ids, w, sorted_tok, expert_offset, work)
 
 
 class BlockNorm(_Plan):

@@ -74,6 +74,14 @@ class BlockNormDesc(C.Structure):
         ("y_codes", _VP), ("y_codes_pitch", _I64), ("y_scales", _VP), ("y_scales_pitch", _I64)]
 
 
+class RouterDesc(C.Structure):
+    """Exl3bRouter (include/exl3b200.h)."""
+    _fields_ = [(n, _I64) for n in ("n_tok", "n_expert", "top_k")] + [
+        (n, C.c_int32) for n in ("dtype", "score", "n_group", "group_keep", "group_top", "renorm")] + [
+        ("scale", C.c_float), ("pad0", C.c_int32), ("logits", _VP), ("logits_pitch", _I64), ("bias", _VP), ("ids", _VP),
+        ("w", _VP), ("n_local", _I64), ("expert_base", _I64), ("sorted_tok", _VP), ("expert_offset", _VP), ("work", _VP)]
+
+
 class ExpertBlockDesc(C.Structure):
     """Exl3bExpertBlockDesc (include/exl3b200.h)."""
     _fields_ = [(n, _I64) for n in ("n_expert", "hidden", "width", "top_k")] + [
@@ -185,9 +193,12 @@ class Native:
         L.exl3b200_expert_block_carve.argtypes = [C.POINTER(ExpertBlockDesc), _I64, _VP, _I64, C.POINTER(ExpertBlockBufs)]
         L.exl3b200_expert_block_forward.argtypes = [C.POINTER(ExpertBlockDesc), C.POINTER(ExpertBlockBufs), _VP, _I64, _VP,
                                                     _VP, _VP]
+        L.exl3b200_f8_quantize.argtypes = [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _I, _VP]
+        L.exl3b200_f8_dequantize.argtypes = [_VP, _I64, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP]
         # descriptors by address: a plan takes its own once (ctypes.addressof), not a byref a call
         L.exl3b200_grouped_mm.argtypes = [_VP, _VP]
         L.exl3b200_block_norm.argtypes = [_VP, _VP]
+        L.exl3b200_router.argtypes = [_VP, _VP]
 
     @staticmethod
     def _check(rc, what):
