@@ -491,9 +491,13 @@ int     exl3b200_router(const Exl3bRouter* router, void* stream);
  * (sorted_tok < 0) are zero, as the EXL3 rows leave them: beside EXL3 experts in one buffer it is called first, over its
  * part of the offsets, and exl3b200_moe_op_live then, which leaves the rows outside its own runs. expert_offset, in
  * ascending order, NULL: one expert holding every row; sorted_tok NULL: no dropped slot, and slot i is i. dtype:
- * RAD_F16, RAD_BF16, or EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form). Pitches in elements
- * (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32), at most 2^26, n_out of 8 (MXFP4
- * out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048. */
+ * RAD_F16, RAD_BF16, EXL3B_MX4 (x and w codes, x_scales row by row, w_scales the tiled form), or EXL3B_F8. Pitches in elements
+ * (two MXFP4 codes a byte), scale pitches in bytes. n_in a multiple of 8 (MXFP4: 32, FP8: 16), at most 2^26, n_out of 8
+ * (MXFP4 out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048.
+ * EXL3B_F8: x and w e4m3 codes, x_scales f32 [x_rows][ceil(n_in / 128)] as f8_quantize writes them, w_scales f32, dense,
+ * [n_expert][blocks][ceil(n_in / 128)], one for 128 weight rows x 128 inputs (SILU_MUL: ceil(n_out / 128) blocks of gate rows
+ * and then as many of up rows): z[n] = sum over blocks b of 128 k of x_scales[t][b] * w_scales[e][n / 128][b] * (the sum over
+ * k of b), each such sum on the tensor cores, the blocks and their scales in f32. y in f32, f16 or bf16. */
 enum { EXL3B_ACT_NONE = 0, EXL3B_ACT_SILU_MUL = 1 };
 typedef struct Exl3bGroupedMm {
     int64_t        n_expert, n_rows, n_out, n_in;

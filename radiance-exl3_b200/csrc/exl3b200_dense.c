@@ -5,7 +5,7 @@
 
 #include <string.h>
 
-/* exl3b200_norm.cu, exl3b200_gmm.cu, exl3b200_moe.cu */
+/* exl3b200_norm.cu, exl3b200_gmm.cu, exl3b200_gmm8.cu, exl3b200_moe.cu */
 int exl3b_cuda_block_norm(const Exl3bNormOp* p, int dtype, int branch_dtype, int vec, int sm_count,
                           void* stream);
 int exl3b_cuda_mx4_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
@@ -15,6 +15,7 @@ int exl3b_cuda_mx4_dequantize(const uint8_t* q, int64_t q_pitch, const uint8_t* 
 int exl3b_cuda_mx4_tile(const uint8_t* s, int64_t s_pitch, int64_t e_pitch, int64_t n_expert, int64_t rows, int64_t cols,
                         int act, int64_t n_blk, int64_t n_k, void* out, void* stream);
 int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream);
+int exl3b_cuda_gmm8(const Exl3bGmmOp* p, int sm_count, void* stream);
 int exl3b_gmm_max_expert(void);
 /* exl3b200_route.cu, exl3b200_f8.cu */
 int exl3b_route_fuses(int64_t n_tok, int64_t n_local);
@@ -246,33 +247,34 @@ int exl3b200_mx4_tile_scales(const uint8_t* scales, int64_t scales_pitch, int64_
 
 int exl3b200_grouped_mm(const Exl3bGroupedMm* d, void* stream) {
     if (!d) return RAD_E_INVAL;
-    const int mx = d->dtype == EXL3B_MX4, mx_out = d->y_dtype == EXL3B_MX4;
-    if (!mx && d->dtype != RAD_F16 && d->dtype != RAD_BF16) return RAD_E_DTYPE;
-    if (!mx_out && !is_float(d->y_dtype)) return RAD_E_DTYPE;
+    const int mx = d->dtype == EXL3B_MX4, f8 = d->dtype == EXL3B_F8, mx_out = d->y_dtype == EXL3B_MX4;
+    if (!mx && !f8 && d->dtype != RAD_F16 && d->dtype != RAD_BF16) return RAD_E_DTYPE;
+    if ((!mx_out || f8) && !is_float(d->y_dtype)) return RAD_E_DTYPE;
     if (d->act != EXL3B_ACT_NONE && d->act != EXL3B_ACT_SILU_MUL) return RAD_E_INVAL;
     if (d->n_expert < 1 || d->n_expert > exl3b_gmm_max_expert() || d->n_rows < 0 || d->n_rows > kMaxDim ||
         d->x_rows < 0 || d->x_rows > kMaxDim || d->top_k < 0 || d->top_k > 4096 || d->n_out < 8 || d->n_out % 8 ||
-        d->n_out > kMaxDim / 2 || d->n_in < 8 || d->n_in > kMaxIn || d->n_in % (mx ? 32 : 8) ||
+        d->n_out > kMaxDim / 2 || d->n_in < 8 || d->n_in > kMaxIn || d->n_in % (mx ? 32 : f8 ? 16 : 8) ||
         (mx_out && d->n_out % 32))
         return RAD_E_SHAPE;
     if (d->n_rows == 0) return RAD_OK;
-    if (!d->x || !d->w || !d->y || (mx && (!d->x_scales || !d->w_scales)) || (mx_out && !d->y_scales)) return RAD_E_INVAL;
+    if (!d->x || !d->w || !d->y || ((mx || f8) && (!d->x_scales || !d->w_scales)) || (mx_out && !d->y_scales)) return RAD_E_INVAL;
     if (!d->expert_offset && d->n_expert != 1) return RAD_E_INVAL;
     if (d->x_rows < 1 || (d->top_k == 0 && d->x_rows < d->n_rows) ||
         (d->top_k > 0 && !d->sorted_tok && d->x_rows < (d->n_rows + d->top_k - 1) / d->top_k))
         return RAD_E_SHAPE;
-    const int64_t w_rows = d->act ? 2 * d->n_out : d->n_out;
+    const int64_t w_rows = d->act ? 2 * d->n_out : d->n_out, kb = (d->n_in + 127) / 128;
     /* units are counted in 32 bits: a group each 32 rows and an expert, a block each 64 outputs */
     if ((d->n_rows / 32 + d->n_expert + 1) * (d->n_out / 64 + 1) > INT32_MAX) return RAD_E_SHAPE;
     if (d->x_pitch < d->n_in || d->w_pitch < d->n_in || (d->n_expert > 1 && d->w_expert_pitch < w_rows * d->w_pitch) ||
         d->y_pitch < d->n_out || (mx && d->x_scales_pitch < d->n_in / 32) ||
-        (mx_out && d->y_scales_pitch < d->n_out / 32))
+        (f8 && d->x_scales_pitch < kb * 4) || (mx_out && d->y_scales_pitch < d->n_out / 32))
         return RAD_E_STRIDE;
     /* TMA reads rows that start on 16-byte boundaries; stores are 16 bytes (MXFP4 codes: 4) */
-    const int64_t xe = mx ? 32 : 8, ye = mx_out ? 8 : 16 / size_of(d->y_dtype);
+    const int64_t xe = mx ? 32 : f8 ? 16 : 8, ye = mx_out ? 8 : 16 / size_of(d->y_dtype);
     if (mis(d->x, 16) || mis(d->w, 16) || d->x_pitch % xe || d->w_pitch % xe ||
         (d->n_expert > 1 && d->w_expert_pitch % xe) || mis(d->y, mx_out ? 4 : 16) || d->y_pitch % ye ||
-        (mx && mis(d->w_scales, 16)) || mis(d->sorted_tok, 4) || mis(d->expert_offset, 4))
+        (mx && mis(d->w_scales, 16)) || (f8 && (mis(d->x_scales, 4) || d->x_scales_pitch % 4 || mis(d->w_scales, 4))) ||
+        mis(d->sorted_tok, 4) || mis(d->expert_offset, 4))
         return RAD_E_ALIGN;
     int sm = 0;
     int32_t* err = 0;
@@ -290,10 +292,11 @@ int exl3b200_grouped_mm(const Exl3bGroupedMm* d, void* stream) {
     p.act = d->act;
     p.y_dtype = d->y_dtype;
     p.x = d->x;
-    p.x_pitch_bytes = mx ? d->x_pitch / 2 : d->x_pitch * 2;
+    const int64_t half_bytes = mx ? 1 : f8 ? 2 : 4;
+    p.x_pitch_bytes = d->x_pitch * half_bytes / 2;
     p.w = d->w;
-    p.w_pitch_bytes = mx ? d->w_pitch / 2 : d->w_pitch * 2;
-    p.w_expert_bytes = d->n_expert > 1 ? (mx ? d->w_expert_pitch / 2 : d->w_expert_pitch * 2) : w_rows * p.w_pitch_bytes;
+    p.w_pitch_bytes = d->w_pitch * half_bytes / 2;
+    p.w_expert_bytes = d->n_expert > 1 ? d->w_expert_pitch * half_bytes / 2 : w_rows * p.w_pitch_bytes;
     p.sorted_tok = d->sorted_tok;
     p.expert_offset = d->expert_offset;
     p.y = d->y;
@@ -305,8 +308,14 @@ int exl3b200_grouped_mm(const Exl3bGroupedMm* d, void* stream) {
     p.w_scales = (const uint8_t*)d->w_scales;
     p.ws_blk_bytes = tile_cols(d->n_in) * 512;
     p.ws_expert_bytes = tile_blocks(w_rows, d->act) * p.ws_blk_bytes;
+    if (f8) {
+        p.ws_blocks = (int32_t)((d->n_out + 127) / 128);
+        p.ws_blk_bytes = kb * 4;
+        p.ws_expert_bytes = p.ws_blocks * (d->act ? 2 : 1) * p.ws_blk_bytes;
+    }
     p.mx4 = mx;
+    p.f8 = f8;
     p.bf16 = d->dtype == RAD_BF16;
     p.err = err;
-    return rc_of(exl3b_cuda_gmm(&p, sm, stream));
+    return rc_of(f8 ? exl3b_cuda_gmm8(&p, sm, stream) : exl3b_cuda_gmm(&p, sm, stream));
 }

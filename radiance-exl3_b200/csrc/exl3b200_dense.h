@@ -72,9 +72,10 @@ typedef struct Exl3bGmmOp {
     int64_t        ys_pitch;
     const uint8_t* x_scales;
     int64_t        xs_pitch;
-    const uint8_t* w_scales;             /* the tiled form */
+    const uint8_t* w_scales;             /* the tiled form; FP8: rows of ws_blk_bytes, a block of 128 weight rows each */
     int64_t        ws_expert_bytes, ws_blk_bytes;
-    int32_t        mx4, bf16;
+    int32_t        ws_blocks;            /* FP8: such rows of a weight (silu_mul: of its gate half, as many of its up half) */
+    int32_t        mx4, f8, bf16;
     int32_t*       err;                  /* device word: set nonzero when a bounded wait gives up */
 } Exl3bGmmOp;
 

@@ -1,0 +1,562 @@
+// exl3b200_gmm8.cu -- grouped_mm over FP8 operands: e4m3 codes with an f32 scale for each 128 values of a row of x and each
+// 128 x 128 of a weight, on the 5th-generation tensor cores. sm_100a only.
+//
+//   z[n] = sum over blocks b of 128 k:  sx[t(i)][b] * sw[e][n / 128][b] * sum over k of b of x[t(i)][k] * w[e][n][k]
+//   y[i][n] = z[n], or silu(z[n]) * z[n_out + n] (act silu_mul), for every sorted row i of expert e
+//
+// The units of work, the operands' way into shared memory and the roles of the warps are grouped_mm's for 16-bit operands
+// (exl3b200_gmm.cu; exl3b200_gmm.cuh): weight rows are the MMA's M, sorted rows its N, a stage 128 bytes of k -- here one block
+// of 128. What differs is the sum over k. The scales are any f32 numbers, so the tensor cores' sums of one block cannot run on
+// into the next one's: each stage's four MMAs (kind::f8f6f4, K 32) start a fresh accumulator in tensor memory, one of several
+// in turn, and the summing warps, which hold the unit's sums in registers, add it times its scales:
+//   sum[n] = fma(d[n], sx * sw, sum[n])    in f32, one rounding a block of 128 and one for the scales' product
+// Three forms, as there: narrow (128 weight rows x up to 32 sorted rows, two CTAs an SM), SPLIT (narrow, a cluster a unit, each
+// CTA a part of its k) and PAIR (cta_group::2, 256 weight rows x up to 256 sorted rows).
+// Warps of a CTA:
+//   0       weights: cp.async.bulk.tensor, 128-byte swizzled
+//   1       MMA issuer (PAIR: of the even CTA; the odd one's reports its filled stages there)
+//   2, 3    scales: sx * sw of 128 (narrow: 32) sorted rows a warp into a ring of stages; silu_mul: for gate rows and up rows
+//   4..7    sorted rows: 16-byte cp.async through sorted_tok
+//   8..     sums: each warp 32 weight rows, half of the slices of 16 sorted rows (narrow: all), then its outputs
+// Every wait is bounded; one that gives up sets the error word, and every role then drains and leaves.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "exl3b200_chain.cuh"
+#include "exl3b200_decode.cuh"
+#include "exl3b200_dense.h"
+#include "exl3b200_gmm.cuh"
+
+using namespace exl3b;
+
+namespace {
+
+constexpr int kScaleSt = 4;                      // stages of scales at once, and what a lane loads of a row at a time
+
+template <bool PAIR, bool SPLIT, bool ACT>
+struct Cfg {
+    static constexpr int NT = PAIR ? 256 : 32;                   // sorted rows a unit at most
+    static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
+    static constexpr int SUM_G = PAIR ? 2 : 1;                   // groups of four summing warps
+    static constexpr int SLICES = NT / kSlice / SUM_G;           // of 16 sorted rows a group
+    static constexpr int THREADS = (kEpiWarp0 + 4 * SUM_G) * 32;
+    static constexpr int X_B = NL * kRowB;
+    static constexpr int STAGE_B = kW_B + X_B;
+    static constexpr int HALVES = ACT ? 2 : 1;                   // scales a sorted row: gate's, up's
+    static constexpr int SC_B = kScaleSt * HALVES * NT * 4;
+    static constexpr int SC_WARPS = PAIR ? 2 : 1;
+    static constexpr int EPI_B = SPLIT ? NT * kEpiLd * 4 : 4 * SUM_G * 1024;
+    static constexpr int DB = PAIR ? 2 : 4;                      // accumulators in turn
+    static constexpr int TMEM = DB * NT;
+    static constexpr int PER_SM = PAIR ? 1 : 2;
+    static constexpr int BARS = 2 * kMaxSt + 2 * DB + 2 * kScaleSt + 1;
+    static constexpr int fixed(int n_expert) { return 1024 + EPI_B + SC_B + 512 + (n_expert + 4) * 4; }
+    static constexpr int stages(int n_expert, int per_sm) {
+        const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kStatic - fixed(n_expert)) / STAGE_B;
+        return n < kMaxSt ? n : kMaxSt;
+    }
+    static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0 && stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4), "tensor or shared memory");
+    static_assert(BARS * 8 + 8 <= 512, "barriers");
+};
+
+// OUT: y_dtype; ACT: silu_mul.
+template <bool PAIR, bool SPLIT, int OUT, bool ACT>
+__global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLIT, ACT>::PER_SM)
+    k_gmm8(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
+    const int ST = sh.st, split = sh.split;
+    using C = Cfg<PAIR, SPLIT, ACT>;
+    constexpr int NT = C::NT, THREADS = C::THREADS, MB = PAIR ? 2 : 1, DB = C::DB;
+    constexpr int blk_out = ACT ? 64 : 128;                   // outputs a block (a CTA's part of a unit)
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* w_ring = smem;                                   // [ST][128 rows][128 B]
+    uint8_t* x_ring = w_ring + ST * kW_B;                     // [ST][NL rows][128 B]
+    float* sc_ring = reinterpret_cast<float*>(x_ring + ST * C::X_B);   // [kScaleSt][HALVES][NT]
+    float* epi = sc_ring + C::SC_B / 4;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(epi) + C::EPI_B);
+    uint64_t* full = bars;                                    // producers (PAIR: and the odd CTA's MMA warp) -> MMA warp
+    uint64_t* empty = full + ST;                              // MMA commit -> producers
+    uint64_t* d_full = empty + ST;                            // MMA commit -> sums [DB]
+    uint64_t* d_empty = d_full + DB;                          // sums (PAIR: of both CTAs) -> MMA [DB]
+    uint64_t* sc_full = d_empty + DB;                         // scales -> sums [kScaleSt]
+    uint64_t* sc_empty = sc_full + kScaleSt;                  // sums -> scales [kScaleSt]
+    uint64_t* part_full = sc_empty + kScaleSt;                // SPLIT: every CTA's partial sums are in its shared memory
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_full + 1);
+    uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
+    uint32_t* prefix = reinterpret_cast<uint32_t*>(bars) + 128;   // [n_expert + 1]
+    __shared__ Unit utab[kTab];
+    __shared__ uint32_t wsum[THREADS / 32];
+
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;        // which half of the unit's weight rows
+    const uint32_t part = SPLIT ? blockIdx.x % split : 0u;    // which part of its k
+    const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / split : blockIdx.x;
+    const uint32_t stride = sh.stride.d;
+    if (tid < ST) {
+        mbar_init(&full[tid], 1 + 32 * kXWarps + (PAIR && rank == 0 ? 1 : 0));
+        mbar_init(&empty[tid], 1);
+    } else if (tid >= 32 && tid < 32 + DB) {
+        mbar_init(&d_full[tid - 32], 1);
+        mbar_init(&d_empty[tid - 32], 4 * C::SUM_G * MB);
+    } else if (tid >= 64 && tid < 64 + kScaleSt) {
+        mbar_init(&sc_full[tid - 64], C::SC_WARPS);
+        mbar_init(&sc_empty[tid - 64], 4 * C::SUM_G);
+    } else if (tid == 96) {
+        *dead = 0;
+        if (SPLIT) mbar_init(part_full, 4 * split);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
+    if (PAIR || SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    chain_wait();                                             // all above needs no memory but the CTA's own
+    scan_units<THREADS, MB>(p, sh, first, prefix, utab, wsum);
+    fence_before();
+    __syncthreads();
+    if (PAIR || SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs' barriers and tensor memory are set up
+    fence_after();
+    chain_next();                                             // every CTA has its tensor memory: a later kernel may ask for its own
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    const uint32_t n_units = prefix[p.n_expert];
+    // SPLIT: the grid has a cluster for every unit that offsets in ascending order can make, so one at most
+    const uint32_t n_mine = n_units > first ? SPLIT ? 1u : exl3b_div_of(n_units - first + stride - 1, sh.stride) : 0u;
+    auto unit_at = [&](uint32_t i) {
+        return i < kTab ? utab[i] : find_unit<MB>(p, prefix, first + i * stride, sh);
+    };
+    const int nck = sh.nck;
+    // this CTA's stages of a unit
+    const int k0 = SPLIT ? (int)(part * (uint32_t)nck / (uint32_t)split) : 0;
+    const int k1 = SPLIT ? (int)((part + 1) * (uint32_t)nck / (uint32_t)split) : nck;
+    volatile uint32_t* vdead = dead;
+    // A bounded wait by a whole warp, which reports nothing: one that gives up marks the CTA dead, every other wait of the
+    // CTA then gives up at its next try, and the roles leave at their next unit.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const uint32_t a = smem_u32(bar);
+        uint64_t t0 = 0;
+        for (;;) {
+            uint32_t done;
+            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+                         " selp.u32 %0, 1, 0, p;\n}\n"
+                         : "=r"(done)
+                         : "r"(a), "r"(parity), "r"(kSuspendNs)
+                         : "memory");
+            if (done || *vdead) break;
+            const uint64_t now = globaltimer_ns();
+            if (!t0) t0 = now;
+            else if (now - t0 > kWaitLimitNs) {
+                *vdead = 1;
+                atomicOr(p.err, 1);
+                break;
+            }
+        }
+        __syncwarp();
+    };
+    Pipe pipe;                                                // of the stages
+    // PAIR: the summing warps' sums need more than the 128 registers a thread that 512 threads start with: 256 x 192 + 256 x 64
+    // are the 512 x 128 of the launch
+    if (warp < kEpiWarp0) {
+        if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0) {
+            // ---------------------------------------------------------------- weights
+            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+                const Unit u = unit_at(i);
+                const int b = u.blk + (int)rank;
+                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
+                    wait(&empty[pipe.s], pipe.ph ^ 1);
+                    mbar_expect_tx_el(&full[pipe.s], kW_B);
+                    uint8_t* dst = w_ring + pipe.s * kW_B;
+                    const int k = ck * 128;
+                    if (!ACT) {
+                        tma_w_el(dst, &wmap, k, b * 128, u.e, &full[pipe.s]);
+                    } else if (p.n_out % 16 == 0) {
+                        tma_w5_el(dst, &wmap, k, b * 4, u.e, &full[pipe.s]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            tma_w_el(dst + q * 4096, &wmap, k, b * 64 + 16 * q, u.e, &full[pipe.s]);
+                            tma_w_el(dst + q * 4096 + 2048, &wmap, k, (int)p.n_out + b * 64 + 16 * q, u.e, &full[pipe.s]);
+                        }
+                    }
+                }
+            }
+            // after a wait that gave up: a millisecond for the copies still in flight, before the CTA's memory goes
+            if (*vdead)
+                for (int j = 0; j < 50; ++j) __nanosleep(20000);
+        } else if (warp == 1 && rank == 1) {
+            // ---------------------------------------------------------------- PAIR, odd CTA: its filled stages, reported
+            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
+                    wait(&full[pipe.s], pipe.ph);
+                    proxy_fence();
+                    if (lane == 0) arrive_even(&full[pipe.s]);
+                    __syncwarp();
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------------------------------------------------------- MMA issuer
+            const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
+            Pipe db;
+            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+                const Unit u = unit_at(i);
+                const uint32_t n = (u.nr + 16 * MB - 1) & ~(16 * MB - 1);
+                // D f32, e4m3 both, both operands K-major, M 128 (PAIR: 256), N n
+                const uint32_t idesc = (n >> 3) << 17 | (8u * MB) << 24 | 1u << 4;
+                for (int ck = k0; ck < k1; ++ck, pipe.next(ST), db.next(DB)) {
+                    wait(&d_empty[db.s], db.ph ^ 1);
+                    wait(&full[pipe.s], pipe.ph);
+                    proxy_fence();
+                    fence_after();
+                    mma4_f8<PAIR>(tmem + db.s * NT, wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd0 + (uint64_t)(pipe.s * C::X_B >> 4),
+                                  idesc, 0u);
+                    commit_el<PAIR>(&empty[pipe.s]);
+                    commit_el<PAIR>(&d_full[db.s]);
+                }
+            }
+        } else if (warp < kXWarp0) {
+            // ---------------------------------------------------------------- scales
+            // A lane has Q neighbouring sorted rows and loads four blocks' scales of each at a time, into two register sets in turn,
+            // one on its way while the other is used, across units; the weight's scales of a batch are one a lane.
+            constexpr int Q = PAIR ? 4 : 1;
+            const int g = warp - 2;
+            if (g < C::SC_WARPS && n_mine) {
+                struct Set {
+                    float x[Q][4], w;
+                };
+                RowAhead<Q> ahead(p, g * 128 + Q * lane, 1);
+                const uint8_t* src[Q];
+                const float* wsrc = nullptr;
+                const bool whole = ((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0;
+                uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
+                int lc = k0, cc = k0;                             // ... and their first stages
+                auto rows = [&](const Unit& u) {
+                    ahead.rows(p.x_scales, p.xs_pitch, src);
+                    const int b = min((u.blk + (int)rank) * blk_out / 128, p.ws_blocks - 1) + (lane & 4 ? p.ws_blocks * (C::HALVES - 1) : 0);
+                    wsrc = reinterpret_cast<const float*>(p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes);
+                };
+                {
+                    const Unit u = unit_at(0);
+                    ahead.fetch(u);
+                    rows(u);
+                    if (n_mine > 1) ahead.fetch(unit_at(1));
+                }
+                auto load = [&](Set& s) {
+                    if (lu >= n_mine) return;
+                    if (whole && lc + 4 <= k1) {
+#pragma unroll
+                        for (int q = 0; q < Q; ++q) {
+                            const float* at = reinterpret_cast<const float*>(src[q]) + lc;
+                            if (lc & 3) {                          // SPLIT: a part that starts inside four blocks
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) s.x[q][j] = at[j];
+                            } else {
+                                const float4 t = *reinterpret_cast<const float4*>(at);
+                                s.x[q][0] = t.x; s.x[q][1] = t.y; s.x[q][2] = t.z; s.x[q][3] = t.w;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < Q; ++q)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                s.x[q][j] = lc + j < k1 ? reinterpret_cast<const float*>(src[q])[lc + j] : 0.f;
+                    }
+                    s.w = lc + (lane & 3) < k1 ? wsrc[lc + (lane & 3)] : 0.f;
+                    if ((lc += 4) >= k1) {
+                        lc = k0;
+                        if (++lu < n_mine) {
+                            rows(unit_at(lu));
+                            if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
+                        }
+                    }
+                };
+                auto use = [&](const Set& s) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (cc + j >= k1) break;
+                        wait(&sc_empty[pipe.s], pipe.ph ^ 1);
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; ++h) {
+                            const float w = __shfl_sync(0xFFFFFFFFu, s.w, 4 * h + j);
+                            float* dst = sc_ring + (pipe.s * C::HALVES + h) * NT + g * 128 + Q * lane;
+                            if constexpr (Q == 4)
+                                *reinterpret_cast<float4*>(dst) = make_float4(s.x[0][j] * w, s.x[1][j] * w, s.x[2][j] * w, s.x[3][j] * w);
+                            else *dst = s.x[0][j] * w;
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sc_full[pipe.s]);
+                        pipe.next(kScaleSt);
+                    }
+                    if ((cc += 4) >= k1) {
+                        cc = k0;
+                        ++cu;
+                    }
+                };
+                Set even = {}, odd = {};
+                load(even);
+                load(odd);
+                while (cu < n_mine && !*vdead) {
+                    use(even);
+                    load(even);
+                    if (cu >= n_mine) break;
+                    use(odd);
+                    load(odd);
+                }
+            }
+        } else {
+            // ---------------------------------------------------------------- sorted rows
+            // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's barrier
+            // when they have landed, and the MMA warp, which sees that, makes them visible to the asynchronous proxy.
+            constexpr int RP = (C::NL + 15) / 16, kStep = 4;      // passes a stage; stages a step of the row pointers
+            const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
+            const int kb = (int)p.n_in;
+            const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
+            RowAhead<RP> ahead(p, rr, 16);
+            auto mine = [&](uint32_t i) {                         // this CTA's rows of its i-th unit; blk: rows of its tile
+                Unit u = unit_at(i);
+                const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
+                u.r0 += (int)rank * nl;
+                u.nr = min(u.nr - (int)rank * nl, nl);
+                u.blk = nl;
+                return u;
+            };
+            Unit u = n_mine ? mine(0) : Unit{};
+            if (n_mine) ahead.fetch(u);
+            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+                const int nl = u.blk;
+                const uint8_t* src[RP];
+                ahead.rows(static_cast<const uint8_t*>(p.x) + k0 * kRowB + c * 16, p.x_pitch_bytes, src);
+                if (i + 1 < n_mine) {
+                    u = mine(i + 1);
+                    ahead.fetch(u);
+                }
+                for (int c0 = k0; c0 < k1; c0 += kStep) {
+#pragma unroll
+                    for (int a = 0; a < kStep; ++a) {
+                        if (c0 + a >= k1) break;
+                        wait(&empty[pipe.s], pipe.ph ^ 1);
+                        const uint32_t dst = dst0 + pipe.s * C::X_B;
+                        if ((c0 + a + 1) * kRowB <= kb) {
+#pragma unroll
+                            for (int j = 0; j < RP; ++j)
+                                if (16 * j < nl) cp16(dst + j * 16 * kRowB, src[j] + a * kRowB);
+                        } else {                                  // the row ends in this stage: zeros behind it
+                            const bool in = (c0 + a) * kRowB + c * 16 < kb;
+#pragma unroll
+                            for (int j = 0; j < RP; ++j)
+                                if (16 * j < nl) cp16_or_zero(dst + j * 16 * kRowB, in ? src[j] + a * kRowB : src[j], in);
+                        }
+                        cp_arrive(&full[pipe.s]);
+                        pipe.next(ST);
+                    }
+#pragma unroll
+                    for (int j = 0; j < RP; ++j) src[j] += kStep * kRowB;
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+    } else {
+        // ---------------------------------------------------------------- sums
+        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
+        constexpr int es = OUT == RAD_F32 ? 4 : 2, G = C::SUM_G, NS = C::SLICES;
+        uint8_t* const y = static_cast<uint8_t*>(p.y);
+        clear_outside<OUT>(p, blockIdx.x * 4 * G + ew, gridDim.x * 4 * G, lane);
+        const int64_t row_b = p.y_pitch * es;
+        // a unit's slots, row 32 b + lane in slot[b]: fetched when its sums begin
+        constexpr int LB = (NT + 31) / 32;
+        Pipe db;
+        for (uint32_t i = 0; i < n_mine; ++i) {
+            const Unit u = unit_at(i);
+            uint32_t live = 0;                                               // which of the unit's rows are, 32 a lane
+#pragma unroll
+            for (int b = 0; b < LB; ++b) {
+                const int32_t slot = p.sorted_tok && 32 * b + lane < u.nr ? p.sorted_tok[u.r0 + 32 * b + lane] : 0;
+                const uint32_t m = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+                if (lane == b) live = m;
+            }
+            // slice s of this group: rows 16 (G s + g) .. of the unit; a thread's 16 sums of it as tmem_ld8x8 has them
+            float acc[NS][16];
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[s][k] = 0.f;
+            const int mine = u.nr > kSlice * g ? (u.nr - kSlice * g + kSlice * G - 1) / (kSlice * G) : 0;   // slices of this group
+            for (int ck = k0; ck < k1; ++ck, db.next(DB), pipe.next(kScaleSt)) {
+                wait(&sc_full[pipe.s], pipe.ph);
+                wait(&d_full[db.s], db.ph);
+                fence_after();
+                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * NT + kSlice * g;
+                const float* sc = sc_ring + pipe.s * C::HALVES * NT + kSlice * g + 2 * (lane & 3);
+                uint32_t a[2][16];
+                if (mine > 0) tmem_ld8x8(d, a[0]);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    if (s >= mine) break;
+                    uint32_t (&now)[16] = a[s & 1];
+                    tmem_wait(now);
+                    if (s + 1 < NS && s + 1 < mine) tmem_ld8x8(d + (s + 1) * kSlice * G, a[(s + 1) & 1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {               // weight rows 0..15 and 16..31 of the warp's 32
+                            const uint64_t f = *reinterpret_cast<const uint64_t*>(sc + (ACT ? half * NT : 0) + s * kSlice * G + 8 * h);
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {
+                                const int k = 8 * half + 4 * h + 2 * v;
+                                const uint64_t r = fma2(f2pk(__uint_as_float(now[k]), __uint_as_float(now[k + 1])), f,
+                                                        f2pk(acc[s][k], acc[s][k + 1]));
+                                f2upk(r, acc[s][k], acc[s][k + 1]);
+                            }
+                        }
+                    }
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (PAIR) arrive_even(&d_empty[db.s]);
+                    else mbar_arrive(&d_empty[db.s]);
+                    mbar_arrive(&sc_empty[pipe.s]);
+                }
+                __syncwarp();
+            }
+            if (__any_sync(0xFFFFFFFFu, *vdead)) break;
+            const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
+            if constexpr (SPLIT) {
+                // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
+                // then sums every split-th row over the CTAs, in their order, and stores it.
+                float* const st = epi;
+                const int c2 = 2 * (lane & 3);
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    if (s < mine) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            st[(s * kSlice + 8 * (k >> 2 & 1) + c2 + (k & 1)) * kEpiLd + 32 * q + 16 * (k >> 3) + 8 * (k >> 1 & 1) + (lane >> 2)] = acc[s][k];
+                    }
+                __syncwarp();                                  // the arrivals publish the whole warp's sums
+                if (lane < split) arrive_at(part_full, lane);
+                __syncwarp();
+                wait(part_full, 0);
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                const bool out_lane = !ACT || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
+                const int64_t n0 = b0 + (ACT ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
+                const uint32_t rows_live = __shfl_sync(0xFFFFFFFFu, live, 0);
+                for (int j = part + split * q; j < u.nr; j += split * 4) {
+                    float f[kMaxSplit][4], v[4];
+#pragma unroll
+                    for (int s = 0; s < kMaxSplit; ++s)       // all on their way before the first is added
+                        if (s < split) ld_cluster(&st[j * kEpiLd + 4 * lane], s, f[s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = f[0][e];
+#pragma unroll
+                        for (int s = 1; s < kMaxSplit; ++s)
+                            if (s < split) v[e] += f[s][e];
+                    }
+                    if (ACT) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float up = __shfl_xor_sync(0xFFFFFFFFu, v[e], 4);
+                            v[e] = v[e] < kSiluLow ? silu_up_low(v[e], up) : silu_up(v[e], up);
+                        }
+                    }
+                    if (!(rows_live >> j & 1)) v[0] = v[1] = v[2] = v[3] = 0.f;        // a dropped slot
+                    if (out_lane && n0 < p.n_out) {
+                        uint8_t* d = y + (u.r0 + j) * row_b + n0 * es;
+                        if constexpr (OUT == RAD_F32) *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2*>(d) = make_uint2(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]));
+                    }
+                }
+                break;
+            }
+            const int64_t n_warp = b0 + (ACT ? 16 : 32) * q;                 // the warp's first output
+            const int c2 = 2 * (lane & 3);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                if (s >= mine) break;
+                const int t0 = kSlice * (G * s + g);
+                uint32_t a[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) a[k] = __float_as_uint(acc[s][k]);
+                constexpr int NV = ACT ? 8 : 16;
+                float v[NV];
+                act_slice<ACT>(a, v);
+                const uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
+                if ((here & 0xFFFFu) != 0xFFFFu) {                                // dropped slots are zero
+#pragma unroll
+                    for (int k = 0; k < NV; ++k)
+                        if (!(here >> (8 * (k >> 2 & 1) + c2 + (k & 1)) & 1)) v[k] = 0.f;
+                }
+                store_slice<OUT, ACT>(v, y + (u.r0 + t0) * row_b, row_b, n_warp, p.n_out, u.nr - t0,
+                                      reinterpret_cast<uint8_t*>(epi) + ew * 1024, lane);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (PAIR || SPLIT) cluster_sync_all();                    // no CTA's memory goes while another uses it
+    if (warp == 1) {
+        fence_after();
+        tmem_free<PAIR>(tmem, C::TMEM);
+    }
+}
+
+typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
+
+// split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
+template <bool PAIR, bool SPLIT, bool ACT>
+int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
+    using C = Cfg<PAIR, SPLIT, ACT>;
+    CUtensorMap map;
+    const int rc = make_map(p, &map);
+    if (rc) return rc;
+    static const Kern kerns[3] = { k_gmm8<PAIR, SPLIT, RAD_F32, ACT>, k_gmm8<PAIR, SPLIT, RAD_F16, ACT>,
+                                   k_gmm8<PAIR, SPLIT, RAD_BF16, ACT> };
+    static bool allowed[64][3];                               // the most shared memory, once a device
+    const int which = p->y_dtype == RAD_F32 ? 0 : p->y_dtype == RAD_F16 ? 1 : 2;
+    const Kern kern = kerns[which];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
+    if (!allowed[dev][which]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
+        allowed[dev][which] = true;
+    }
+    const int ctas = PAIR ? 2 : split;                        // of a cluster
+    const int nt = PAIR ? pair_rows(p, C::NT, sm_count) : C::NT;
+    const int64_t most = most_units(p, nt, PAIR ? 2 : 1);
+    // few units: one CTA an SM, with the whole of its shared memory for stages in flight; clusters of three or four do not
+    // fill the SMs of every processing cluster
+    const int64_t alone = ctas > 2 ? sm_count - sm_count / 8 : sm_count;
+    const int per_sm = !PAIR && most * ctas <= alone ? 1 : C::PER_SM;
+    const int64_t room = (int64_t)sm_count * per_sm / ctas;
+    const int stages = C::stages(p->n_expert, per_sm);
+    const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
+    const Shape sh = { exl3b_div((uint32_t)((p->n_out + blk - 1) / blk)), exl3b_div((uint32_t)units), exl3b_div((uint32_t)nt),
+                       (int32_t)((p->n_in + 127) / 128), stages, split };
+    return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
+                        ctas, st, map, *p, sh);
+}
+
+template <bool ACT>
+int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
+    const int64_t few = p->w_rows < 512 ? 96 : 16;
+    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4)
+        return launch<true, false, ACT>(p, sm_count, 1, st);
+    const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 127) / 128;
+    int64_t split = sm_count / most;                          // so the grid has room for a cluster a unit: the kernel counts on it
+    if (split > nck / 4) split = nck / 4;
+    if (split > kMaxSplit) split = kMaxSplit;
+    if (split >= 2) return launch<false, true, ACT>(p, sm_count, (int)split, st);
+    return launch<false, false, ACT>(p, sm_count, 1, st);
+}
+
+}  // namespace
+
+extern "C" int exl3b_cuda_gmm8(const Exl3bGmmOp* p, int sm_count, void* stream) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return p->act ? launch_form<true>(p, sm_count, st) : launch_form<false>(p, sm_count, st);
+}

@@ -187,14 +187,15 @@ class GroupedMm(_Plan):
     of w's rows times the second).
 
     x [x_rows, n_in] and w [experts, w_rows, n_in] in f16 or bf16; or MXFP4 codes (uint8, half as wide) with x_scales
-    [x_rows, n_in / 32] and w_scales from mx4_tile_scales. y [rows, n_out] in f32, f16 or bf16, or MXFP4 codes with
-    y_scales. expert_offset i32 [experts + 1] (None: one expert); sorted_tok i32 [rows] (None: no dropped slot). top_k:
+    [x_rows, n_in / 32] and w_scales from mx4_tile_scales; or FP8 (float8_e4m3fn) with f32 x_scales [x_rows, ceil(n_in / 128)]
+    and w_scales [experts, blocks, ceil(n_in / 128)], a block each 128 weight rows (silu_mul: ceil(n_out / 128) blocks of gate
+    rows, then as many of up rows). y [rows, n_out] in f32, f16 or bf16, or (not from FP8) MXFP4 codes with y_scales. expert_offset i32 [experts + 1] (None: one expert); sorted_tok i32 [rows] (None: no dropped slot). top_k:
     row i reads x row sorted_tok[i] // top_k; 0: x is sorted already."""
     _entry = "exl3b200_grouped_mm"
 
     def __init__(self, *, x, w, y, expert_offset=None, sorted_tok=None, top_k=0, act="none", x_scales=None,
                  w_scales=None, y_scales=None):
-        mx, mx_out = w.dtype == torch.uint8, y.dtype == torch.uint8
+        mx, f8, mx_out = w.dtype == torch.uint8, w.dtype == torch.float8_e4m3fn, y.dtype == torch.uint8
         d = GroupedMmDesc()
         per, per_out = 2 if mx else 1, 2 if mx_out else 1
         if x.dtype != w.dtype:
@@ -204,7 +205,7 @@ class GroupedMm(_Plan):
         dev = x.get_device()
         d.n_expert, d.n_rows, d.x_rows, d.top_k = w.shape[0], y.shape[0], x.shape[0], top_k
         d.n_out, d.n_in, d.act = y.shape[1] * per_out, x.shape[1] * per, ACTS[act]
-        d.dtype, d.y_dtype = MX4 if mx else _dtype(x), MX4 if mx_out else _dtype(y)
+        d.dtype, d.y_dtype = MX4 if mx else F8 if f8 else _dtype(x), MX4 if mx_out else _dtype(y)
         _rows(w, "w", dev, (d.n_expert, d.n_out * (2 if d.act else 1), x.shape[1]))
         d.x, pitch = _rows(x, "x", dev)
         d.x_pitch = pitch * per
@@ -216,6 +217,14 @@ class GroupedMm(_Plan):
             d.x_scales, d.x_scales_pitch = _rows(x_scales, "x_scales", dev, (d.x_rows, d.n_in // 32), torch.uint8)
             want = native().mx4_tiled_bytes(d.n_expert, w.shape[1], d.n_in, d.act)
             d.w_scales, _ = _rows(w_scales, "w_scales", dev, (want,), torch.uint8)
+        if f8:
+            kb = (d.n_in + 127) // 128
+            d.x_scales, pitch = _rows(x_scales, "x_scales", dev, (d.x_rows, kb), torch.float32)
+            d.x_scales_pitch = pitch * 4
+            blocks = (d.n_out + 127) // 128 * (2 if d.act else 1)
+            d.w_scales, _ = _rows(w_scales, "w_scales", dev, (d.n_expert, blocks, kb), torch.float32)
+            if not w_scales.is_contiguous():
+                raise ValueError("w_scales is strided")
         if mx_out:
             d.y_scales, d.y_scales_pitch = _rows(y_scales, "y_scales", dev, (d.n_rows, d.n_out // 32), torch.uint8)
         if expert_offset is not None:
