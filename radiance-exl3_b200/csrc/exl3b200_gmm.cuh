@@ -373,19 +373,20 @@ __device__ __forceinline__ void clear_outside(const Exl3bGmmOp& p, uint32_t w, u
 }
 
 // A slice: v, a warp's outputs from n_warp on of up to 16 rows (`left` of them) at d. Thread t has outputs o = t / 4 and o + 8
-// (act NONE: and 16 more) of rows c2 = 2 (t % 4), c2 + 1, 8 + c2, 9 + c2. sw: 1 KB of shared memory of the warp's own.
-template <int OUT, bool ACT>
+// (act NONE: and 16 more) of four rows: 2 (t % 4), the next one, and 8 more each (tmem_ld8x8's), or with BY4 t % 4, 4 + t % 4,
+// and 8 more each (tmem_ld4's). sw: 1 KB of shared memory of the warp's own.
+template <int OUT, bool ACT, bool BY4 = false>
 __device__ __forceinline__ void store_slice(const float (&v)[ACT ? 8 : 16], uint8_t* d, int64_t row_b, int64_t n_warp,
                                             int64_t n_out, int left, uint8_t* sw, int lane) {
     constexpr int NV = ACT ? 8 : 16;
     if constexpr (OUT == RAD_F32) {
         // straight from the registers: a warp's store is 32 bytes each of four rows
-        const int o = lane >> 2, c2 = 2 * (lane & 3);
+        const int o = lane >> 2, c2 = (BY4 ? 1 : 2) * (lane & 3);
         const int64_t n = n_warp + o;
         d += c2 * row_b + n * 4;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int j = 8 * (k >> 2 & 1) + (k & 1), m = 16 * (k >> 3) + 8 * (k >> 1 & 1);
+            const int j = 8 * (k >> 2 & 1) + (BY4 ? 4 : 1) * (k & 1), m = 16 * (k >> 3) + 8 * (k >> 1 & 1);
             if (c2 + j < left && n + m < n_out) *reinterpret_cast<float*>(d + j * row_b + 4 * m) = v[k];
         }
     } else {
@@ -394,12 +395,13 @@ __device__ __forceinline__ void store_slice(const float (&v)[ACT ? 8 : 16], uint
         // against 177 us at 16 experts, 16067 rows, 1536 -> 4096.)
         constexpr int P = NV / 4, SH = ACT ? 2 : 1;                   // 16-byte pieces a row; rows that share banks
         auto at = [](int row, int piece) { return (row * P + (piece ^ (row >> SH & (P - 1)))) * 16; };
+        const int m = BY4 ? (lane >> 1 & 3) + 4 * (lane & 1) : lane & 7;
 #pragma unroll
         for (int s = 0; s < NV / 8; ++s) {
             uint32_t w[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m) w[m] = pack2<OUT>(v[8 * s + 2 * m], v[8 * s + 2 * m + 1]);
-            st8x8t(smem_u32(sw) + at(8 * (lane >> 4) + (lane & 7), 2 * s + (lane >> 3 & 1)), w);
+            st8x8t(smem_u32(sw) + at(8 * (lane >> 4) + m, 2 * s + (lane >> 3 & 1)), w);
         }
         __syncwarp();
 #pragma unroll
@@ -432,17 +434,18 @@ static inline EncodeTiledFn encode_fn() {
 // Weights, boxes of 128 bytes of k: [expert][row][k] and a block's 128 rows; for silu_mul [expert][group of 16 rows]
 // [gate, up][16][k] and a block's four groups, in one box (eight boxes of 16 rows a stage kept the issuing warp busy, 550
 // cycles a stage) unless the last group is half a one and the box would leave the weight: then a box a half group.
-static inline int make_map(const Exl3bGmmOp* p, CUtensorMap* map) {
+// box_rows: a box of so many rows instead, whatever the act.
+static inline int make_map(const Exl3bGmmOp* p, CUtensorMap* map, int box_rows = 0) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return -6;
     const CUtensorMapDataType dt = p->mx4 || p->f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                           : p->bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const cuuint64_t k = (cuuint64_t)(p->mx4 ? p->n_in / 2 : p->n_in), pitch = (cuuint64_t)p->w_pitch_bytes;
     const cuuint32_t kb = p->mx4 || p->f8 ? 128u : 64u, one[5] = { 1, 1, 1, 1, 1 };
-    const bool whole = p->act && p->n_out % 16 == 0;
+    const bool whole = !box_rows && p->act && p->n_out % 16 == 0;
     const cuuint64_t dims3[3] = { k, (cuuint64_t)p->w_rows, (cuuint64_t)p->n_expert };
     const cuuint64_t strides3[2] = { pitch, (cuuint64_t)p->w_expert_bytes };
-    const cuuint32_t box3[3] = { kb, p->act ? 16u : 128u, 1u };
+    const cuuint32_t box3[3] = { kb, box_rows ? (cuuint32_t)box_rows : p->act ? 16u : 128u, 1u };
     const cuuint64_t dims5[5] = { k, 16, 2, (cuuint64_t)(p->n_out / 16), (cuuint64_t)p->n_expert };
     const cuuint64_t strides5[4] = { pitch, (cuuint64_t)p->n_out * pitch, 16 * pitch, (cuuint64_t)p->w_expert_bytes };
     const cuuint32_t box5[5] = { kb, 16, 2, 4, 1 };

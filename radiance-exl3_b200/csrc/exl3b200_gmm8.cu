@@ -29,6 +29,7 @@
 #include "exl3b200_decode.cuh"
 #include "exl3b200_dense.h"
 #include "exl3b200_gmm.cuh"
+#include "exl3b200_gmm8w.cuh"
 
 using namespace exl3b;
 
@@ -40,17 +41,19 @@ template <bool PAIR, bool SPLIT, bool ACT>
 struct Cfg {
     static constexpr int NT = PAIR ? 256 : 32;                   // sorted rows a unit at most
     static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
-    static constexpr int SUM_G = PAIR ? 2 : 1;                   // groups of four summing warps
-    static constexpr int SLICES = NT / kSlice / SUM_G;           // of 16 sorted rows a group
+    static constexpr int SUM_G = PAIR ? 2 : 1;                   // groups of four summing warps, each for a CTA's sorted rows
+    static constexpr int PARTS = PAIR ? 2 : 1;                   // MMAs a 32 k at most, each of up to PART of a CTA's sorted rows
+    static constexpr int PART = NL / PARTS;
     static constexpr int THREADS = (kEpiWarp0 + 4 * SUM_G) * 32;
     static constexpr int X_B = NL * kRowB;
     static constexpr int STAGE_B = kW_B + X_B;
     static constexpr int HALVES = ACT ? 2 : 1;                   // scales a sorted row: gate's, up's
-    static constexpr int SC_B = kScaleSt * HALVES * NT * 4;
+    static constexpr int SC_ROWS = NT * 2;                       // floats of a half's scales: each twice
+    static constexpr int SC_B = kScaleSt * HALVES * SC_ROWS * 4;
     static constexpr int SC_WARPS = PAIR ? 2 : 1;
     static constexpr int EPI_B = SPLIT ? NT * kEpiLd * 4 : 4 * SUM_G * 1024;
-    static constexpr int DB = PAIR ? 2 : 4;                      // accumulators in turn
-    static constexpr int TMEM = DB * NT;
+    static constexpr int DB = 4, DCOLS = PART * (PAIR ? 2 : 1);  // accumulators in turn, of so many columns
+    static constexpr int TMEM = DB * DCOLS;
     static constexpr int PER_SM = PAIR ? 1 : 2;
     static constexpr int BARS = 2 * kMaxSt + 2 * DB + 2 * kScaleSt + 1;
     static constexpr int fixed(int n_expert) { return 1024 + EPI_B + SC_B + 512 + (n_expert + 4) * 4; }
@@ -61,6 +64,33 @@ struct Cfg {
     static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0 && stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4), "tensor or shared memory");
     static_assert(BARS * 8 + 8 <= 512, "barriers");
 };
+
+// The sorted rows of a unit that a CTA brings, and those of them in the first MMA's part (the rest is in the second's).
+struct Parts {
+    int nl, p0;
+};
+template <typename C, int MB>
+__device__ __forceinline__ Parts parts_of(const Unit& u) {
+    Parts r;
+    r.nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
+    r.p0 = r.nl <= C::PART ? r.nl : (r.nl / 16 + 1) / 2 * 16;
+    return r;
+}
+
+// Where row r's scale lies in the ring, twice: with those of row r + 4, when r % 8 < 4, 16 bytes that a thread of tmem_ld4's
+// rows loads at once.
+__device__ __forceinline__ int scale_at(int r) { return (r >> 3) * 16 + (r & 3) * 4 + (r & 4) / 2; }
+
+// 32 columns of 16 lanes: r[2 i + v] is lane t / 4 + 8 v, column 4 i + t % 4 in thread t. (Of the ways to read 16 lanes at a time
+// this moves 128 bytes a cycle, tmem_ld8x8's 64.)
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t r[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x128b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
 
 // OUT: y_dtype; ACT: silu_mul.
 template <bool PAIR, bool SPLIT, int OUT, bool ACT>
@@ -74,7 +104,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* w_ring = smem;                                   // [ST][128 rows][128 B]
     uint8_t* x_ring = w_ring + ST * kW_B;                     // [ST][NL rows][128 B]
-    float* sc_ring = reinterpret_cast<float*>(x_ring + ST * C::X_B);   // [kScaleSt][HALVES][NT]
+    float* sc_ring = reinterpret_cast<float*>(x_ring + ST * C::X_B);   // [kScaleSt][HALVES][SC_ROWS]
     float* epi = sc_ring + C::SC_B / 4;
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(epi) + C::EPI_B);
     uint64_t* full = bars;                                    // producers (PAIR: and the odd CTA's MMA warp) -> MMA warp
@@ -201,19 +231,24 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
             const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
             Pipe db;
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                const Unit u = unit_at(i);
-                const uint32_t n = (u.nr + 16 * MB - 1) & ~(16 * MB - 1);
-                // D f32, e4m3 both, both operands K-major, M 128 (PAIR: 256), N n
-                const uint32_t idesc = (n >> 3) << 17 | (8u * MB) << 24 | 1u << 4;
-                for (int ck = k0; ck < k1; ++ck, pipe.next(ST), db.next(DB)) {
-                    wait(&d_empty[db.s], db.ph ^ 1);
+                const Parts pt = parts_of<C, MB>(unit_at(i));
+                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
                     wait(&full[pipe.s], pipe.ph);
                     proxy_fence();
-                    fence_after();
-                    mma4_f8<PAIR>(tmem + db.s * NT, wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd0 + (uint64_t)(pipe.s * C::X_B >> 4),
-                                  idesc, 0u);
+#pragma unroll
+                    for (int h = 0; h < C::PARTS; ++h) {
+                        const uint32_t n = MB * (h ? pt.nl - pt.p0 : pt.p0);
+                        if (n == 0) break;
+                        // D f32, e4m3 both, both operands K-major, M 128 (PAIR: 256), N n
+                        const uint32_t idesc = (n >> 3) << 17 | (8u * MB) << 24 | 1u << 4;
+                        wait(&d_empty[db.s], db.ph ^ 1);
+                        fence_after();
+                        mma4_f8<PAIR>(tmem + db.s * C::DCOLS, wd0 + (uint64_t)(pipe.s * kW_B >> 4),
+                                      xd0 + (uint64_t)((pipe.s * C::X_B + (h ? pt.p0 * kRowB : 0)) >> 4), idesc, 0u);
+                        commit_el<PAIR>(&d_full[db.s]);
+                        db.next(DB);
+                    }
                     commit_el<PAIR>(&empty[pipe.s]);
-                    commit_el<PAIR>(&d_full[db.s]);
                 }
             }
         } else if (warp < kXWarp0) {
@@ -281,10 +316,12 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
 #pragma unroll
                         for (int h = 0; h < C::HALVES; ++h) {
                             const float w = __shfl_sync(0xFFFFFFFFu, s.w, 4 * h + j);
-                            float* dst = sc_ring + (pipe.s * C::HALVES + h) * NT + g * 128 + Q * lane;
-                            if constexpr (Q == 4)
-                                *reinterpret_cast<float4*>(dst) = make_float4(s.x[0][j] * w, s.x[1][j] * w, s.x[2][j] * w, s.x[3][j] * w);
-                            else *dst = s.x[0][j] * w;
+                            float* dst = sc_ring + (pipe.s * C::HALVES + h) * C::SC_ROWS;
+#pragma unroll
+                            for (int q = 0; q < Q; ++q) {
+                                const float f = s.x[q][j] * w;
+                                *reinterpret_cast<float2*>(dst + scale_at(g * 128 + Q * lane + q)) = make_float2(f, f);
+                            }
                         }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sc_full[pipe.s]);
@@ -362,66 +399,85 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
         // ---------------------------------------------------------------- sums
         if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
-        constexpr int es = OUT == RAD_F32 ? 4 : 2, G = C::SUM_G, NS = C::SLICES;
+        constexpr int es = OUT == RAD_F32 ? 4 : 2, G = C::SUM_G;
         uint8_t* const y = static_cast<uint8_t*>(p.y);
         clear_outside<OUT>(p, blockIdx.x * 4 * G + ew, gridDim.x * 4 * G, lane);
         const int64_t row_b = p.y_pitch * es;
-        // a unit's slots, row 32 b + lane in slot[b]: fetched when its sums begin
+        // which of a unit's rows are live, 32 a lane: its slots are fetched a unit ahead
         constexpr int LB = (NT + 31) / 32;
+        int32_t slot[LB];
+        auto fetch = [&](const Unit& n) {
+#pragma unroll
+            for (int b = 0; b < LB; ++b) slot[b] = p.sorted_tok && 32 * b + lane < n.nr ? p.sorted_tok[n.r0 + 32 * b + lane] : 0;
+        };
+        auto votes = [&]() {
+            uint32_t r = 0;
+#pragma unroll
+            for (int b = 0; b < LB; ++b) {
+                const uint32_t m = __ballot_sync(0xFFFFFFFFu, slot[b] >= 0);
+                if (lane == b) r = m;
+            }
+            return r;
+        };
+        if (n_mine) fetch(unit_at(0));
+        uint32_t live = votes();
         Pipe db;
         for (uint32_t i = 0; i < n_mine; ++i) {
             const Unit u = unit_at(i);
-            uint32_t live = 0;                                               // which of the unit's rows are, 32 a lane
+            const Parts pt = parts_of<C, MB>(u);
+            // the group's rows are those that CTA g brings: row 32 b + .. of part h, its 16 sums of each half of the lanes as
+            // tmem_ld4 has them, two a word (as floats the compiler moved them into pairs and out again for each fma2: 194
+            // against 115 us at 16 experts, 16060 rows, 4096 -> 1536)
+            uint64_t acc[C::PARTS][C::PART / 32][2][8];
 #pragma unroll
-            for (int b = 0; b < LB; ++b) {
-                const int32_t slot = p.sorted_tok && 32 * b + lane < u.nr ? p.sorted_tok[u.r0 + 32 * b + lane] : 0;
-                const uint32_t m = __ballot_sync(0xFFFFFFFFu, slot >= 0);
-                if (lane == b) live = m;
-            }
-            // slice s of this group: rows 16 (G s + g) .. of the unit; a thread's 16 sums of it as tmem_ld8x8 has them
-            float acc[NS][16];
+            for (int h = 0; h < C::PARTS; ++h)
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+                for (int b = 0; b < C::PART / 32; ++b)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) acc[s][k] = 0.f;
-            const int mine = u.nr > kSlice * g ? (u.nr - kSlice * g + kSlice * G - 1) / (kSlice * G) : 0;   // slices of this group
-            for (int ck = k0; ck < k1; ++ck, db.next(DB), pipe.next(kScaleSt)) {
+                    for (int k = 0; k < 16; ++k) acc[h][b][k >> 3][k & 7] = 0;
+            for (int ck = k0; ck < k1; ++ck, pipe.next(kScaleSt)) {
                 wait(&sc_full[pipe.s], pipe.ph);
-                wait(&d_full[db.s], db.ph);
-                fence_after();
-                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * NT + kSlice * g;
-                const float* sc = sc_ring + pipe.s * C::HALVES * NT + kSlice * g + 2 * (lane & 3);
-                uint32_t a[2][16];
-                if (mine > 0) tmem_ld8x8(d, a[0]);
+                const float* sc = sc_ring + pipe.s * C::HALVES * C::SC_ROWS + 2 * g * pt.nl + 4 * (lane & 3);
 #pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    if (s >= mine) break;
-                    uint32_t (&now)[16] = a[s & 1];
-                    tmem_wait(now);
-                    if (s + 1 < NS && s + 1 < mine) tmem_ld8x8(d + (s + 1) * kSlice * G, a[(s + 1) & 1]);
+                for (int h = 0; h < C::PARTS; ++h) {
+                    const int ph = h ? pt.nl - pt.p0 : pt.p0;
+                    if (ph == 0) break;
+                    wait(&d_full[db.s], db.ph);
+                    fence_after();
+                    const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * C::DCOLS + g * ph;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int b = 0; b < C::PART / 32; ++b) {
+                        if (b && 32 * b >= ph) break;
+                        const bool last = 32 * (b + 1) >= (b + 1 < C::PART / 32 ? ph : 0);
+                        uint32_t a[16];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {               // weight rows 0..15 and 16..31 of the warp's 32
-                            const uint64_t f = *reinterpret_cast<const uint64_t*>(sc + (ACT ? half * NT : 0) + s * kSlice * G + 8 * h);
+                        for (int s = 0; s < 2; ++s) {
+                            tmem_ld4(d + ((16u * s) << 16) + 32 * b, a);
+                            tmem_wait(a);
+                            if (last && s == 1) {
+                                fence_before();
+                                __syncwarp();
+                                if (lane == 0) {
+                                    if (PAIR) arrive_even(&d_empty[db.s]);
+                                    else mbar_arrive(&d_empty[db.s]);
+                                }
+                            }
 #pragma unroll
-                            for (int v = 0; v < 2; ++v) {
-                                const int k = 8 * half + 4 * h + 2 * v;
-                                const uint64_t r = fma2(f2pk(__uint_as_float(now[k]), __uint_as_float(now[k + 1])), f,
-                                                        f2pk(acc[s][k], acc[s][k + 1]));
-                                f2upk(r, acc[s][k], acc[s][k + 1]);
+                            for (int e = 0; e < 4; ++e) {                    // eight rows: two of them this thread's
+                                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + (ACT ? s * C::SC_ROWS : 0) + 2 * (h * pt.p0 + 32 * b) + 16 * e);
+#pragma unroll
+                                for (int v = 0; v < 2; ++v) {
+                                    uint64_t& t = acc[h][b][s][2 * e + v];
+                                    const int k = 4 * e + 2 * v;
+                                    t = fma2(f2pk(__uint_as_float(a[k]), __uint_as_float(a[k + 1])), v ? f.y : f.x, t);
+                                }
                             }
                         }
                     }
-                }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (PAIR) arrive_even(&d_empty[db.s]);
-                    else mbar_arrive(&d_empty[db.s]);
-                    mbar_arrive(&sc_empty[pipe.s]);
+                    db.next(DB);
                 }
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_empty[pipe.s]);
             }
             if (__any_sync(0xFFFFFFFFu, *vdead)) break;
             const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
@@ -429,14 +485,10 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
                 // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
                 // then sums every split-th row over the CTAs, in their order, and stores it.
                 float* const st = epi;
-                const int c2 = 2 * (lane & 3);
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
-                    if (s < mine) {
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            st[(s * kSlice + 8 * (k >> 2 & 1) + c2 + (k & 1)) * kEpiLd + 32 * q + 16 * (k >> 3) + 8 * (k >> 1 & 1) + (lane >> 2)] = acc[s][k];
-                    }
+                for (int k = 0; k < 32; ++k)
+                    st[(4 * (k >> 1 & 7) + (lane & 3)) * kEpiLd + 32 * q + 16 * (k >> 4) + 8 * (k & 1) + (lane >> 2)] =
+                        __uint_as_float((uint32_t)(acc[0][0][k >> 4][k >> 1 & 7] >> (32 * (k & 1))));
                 __syncwarp();                                  // the arrivals publish the whole warp's sums
                 if (lane < split) arrive_at(part_full, lane);
                 __syncwarp();
@@ -473,27 +525,43 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
                 }
                 break;
             }
+            if (i + 1 < n_mine) fetch(unit_at(i + 1));
             const int64_t n_warp = b0 + (ACT ? 16 : 32) * q;                 // the warp's first output
-            const int c2 = 2 * (lane & 3);
+            // 32 rows a turn, the sums moved down between: unrolled over all of a unit's slices the code is read from far away
+            // each time (215 against 120 us at 16 experts, 16060 rows, 4096 -> 1536)
+            constexpr int TURNS = C::PARTS * C::PART / 32;
+            uint64_t (&flat)[TURNS][2][8] = reinterpret_cast<uint64_t (&)[TURNS][2][8]>(acc);
+#pragma unroll 1
+            for (int it = 0; it < TURNS; ++it) {
+                const int h = it * 32 >= C::PART, b = it - h * (C::PART / 32);
+                const int in = h ? pt.nl - pt.p0 : pt.p0;                        // rows of the part
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                if (s >= mine) break;
-                const int t0 = kSlice * (G * s + g);
-                uint32_t a[16];
+                for (int sl = 0; sl < 2; ++sl) {
+                    const int at = 32 * b + kSlice * sl, t0 = g * pt.nl + h * pt.p0 + at;
+                    if (at < in && t0 < u.nr) {
+                        uint32_t a[16];                                           // as act_slice takes them
 #pragma unroll
-                for (int k = 0; k < 16; ++k) a[k] = __float_as_uint(acc[s][k]);
-                constexpr int NV = ACT ? 8 : 16;
-                float v[NV];
-                act_slice<ACT>(a, v);
-                const uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
-                if ((here & 0xFFFFu) != 0xFFFFu) {                                // dropped slots are zero
+                        for (int k = 0; k < 16; ++k)
+                            a[k] = (uint32_t)(flat[0][k >> 3][4 * sl + 2 * (k >> 2 & 1) + (k & 1)] >> (32 * (k >> 1 & 1)));
+                        constexpr int NV = ACT ? 8 : 16;
+                        float v[NV];
+                        act_slice<ACT>(a, v);
+                        const uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
+                        if ((here & 0xFFFFu) != 0xFFFFu) {                        // dropped slots are zero
 #pragma unroll
-                    for (int k = 0; k < NV; ++k)
-                        if (!(here >> (8 * (k >> 2 & 1) + c2 + (k & 1)) & 1)) v[k] = 0.f;
+                            for (int k = 0; k < NV; ++k)
+                                if (!(here >> (8 * (k >> 2 & 1) + 4 * (k & 1) + (lane & 3)) & 1)) v[k] = 0.f;
+                        }
+                        store_slice<OUT, ACT, true>(v, y + (u.r0 + t0) * row_b, row_b, n_warp, p.n_out, u.nr - t0,
+                                                    reinterpret_cast<uint8_t*>(epi) + ew * 1024, lane);
+                    }
                 }
-                store_slice<OUT, ACT>(v, y + (u.r0 + t0) * row_b, row_b, n_warp, p.n_out, u.nr - t0,
-                                      reinterpret_cast<uint8_t*>(epi) + ew * 1024, lane);
+#pragma unroll
+                for (int k = 0; k + 1 < TURNS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) flat[k][j >> 3][j & 7] = flat[k + 1][j >> 3][j & 7];
             }
+            live = votes();
         }
     }
     fence_before();
@@ -545,7 +613,7 @@ template <bool ACT>
 int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     const int64_t few = p->w_rows < 512 ? 96 : 16;
     if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4)
-        return launch<true, false, ACT>(p, sm_count, 1, st);
+        return p->n_rows > 128 * (int64_t)p->n_expert ? wide::launch<true, ACT>(p, sm_count, st) : wide::launch<false, ACT>(p, sm_count, st);
     const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 127) / 128;
     int64_t split = sm_count / most;                          // so the grid has room for a cluster a unit: the kernel counts on it
     if (split > nck / 4) split = nck / 4;
