@@ -434,7 +434,7 @@ static inline EncodeTiledFn encode_fn() {
 // Weights, boxes of 128 bytes of k: [expert][row][k] and a block's 128 rows; for silu_mul [expert][group of 16 rows]
 // [gate, up][16][k] and a block's four groups, in one box (eight boxes of 16 rows a stage kept the issuing warp busy, 550
 // cycles a stage) unless the last group is half a one and the box would leave the weight: then a box a half group.
-// box_rows: a box of so many rows instead, whatever the act.
+// box_rows: plain boxes [1][box_rows][k] instead, whatever the act.
 static inline int make_map(const Exl3bGmmOp* p, CUtensorMap* map, int box_rows = 0) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return -6;

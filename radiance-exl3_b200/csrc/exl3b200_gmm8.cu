@@ -5,19 +5,20 @@
 //   y[i][n] = z[n], or silu(z[n]) * z[n_out + n] (act silu_mul), for every sorted row i of expert e
 //
 // The units of work, the operands' way into shared memory and the roles of the warps are grouped_mm's for 16-bit operands
-// (exl3b200_gmm.cu; exl3b200_gmm.cuh): weight rows are the MMA's M, sorted rows its N, a stage 128 bytes of k -- here one block
-// of 128. What differs is the sum over k. The scales are any f32 numbers, so the tensor cores' sums of one block cannot run on
-// into the next one's: each stage's four MMAs (kind::f8f6f4, K 32) start a fresh accumulator in tensor memory, one of several
-// in turn, and the summing warps, which hold the unit's sums in registers, add it times its scales:
+// (exl3b200_gmm.cu; exl3b200_gmm.cuh); a stage is 128 bytes of k, here one block of 128. What differs is the sum over k. The
+// scales are any f32 numbers, so the tensor cores' sums of one block cannot run on into the next one's: each stage's four MMAs
+// (kind::f8f6f4, K 32) start a fresh accumulator in tensor memory, one of several in turn, and the summing warps, which hold the
+// unit's sums in registers, add it times its scales:
 //   sum[n] = fma(d[n], sx * sw, sum[n])    in f32, one rounding a block of 128 and one for the scales' product
-// Three forms, as there: narrow (128 weight rows x up to 32 sorted rows, two CTAs an SM), SPLIT (narrow, a cluster a unit, each
-// CTA a part of its k) and PAIR (cta_group::2, 256 weight rows x up to 256 sorted rows).
+// Where experts have many rows, exl3b200_gmm8w.cuh's kernel does it; here, where they have few, the WEIGHT rows are the MMA's M
+// (128) and up to 32 sorted rows its N, in steps of 16, two CTAs an SM. With few units (SPLIT) a cluster for each of them, every
+// CTA a part of its k, the parts summed through distributed shared memory in the CTAs' order.
 // Warps of a CTA:
 //   0       weights: cp.async.bulk.tensor, 128-byte swizzled
-//   1       MMA issuer (PAIR: of the even CTA; the odd one's reports its filled stages there)
-//   2, 3    scales: sx * sw of 128 (narrow: 32) sorted rows a warp into a ring of stages; silu_mul: for gate rows and up rows
+//   1       MMA issuer
+//   2       scales: sx * sw of the sorted rows into a ring of stages; silu_mul: for gate rows and for up rows
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok
-//   8..     sums: each warp 32 weight rows, half of the slices of 16 sorted rows (narrow: all), then its outputs
+//   8..11   sums: each warp 32 weight rows, then its outputs
 // Every wait is bounded; one that gives up sets the error word, and every role then drains and leaves.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -35,47 +36,28 @@ using namespace exl3b;
 
 namespace {
 
-constexpr int kScaleSt = 4;                      // stages of scales at once, and what a lane loads of a row at a time
+constexpr int kScaleSt = 4;                      // stages of scales at once
 
-template <bool PAIR, bool SPLIT, bool ACT>
+template <bool SPLIT, bool ACT>
 struct Cfg {
-    static constexpr int NT = PAIR ? 256 : 32;                   // sorted rows a unit at most
-    static constexpr int NL = PAIR ? NT / 2 : NT;                // ... of which this CTA brings
-    static constexpr int SUM_G = PAIR ? 2 : 1;                   // groups of four summing warps, each for a CTA's sorted rows
-    static constexpr int PARTS = PAIR ? 2 : 1;                   // MMAs a 32 k at most, each of up to PART of a CTA's sorted rows
-    static constexpr int PART = NL / PARTS;
-    static constexpr int THREADS = (kEpiWarp0 + 4 * SUM_G) * 32;
-    static constexpr int X_B = NL * kRowB;
+    static constexpr int NT = 32;                                // sorted rows a unit at most
+    static constexpr int THREADS = (kEpiWarp0 + 4) * 32;
+    static constexpr int X_B = NT * kRowB;
     static constexpr int STAGE_B = kW_B + X_B;
     static constexpr int HALVES = ACT ? 2 : 1;                   // scales a sorted row: gate's, up's
     static constexpr int SC_ROWS = NT * 2;                       // floats of a half's scales: each twice
     static constexpr int SC_B = kScaleSt * HALVES * SC_ROWS * 4;
-    static constexpr int SC_WARPS = PAIR ? 2 : 1;
-    static constexpr int EPI_B = SPLIT ? NT * kEpiLd * 4 : 4 * SUM_G * 1024;
-    static constexpr int DB = 4, DCOLS = PART * (PAIR ? 2 : 1);  // accumulators in turn, of so many columns
-    static constexpr int TMEM = DB * DCOLS;
-    static constexpr int PER_SM = PAIR ? 1 : 2;
+    static constexpr int EPI_B = SPLIT ? NT * kEpiLd * 4 : 4 * 1024;
+    static constexpr int DB = 4;                                 // accumulators in turn, of NT columns
+    static constexpr int PER_SM = 2;
     static constexpr int BARS = 2 * kMaxSt + 2 * DB + 2 * kScaleSt + 1;
     static constexpr int fixed(int n_expert) { return 1024 + EPI_B + SC_B + 512 + (n_expert + 4) * 4; }
     static constexpr int stages(int n_expert, int per_sm) {
         const int n = ((per_sm == 1 ? 227 : 113) * 1024 - kStatic - fixed(n_expert)) / STAGE_B;
         return n < kMaxSt ? n : kMaxSt;
     }
-    static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0 && stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4), "tensor or shared memory");
-    static_assert(BARS * 8 + 8 <= 512, "barriers");
+    static_assert(stages(kMaxExpert, PER_SM) >= (SPLIT ? 3 : 4) && BARS * 8 + 8 <= 512, "shared memory");
 };
-
-// The sorted rows of a unit that a CTA brings, and those of them in the first MMA's part (the rest is in the second's).
-struct Parts {
-    int nl, p0;
-};
-template <typename C, int MB>
-__device__ __forceinline__ Parts parts_of(const Unit& u) {
-    Parts r;
-    r.nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
-    r.p0 = r.nl <= C::PART ? r.nl : (r.nl / 16 + 1) / 2 * 16;
-    return r;
-}
 
 // Where row r's scale lies in the ring, twice: with those of row r + 4, when r % 8 < 4, 16 bytes that a thread of tmem_ld4's
 // rows loads at once.
@@ -93,24 +75,24 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t r[16]) {
 }
 
 // OUT: y_dtype; ACT: silu_mul.
-template <bool PAIR, bool SPLIT, int OUT, bool ACT>
-__global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLIT, ACT>::PER_SM)
+template <bool SPLIT, int OUT, bool ACT>
+__global__ void __launch_bounds__(Cfg<SPLIT, ACT>::THREADS, Cfg<SPLIT, ACT>::PER_SM)
     k_gmm8(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
     const int ST = sh.st, split = sh.split;
-    using C = Cfg<PAIR, SPLIT, ACT>;
-    constexpr int NT = C::NT, THREADS = C::THREADS, MB = PAIR ? 2 : 1, DB = C::DB;
+    using C = Cfg<SPLIT, ACT>;
+    constexpr int NT = C::NT, THREADS = C::THREADS, DB = C::DB;
     constexpr int blk_out = ACT ? 64 : 128;                   // outputs a block (a CTA's part of a unit)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* w_ring = smem;                                   // [ST][128 rows][128 B]
-    uint8_t* x_ring = w_ring + ST * kW_B;                     // [ST][NL rows][128 B]
+    uint8_t* x_ring = w_ring + ST * kW_B;                     // [ST][32 rows][128 B]
     float* sc_ring = reinterpret_cast<float*>(x_ring + ST * C::X_B);   // [kScaleSt][HALVES][SC_ROWS]
     float* epi = sc_ring + C::SC_B / 4;
     uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(epi) + C::EPI_B);
-    uint64_t* full = bars;                                    // producers (PAIR: and the odd CTA's MMA warp) -> MMA warp
+    uint64_t* full = bars;                                    // producers -> MMA warp
     uint64_t* empty = full + ST;                              // MMA commit -> producers
     uint64_t* d_full = empty + ST;                            // MMA commit -> sums [DB]
-    uint64_t* d_empty = d_full + DB;                          // sums (PAIR: of both CTAs) -> MMA [DB]
+    uint64_t* d_empty = d_full + DB;                          // sums -> MMA [DB]
     uint64_t* sc_full = d_empty + DB;                         // scales -> sums [kScaleSt]
     uint64_t* sc_empty = sc_full + kScaleSt;                  // sums -> scales [kScaleSt]
     uint64_t* part_full = sc_empty + kScaleSt;                // SPLIT: every CTA's partial sums are in its shared memory
@@ -121,19 +103,18 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
     __shared__ uint32_t wsum[THREADS / 32];
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;        // which half of the unit's weight rows
     const uint32_t part = SPLIT ? blockIdx.x % split : 0u;    // which part of its k
-    const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / split : blockIdx.x;
+    const uint32_t first = SPLIT ? blockIdx.x / split : blockIdx.x;
     const uint32_t stride = sh.stride.d;
     if (tid < ST) {
-        mbar_init(&full[tid], 1 + 32 * kXWarps + (PAIR && rank == 0 ? 1 : 0));
+        mbar_init(&full[tid], 1 + 32 * kXWarps);
         mbar_init(&empty[tid], 1);
     } else if (tid >= 32 && tid < 32 + DB) {
         mbar_init(&d_full[tid - 32], 1);
-        mbar_init(&d_empty[tid - 32], 4 * C::SUM_G * MB);
+        mbar_init(&d_empty[tid - 32], 4);
     } else if (tid >= 64 && tid < 64 + kScaleSt) {
-        mbar_init(&sc_full[tid - 64], C::SC_WARPS);
-        mbar_init(&sc_empty[tid - 64], 4 * C::SUM_G);
+        mbar_init(&sc_full[tid - 64], 1);
+        mbar_init(&sc_empty[tid - 64], 4);
     } else if (tid == 96) {
         *dead = 0;
         if (SPLIT) mbar_init(part_full, 4 * split);
@@ -141,13 +122,13 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
-    if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C::TMEM);
-    if (PAIR || SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (warp == 1) tmem_alloc<false>(tmem_slot, DB * NT);
+    if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     chain_wait();                                             // all above needs no memory but the CTA's own
-    scan_units<THREADS, MB>(p, sh, first, prefix, utab, wsum);
+    scan_units<THREADS, 1>(p, sh, first, prefix, utab, wsum);
     fence_before();
     __syncthreads();
-    if (PAIR || SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs' barriers and tensor memory are set up
+    if (SPLIT) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs' barriers and tensor memory are set up
     fence_after();
     chain_next();                                             // every CTA has its tensor memory: a later kernel may ask for its own
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
@@ -155,7 +136,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
     // SPLIT: the grid has a cluster for every unit that offsets in ascending order can make, so one at most
     const uint32_t n_mine = n_units > first ? SPLIT ? 1u : exl3b_div_of(n_units - first + stride - 1, sh.stride) : 0u;
     auto unit_at = [&](uint32_t i) {
-        return i < kTab ? utab[i] : find_unit<MB>(p, prefix, first + i * stride, sh);
+        return i < kTab ? utab[i] : find_unit<1>(p, prefix, first + i * stride, sh);
     };
     const int nck = sh.nck;
     // this CTA's stages of a unit
@@ -186,301 +167,215 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
         __syncwarp();
     };
     Pipe pipe;                                                // of the stages
-    // PAIR: the summing warps' sums need more than the 128 registers a thread that 512 threads start with: 256 x 192 + 256 x 64
-    // are the 512 x 128 of the launch
-    if (warp < kEpiWarp0) {
-        if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 0) {
-            // ---------------------------------------------------------------- weights
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                const Unit u = unit_at(i);
-                const int b = u.blk + (int)rank;
-                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
-                    wait(&empty[pipe.s], pipe.ph ^ 1);
-                    mbar_expect_tx_el(&full[pipe.s], kW_B);
-                    uint8_t* dst = w_ring + pipe.s * kW_B;
-                    const int k = ck * 128;
-                    if (!ACT) {
-                        tma_w_el(dst, &wmap, k, b * 128, u.e, &full[pipe.s]);
-                    } else if (p.n_out % 16 == 0) {
-                        tma_w5_el(dst, &wmap, k, b * 4, u.e, &full[pipe.s]);
-                    } else {
+    if (warp == 0) {
+        // ---------------------------------------------------------------- weights
+        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+            const Unit u = unit_at(i);
+            for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
+                wait(&empty[pipe.s], pipe.ph ^ 1);
+                mbar_expect_tx_el(&full[pipe.s], kW_B);
+                uint8_t* dst = w_ring + pipe.s * kW_B;
+                const int k = ck * 128;
+                if (!ACT) {
+                    tma_w_el(dst, &wmap, k, u.blk * 128, u.e, &full[pipe.s]);
+                } else if (p.n_out % 16 == 0) {
+                    tma_w5_el(dst, &wmap, k, u.blk * 4, u.e, &full[pipe.s]);
+                } else {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            tma_w_el(dst + q * 4096, &wmap, k, b * 64 + 16 * q, u.e, &full[pipe.s]);
-                            tma_w_el(dst + q * 4096 + 2048, &wmap, k, (int)p.n_out + b * 64 + 16 * q, u.e, &full[pipe.s]);
-                        }
+                    for (int q = 0; q < 4; ++q) {
+                        tma_w_el(dst + q * 4096, &wmap, k, u.blk * 64 + 16 * q, u.e, &full[pipe.s]);
+                        tma_w_el(dst + q * 4096 + 2048, &wmap, k, (int)p.n_out + u.blk * 64 + 16 * q, u.e, &full[pipe.s]);
                     }
                 }
             }
-            // after a wait that gave up: a millisecond for the copies still in flight, before the CTA's memory goes
-            if (*vdead)
-                for (int j = 0; j < 50; ++j) __nanosleep(20000);
-        } else if (warp == 1 && rank == 1) {
-            // ---------------------------------------------------------------- PAIR, odd CTA: its filled stages, reported
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
-                    wait(&full[pipe.s], pipe.ph);
-                    proxy_fence();
-                    if (lane == 0) arrive_even(&full[pipe.s]);
-                    __syncwarp();
-                }
-            }
-        } else if (warp == 1) {
-            // ---------------------------------------------------------------- MMA issuer
-            const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
-            Pipe db;
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                const Parts pt = parts_of<C, MB>(unit_at(i));
-                for (int ck = k0; ck < k1; ++ck, pipe.next(ST)) {
-                    wait(&full[pipe.s], pipe.ph);
-                    proxy_fence();
-#pragma unroll
-                    for (int h = 0; h < C::PARTS; ++h) {
-                        const uint32_t n = MB * (h ? pt.nl - pt.p0 : pt.p0);
-                        if (n == 0) break;
-                        // D f32, e4m3 both, both operands K-major, M 128 (PAIR: 256), N n
-                        const uint32_t idesc = (n >> 3) << 17 | (8u * MB) << 24 | 1u << 4;
-                        wait(&d_empty[db.s], db.ph ^ 1);
-                        fence_after();
-                        mma4_f8<PAIR>(tmem + db.s * C::DCOLS, wd0 + (uint64_t)(pipe.s * kW_B >> 4),
-                                      xd0 + (uint64_t)((pipe.s * C::X_B + (h ? pt.p0 * kRowB : 0)) >> 4), idesc, 0u);
-                        commit_el<PAIR>(&d_full[db.s]);
-                        db.next(DB);
-                    }
-                    commit_el<PAIR>(&empty[pipe.s]);
-                }
-            }
-        } else if (warp < kXWarp0) {
-            // ---------------------------------------------------------------- scales
-            // A lane has Q neighbouring sorted rows and loads four blocks' scales of each at a time, into two register sets in turn,
-            // one on its way while the other is used, across units; the weight's scales of a batch are one a lane.
-            constexpr int Q = PAIR ? 4 : 1;
-            const int g = warp - 2;
-            if (g < C::SC_WARPS && n_mine) {
-                struct Set {
-                    float x[Q][4], w;
-                };
-                RowAhead<Q> ahead(p, g * 128 + Q * lane, 1);
-                const uint8_t* src[Q];
-                const float* wsrc = nullptr;
-                const bool whole = ((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0;
-                uint32_t lu = 0, cu = 0;                          // units of the next load and of the next batch used
-                int lc = k0, cc = k0;                             // ... and their first stages
-                auto rows = [&](const Unit& u) {
-                    ahead.rows(p.x_scales, p.xs_pitch, src);
-                    const int b = min((u.blk + (int)rank) * blk_out / 128, p.ws_blocks - 1) + (lane & 4 ? p.ws_blocks * (C::HALVES - 1) : 0);
-                    wsrc = reinterpret_cast<const float*>(p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes);
-                };
-                {
-                    const Unit u = unit_at(0);
-                    ahead.fetch(u);
-                    rows(u);
-                    if (n_mine > 1) ahead.fetch(unit_at(1));
-                }
-                auto load = [&](Set& s) {
-                    if (lu >= n_mine) return;
-                    if (whole && lc + 4 <= k1) {
-#pragma unroll
-                        for (int q = 0; q < Q; ++q) {
-                            const float* at = reinterpret_cast<const float*>(src[q]) + lc;
-                            if (lc & 3) {                          // SPLIT: a part that starts inside four blocks
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) s.x[q][j] = at[j];
-                            } else {
-                                const float4 t = *reinterpret_cast<const float4*>(at);
-                                s.x[q][0] = t.x; s.x[q][1] = t.y; s.x[q][2] = t.z; s.x[q][3] = t.w;
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < Q; ++q)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                s.x[q][j] = lc + j < k1 ? reinterpret_cast<const float*>(src[q])[lc + j] : 0.f;
-                    }
-                    s.w = lc + (lane & 3) < k1 ? wsrc[lc + (lane & 3)] : 0.f;
-                    if ((lc += 4) >= k1) {
-                        lc = k0;
-                        if (++lu < n_mine) {
-                            rows(unit_at(lu));
-                            if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
-                        }
-                    }
-                };
-                auto use = [&](const Set& s) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (cc + j >= k1) break;
-                        wait(&sc_empty[pipe.s], pipe.ph ^ 1);
-#pragma unroll
-                        for (int h = 0; h < C::HALVES; ++h) {
-                            const float w = __shfl_sync(0xFFFFFFFFu, s.w, 4 * h + j);
-                            float* dst = sc_ring + (pipe.s * C::HALVES + h) * C::SC_ROWS;
-#pragma unroll
-                            for (int q = 0; q < Q; ++q) {
-                                const float f = s.x[q][j] * w;
-                                *reinterpret_cast<float2*>(dst + scale_at(g * 128 + Q * lane + q)) = make_float2(f, f);
-                            }
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sc_full[pipe.s]);
-                        pipe.next(kScaleSt);
-                    }
-                    if ((cc += 4) >= k1) {
-                        cc = k0;
-                        ++cu;
-                    }
-                };
-                Set even = {}, odd = {};
-                load(even);
-                load(odd);
-                while (cu < n_mine && !*vdead) {
-                    use(even);
-                    load(even);
-                    if (cu >= n_mine) break;
-                    use(odd);
-                    load(odd);
-                }
-            }
-        } else {
-            // ---------------------------------------------------------------- sorted rows
-            // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's barrier
-            // when they have landed, and the MMA warp, which sees that, makes them visible to the asynchronous proxy.
-            constexpr int RP = (C::NL + 15) / 16, kStep = 4;      // passes a stage; stages a step of the row pointers
-            const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
-            const int kb = (int)p.n_in;
-            const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
-            RowAhead<RP> ahead(p, rr, 16);
-            auto mine = [&](uint32_t i) {                         // this CTA's rows of its i-th unit; blk: rows of its tile
-                Unit u = unit_at(i);
-                const int nl = ((u.nr + 16 * MB - 1) & ~(16 * MB - 1)) / MB;
-                u.r0 += (int)rank * nl;
-                u.nr = min(u.nr - (int)rank * nl, nl);
-                u.blk = nl;
-                return u;
-            };
-            Unit u = n_mine ? mine(0) : Unit{};
-            if (n_mine) ahead.fetch(u);
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                const int nl = u.blk;
-                const uint8_t* src[RP];
-                ahead.rows(static_cast<const uint8_t*>(p.x) + k0 * kRowB + c * 16, p.x_pitch_bytes, src);
-                if (i + 1 < n_mine) {
-                    u = mine(i + 1);
-                    ahead.fetch(u);
-                }
-                for (int c0 = k0; c0 < k1; c0 += kStep) {
-#pragma unroll
-                    for (int a = 0; a < kStep; ++a) {
-                        if (c0 + a >= k1) break;
-                        wait(&empty[pipe.s], pipe.ph ^ 1);
-                        const uint32_t dst = dst0 + pipe.s * C::X_B;
-                        if ((c0 + a + 1) * kRowB <= kb) {
-#pragma unroll
-                            for (int j = 0; j < RP; ++j)
-                                if (16 * j < nl) cp16(dst + j * 16 * kRowB, src[j] + a * kRowB);
-                        } else {                                  // the row ends in this stage: zeros behind it
-                            const bool in = (c0 + a) * kRowB + c * 16 < kb;
-#pragma unroll
-                            for (int j = 0; j < RP; ++j)
-                                if (16 * j < nl) cp16_or_zero(dst + j * 16 * kRowB, in ? src[j] + a * kRowB : src[j], in);
-                        }
-                        cp_arrive(&full[pipe.s]);
-                        pipe.next(ST);
-                    }
-#pragma unroll
-                    for (int j = 0; j < RP; ++j) src[j] += kStep * kRowB;
-                }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-    } else {
-        // ---------------------------------------------------------------- sums
-        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
-        constexpr int es = OUT == RAD_F32 ? 4 : 2, G = C::SUM_G;
-        uint8_t* const y = static_cast<uint8_t*>(p.y);
-        clear_outside<OUT>(p, blockIdx.x * 4 * G + ew, gridDim.x * 4 * G, lane);
-        const int64_t row_b = p.y_pitch * es;
-        // which of a unit's rows are live, 32 a lane: its slots are fetched a unit ahead
-        constexpr int LB = (NT + 31) / 32;
-        int32_t slot[LB];
-        auto fetch = [&](const Unit& n) {
-#pragma unroll
-            for (int b = 0; b < LB; ++b) slot[b] = p.sorted_tok && 32 * b + lane < n.nr ? p.sorted_tok[n.r0 + 32 * b + lane] : 0;
-        };
-        auto votes = [&]() {
-            uint32_t r = 0;
-#pragma unroll
-            for (int b = 0; b < LB; ++b) {
-                const uint32_t m = __ballot_sync(0xFFFFFFFFu, slot[b] >= 0);
-                if (lane == b) r = m;
+        // after a wait that gave up: a millisecond for the copies still in flight, before the CTA's memory goes
+        if (*vdead)
+            for (int j = 0; j < 50; ++j) __nanosleep(20000);
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
+        Pipe db;
+        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+            // D f32, e4m3 both, both operands K-major, M 128, N the rows in steps of 16
+            const uint32_t idesc = ((uint32_t)unit_at(i).nr + 15) / 16 << 18 | 8u << 24 | 1u << 4;
+            for (int ck = k0; ck < k1; ++ck, pipe.next(ST), db.next(DB)) {
+                wait(&full[pipe.s], pipe.ph);
+                proxy_fence();
+                wait(&d_empty[db.s], db.ph ^ 1);
+                fence_after();
+                mma4_f8<false>(tmem + db.s * NT, wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd0 + (uint64_t)(pipe.s * C::X_B >> 4), idesc, 0u);
+                commit_el<false>(&d_full[db.s]);
+                commit_el<false>(&empty[pipe.s]);
             }
-            return r;
+        }
+    } else if (warp == 2) {
+        // ---------------------------------------------------------------- scales
+        // A lane has a sorted row and loads four blocks' scales of it at a time, into two register sets in turn, one on its way
+        // while the other is used, across units; the weight's scales of a batch are one a lane (lanes 4 .. 7: up's).
+        struct Set {
+            float x[4], w;
         };
+        RowAhead<1> ahead(p, lane, 1);
+        const uint8_t* src[1];
+        const float* wsrc = nullptr;
+        const bool whole = ((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0;
+        uint32_t lu = 0, cu = 0;                              // units of the next load and of the next batch used
+        int lc = k0, cc = k0;                                 // ... and their first stages
+        auto rows = [&](const Unit& u) {
+            ahead.rows(p.x_scales, p.xs_pitch, src);
+            const int b = u.blk * blk_out / 128 + (lane & 4 ? p.ws_blocks * (C::HALVES - 1) : 0);
+            wsrc = reinterpret_cast<const float*>(p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes);
+        };
+        if (n_mine) {
+            const Unit u = unit_at(0);
+            ahead.fetch(u);
+            rows(u);
+            if (n_mine > 1) ahead.fetch(unit_at(1));
+        }
+        auto load = [&](Set& s) {
+            if (lu >= n_mine) return;
+            const float* at = reinterpret_cast<const float*>(src[0]) + lc;
+            if (whole && lc + 4 <= k1 && (lc & 3) == 0) {     // SPLIT: a part may start inside four blocks
+                const float4 t = *reinterpret_cast<const float4*>(at);
+                s.x[0] = t.x; s.x[1] = t.y; s.x[2] = t.z; s.x[3] = t.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s.x[j] = lc + j < k1 ? at[j] : 0.f;
+            }
+            s.w = lc + (lane & 3) < k1 ? wsrc[lc + (lane & 3)] : 0.f;
+            if ((lc += 4) >= k1) {
+                lc = k0;
+                if (++lu < n_mine) {
+                    rows(unit_at(lu));
+                    if (lu + 1 < n_mine) ahead.fetch(unit_at(lu + 1));
+                }
+            }
+        };
+        auto use = [&](const Set& s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (cc + j >= k1) break;
+                wait(&sc_empty[pipe.s], pipe.ph ^ 1);
+#pragma unroll
+                for (int h = 0; h < C::HALVES; ++h) {
+                    const float f = s.x[j] * __shfl_sync(0xFFFFFFFFu, s.w, 4 * h + j);
+                    *reinterpret_cast<float2*>(sc_ring + (pipe.s * C::HALVES + h) * C::SC_ROWS + scale_at(lane)) = make_float2(f, f);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_full[pipe.s]);
+                pipe.next(kScaleSt);
+            }
+            if ((cc += 4) >= k1) {
+                cc = k0;
+                ++cu;
+            }
+        };
+        Set even = {}, odd = {};
+        load(even);
+        load(odd);
+        while (cu < n_mine && !*vdead) {
+            use(even);
+            load(even);
+            if (cu >= n_mine) break;
+            use(odd);
+            load(odd);
+        }
+    } else if (warp >= kXWarp0 && warp < kEpiWarp0) {
+        // ---------------------------------------------------------------- sorted rows
+        // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's barrier
+        // when they have landed, and the MMA warp, which sees that, makes them visible to the asynchronous proxy.
+        constexpr int RP = NT / 16, kStep = 4;                // passes a stage; stages a step of the row pointers
+        const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
+        const int kb = (int)p.n_in;
+        const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
+        RowAhead<RP> ahead(p, rr, 16);
+        Unit u = n_mine ? unit_at(0) : Unit{};
+        if (n_mine) ahead.fetch(u);
+        for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
+            const int nl = u.nr;
+            const uint8_t* src[RP];
+            ahead.rows(static_cast<const uint8_t*>(p.x) + k0 * kRowB + c * 16, p.x_pitch_bytes, src);
+            if (i + 1 < n_mine) {
+                u = unit_at(i + 1);
+                ahead.fetch(u);
+            }
+            for (int c0 = k0; c0 < k1; c0 += kStep) {
+#pragma unroll
+                for (int a = 0; a < kStep; ++a) {
+                    if (c0 + a >= k1) break;
+                    wait(&empty[pipe.s], pipe.ph ^ 1);
+                    const uint32_t dst = dst0 + pipe.s * C::X_B;
+                    if ((c0 + a + 1) * kRowB <= kb) {
+#pragma unroll
+                        for (int j = 0; j < RP; ++j)
+                            if (16 * j < nl) cp16(dst + j * 16 * kRowB, src[j] + a * kRowB);
+                    } else {                                  // the row ends in this stage: zeros behind it
+                        const bool in = (c0 + a) * kRowB + c * 16 < kb;
+#pragma unroll
+                        for (int j = 0; j < RP; ++j)
+                            if (16 * j < nl) cp16_or_zero(dst + j * 16 * kRowB, in ? src[j] + a * kRowB : src[j], in);
+                    }
+                    cp_arrive(&full[pipe.s]);
+                    pipe.next(ST);
+                }
+#pragma unroll
+                for (int j = 0; j < RP; ++j) src[j] += kStep * kRowB;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp >= kEpiWarp0) {
+        // ---------------------------------------------------------------- sums
+        const int q = warp & 3;
+        constexpr int es = OUT == RAD_F32 ? 4 : 2;
+        uint8_t* const y = static_cast<uint8_t*>(p.y);
+        clear_outside<OUT>(p, blockIdx.x * 4 + q, gridDim.x * 4, lane);
+        const int64_t row_b = p.y_pitch * es;
+        // which of a unit's rows are live: its slots are fetched a unit ahead
+        int32_t slot = 0;
+        auto fetch = [&](const Unit& n) { slot = p.sorted_tok && lane < n.nr ? p.sorted_tok[n.r0 + lane] : 0; };
         if (n_mine) fetch(unit_at(0));
-        uint32_t live = votes();
         Pipe db;
         for (uint32_t i = 0; i < n_mine; ++i) {
             const Unit u = unit_at(i);
-            const Parts pt = parts_of<C, MB>(u);
-            // the group's rows are those that CTA g brings: row 32 b + .. of part h, its 16 sums of each half of the lanes as
-            // tmem_ld4 has them, two a word (as floats the compiler moved them into pairs and out again for each fma2: 194
-            // against 115 us at 16 experts, 16060 rows, 4096 -> 1536)
-            uint64_t acc[C::PARTS][C::PART / 32][2][8];
+            const uint32_t live = __ballot_sync(0xFFFFFFFFu, slot >= 0);
+            if (i + 1 < n_mine) fetch(unit_at(i + 1));
+            uint64_t acc[2][8];                               // sums of each half of the lanes as tmem_ld4 has them, two a word
 #pragma unroll
-            for (int h = 0; h < C::PARTS; ++h)
-#pragma unroll
-                for (int b = 0; b < C::PART / 32; ++b)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) acc[h][b][k >> 3][k & 7] = 0;
-            for (int ck = k0; ck < k1; ++ck, pipe.next(kScaleSt)) {
+            for (int k = 0; k < 16; ++k) acc[k >> 3][k & 7] = 0;
+            for (int ck = k0; ck < k1; ++ck, pipe.next(kScaleSt), db.next(DB)) {
                 wait(&sc_full[pipe.s], pipe.ph);
-                const float* sc = sc_ring + pipe.s * C::HALVES * C::SC_ROWS + 2 * g * pt.nl + 4 * (lane & 3);
+                wait(&d_full[db.s], db.ph);
+                fence_after();
+                const float* sc = sc_ring + pipe.s * C::HALVES * C::SC_ROWS + 4 * (lane & 3);
+                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * NT;
+                // one half's 16 registers at a time: with both, the pairs did not fit (13.8 against 10.7 us at one token)
+                uint32_t a[16];
 #pragma unroll
-                for (int h = 0; h < C::PARTS; ++h) {
-                    const int ph = h ? pt.nl - pt.p0 : pt.p0;
-                    if (ph == 0) break;
-                    wait(&d_full[db.s], db.ph);
-                    fence_after();
-                    const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * C::DCOLS + g * ph;
+                for (int s = 0; s < 2; ++s) {
+                    tmem_ld4(d + ((16u * s) << 16), a);
+                    tmem_wait(a);
+                    if (s == 1) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&d_empty[db.s]);
+                    }
 #pragma unroll
-                    for (int b = 0; b < C::PART / 32; ++b) {
-                        if (b && 32 * b >= ph) break;
-                        const bool last = 32 * (b + 1) >= (b + 1 < C::PART / 32 ? ph : 0);
-                        uint32_t a[16];
+                    for (int e = 0; e < 4; ++e) {             // eight rows: two of them this thread's
+                        const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + (ACT ? s * C::SC_ROWS : 0) + 16 * e);
 #pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            tmem_ld4(d + ((16u * s) << 16) + 32 * b, a);
-                            tmem_wait(a);
-                            if (last && s == 1) {
-                                fence_before();
-                                __syncwarp();
-                                if (lane == 0) {
-                                    if (PAIR) arrive_even(&d_empty[db.s]);
-                                    else mbar_arrive(&d_empty[db.s]);
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {                    // eight rows: two of them this thread's
-                                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + (ACT ? s * C::SC_ROWS : 0) + 2 * (h * pt.p0 + 32 * b) + 16 * e);
-#pragma unroll
-                                for (int v = 0; v < 2; ++v) {
-                                    uint64_t& t = acc[h][b][s][2 * e + v];
-                                    const int k = 4 * e + 2 * v;
-                                    t = fma2(f2pk(__uint_as_float(a[k]), __uint_as_float(a[k + 1])), v ? f.y : f.x, t);
-                                }
-                            }
+                        for (int v = 0; v < 2; ++v) {
+                            uint64_t& t = acc[s][2 * e + v];
+                            const int k = 4 * e + 2 * v;
+                            t = fma2(f2pk(__uint_as_float(a[k]), __uint_as_float(a[k + 1])), v ? f.y : f.x, t);
                         }
                     }
-                    db.next(DB);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[pipe.s]);
             }
             if (__any_sync(0xFFFFFFFFu, *vdead)) break;
-            const int64_t b0 = (int64_t)(u.blk + rank) * blk_out;           // the block's first output
+            const int64_t b0 = (int64_t)u.blk * blk_out;           // the block's first output
             if constexpr (SPLIT) {
                 // The parts' sums meet through distributed shared memory: every CTA puts its own into its shared memory,
                 // then sums every split-th row over the CTAs, in their order, and stores it.
@@ -488,7 +383,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
                     st[(4 * (k >> 1 & 7) + (lane & 3)) * kEpiLd + 32 * q + 16 * (k >> 4) + 8 * (k & 1) + (lane >> 2)] =
-                        __uint_as_float((uint32_t)(acc[0][0][k >> 4][k >> 1 & 7] >> (32 * (k & 1))));
+                        __uint_as_float((uint32_t)(acc[k >> 4][k >> 1 & 7] >> (32 * (k & 1))));
                 __syncwarp();                                  // the arrivals publish the whole warp's sums
                 if (lane < split) arrive_at(part_full, lane);
                 __syncwarp();
@@ -496,7 +391,6 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
                 asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 const bool out_lane = !ACT || !(lane & 4);    // silu_mul: 16 gate columns, then their 16 up columns
                 const int64_t n0 = b0 + (ACT ? 16 * (lane >> 3) + 4 * (lane & 3) : 4 * lane);
-                const uint32_t rows_live = __shfl_sync(0xFFFFFFFFu, live, 0);
                 for (int j = part + split * q; j < u.nr; j += split * 4) {
                     float f[kMaxSplit][4], v[4];
 #pragma unroll
@@ -516,7 +410,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
                             v[e] = v[e] < kSiluLow ? silu_up_low(v[e], up) : silu_up(v[e], up);
                         }
                     }
-                    if (!(rows_live >> j & 1)) v[0] = v[1] = v[2] = v[3] = 0.f;        // a dropped slot
+                    if (!(live >> j & 1)) v[0] = v[1] = v[2] = v[3] = 0.f;        // a dropped slot
                     if (out_lane && n0 < p.n_out) {
                         uint8_t* d = y + (u.r0 + j) * row_b + n0 * es;
                         if constexpr (OUT == RAD_F32) *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -525,65 +419,48 @@ __global__ void __launch_bounds__(Cfg<PAIR, SPLIT, ACT>::THREADS, Cfg<PAIR, SPLI
                 }
                 break;
             }
-            if (i + 1 < n_mine) fetch(unit_at(i + 1));
             const int64_t n_warp = b0 + (ACT ? 16 : 32) * q;                 // the warp's first output
-            // 32 rows a turn, the sums moved down between: unrolled over all of a unit's slices the code is read from far away
-            // each time (215 against 120 us at 16 experts, 16060 rows, 4096 -> 1536)
-            constexpr int TURNS = C::PARTS * C::PART / 32;
-            uint64_t (&flat)[TURNS][2][8] = reinterpret_cast<uint64_t (&)[TURNS][2][8]>(acc);
-#pragma unroll 1
-            for (int it = 0; it < TURNS; ++it) {
-                const int h = it * 32 >= C::PART, b = it - h * (C::PART / 32);
-                const int in = h ? pt.nl - pt.p0 : pt.p0;                        // rows of the part
 #pragma unroll
-                for (int sl = 0; sl < 2; ++sl) {
-                    const int at = 32 * b + kSlice * sl, t0 = g * pt.nl + h * pt.p0 + at;
-                    if (at < in && t0 < u.nr) {
-                        uint32_t a[16];                                           // as act_slice takes them
+            for (int sl = 0; sl < NT / kSlice; ++sl) {
+                const int t0 = kSlice * sl;
+                if (t0 >= u.nr) break;
+                uint32_t a[16];                                               // as act_slice takes them
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            a[k] = (uint32_t)(flat[0][k >> 3][4 * sl + 2 * (k >> 2 & 1) + (k & 1)] >> (32 * (k >> 1 & 1)));
-                        constexpr int NV = ACT ? 8 : 16;
-                        float v[NV];
-                        act_slice<ACT>(a, v);
-                        const uint32_t here = __shfl_sync(0xFFFFFFFFu, live, t0 >> 5) >> (t0 & 31);
-                        if ((here & 0xFFFFu) != 0xFFFFu) {                        // dropped slots are zero
+                for (int k = 0; k < 16; ++k)
+                    a[k] = (uint32_t)(acc[k >> 3][4 * sl + 2 * (k >> 2 & 1) + (k & 1)] >> (32 * (k >> 1 & 1)));
+                constexpr int NV = ACT ? 8 : 16;
+                float v[NV];
+                act_slice<ACT>(a, v);
+                const uint32_t here = live >> t0;
+                if ((here & 0xFFFFu) != 0xFFFFu) {                            // dropped slots are zero
 #pragma unroll
-                            for (int k = 0; k < NV; ++k)
-                                if (!(here >> (8 * (k >> 2 & 1) + 4 * (k & 1) + (lane & 3)) & 1)) v[k] = 0.f;
-                        }
-                        store_slice<OUT, ACT, true>(v, y + (u.r0 + t0) * row_b, row_b, n_warp, p.n_out, u.nr - t0,
-                                                    reinterpret_cast<uint8_t*>(epi) + ew * 1024, lane);
-                    }
+                    for (int k = 0; k < NV; ++k)
+                        if (!(here >> (8 * (k >> 2 & 1) + 4 * (k & 1) + (lane & 3)) & 1)) v[k] = 0.f;
                 }
-#pragma unroll
-                for (int k = 0; k + 1 < TURNS; ++k)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) flat[k][j >> 3][j & 7] = flat[k + 1][j >> 3][j & 7];
+                store_slice<OUT, ACT, true>(v, y + (u.r0 + t0) * row_b, row_b, n_warp, p.n_out, u.nr - t0,
+                                            reinterpret_cast<uint8_t*>(epi) + q * 1024, lane);
             }
-            live = votes();
         }
     }
     fence_before();
     __syncthreads();
-    if (PAIR || SPLIT) cluster_sync_all();                    // no CTA's memory goes while another uses it
+    if (SPLIT) cluster_sync_all();                            // no CTA's memory goes while another uses it
     if (warp == 1) {
         fence_after();
-        tmem_free<PAIR>(tmem, C::TMEM);
+        tmem_free<false>(tmem, DB * NT);
     }
 }
 
 typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
 
-// split: CTAs a unit, each a part of its k (SPLIT); PAIR: two CTAs a unit all the same.
-template <bool PAIR, bool SPLIT, bool ACT>
+// split: CTAs a unit, each a part of its k (SPLIT).
+template <bool SPLIT, bool ACT>
 int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
-    using C = Cfg<PAIR, SPLIT, ACT>;
+    using C = Cfg<SPLIT, ACT>;
     CUtensorMap map;
     const int rc = make_map(p, &map);
     if (rc) return rc;
-    static const Kern kerns[3] = { k_gmm8<PAIR, SPLIT, RAD_F32, ACT>, k_gmm8<PAIR, SPLIT, RAD_F16, ACT>,
-                                   k_gmm8<PAIR, SPLIT, RAD_BF16, ACT> };
+    static const Kern kerns[3] = { k_gmm8<SPLIT, RAD_F32, ACT>, k_gmm8<SPLIT, RAD_F16, ACT>, k_gmm8<SPLIT, RAD_BF16, ACT> };
     static bool allowed[64][3];                               // the most shared memory, once a device
     const int which = p->y_dtype == RAD_F32 ? 0 : p->y_dtype == RAD_F16 ? 1 : 2;
     const Kern kern = kerns[which];
@@ -593,33 +470,30 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
         allowed[dev][which] = true;
     }
-    const int ctas = PAIR ? 2 : split;                        // of a cluster
-    const int nt = PAIR ? pair_rows(p, C::NT, sm_count) : C::NT;
-    const int64_t most = most_units(p, nt, PAIR ? 2 : 1);
+    const int64_t most = most_units(p, C::NT, 1);
     // few units: one CTA an SM, with the whole of its shared memory for stages in flight; clusters of three or four do not
     // fill the SMs of every processing cluster
-    const int64_t alone = ctas > 2 ? sm_count - sm_count / 8 : sm_count;
-    const int per_sm = !PAIR && most * ctas <= alone ? 1 : C::PER_SM;
-    const int64_t room = (int64_t)sm_count * per_sm / ctas;
+    const int64_t alone = split > 2 ? sm_count - sm_count / 8 : sm_count;
+    const int per_sm = most * split <= alone ? 1 : C::PER_SM;
+    const int64_t room = (int64_t)sm_count * per_sm / split, units = most < room ? most : room;
     const int stages = C::stages(p->n_expert, per_sm);
-    const int64_t units = most < room ? most : room, blk = (p->act ? 64 : 128) * (PAIR ? 2 : 1);
-    const Shape sh = { exl3b_div((uint32_t)((p->n_out + blk - 1) / blk)), exl3b_div((uint32_t)units), exl3b_div((uint32_t)nt),
+    const int64_t blk = ACT ? 64 : 128;
+    const Shape sh = { exl3b_div((uint32_t)((p->n_out + blk - 1) / blk)), exl3b_div((uint32_t)units), exl3b_div((uint32_t)C::NT),
                        (int32_t)((p->n_in + 127) / 128), stages, split };
-    return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
-                        ctas, st, map, *p, sh);
+    return chain_launch(kern, dim3((unsigned)(units * split)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B, split, st,
+                        map, *p, sh);
 }
 
 template <bool ACT>
 int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     const int64_t few = p->w_rows < 512 ? 96 : 16;
-    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4)
-        return p->n_rows > 128 * (int64_t)p->n_expert ? wide::launch<true, ACT>(p, sm_count, st) : wide::launch<false, ACT>(p, sm_count, st);
+    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4) return wide::launch<ACT>(p, sm_count, st);
     const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 127) / 128;
     int64_t split = sm_count / most;                          // so the grid has room for a cluster a unit: the kernel counts on it
     if (split > nck / 4) split = nck / 4;
     if (split > kMaxSplit) split = kMaxSplit;
-    if (split >= 2) return launch<false, true, ACT>(p, sm_count, (int)split, st);
-    return launch<false, false, ACT>(p, sm_count, 1, st);
+    if (split >= 2) return launch<true, ACT>(p, sm_count, (int)split, st);
+    return launch<false, ACT>(p, sm_count, 1, st);
 }
 
 }  // namespace

@@ -1,16 +1,20 @@
-// exl3b200_gmm8w.cuh -- grouped_mm over FP8 operands where experts have many rows: the SORTED rows are the MMA's M and the
-// weight rows its N, the other way round than in exl3b200_gmm8.cu's narrow form. A thread of the summing warps then has one
-// sorted row and 128 of its outputs, so that a block's scale is one number a thread (sx of its row times sw of its columns'
-// block): the sums cost an LDTM and half an FFMA2 a value and no shared memory. (With the weight rows as M every column has a
-// scale of its own, read from shared memory four bytes a lane: 215 against X us at 16 experts, 16060 rows, 4096 -> 1536.)
+// exl3b200_gmm8w.cuh -- grouped_mm over FP8 operands where experts have many rows: the SORTED rows are the MMA's M (128) and the
+// weight rows its N, the other way round than in exl3b200_gmm8.cu. A thread of the summing warps then has one sorted row and 128
+// of its columns, so that a block's scale is one number a thread (sx of its row times sw of its columns' block): the sums cost
+// an FMA a value and no shared memory. (With the weight rows as M every column has a scale of its own, which a thread reads from
+// shared memory, four bytes a lane a cycle: 174 against 138 us at 16 experts, 16060 rows, 4096 -> 1536, and 253 against 182 at
+// 418 experts of 20072 rows, 2048 -> 512 silu_mul.)
 //
-// Two forms, persistent over units (expert, a group of its sorted rows, a block of 256 weight rows; silu_mul: 128 gate rows and
-// their 128 up rows):
-//   SOLO   one CTA, up to 128 sorted rows: experts of few rows, where the weights' bytes count
-//   PAIR   two CTAs (a cluster), up to 256 sorted rows, tcgen05 cta_group::2: each CTA brings half of the sorted rows and half
-//          of the weight rows, and both multiply by all of them
-// Columns: act NONE: the block's weight rows in order. silu_mul: 64 gate rows, their 64 up rows, and the next 64 of each, so
-// that a thread has both of its 64 outputs.
+// Persistent over units (expert, a group of up to 128 of its sorted rows, a block of 256 weight rows; silu_mul: 128 gate rows and
+// their 128 up rows), one CTA an SM. A unit's weight rows are two groups of 128, an MMA and four summing warps each: act NONE in
+// order; silu_mul 64 gate rows and their 64 up rows, and the next 64 of each, so that a thread has both of its 64 outputs.
+// Warps of a CTA:
+//   0       weights: cp.async.bulk.tensor, 128-byte swizzled
+//   1       MMA issuer: eight tcgen05.mma (kind::f8f6f4, M 128, N 128, K 32) a stage of 128 k, four a group, into the group's
+//           next accumulator (two each, in tensor memory)
+//   2, 3    nothing: they leave their registers to the summing warps
+//   4..7    sorted rows: 16-byte cp.async through sorted_tok
+//   8..15   sums: 32 sorted rows and a group's 128 columns each, then their outputs
 #pragma once
 
 #include <cuda.h>
@@ -25,98 +29,69 @@
 namespace exl3b {
 namespace wide {
 
-template <bool PAIR>
-struct Cfg {
-    static constexpr int NL = 128;                               // sorted rows a CTA at most: the MMA's lanes
-    static constexpr int NT = PAIR ? 2 * NL : NL;                // ... and a unit
-    static constexpr int WR = PAIR ? 128 : 256;                  // weight rows that a CTA brings
-    static constexpr int COLS = 256;                             // of an accumulator: a unit's weight rows
-    static constexpr int DB = 2;                                 // accumulators in turn
-    static constexpr int SUM_G = 2;                              // groups of four summing warps, 128 columns each
-    static constexpr int THREADS = (kEpiWarp0 + 4 * SUM_G) * 32;
-    static constexpr int W_B = WR * kRowB, X_B = NL * kRowB, STAGE_B = W_B + X_B;
-    static constexpr int BARS = 2 * kMaxSt + 2 * DB;
-    static constexpr int fixed(int n_expert) { return 1024 + 512 + (n_expert + 4) * 4; }
-    static constexpr int stages(int n_expert) {
-        const int n = (227 * 1024 - kStatic - fixed(n_expert)) / STAGE_B;
-        return n < kMaxSt ? n : kMaxSt;
-    }
-    static_assert(stages(kMaxExpert) >= 4 && BARS * 8 + 8 <= 512, "shared memory");
-};
-
-// 32 columns of this warp's 32 lanes, lane l's in thread l; tmem_wait32 before the registers are read.
-__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t r[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(t));
+constexpr int kGroups = 2;                                   // of four summing warps, each for 128 weight rows
+constexpr int kThreads = (kEpiWarp0 + 4 * kGroups) * 32;
+constexpr int kRows = 128;                                   // sorted rows a unit at most: the MMA's lanes
+constexpr int kCols = 128;                                   // of an accumulator: a group's weight rows
+constexpr int kDb = 2 * kGroups;                             // accumulators: two of each group in turn
+constexpr int kWideW_B = kGroups * kW_B, kX_B = kRows * kRowB, kStageB = kWideW_B + kX_B;
+constexpr int fixed_bytes(int n_expert) { return 1024 + 512 + (n_expert + 4) * 4; }
+constexpr int stages_of(int n_expert) {
+    const int n = (227 * 1024 - kStatic - fixed_bytes(n_expert)) / kStageB;
+    return n < kMaxSt ? n : kMaxSt;
 }
-__device__ __forceinline__ void tmem_wait32(uint32_t r[32]) {
-    tmem_wait(r);
-    tmem_wait(r + 16);
-}
+static_assert(stages_of(kMaxExpert) >= 4 && (2 * kMaxSt + 2 * kDb) * 8 + 8 <= 512, "shared memory");
 
-// The sorted rows of a unit that CTA `rank` brings: `nl` from `first` on, in tiles alike (PAIR: halves in steps of 16).
-struct Rows {
-    int first, n;
-};
-template <bool PAIR>
-__device__ __forceinline__ Rows rows_of(const Unit& u, uint32_t rank) {
-    if (!PAIR) return Rows{ u.r0, u.nr };
-    const int nl = (u.nr + 31) / 32 * 16;
-    return Rows{ u.r0 + (int)rank * nl, rank ? max(u.nr - nl, 0) : min(u.nr, nl) };
+// One arrival, by one lane of a whole warp.
+__device__ __forceinline__ void arrive_el(uint64_t* bar) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// A number from global memory if `ok`, else v as it was. In place: a value that met another one on the way would be waited for
+// where they meet.
+__device__ __forceinline__ void ld_if(float& v, const float* p, bool ok) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p ld.global.f32 %0, [%1];\n}\n" : "+f"(v) : "l"(p), "r"((uint32_t)ok));
 }
 
 // OUT: y_dtype; ACT: silu_mul.
-template <bool PAIR, int OUT, bool ACT>
-__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
-    k_gmm8w(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
+template <int OUT, bool ACT>
+__global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ CUtensorMap wmap, const Exl3bGmmOp p, const Shape sh) {
     const int ST = sh.st;
-    using C = Cfg<PAIR>;
-    constexpr int THREADS = C::THREADS, MB = PAIR ? 2 : 1, DB = C::DB;
     constexpr int blk_out = ACT ? 128 : 256;                  // outputs of a unit
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t* w_ring = smem;                                   // [ST][WR rows][128 B]
-    uint8_t* x_ring = w_ring + ST * C::W_B;                   // [ST][NL rows][128 B]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(x_ring + ST * C::X_B);
-    uint64_t* full = bars;                                    // producers (PAIR: and the odd CTA's MMA warp) -> MMA warp
+    uint8_t* w_ring = smem;                                   // [ST][256 rows][128 B]
+    uint8_t* x_ring = w_ring + ST * kWideW_B;                 // [ST][128 rows][128 B]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(x_ring + ST * kX_B);
+    uint64_t* full = bars;                                    // producers -> MMA warp
     uint64_t* empty = full + ST;                              // MMA commit -> producers
-    uint64_t* d_full = empty + ST;                            // MMA commit -> sums [DB]
-    uint64_t* d_empty = d_full + DB;                          // sums (PAIR: of both CTAs) -> MMA [DB]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + DB);
+    uint64_t* d_full = empty + ST;                            // MMA commit -> sums [kDb]
+    uint64_t* d_empty = d_full + kDb;                         // sums -> MMA [kDb]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + kDb);
     uint32_t* dead = tmem_slot + 1;                           // a wait gave up: everyone leaves
     uint32_t* prefix = reinterpret_cast<uint32_t*>(bars) + 128;   // [n_expert + 1]
     __shared__ Unit utab[kTab];
-    __shared__ uint32_t wsum[THREADS / 32];
+    __shared__ uint32_t wsum[kThreads / 32];
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u;
-    const uint32_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const uint32_t stride = sh.stride.d;
+    const uint32_t first = blockIdx.x, stride = sh.stride.d;
     if (tid < ST) {
-        mbar_init(&full[tid], 1 + 32 * kXWarps + (PAIR && rank == 0 ? 1 : 0));
+        mbar_init(&full[tid], 1 + 32 * kXWarps);
         mbar_init(&empty[tid], 1);
-    } else if (tid >= 32 && tid < 32 + DB) {
+    } else if (tid >= 32 && tid < 32 + kDb) {
         mbar_init(&d_full[tid - 32], 1);
-        mbar_init(&d_empty[tid - 32], 4 * C::SUM_G * MB);
+        mbar_init(&d_empty[tid - 32], 4);
     } else if (tid == 64) {
         *dead = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
-    if (warp == 1) tmem_alloc<PAIR>(tmem_slot, DB * C::COLS);
-    if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (warp == 1) tmem_alloc<false>(tmem_slot, kDb * kCols);
     chain_wait();                                             // all above needs no memory but the CTA's own
-    scan_units<THREADS, 1>(p, sh, first, prefix, utab, wsum);
+    scan_units<kThreads, 1>(p, sh, first, prefix, utab, wsum);
     fence_before();
     __syncthreads();
-    if (PAIR) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // both CTAs' barriers and tensor memory are set up
     fence_after();
     chain_next();                                             // every CTA has its tensor memory: a later kernel may ask for its own
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
@@ -162,51 +137,38 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
                 const Unit u = unit_at(i);
                 for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                     wait(&empty[pipe.s], pipe.ph ^ 1);
-                    mbar_expect_tx_el(&full[pipe.s], C::W_B);
-                    uint8_t* dst = w_ring + pipe.s * C::W_B;
+                    mbar_expect_tx_el(&full[pipe.s], kWideW_B);
+                    uint8_t* dst = w_ring + pipe.s * kWideW_B;
                     const int k = ck * 128;
 #pragma unroll
-                    for (int h = 0; h < C::WR / 128; ++h) {      // 128 columns at a time
-                        const int at = h + (int)rank;
-                        if (!ACT) {
-                            tma_w_el(dst + h * kW_B, &wmap, k, u.blk * 256 + 128 * at, u.e, &full[pipe.s]);
-                        } else {
-                            const int o = u.blk * 128 + 64 * at;
-                            tma_w_el(dst + h * kW_B, &wmap, k, o, u.e, &full[pipe.s]);
-                            tma_w_el(dst + h * kW_B + kW_B / 2, &wmap, k, (int)p.n_out + o, u.e, &full[pipe.s]);
-                        }
+                    for (int h = 0; h < 4; ++h) {                // 64 rows a box, two boxes a group
+                        const int row = ACT ? u.blk * 128 + 64 * (h >> 1) + (h & 1 ? (int)p.n_out : 0) : u.blk * 256 + 64 * h;
+                        tma_w_el(dst + h * (64 * kRowB), &wmap, k, row, u.e, &full[pipe.s]);
                     }
                 }
             }
             // after a wait that gave up: a millisecond for the copies still in flight, before the CTA's memory goes
             if (*vdead)
                 for (int j = 0; j < 50; ++j) __nanosleep(20000);
-        } else if (warp == 1 && rank == 1) {
-            // ------------------------------------------------------------ PAIR, odd CTA: its filled stages, reported
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ MMA issuer
+            const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
+            // D f32, e4m3 both, both operands K-major, M 128, N 128
+            constexpr uint32_t idesc = (uint32_t)kCols >> 3 << 17 | 8u << 24 | 1u << 4;
+            Pipe db;
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
                 for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                     wait(&full[pipe.s], pipe.ph);
                     proxy_fence();
-                    if (lane == 0) arrive_even(&full[pipe.s]);
-                    __syncwarp();
-                }
-            }
-        } else if (warp == 1) {
-            // ------------------------------------------------------------ MMA issuer
-            const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
-            // D f32, e4m3 both, both operands K-major, M 128 (PAIR: 256), N 256
-            const uint32_t idesc = (uint32_t)C::COLS >> 3 << 17 | (8u * MB) << 24 | 1u << 4;
-            Pipe db;
-            for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
-                for (int ck = 0; ck < nck; ++ck, pipe.next(ST), db.next(DB)) {
-                    wait(&full[pipe.s], pipe.ph);
-                    proxy_fence();
-                    wait(&d_empty[db.s], db.ph ^ 1);
-                    fence_after();
-                    mma4_f8<PAIR>(tmem + db.s * C::COLS, xd0 + (uint64_t)(pipe.s * C::X_B >> 4), wd0 + (uint64_t)(pipe.s * C::W_B >> 4),
-                                  idesc, 0u);
-                    commit_el<PAIR>(&d_full[db.s]);
-                    commit_el<PAIR>(&empty[pipe.s]);
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g, db.next(kDb)) {
+                        wait(&d_empty[db.s], db.ph ^ 1);
+                        fence_after();
+                        mma4_f8<false>(tmem + db.s * kCols, xd0 + (uint64_t)(pipe.s * kX_B >> 4),
+                                      wd0 + (uint64_t)((pipe.s * kWideW_B + g * kW_B) >> 4), idesc, 0u);
+                        commit_el<false>(&d_full[db.s]);
+                    }
+                    commit_el<false>(&empty[pipe.s]);
                 }
             }
         } else if (warp >= kXWarp0) {
@@ -214,26 +176,19 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
             // Eight lanes a row of a stage, 16 rows a pass of the four warps; each thread's copies arrive on the stage's
             // barrier when they have landed, and the MMA warp, which sees that, makes them visible to the asynchronous proxy.
             // Rows past the unit's are left as they were: their sums are nobody's.
-            constexpr int RP = C::NL / 16, kStep = 4;             // passes a stage; stages a step of the row pointers
+            constexpr int RP = kRows / 16, kStep = 4;             // passes a stage; stages a step of the row pointers
             const int xt = tid - kXWarp0 * 32, c = xt & 7, rr = xt >> 3;
             const int kb = (int)p.n_in;
             const uint32_t dst0 = smem_u32(x_ring) + rr * kRowB + ((c ^ (rr & 7)) << 4);
             RowAhead<RP> ahead(p, rr, 16);
-            auto mine = [&](uint32_t i) {
-                Unit u = unit_at(i);
-                const Rows r = rows_of<PAIR>(u, rank);
-                u.r0 = r.first;
-                u.nr = r.n;
-                return u;
-            };
-            Unit u = n_mine ? mine(0) : Unit{};
+            Unit u = n_mine ? unit_at(0) : Unit{};
             if (n_mine) ahead.fetch(u);
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
                 const int nl = u.nr;
                 const uint8_t* src[RP];
                 ahead.rows(static_cast<const uint8_t*>(p.x) + c * 16, p.x_pitch_bytes, src);
                 if (i + 1 < n_mine) {
-                    u = mine(i + 1);
+                    u = unit_at(i + 1);
                     ahead.fetch(u);
                 }
                 for (int c0 = 0; c0 < nck; c0 += kStep) {
@@ -241,7 +196,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
                     for (int a = 0; a < kStep; ++a) {
                         if (c0 + a >= nck) break;
                         wait(&empty[pipe.s], pipe.ph ^ 1);
-                        const uint32_t dst = dst0 + pipe.s * C::X_B;
+                        const uint32_t dst = dst0 + pipe.s * kX_B;
                         if ((c0 + a + 1) * kRowB <= kb) {
 #pragma unroll
                             for (int j = 0; j < RP; ++j)
@@ -266,135 +221,139 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
         constexpr int es = OUT == RAD_F32 ? 4 : 2;
-        clear_outside<OUT>(p, blockIdx.x * 4 * C::SUM_G + ew, gridDim.x * 4 * C::SUM_G, lane);
-        const bool whole = ((reinterpret_cast<uintptr_t>(p.x_scales) | (uintptr_t)p.xs_pitch) & 15) == 0;
+        clear_outside<OUT>(p, blockIdx.x * 4 * kGroups + ew, gridDim.x * 4 * kGroups, lane);
+        const bool sectors = ((reinterpret_cast<uintptr_t>(p.y) | (uintptr_t)(p.y_pitch * es)) & 31) == 0;
         RowAhead<1> ahead(p, 32 * q + lane, 1);
-        // four blocks' scales: of the thread's row, and of the weight, one a lane (lanes 4 .. 7: silu_mul's up rows)
+        // four blocks' scales: of the thread's row, and of its columns' block of the weight (silu_mul: of gate's and of up's)
         struct Scales {
-            float x[4], w;
+            float x[4], w[ACT ? 8 : 4];
         };
         const float *xs = nullptr, *ws = nullptr;
+        const int64_t ws_up = p.ws_blocks * p.ws_blk_bytes / 4;
         auto load = [&](Scales& s, int ck) {
-            if (whole && ck + 4 <= nck) {
-                const float4 t = *reinterpret_cast<const float4*>(xs + ck);
-                s.x[0] = t.x; s.x[1] = t.y; s.x[2] = t.z; s.x[3] = t.w;
-            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s.x[j] = ck + j < nck ? xs[ck + j] : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                ld_if(s.x[j], xs + ck + j, ck + j < nck);
+                ld_if(s.w[j], ws + ck + j, ck + j < nck);
+                if (ACT) ld_if(s.w[(4 + j) % (ACT ? 8 : 4)], ws + ws_up + ck + j, ck + j < nck);
             }
-            s.w = ck + (lane & 3) < nck ? ws[ck + (lane & 3)] : 0.f;
         };
-        Scales next;
+        Scales next = {};
         bool live_next = false;
         auto begin = [&](uint32_t i) {                        // unit i's rows and first scales; its slots are there
             const Unit u = unit_at(i);
             const uint8_t* at[1];
             ahead.rows(p.x_scales, p.xs_pitch, at);
             xs = reinterpret_cast<const float*>(at[0]);
-            const int b = ACT ? u.blk + (lane & 4 ? p.ws_blocks : 0) : min(2 * u.blk + g, p.ws_blocks - 1);
+            const int b = ACT ? u.blk : min(2 * u.blk + g, p.ws_blocks - 1);
             ws = reinterpret_cast<const float*>(p.w_scales + u.e * p.ws_expert_bytes + b * p.ws_blk_bytes);
             load(next, 0);
         };
         auto fetch = [&](uint32_t i) {                        // ... are asked for
-            Unit u = unit_at(i);
-            const Rows r = rows_of<PAIR>(u, rank);
-            u.r0 = r.first;
-            u.nr = r.n;
+            const Unit u = unit_at(i);
             ahead.fetch(u);
-            const int at = r.first + 32 * q + lane;
-            live_next = 32 * q + lane < r.n && (!p.sorted_tok || p.sorted_tok[at] >= 0);
+            live_next = 32 * q + lane < u.nr && (!p.sorted_tok || p.sorted_tok[u.r0 + 32 * q + lane] >= 0);
         };
         if (n_mine) {
             fetch(0);
             begin(0);
         }
+        // the group's accumulators: g, then g + 2
         Pipe db;
         for (uint32_t i = 0; i < n_mine; ++i) {
             const Unit u = unit_at(i);
-            const Rows r = rows_of<PAIR>(u, rank);
-            const bool any = 32 * q < r.n, live = live_next;
+            const bool any = 32 * q < u.nr, live = live_next;
             if (i + 1 < n_mine) fetch(i + 1);
-            uint64_t acc[4][16];                              // 128 columns, two a word
+            uint64_t acc[8][8];                               // 128 columns, two a word
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 8; ++c)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) acc[c][k] = 0;
-            Scales s = next;
+                for (int k = 0; k < 8; ++k) acc[c][k] = 0;
+            float f[ACT ? 8 : 4];                             // of the next four stages: for columns 0 .. 63, silu_mul: 64 .. 127
 #pragma unroll 1
-            for (int ck = 0; ck < nck; ++ck, db.next(DB)) {
+            for (int ck = 0; ck < nck; ++ck) {
                 if ((ck & 3) == 0) {
-                    s = next;
+#pragma unroll
+                    for (int j = 0; j < (ACT ? 8 : 4); ++j) f[j] = next.x[j & 3] * next.w[j];
                     if (ck + 4 < nck) load(next, ck + 4);
                 }
-                float f[2];
-                f[0] = s.x[0] * __shfl_sync(0xFFFFFFFFu, s.w, ck & 3);
-                f[1] = ACT ? s.x[0] * __shfl_sync(0xFFFFFFFFu, s.w, 4 + (ck & 3)) : f[0];
-                s.x[0] = s.x[1]; s.x[1] = s.x[2]; s.x[2] = s.x[3];
-                wait(&d_full[db.s], db.ph);
-                fence_after();
-                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + db.s * C::COLS + 128 * g;
+                const uint64_t f0 = f2pk(f[0], f[0]), f1 = ACT ? f2pk(f[ACT ? 4 : 0], f[ACT ? 4 : 0]) : f0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t a[32];
-                    if (any) {
-                        tmem_ld32(d + 32 * c, a);
-                        tmem_wait32(a);
-                    }
-                    if (c == 3) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) arrive_even(&d_empty[db.s]);
-                            else mbar_arrive(&d_empty[db.s]);
+                for (int j = 0; j < (ACT ? 8 : 4); ++j)
+                    if ((j & 3) < 3) f[j] = f[j + 1];
+                wait(&d_full[2 * db.s + g], db.ph);
+                fence_after();
+                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + (2 * db.s + g) * kCols;
+                uint64_t* const done = &d_empty[2 * db.s + g];
+                db.next(2);
+                if (any) {
+                    uint32_t a[2][16];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {             // 32 columns at a time
+                        tmem_ld16(d + 32 * c, a[0]);
+                        tmem_ld16(d + 32 * c + 16, a[1]);
+                        tmem_wait(a[0]);
+                        tmem_wait(a[1]);
+                        if (c == 3) {
+                            fence_before();
+                            arrive_el(done);
                         }
-                    }
-                    if (any) {
-                        const uint64_t ff = f2pk(f[c >> 1], f[c >> 1]);
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            acc[c][k] = fma2(f2pk(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1])), ff, acc[c][k]);
+                            acc[2 * c + (k >> 3)][k & 7] = fma2(f2pk(__uint_as_float(a[k >> 3][2 * (k & 7)]), __uint_as_float(a[k >> 3][2 * (k & 7) + 1])), c < 2 ? f0 : f1, acc[2 * c + (k >> 3)][k & 7]);
                     }
+                } else {
+                    arrive_el(done);
                 }
             }
             if (__any_sync(0xFFFFFFFFu, *vdead)) break;
             if (i + 1 < n_mine) begin(i + 1);                 // its first scales, on their way under the epilogue
             const int row = 32 * q + lane;
-            if (row < r.n) {
+            if (row < u.nr) {
                 constexpr int NV = ACT ? 64 : 128;
                 const int64_t n0 = (int64_t)u.blk * blk_out + NV * g;            // the thread's first output
-                uint8_t* d = static_cast<uint8_t*>(p.y) + (r.first + row) * (p.y_pitch * es) + n0 * es;
+                uint8_t* d = static_cast<uint8_t*>(p.y) + (u.r0 + row) * (p.y_pitch * es) + n0 * es;
                 const int left = (int)min((int64_t)NV, p.n_out - n0);
+                // 32 bytes a store, whole sectors, where they are aligned
+                constexpr int VS = 32 / es;
 #pragma unroll
-                for (int j = 0; j < NV / 8; ++j) {
-                    if (8 * j >= left) break;
-                    float v[8];
+                for (int j = 0; j < NV / VS; ++j) {
+                    if (VS * j >= left) break;
+                    float v[VS];
+                    auto two = [&](int k, float& a, float& b) { f2upk(acc[k >> 4][k >> 1 & 7], a, b); };   // columns k, k + 1
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) f2upk(acc[j >> 2][4 * (j & 3) + k], v[2 * k], v[2 * k + 1]);
+                    for (int k = 0; k < VS; k += 2) two(VS * j + k, v[k], v[k + 1]);
                     if constexpr (ACT) {
-                        float up[8];
+                        float up[VS], least = v[0];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) f2upk(acc[2 + (j >> 2)][4 * (j & 3) + k], up[2 * k], up[2 * k + 1]);
-                        float least = v[0];
+                        for (int k = 0; k < VS; k += 2) two((64 + VS * j + k) & 127, up[k], up[k + 1]);
 #pragma unroll
-                        for (int k = 1; k < 8; ++k) least = fminf(least, v[k]);
+                        for (int k = 1; k < VS; ++k) least = fminf(least, v[k]);
                         if (least < kSiluLow) {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = v[k] < kSiluLow ? silu_up_low(v[k], up[k]) : silu_up(v[k], up[k]);
+                            for (int k = 0; k < VS; ++k) v[k] = v[k] < kSiluLow ? silu_up_low(v[k], up[k]) : silu_up(v[k], up[k]);
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = silu_up(v[k], up[k]);
+                            for (int k = 0; k < VS; ++k) v[k] = silu_up(v[k], up[k]);
                         }
                     }
                     if (!live) {                                                  // a dropped slot
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+                        for (int k = 0; k < VS; ++k) v[k] = 0.f;
                     }
-                    if constexpr (OUT == RAD_F32) {
-                        *reinterpret_cast<float4*>(d + 32 * j) = make_float4(v[0], v[1], v[2], v[3]);
-                        *reinterpret_cast<float4*>(d + 32 * j + 16) = make_float4(v[4], v[5], v[6], v[7]);
+                    uint32_t w[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if constexpr (OUT == RAD_F32) w[k] = __float_as_uint(v[k]);
+                        else w[k] = pack2<OUT>(v[(2 * k) % VS], v[(2 * k + 1) % VS]);
+                    }
+                    if (sectors && VS * (j + 1) <= left) {
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(d + 32 * j), "r"(w[0]), "r"(w[1]),
+                                     "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                     : "memory");
                     } else {
-                        *reinterpret_cast<uint4*>(d + 16 * j) = make_uint4(pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3]),
-                                                                            pack2<OUT>(v[4], v[5]), pack2<OUT>(v[6], v[7]));
+                        *reinterpret_cast<uint4*>(d + 32 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (VS * j + VS / 2 < left) *reinterpret_cast<uint4*>(d + 32 * j + 16) = make_uint4(w[4], w[5], w[6], w[7]);
                     }
                 }
             }
@@ -403,21 +362,19 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
     }
     fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();                             // no CTA's memory goes while another uses it
     if (warp == 1) {
         fence_after();
-        tmem_free<PAIR>(tmem, DB * C::COLS);
+        tmem_free<false>(tmem, kDb * kCols);
     }
 }
 
-template <bool PAIR, bool ACT>
+template <bool ACT>
 int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
-    using C = Cfg<PAIR>;
     typedef void (*Kern)(CUtensorMap, Exl3bGmmOp, Shape);
     CUtensorMap map;
-    const int rc = make_map(p, &map, ACT ? 64 : 128);
+    const int rc = make_map(p, &map, 64);
     if (rc) return rc;
-    static const Kern kerns[3] = { k_gmm8w<PAIR, RAD_F32, ACT>, k_gmm8w<PAIR, RAD_F16, ACT>, k_gmm8w<PAIR, RAD_BF16, ACT> };
+    static const Kern kerns[3] = { k_gmm8w<RAD_F32, ACT>, k_gmm8w<RAD_F16, ACT>, k_gmm8w<RAD_BF16, ACT> };
     static bool allowed[64][3];                               // the most shared memory, once a device
     const int which = p->y_dtype == RAD_F32 ? 0 : p->y_dtype == RAD_F16 ? 1 : 2;
     const Kern kern = kerns[which];
@@ -427,15 +384,15 @@ int launch(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - kStatic) != cudaSuccess) return -6;
         allowed[dev][which] = true;
     }
-    const int ctas = PAIR ? 2 : 1;
     const int64_t blk = ACT ? 128 : 256, n_mb = (p->n_out + blk - 1) / blk;
     const int64_t live = p->n_expert < p->n_rows ? p->n_expert : p->n_rows;
-    const int64_t most = (live + p->n_rows / C::NT) * n_mb, room = sm_count / ctas, units = most < room ? most : room;
-    const int stages = C::stages(p->n_expert);
-    const Shape sh = { exl3b_div((uint32_t)n_mb), exl3b_div((uint32_t)units), exl3b_div((uint32_t)C::NT),
+    const int64_t most = (live + p->n_rows / kRows) * n_mb;
+    const int64_t units = most < sm_count ? most : sm_count;
+    const int stages = stages_of(p->n_expert);
+    const Shape sh = { exl3b_div((uint32_t)n_mb), exl3b_div((uint32_t)units), exl3b_div((uint32_t)kRows),
                        (int32_t)((p->n_in + 127) / 128), stages, 1 };
-    return chain_launch(kern, dim3((unsigned)(units * ctas)), dim3(C::THREADS), C::fixed(p->n_expert) + stages * C::STAGE_B,
-                        ctas, st, map, *p, sh);
+    return chain_launch(kern, dim3((unsigned)units), dim3(kThreads), fixed_bytes(p->n_expert) + stages * kStageB, 1, st, map,
+                        *p, sh);
 }
 
 }  // namespace wide
