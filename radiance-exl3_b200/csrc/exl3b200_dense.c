@@ -174,9 +174,9 @@ int exl3b200_router(const Exl3bRouter* d, void* stream) {
         G > 32 || E % G || d->group_keep < 1 || d->group_keep > G || d->group_top < 1 || d->group_top > 2 ||
         d->top_k > E / G * d->group_keep)
         return RAD_E_SHAPE;
-    int lanes = 32;                      /* of a group */
-    while (lanes * G > 32) lanes /= 2;
-    const int64_t per = (E / G + lanes - 1) / lanes;
+    int shift = 5;                       /* lanes of a group */
+    while (G << shift > 32) --shift;
+    const int64_t per = (E / G + (1 << shift) - 1) >> shift;
     if (per > 64) return RAD_E_SHAPE;
     const int sort = d->expert_offset != 0;
     if (d->n_tok > 0 && sort != (d->sorted_tok != 0)) return RAD_E_INVAL;
@@ -202,8 +202,11 @@ int exl3b200_router(const Exl3bRouter* d, void* stream) {
         p.group_keep = d->group_keep;
         p.group_top = d->group_top;
         p.group_size = (int32_t)(E / G);
-        p.group_lanes = lanes;
+        p.group_shift = shift;
         p.lane_experts = (int32_t)per;
+        const int64_t es = size_of(d->dtype);
+        if (E / G % per == 0 && per * es % 16 == 0 && !mis(d->logits, 16) && d->logits_pitch * es % 16 == 0) p.vec |= 1;
+        if (E / G % per == 0 && per % 4 == 0 && !mis(d->bias, 16)) p.vec |= 2;
         p.scale = d->scale;
         p.ids = d->ids;
         p.w = d->w;

@@ -79,14 +79,15 @@ typedef struct Exl3bGmmOp {
     int32_t*       err;                  /* device word: set nonzero when a bounded wait gives up */
 } Exl3bGmmOp;
 
-/* router (exl3b200_route.cu). A group has group_lanes lanes of a warp, each lane_experts neighbouring experts of it. */
+/* router (exl3b200_route.cu). A group has 2^group_shift lanes of a warp, each lane_experts neighbouring experts of it. */
 typedef struct Exl3bRouteOp {
     int64_t      n_tok;
     const void*  logits;
     int64_t      logits_pitch;           /* elements */
     const float* bias;
     int32_t      score, top_k, renorm;
-    int32_t      n_group, group_keep, group_top, group_size, group_lanes, lane_experts;
+    int32_t      n_group, group_keep, group_top, group_size, group_shift, lane_experts;
+    int32_t      vec;                    /* a lane's logits (1) and biases (2) can be read 16 bytes at a time */
     float        scale;
     int32_t*     ids;
     float*       w;

@@ -395,13 +395,13 @@ __device__ __forceinline__ void store_slice(const float (&v)[ACT ? 8 : 16], uint
         // against 177 us at 16 experts, 16067 rows, 1536 -> 4096.)
         constexpr int P = NV / 4, SH = ACT ? 2 : 1;                   // 16-byte pieces a row; rows that share banks
         auto at = [](int row, int piece) { return (row * P + (piece ^ (row >> SH & (P - 1)))) * 16; };
-        const int m = BY4 ? (lane >> 1 & 3) + 4 * (lane & 1) : lane & 7;
+        const int col = BY4 ? (lane >> 1 & 3) + 4 * (lane & 1) : lane & 7;
 #pragma unroll
         for (int s = 0; s < NV / 8; ++s) {
             uint32_t w[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m) w[m] = pack2<OUT>(v[8 * s + 2 * m], v[8 * s + 2 * m + 1]);
-            st8x8t(smem_u32(sw) + at(8 * (lane >> 4) + m, 2 * s + (lane >> 3 & 1)), w);
+            st8x8t(smem_u32(sw) + at(8 * (lane >> 4) + col, 2 * s + (lane >> 3 & 1)), w);
         }
         __syncwarp();
 #pragma unroll

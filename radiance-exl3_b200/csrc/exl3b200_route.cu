@@ -10,11 +10,20 @@
 // a power of two of groups leaves each), so that a group's maximum is a few shuffles and the lower of two lanes has the lower
 // experts. Experts that are masked (a logit or a c that is -inf or NaN) have key 0, below every other key.
 //
-// Choices are made as the real numbers order them, not as their roundings do: without a bias and without sums of two, the
-// logits themselves are compared (both scores grow with them), else c in 64 bits.
+// Choices are made as the real numbers order them, not as their roundings do. Without a bias and without sums of two the logits
+// are compared (both scores grow with them), else c. Each expert has a 32-bit key that orders as the number does, but for its
+// last bits, which hold the expert's place in the lane: one maximum finds both. 16-bit logits leave room for the whole expert,
+// and their keys are exact. Where two neighbours among the chosen ones, or the last chosen and the next, or the worst group kept
+// and the best one dropped, are nearer than the keys and the f32 scores behind them can tell, the token is routed again with
+// 64-bit scores, exactly (`again`; about one token in a hundred at most, unless logits are equal).
+//
+// Bound by instructions: a round is a maximum over the warp, its lane and the next key of that lane. Measured on one B200:
+// 16384 tokens, 256 experts, sigmoid, bias, four of eight groups, eight chosen: @T1 us (all in 64 bits 43); the 17 MB are 2.7.
 #include <cuda_runtime.h>
 #include <float.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "exl3b200_chain.cuh"
 #include "exl3b200_dense.h"
@@ -32,6 +41,7 @@ __device__ __forceinline__ uint32_t key_of(float f) {
     const uint32_t b = __float_as_uint(f == 0.f ? 0.f : f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
 __device__ __forceinline__ uint64_t key_of(double f) {
     const uint64_t b = (uint64_t)__double_as_longlong(f == 0. ? 0. : f);
     return (b >> 63) ? ~b : (b | 1ull << 63);
@@ -45,12 +55,8 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     const uint32_t lo = __reduce_max_sync(kAll, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
     return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(kAll, v, m);
-    return v;
-}
-__device__ __forceinline__ double warp_sum(double v) {
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
     for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(kAll, v, m);
     return v;
@@ -61,168 +67,366 @@ __device__ __forceinline__ float warp_max_of(float v) {
     return v;
 }
 
-// The keys of experts outside the kept groups to 0. Called by whole warps.
-template <int RPL, typename K>
-__device__ __forceinline__ void keep_groups(const Exl3bRouteOp& p, K key[RPL], int lane) {
-    K a = 0, b = 0;                                            // the lane's, then the group's, two largest
-#pragma unroll
-    for (int q = 0; q < RPL; ++q) {
-        const K lo = min(a, key[q]);
-        a = max(a, key[q]);
-        b = max(b, lo);
-    }
-    for (int m = 1; m < p.group_lanes; m <<= 1) {
+// 1 / (1 + e^-z); below -20 its exponential, which it is to within 2^-28, and which stays in range while the value does.
+__device__ __forceinline__ float sigmoid(float z) { return z < -20.f ? expf(z) : 1.f / (1.f + expf(-z)); }
+
+// e^x from the special-function unit: within 2^-22 + |x| 2^-24 of the value.
+__device__ __forceinline__ float exp_near(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+    return r;
+}
+__device__ __forceinline__ float sigmoid_near(float z) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp_near(-z)));
+    return r;
+}
+
+// A logit: NaN as -inf, +inf as the largest number, which it stands for.
+__device__ __forceinline__ float logit_of(float v) { return v == v ? fminf(v, FLT_MAX) : -INFINITY; }
+
+// The experts of a lane: n from e0 on.
+struct Span {
+    int e0, n;
+};
+__device__ __forceinline__ Span span_of(const Exl3bRouteOp& p, int lane) {
+    const int g = lane >> p.group_shift, first = (lane - (g << p.group_shift)) * p.lane_experts;
+    return Span{ g * p.group_size + first, g < p.n_group ? max(min(p.group_size - first, p.lane_experts), 0) : 0 };
+}
+
+// The two largest of a lane's keys -> those of its group's lanes.
+template <typename K>
+__device__ __forceinline__ void group_top(const Exl3bRouteOp& p, K& a, K& b) {
+    for (int m = 1; m >> p.group_shift == 0; m <<= 1) {
         const K oa = __shfl_xor_sync(kAll, a, m), ob = __shfl_xor_sync(kAll, b, m);
         b = max(min(a, oa), max(b, ob));
         a = max(a, oa);
     }
-    if constexpr (sizeof(K) == 8) {
-        if (p.group_top == 2 && b) a = key_of(value_of(a) + value_of(b));
-    }
-    const int g = lane / p.group_lanes;
+}
+// Whether the lane's group is among the group_keep with the largest score, the lower one among equals.
+template <typename K>
+__device__ __forceinline__ bool group_kept(const Exl3bRouteOp& p, K score, int lane) {
+    const int g = lane >> p.group_shift;
     int ahead = 0;
     for (int j = 0; j < p.n_group; ++j) {
-        const K o = __shfl_sync(kAll, a, j * p.group_lanes);
-        ahead += o > a || (o == a && j < g);
+        const K o = __shfl_sync(kAll, score, j << p.group_shift);
+        ahead += o > score || (o == score && j < g);
     }
-    if (ahead >= p.group_keep) {
-#pragma unroll
-        for (int q = 0; q < RPL; ++q) key[q] = 0;
-    }
+    return ahead < p.group_keep;
 }
 
-// The expert of lane r's round, r < top_k: the largest key left, the lowest expert among equals; -1 when none is left.
-template <int RPL, typename K>
-__device__ __forceinline__ int pick(K key[RPL], int e0, int top_k, int lane) {
-    K best;
-    int at;
-    auto look = [&]() {
-        best = key[0];
-        at = 0;
+// The choice in 64 bits: lane r's is round r's expert, -1 when none is left. A lane of up to 16 experts holds their keys; of
+// more, it works them out as often as it looks at them.
+template <int RPL, int DT, bool WIDE>
+__device__ __noinline__ int again(const Exl3bRouteOp& p, const typename El<DT>::T* row, float top, int lane) {
+    constexpr bool HOLD = RPL <= 16;
+    const Span s = span_of(p, lane);
+    const bool softmax = p.score == EXL3B_SCORE_SOFTMAX;
+    auto each = [&](auto&& f) {                                // of the lane's experts
+        if constexpr (HOLD) {
 #pragma unroll
-        for (int q = 1; q < RPL; ++q)
-            if (key[q] > best) {
-                best = key[q];
+            for (int q = 0; q < RPL; ++q) f(q);
+        } else {
+            for (int q = 0; q < s.n; ++q) f(q);
+        }
+    };
+    auto logit = [&](int q) { return q < s.n ? logit_of(El<DT>::to(row[s.e0 + q])) : -INFINITY; };
+    double sum = 0.;
+    if (WIDE && softmax) {
+        each([&](int q) { sum += exp((double)logit(q) - (double)top); });
+        sum = warp_sum(sum);
+    }
+    auto key = [&](int q) -> uint64_t {
+        const float l = logit(q);
+        double c = l;
+        if (WIDE) {
+            c = softmax ? exp((double)l - (double)top) / sum : 1. / (1. + exp(-(double)l));
+            if (p.bias && q < s.n) c += (double)p.bias[s.e0 + q];
+        }
+        return l > -INFINITY && c > -INFINITY ? key_of(c) : 0;
+    };
+    uint64_t held[HOLD ? RPL : 1];
+    if constexpr (HOLD) each([&](int q) { held[q] = key(q); });
+    uint64_t taken = 0;                                        // of the lane's experts
+    auto left = [&](int q) -> uint64_t {
+        if (taken >> q & 1) return 0;
+        if constexpr (HOLD) return held[q];
+        else return key(q);
+    };
+    if (p.group_keep < p.n_group) {
+        uint64_t a = 0, b = 0;
+        each([&](int q) {
+            const uint64_t k = left(q);
+            b = max(b, min(a, k));
+            a = max(a, k);
+        });
+        group_top(p, a, b);
+        if (p.group_top == 2 && b) a = key_of(value_of(a) + value_of(b));
+        if (!group_kept(p, a, lane)) taken = ~0ull;
+    }
+    int mine = -1;
+    for (int r = 0; r < p.top_k; ++r) {
+        uint64_t best = 0;
+        int at = 0;
+        each([&](int q) {
+            const uint64_t k = left(q);
+            if (k > best) {
+                best = k;
                 at = q;
             }
-    };
-    look();
-    int mine = -1;
-    for (int r = 0; r < top_k; ++r) {
-        const K top = warp_max(best);
-        if (top == 0) break;
-        const int from = __ffs(__ballot_sync(kAll, best == top)) - 1;
-        const int id = __shfl_sync(kAll, e0 + at, from);
+        });
+        const uint64_t most = warp_max(best);
+        if (most == 0) break;
+        const int from = __ffs(__ballot_sync(kAll, best == most)) - 1;
+        const int id = __shfl_sync(kAll, s.e0 + at, from);
         if (lane == r) mine = id;
-        if (lane == from) {
-#pragma unroll
-            for (int q = 0; q < RPL; ++q)
-                if (q == at) key[q] = 0;
-            look();
-        }
+        if (lane == from) taken |= 1ull << at;
     }
     return mine;
 }
 
-// 1 / (1 + e^-z); below -20 its exponential, which it is to within 2^-28, and which stays in range while the value does.
-__device__ __forceinline__ float sigmoid(float z) { return z < -20.f ? expf(z) : 1.f / (1.f + expf(-z)); }
+// A lane's n values from p on as f32; `vec`: n is all of them or none, 16 bytes aligned.
+template <int N, typename T>
+__device__ __forceinline__ void load_lane(const T* p, int n, bool vec, float (&v)[N]) {
+    constexpr int V = 16 / (int)sizeof(T);
+    typedef El<sizeof(T) == 4 ? RAD_F32 : std::is_same<T, __half>::value ? RAD_F16 : RAD_BF16> E;
+    if (N >= V && vec) {
+#pragma unroll
+        for (int q = 0; q + V <= N; q += V) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (q < n) w = *reinterpret_cast<const uint4*>(p + q);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[q + i] = E::to(reinterpret_cast<const T*>(&w)[i]);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = q < n ? E::to(p[q]) : 0.f;
+    }
+}
 
-// One token, by a whole warp.
+// Descending, by Batcher's odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+        for (int q = p; q; q >>= 1)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+                        k[i + j] = hi;
+                        k[i + j + q] = lo;
+                    }
+}
+
+// One token, by a whole warp; its ids also to `local` (shared memory), if given.
 template <int RPL, int DT, bool WIDE>
-__device__ __forceinline__ void route(const Exl3bRouteOp& p, int64_t t, int lane) {
+__device__ __forceinline__ void route(const Exl3bRouteOp& p, int64_t t, int lane, int32_t* local = nullptr) {
     typedef typename El<DT>::T T;
+    constexpr bool EXACT = !WIDE && DT != RAD_F32;             // the keys are: 16 bits and the expert
+    constexpr uint32_t LOW = EXACT ? 0xFFFFu : RPL <= 8 ? 7u : RPL <= 16 ? 15u : RPL <= 32 ? 31u : 63u;
+    constexpr bool SORT = RPL <= 16;                           // a lane's keys are sorted, or searched each round
     const T* row = static_cast<const T*>(p.logits) + t * p.logits_pitch;
-    const int g = lane / p.group_lanes, j = lane % p.group_lanes;
-    const int first = j * p.lane_experts, left = p.group_size - first;
-    const int n = g < p.n_group ? max(min(left, p.lane_experts), 0) : 0, e0 = g * p.group_size + first;
-    float l[RPL];                                              // NaN as -inf; +inf as the largest number, which it stands for
-    float top = -INFINITY;
+    const Span span = span_of(p, lane);
+    const int n = span.n, e0 = span.e0;
+    const bool softmax = p.score == EXL3B_SCORE_SOFTMAX;
+    float l[RPL], bias[WIDE ? RPL : 1];
+    load_lane<RPL>(row + e0, n, p.vec & 1, l);
+    if (WIDE) {
+        if (p.bias) load_lane<WIDE ? RPL : 1>(p.bias + e0, n, p.vec & 2, bias);
+        else
+#pragma unroll
+            for (int q = 0; q < RPL; ++q) bias[WIDE ? q : 0] = 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < RPL; ++q) l[q] = q < n ? logit_of(l[q]) : -INFINITY;
+    float top = 0.f, inv = 1.f;                                // softmax: the largest logit, one over the sum
+    if (softmax && (WIDE || !p.renorm)) {
+        top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < RPL; ++q) top = fmaxf(top, l[q]);
+        top = fmaxf(warp_max_of(top), -FLT_MAX);               // a row with nothing in it: any number does
+        float sum = 0.f;
+#pragma unroll
+        for (int q = 0; q < RPL; ++q) sum += expf(l[q] - top);
+        inv = 1.f / warp_sum(sum);
+    }
+    uint32_t key[RPL];
 #pragma unroll
     for (int q = 0; q < RPL; ++q) {
-        const float v = q < n ? El<DT>::to(row[e0 + q]) : -INFINITY;
-        l[q] = v == v ? fminf(v, FLT_MAX) : -INFINITY;
-        top = fmaxf(top, l[q]);
-    }
-    const bool softmax = p.score == EXL3B_SCORE_SOFTMAX;
-    if (softmax) top = fmaxf(warp_max_of(top), -FLT_MAX);      // a row with nothing in it: any number does
-    int id;
-    if constexpr (WIDE) {
-        double s[RPL];
-        double sum = 0.;
-#pragma unroll
-        for (int q = 0; q < RPL; ++q) {
-            s[q] = softmax ? exp((double)l[q] - (double)top) : 1. / (1. + exp(-(double)l[q]));
-            sum += s[q];
+        float c = l[q];
+        if (WIDE) {
+            c = (softmax ? exp_near(c - top) * inv : sigmoid_near(c)) + bias[WIDE ? q : 0];
         }
-        if (softmax) sum = warp_sum(sum);
-        uint64_t key[RPL];
-#pragma unroll
-        for (int q = 0; q < RPL; ++q) {
-            const double c = (softmax ? s[q] / sum : s[q]) + (p.bias && q < n ? (double)p.bias[e0 + q] : 0.);
-            key[q] = l[q] > -INFINITY && c > -INFINITY ? key_of(c) : 0;
+        const bool in = l[q] > -INFINITY && c > -INFINITY;
+        if constexpr (DT == RAD_F16 && EXACT) {                // f16's own order: its 19 significant bits of an f32 are too many
+            const uint32_t h = __half_as_ushort(__float2half_rn(c == 0.f ? 0.f : c));     // the largest f32: +inf, as it was
+            key[q] = in ? ((h & 0x8000u) ? ~h & 0xFFFFu : h | 0x8000u) << 16 | (LOW - (uint32_t)(e0 + q)) : 0u;
+        } else {
+            if (EXACT && c == FLT_MAX) c = INFINITY;           // bf16's own largest number has the same 16 bits
+            key[q] = in ? (key_of(c) & ~LOW) | (LOW - (uint32_t)(EXACT ? e0 + q : q)) : 0u;
         }
-        if (p.group_keep < p.n_group) keep_groups<RPL>(p, key, lane);
-        id = pick<RPL>(key, e0, p.top_k, lane);
-    } else {
-        uint32_t key[RPL];
-#pragma unroll
-        for (int q = 0; q < RPL; ++q) key[q] = l[q] > -INFINITY ? key_of(l[q]) : 0;
-        if (p.group_keep < p.n_group) keep_groups<RPL>(p, key, lane);
-        id = pick<RPL>(key, e0, p.top_k, lane);
     }
+    // Nearer than this two c cannot be told apart: twice an f32 score's error and, relative to c, its own rounding and the bits of
+    // the key that hold a place. A sigmoid s is off by s (1 - s) (2^-22 + |z| 2^-24) for the exponential and s 1.5 2^-23 for
+    // the sum and the reciprocal, below 2^-22 in all. A softmax's exponentials are off by 2^-22 + 0.4 2^-24 of the largest
+    // score, `inv`, at most, their sum (the same way for all) by as much and one rounding a term, at most 69 of 2^-24.
+    const float near = softmax ? 0x1p-16f * inv : 0x1p-20f;
+    constexpr float near_rel = 0x1p-22f + (float)(LOW + 1) * 0x1p-23f;
+    bool unsure = false;
+    auto compare = [&](uint32_t hi, uint32_t lo, float times) {
+        if constexpr (WIDE) {
+            const float a = value_of(hi & ~LOW), b = value_of(lo & ~LOW);
+            unsure = unsure || !(a - b > times * (near + near_rel * fmaxf(fabsf(a), fabsf(b))));
+        } else if constexpr (!EXACT) {
+            unsure = unsure || ((hi ^ lo) & ~LOW) == 0;
+        }
+    };
+    if (SORT) sort_down(key);
+    if (p.group_keep < p.n_group) {
+        uint32_t a = key[0], b = key[1];
+        if (!SORT) {
+            a = b = 0;
+#pragma unroll
+            for (int q = 0; q < RPL; ++q) {
+                b = max(b, min(a, key[q]));
+                a = max(a, key[q]);
+            }
+        }
+        group_top(p, a, b);
+        const bool two = WIDE && p.group_top == 2;
+        if (two && b) a = key_of(value_of(a & ~LOW) + value_of(b & ~LOW));
+        const bool kept = group_kept(p, a, lane);
+        if (!EXACT) {                                          // a sum's error is its terms', whose magnitudes it may not show
+            const uint32_t worst = ~warp_max(kept && lane >> p.group_shift < p.n_group ? ~a : 0u), best = warp_max(kept ? 0u : a);
+            float size = 0.f;
+            if (two && b) size = fabsf(value_of(b & ~LOW)) + fabsf(value_of(a));
+            if (two) size = warp_max_of(size);
+            if (best) compare(worst, best, 2.f);
+            if (two && best) unsure = unsure || !(value_of(worst) - value_of(best) > 2.f * near + 4.f * near_rel * size);
+        }
+        if (!kept) {
+#pragma unroll
+            for (int q = 0; q < RPL; ++q) key[q] = 0;
+        }
+    }
+    auto largest = [&]() {
+        uint32_t m = key[0];
+        if (!SORT) {
+#pragma unroll
+            for (int q = 1; q < RPL; ++q) m = max(m, key[q]);
+        }
+        return m;
+    };
+    uint32_t best = largest(), last = 0;
+    int id = -1;
+    for (int r = 0; r <= p.top_k; ++r) {
+        const uint32_t most = warp_max(best);
+        if (most == 0) break;
+        if (r > 0) compare(last, most, 1.f);
+        if (r == p.top_k) break;
+        last = most;
+        const int from = __ffs(__ballot_sync(kAll, best == most)) - 1;
+        const int at = (int)(LOW - (most & LOW)), here = EXACT ? at : __shfl_sync(kAll, e0, from) + at;
+        if (lane == r) id = here;
+        const bool win = lane == from;
+        if (SORT) {
+#pragma unroll
+            for (int q = 0; q < RPL; ++q) key[q] = win ? (q + 1 < RPL ? key[(q + 1) % RPL] : 0u) : key[q];
+        } else {
+#pragma unroll
+            for (int q = 0; q < RPL; ++q) key[q] = win && key[q] == most ? 0u : key[q];
+        }
+        best = largest();
+    }
+    if (!EXACT && unsure) id = again<RPL, DT, WIDE>(p, row, top, lane);
     // lane r has round r's expert. Renormalised weights come from the chosen logits alone; softmax's, and those of sigmoids all
     // below -20, less the largest of them, in range however small the scores are
     float z = -INFINITY;
     if (id >= 0) z = fminf(El<DT>::to(row[id]), FLT_MAX);
     float w;
-    if (softmax || p.renorm) {
+    if (p.renorm) {
         const float most = fmaxf(warp_max_of(z), -FLT_MAX);
-        if (softmax && !p.renorm) {
-            float sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < RPL; ++q) sum += expf(l[q] - top);
-            w = expf(z - top) / warp_sum(sum);
-        } else {
-            w = softmax || most < -20.f ? expf(z - most) : sigmoid(z);
-            w /= warp_sum(w);
-        }
+        w = softmax || most < -20.f ? expf(z - most) : sigmoid(z);
+        w /= warp_sum(w);
     } else {
-        w = sigmoid(z);
+        w = softmax ? expf(z - top) * inv : sigmoid(z);
     }
     if (lane < p.top_k) {
         p.ids[t * p.top_k + lane] = id;
         p.w[t * p.top_k + lane] = id < 0 ? 0.f : w * p.scale;
+        if (local) local[t * p.top_k + lane] = id;
     }
 }
 
 template <int RPL, int DT, bool WIDE>
-__global__ void __launch_bounds__(128) k_route(const Exl3bRouteOp p) {
+__global__ void __launch_bounds__(128) k_route(const __grid_constant__ Exl3bRouteOp p) {
     chain_wait();
     chain_next();
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (t < p.n_tok) route<RPL, DT, WIDE>(p, t, threadIdx.x & 31);
 }
 
-// A few tokens: their routing and the whole sort in one block.
-constexpr int kFusedTokens = 32;
+// A few tokens: their routing and the whole sort in one block, as moe_scatter sorts: experts counted, the counts summed up, and
+// each pair placed behind those of its expert in earlier warps (whose leading lanes note their counts, a row a warp) and lanes.
+constexpr int kFusedTokens = 32, kFusedThreads = 512;
+__device__ __forceinline__ int32_t* fused_counts(int* sm, const Exl3bRouteOp& p) { return sm + ((int)p.n_tok * p.top_k + 3) / 4 * 4; }
 template <int RPL, int DT, bool WIDE>
-__global__ void __launch_bounds__(512) k_route_sort(const Exl3bRouteOp p) {
+__global__ void __launch_bounds__(kFusedThreads) k_route_sort(const __grid_constant__ Exl3bRouteOp p) {
     extern __shared__ int sm[];
+    __shared__ int wtot[32];
+    int* const ids = sm;                                       // [n_tok * top_k]
+    int* const cnt = fused_counts(sm, p);                      // [n_local + 1], then [warps of pairs][n_local]
+    const int tid = threadIdx.x, lane = tid & 31, E = p.n_local, P = (int)p.n_tok * p.top_k;
+    int* const wcnt = cnt + E + 1;
+    for (int x = tid; x < E + 1 + (P + 31) / 32 * E; x += kFusedThreads) cnt[x] = 0;
     chain_wait();
     chain_next();
-    for (int64_t t = threadIdx.x >> 5; t < p.n_tok; t += 16) route<RPL, DT, WIDE>(p, t, threadIdx.x & 31);
+    for (int64_t t = tid >> 5; t < p.n_tok; t += kFusedThreads / 32) route<RPL, DT, WIDE>(p, t, lane, ids);
     __syncthreads();
-    scatter_block(p.ids, p.n_tok * p.top_k, p.n_local, p.expert_base, p.sorted_tok, p.expert_offset, sm);
+    for (int f0 = 0; f0 < P; f0 += kFusedThreads) {
+        const int f = f0 + tid, e = f < P ? local_expert(ids[f], p.expert_base, E) : -1;
+        const unsigned peers = __match_any_sync(kAll, e);
+        if (e >= 0 && lane == __ffs(peers) - 1) {
+            wcnt[(f >> 5) * E + e] = __popc(peers);
+            atomicAdd(&cnt[e], __popc(peers));
+        }
+    }
+    __syncthreads();
+    const int live = block_scan_excl(cnt, E, wtot);
+    for (int e = tid; e < E; e += kFusedThreads) {
+        int at = cnt[e];
+        p.expert_offset[e] = at;
+        for (int w = 0; w < (P + 31) / 32; ++w) {
+            const int c = wcnt[w * E + e];
+            if (c) {
+                wcnt[w * E + e] = at;
+                at += c;
+            }
+        }
+    }
+    if (tid == 0) p.expert_offset[E] = live;
+    for (int f = live + tid; f < P; f += kFusedThreads) p.sorted_tok[f] = -1;
+    __syncthreads();
+    for (int f0 = 0; f0 < P; f0 += kFusedThreads) {
+        const int f = f0 + tid, e = f < P ? local_expert(ids[f], p.expert_base, E) : -1;
+        const unsigned peers = __match_any_sync(kAll, e);
+        if (e >= 0) p.sorted_tok[wcnt[(f >> 5) * E + e] + __popc(peers & ((1u << lane) - 1u))] = f;
+    }
 }
 
 template <int RPL, int DT, bool WIDE>
 int launch(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
     if (!fused) return chain_launch(k_route<RPL, DT, WIDE>, dim3((unsigned)((p->n_tok + 3) / 4)), dim3(128), 0, 1, st, *p);
     auto kern = k_route_sort<RPL, DT, WIDE>;
-    const size_t smem = (size_t)(p->n_local + 1) * 4 + (size_t)32 * p->n_local * 4;
+    const int64_t pairs = p->n_tok * p->top_k;
+    const size_t smem = (size_t)((pairs + 3) / 4 * 4 + p->n_local + 1 + (pairs + 31) / 32 * p->n_local) * 4;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return -6;
-    return chain_launch(kern, dim3(1), dim3(512), smem, 1, st, *p);
+    return chain_launch(kern, dim3(1), dim3(kFusedThreads), smem, 1, st, *p);
 }
 template <int RPL, int DT>
 int launch_wide(const Exl3bRouteOp* p, int fused, cudaStream_t st) {

@@ -177,6 +177,31 @@ def test_scores_that_differ_by_less_than_their_rounding():
     check(l, 8, score="sigmoid", bias=b)
 
 
+@pytest.mark.parametrize("E,k,groups,keep", [(40, 5, 1, 1), (256, 8, 8, 4), (512, 10, 16, 5), (1024, 10, 4, 2), (2048, 16, 32, 9)])
+@pytest.mark.parametrize("gap", [0.0, 2.0 ** -24, 2.0 ** -20, 2.0 ** -16])
+def test_neighbours_among_the_chosen(E, k, groups, keep, gap):
+    """Scores in pairs that are equal or next to equal, at every place of a lane and across lanes and groups."""
+    g = torch.Generator(device="cuda").manual_seed(E + groups)
+    half = torch.randn((60, E // 2), generator=g, device="cuda")
+    l = torch.cat((half, half * (1 + gap)), 1)[:, torch.randperm(E, generator=g, device="cuda")].contiguous()
+    b = torch.zeros(E, device="cuda")
+    for kw in (dict(), dict(score="sigmoid", bias=b), dict(score="softmax", bias=b + 0.25),
+               dict(score="sigmoid", groups=groups, keep_groups=keep, group_top=2), dict(groups=groups, keep_groups=keep)):
+        check(l, k, renorm=True, **kw)
+        check(l.to(BF16), k, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_infinity_is_above_the_largest_number(dtype):
+    l = logits_of(8, 3, 64, dtype)
+    l[0, 9], l[0, 40] = torch.finfo(dtype).max, torch.inf
+    l[1, 40], l[1, 9] = torch.finfo(dtype).max, torch.inf
+    l[2, 5], l[2, 6], l[2, 7] = torch.finfo(dtype).min, 0.0, -0.0
+    if dtype != F32:                    # in f32 it is the largest number
+        check(l, 8)
+    check(l, 32, score="sigmoid", bias=torch.zeros(64, device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strided_logits_and_neighbours_left_alone(dtype):
     big = torch.full((21, 700), 9.0, dtype=dtype, device="cuda")
