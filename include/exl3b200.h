@@ -559,8 +559,11 @@ int     exl3b200_block_norm(const Exl3bBlockNorm* norm, void* stream);
  * over block_norm, grouped_mm and the routing entries above. x, out and next are [T][hidden] of `dtype` (RAD_F16 or
  * RAD_BF16), as are router_w [n_expert][hidden] and the norms' and the gate's [hidden] (post_w, gate, next_w may be NULL).
  * weights: `dtype`, or EXL3B_MX4 (gu_w [n_expert][2 width][hidden] and dn_w [n_expert][hidden][width] as codes, the
- * scales tiled: gu_scales for SILU_MUL; xn is then also quantised for them, and h is MXFP4). `out` may be x; `next` is
- * optional. n_expert a multiple of 8, at most 2048; hidden and width multiples of 8 (MXFP4: 32).
+ * scales tiled: gu_scales for SILU_MUL; xn is then also quantised for them, and h is MXFP4), or EXL3B_F8 (codes, the scales
+ * f32 as grouped_mm takes them; xn, and h, which is of `dtype`, go through f8_quantize). `out` may be x; `next` is
+ * optional. n_expert a multiple of 8, at most 2048; hidden and width multiples of 8 (MXFP4: 32, FP8: 16).
+ * exl3b200_expert_block_forward_routed takes another router: its score, groups, renorm, scale and bias are `router`'s (the rest
+ * of *router is the block's own and not read); NULL: router_scatter.
  * exl3b200_expert_block_work_bytes sizes one device block for up to max_tokens tokens a pass (-1: refused),
  * exl3b200_expert_block_carve cuts it, and a forward only enqueues (it can be captured in a CUDA graph). */
 typedef struct Exl3bExpertBlockDesc {
@@ -588,7 +591,7 @@ typedef struct Exl3bExpertBlockBufs {
     int32_t*  sorted_tok;     /* [max_tokens * top_k] */
     int32_t*  expert_offset;  /* [n_expert + 1] */
     void*     scatter_work;
-    void*     h;              /* [max_tokens * top_k][width], elements or codes */
+    void*     h;              /* [max_tokens * top_k][width], elements or codes; FP8: elements, codes 256-byte aligned behind */
     uint8_t*  h_scales;
     uint16_t* y_rows;         /* bf16 [max_tokens * top_k][hidden] */
     float*    branch;         /* [max_tokens][hidden] */
@@ -599,6 +602,9 @@ int     exl3b200_expert_block_carve(const Exl3bExpertBlockDesc* desc, int64_t ma
                                     Exl3bExpertBlockBufs* bufs);
 int     exl3b200_expert_block_forward(const Exl3bExpertBlockDesc* desc, const Exl3bExpertBlockBufs* bufs, const void* x,
                                       int64_t n_tok, void* out, void* next, void* stream);
+int     exl3b200_expert_block_forward_routed(const Exl3bExpertBlockDesc* desc, const Exl3bRouter* router,
+                                             const Exl3bExpertBlockBufs* bufs, const void* x, int64_t n_tok, void* out,
+                                             void* next, void* stream);
 
 /* How long a kernel that waits on another rank's flag (p2p_wait_dispatch, p2p_wait_combine, tp_reduce, tp_pull)
  * waits before it gives up, sets its status and the error word, and returns: `ns` nanoseconds, or the default 5 s

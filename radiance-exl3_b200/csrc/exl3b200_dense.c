@@ -165,7 +165,17 @@ int exl3b200_f8_dequantize(const uint8_t* codes, int64_t codes_pitch, const floa
     return rc_of(exl3b_cuda_f8_dequantize(codes, codes_pitch, scales, scales_pitch, rows, cols, y, y_dtype, y_pitch, stream));
 }
 
-int exl3b200_router(const Exl3bRouter* d, void* stream) {
+/* How many neighbouring experts a lane holds; 2^*shift lanes a group: as many as a power of two of groups leaves each. */
+static int64_t lane_experts(const Exl3bRouter* d, int* shift) {
+    int s = 5;
+    while ((int64_t)d->n_group << s > 32) --s;
+    if (shift) *shift = s;
+    return (d->n_expert / d->n_group + (1 << s) - 1) >> s;
+}
+
+/* Also exl3b200_expert_block.c's, before its first step. */
+int exl3b_router_check(const Exl3bRouter* d);
+int exl3b_router_check(const Exl3bRouter* d) {
     if (!d) return RAD_E_INVAL;
     if (!is_float(d->dtype)) return RAD_E_DTYPE;
     if ((d->score != EXL3B_SCORE_SOFTMAX && d->score != EXL3B_SCORE_SIGMOID) || !(d->scale - d->scale == 0.f)) return RAD_E_INVAL;
@@ -174,10 +184,7 @@ int exl3b200_router(const Exl3bRouter* d, void* stream) {
         G > 32 || E % G || d->group_keep < 1 || d->group_keep > G || d->group_top < 1 || d->group_top > 2 ||
         d->top_k > E / G * d->group_keep)
         return RAD_E_SHAPE;
-    int shift = 5;                       /* lanes of a group */
-    while (G << shift > 32) --shift;
-    const int64_t per = (E / G + (1 << shift) - 1) >> shift;
-    if (per > 64) return RAD_E_SHAPE;
+    if (lane_experts(d, 0) > 64) return RAD_E_SHAPE;
     const int sort = d->expert_offset != 0;
     if (d->n_tok > 0 && sort != (d->sorted_tok != 0)) return RAD_E_INVAL;
     if (sort && (d->n_local < 1 || d->n_local > 16384)) return RAD_E_SHAPE;
@@ -187,8 +194,18 @@ int exl3b200_router(const Exl3bRouter* d, void* stream) {
     if (mis(d->logits, size_of(d->dtype)) || mis(d->bias, 4) || mis(d->ids, 4) || mis(d->w, 4) || mis(d->sorted_tok, 4) ||
         mis(d->expert_offset, 4) || (sort && mis(d->work, 4)))
         return RAD_E_ALIGN;
+    return RAD_OK;
+}
+
+int exl3b200_router(const Exl3bRouter* d, void* stream) {
+    const int bad = exl3b_router_check(d);
+    if (bad) return bad;
+    const int64_t E = d->n_expert, G = d->n_group;
+    const int sort = d->expert_offset != 0;
     if (d->n_tok > 0) {
         const int fused = sort && exl3b_route_fuses(d->n_tok, d->n_local);
+        int shift = 0;
+        const int64_t per = lane_experts(d, &shift);
         Exl3bRouteOp p;
         memset(&p, 0, sizeof p);
         p.n_tok = d->n_tok;

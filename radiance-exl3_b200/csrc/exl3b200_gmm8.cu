@@ -484,11 +484,24 @@ int launch(const Exl3bGmmOp* p, int sm_count, int split, cudaStream_t st) {
                         map, *p, sh);
 }
 
+// About how many units there will be: groups of nt rows, half a one more an expert for its remainder, one an expert at least.
+int64_t likely_units(const Exl3bGmmOp* p, int nt, int64_t blk) {
+    const int64_t live = p->n_expert < p->n_rows ? p->n_expert : p->n_rows, some = p->n_rows / nt + live / 2;
+    return (some > live ? some : live) * ((p->n_out + blk - 1) / blk);
+}
+
 template <bool ACT>
 int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
-    const int64_t few = p->w_rows < 512 ? 96 : 16;
-    if (p->n_rows > few * (int64_t)p->n_expert && most_units(p, 96, 2) >= sm_count / 4) return wide::launch<ACT>(p, sm_count, st);
-    const int64_t most = most_units(p, 32, 1), nck = (p->n_in + 127) / 128;
+    // The wide form where its units cost less: a unit's stage there takes 3.1 times as long as a narrow one's (2 times where the
+    // SMs have a unit each at most), and its start and end as long as five of those; narrow units run two an SM. Narrow and wide,
+    // us: 64 experts, 2048 -> 512 silu_mul, 28 rows each 28.2 and 29.8, 40 rows 33.0 and 30.4, 130 rows 62.7 and 41.5; 640 ->
+    // 2560, 40 rows 27.4 and 30.8, 96 rows 47.6 and 41.5; 300 experts of 96 rows, 448 -> 160 silu_mul 30.9 and 33.4; one expert,
+    // 4096 -> 1536, 512 rows 17.7 and 25.0, 1024 rows 30.1 and 25.2.
+    const int64_t nck = (p->n_in + 127) / 128, sm = sm_count;
+    const int64_t wide_units = likely_units(p, 128, ACT ? 128 : 256), narrow_units = likely_units(p, 32, ACT ? 64 : 128);
+    const int64_t wide_cost = wide_units > sm ? wide_units * (31 * nck + 50) : sm * (20 * nck + 50);
+    if (wide_cost < 10 * nck * (narrow_units > 2 * sm ? narrow_units : 2 * sm)) return wide::launch<ACT>(p, sm_count, st);
+    const int64_t most = most_units(p, 32, 1);
     int64_t split = sm_count / most;                          // so the grid has room for a cluster a unit: the kernel counts on it
     if (split > nck / 4) split = nck / 4;
     if (split > kMaxSplit) split = kMaxSplit;

@@ -324,22 +324,26 @@ class ExpertBlock:
 
     router_w [experts, hidden] in f16 or bf16 sets the stream's type, which pre_w, post_w, gate (a scale a channel) and
     next_w [hidden] share. gu_w [experts, 2 width, hidden] and dn_w [experts, hidden, width] are of that type, or uint8
-    MXFP4 codes with gu_scales and dn_scales [experts, rows, cols / 32] (tiled here, once).
+    MXFP4 codes with gu_scales and dn_scales [experts, rows, cols / 32] (tiled here, once), or float8_e4m3fn with f32 gu_scales
+    [experts, 2 ceil(width / 128), ceil(hidden / 128)] and dn_scales [experts, ceil(hidden / 128), ceil(width / 128)].
+
+    router: None (softmax over all experts, the top_k), or a dict of Router's score, bias, groups, keep_groups, group_top,
+    renorm and scale.
 
     A block has one work buffer: its forwards run one after another, on one stream or on streams that wait for each other,
     and it is kept until they are done."""
 
     def __init__(self, *, router_w, gu_w, dn_w, pre_w, post_w=None, gate=None, next_w=None, gu_scales=None, dn_scales=None,
-                 top_k, eps=1e-6, res_scale=1.0, max_tokens=2048):
+                 top_k, eps=1e-6, res_scale=1.0, max_tokens=2048, router=None):
         E, H = router_w.shape
         dev = self._dev = router_w.get_device()
-        mx = gu_w.dtype == torch.uint8
+        mx, f8 = gu_w.dtype == torch.uint8, gu_w.dtype == torch.float8_e4m3fn
         per, dt = 2 if mx else 1, router_w.dtype
         W = dn_w.shape[2] * per
         d = self.desc = ExpertBlockDesc()
         d.n_expert, d.hidden, d.width, d.top_k, d.eps, d.res_scale = E, H, W, top_k, eps, res_scale
-        d.dtype, d.weights = _dtype(router_w), MX4 if mx else _dtype(gu_w)
-        want = torch.uint8 if mx else dt
+        d.dtype, d.weights = _dtype(router_w), MX4 if mx else F8 if f8 else _dtype(gu_w)
+        want = torch.uint8 if mx else torch.float8_e4m3fn if f8 else dt
         keep = [router_w, gu_w, dn_w, pre_w, post_w, gate, next_w]
         for name, t, shape, kind in (("router_w", router_w, (E, H), dt), ("gu_w", gu_w, (E, 2 * W, H // per), want),
                                      ("dn_w", dn_w, (E, H, W // per), want), ("pre_w", pre_w, (H,), dt),
@@ -353,6 +357,23 @@ class ExpertBlock:
             _rows(dn_scales, "dn_scales", dev, (E, H, W // 32), torch.uint8)
             keep += [mx4_tile_scales(gu_scales, "silu_mul"), mx4_tile_scales(dn_scales)]
             d.gu_scales, d.dn_scales = keep[-2].data_ptr(), keep[-1].data_ptr()
+        if f8:
+            h, w = (H + 127) // 128, (W + 127) // 128
+            for name, t, shape in (("gu_scales", gu_scales, (E, 2 * w, h)), ("dn_scales", dn_scales, (E, h, w))):
+                setattr(d, name, _rows(t, name, dev, shape, torch.float32)[0])
+                if not t.is_contiguous():
+                    raise ValueError(f"{name} is strided")
+            keep += [gu_scales, dn_scales]
+        self.router = None
+        if router is not None:
+            o = {**dict(score="softmax", bias=None, groups=1, keep_groups=1, group_top=1, renorm=False, scale=1.0), **router}
+            if len(o) != 7:
+                raise ValueError(f"router has {sorted(set(o))}")
+            r = self.router = RouterDesc(score=SCORES[o["score"]], n_group=o["groups"], group_keep=o["keep_groups"],
+                                         group_top=o["group_top"], renorm=o["renorm"], scale=o["scale"])
+            if o["bias"] is not None:
+                r.bias, _ = _rows(o["bias"], "bias", dev, (E,), torch.float32)
+            keep.append(o["bias"])
         self._keep, self.dtype, self.hidden, self.max_tokens = keep, dt, H, max_tokens
         n = native().expert_block_work_bytes(d, max_tokens)
         self.work = torch.empty(n, dtype=torch.uint8, device=router_w.device)
@@ -372,5 +393,5 @@ class ExpertBlock:
             _check_current(self._dev)
         native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
                                       next_out.data_ptr() if next_out is not None else None,
-                                      _current_stream(self._dev) if stream is None else stream)
+                                      _current_stream(self._dev) if stream is None else stream, self.router)
         return out

@@ -193,6 +193,8 @@ class Native:
         L.exl3b200_expert_block_carve.argtypes = [C.POINTER(ExpertBlockDesc), _I64, _VP, _I64, C.POINTER(ExpertBlockBufs)]
         L.exl3b200_expert_block_forward.argtypes = [C.POINTER(ExpertBlockDesc), C.POINTER(ExpertBlockBufs), _VP, _I64, _VP,
                                                     _VP, _VP]
+        L.exl3b200_expert_block_forward_routed.argtypes = [C.POINTER(ExpertBlockDesc), C.POINTER(RouterDesc),
+                                                           C.POINTER(ExpertBlockBufs), _VP, _I64, _VP, _VP, _VP]
         L.exl3b200_f8_quantize.argtypes = [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _I, _VP]
         L.exl3b200_f8_dequantize.argtypes = [_VP, _I64, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP]
         # descriptors by address: a plan takes its own once (ctypes.addressof), not a byref a call
@@ -468,6 +470,7 @@ class Native:
                     "exl3b200_expert_block_carve")
         return b
 
-    def expert_block_forward(self, desc, bufs, x, n_tok, out, next_, stream=0):
-        self._check(self.lib.exl3b200_expert_block_forward(C.byref(desc), C.byref(bufs), x, n_tok, out, next_, stream),
-                    "exl3b200_expert_block_forward")
+    def expert_block_forward(self, desc, bufs, x, n_tok, out, next_, stream=0, router=None):
+        self._check(self.lib.exl3b200_expert_block_forward_routed(C.byref(desc), None if router is None else C.byref(router),
+                                                                  C.byref(bufs), x, n_tok, out, next_, stream),
+                    "exl3b200_expert_block_forward_routed")

@@ -104,7 +104,8 @@ def test_grouped_mm_f8(kind, K, N, act):
         close(y, want, tol, out)
 
 
-FORMS = {"split": ([1, 3], 1024, 128), "narrow": ([5] * 40, 512, 512), "pair": ([300, 0, 41, 700], 512, 640)}
+FORMS = {"split": ([1, 3], 1024, 128), "narrow": ([5] * 40, 512, 512),
+         "wide": ([300, 0, 41, 700, 128, 257, 90, 500], 1024, 1280)}
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -121,7 +122,7 @@ def test_every_form_with_dropped_slots_and_rows_outside(form, act, out):
     close(y[~dead], want[~dead], tol[~dead], out)
 
 
-@pytest.mark.parametrize("rows", [1, 31, 33, 97, 255, 257, 1024, 2869, 4100])
+@pytest.mark.parametrize("rows", [1, 31, 33, 97, 255, 257, 1024, 2869, 4100, 9001])
 @pytest.mark.parametrize("N,act", [(248, "silu_mul"), (512, "none"), (1064, "none"), (192, "silu_mul")])
 def test_one_expert_of_many_rows(rows, N, act):
     y, _, (want, tol), _ = case(rows, [rows], 272, N, act)
@@ -129,11 +130,11 @@ def test_one_expert_of_many_rows(rows, N, act):
 
 
 @pytest.mark.parametrize("K", [16, 272, 640, 3824])
-@pytest.mark.parametrize("form", ["narrow", "pair", "split"])
+@pytest.mark.parametrize("form", ["narrow", "wide", "split"])
 @pytest.mark.parametrize("shift,extra", [(0, 0), (1, 0), (3, 2), (4, 4), (2, 5)])
 def test_scales_at_any_alignment(K, form, shift, extra):
     """x's scales any number of floats into their memory and any pitch apart, poison between them."""
-    rows, N, E = {"narrow": (50, 1048, 20), "pair": (700, 640, 2), "split": (9, 128, 2)}[form]
+    rows, N, E = {"narrow": (50, 1048, 20), "wide": (2100, 2048, 2), "split": (9, 128, 2)}[form]
     xq, xs, w, ws, xv = operands(K + shift, E, rows, K, N, "none")
     kb = -(-K // 128)
     mem = torch.full((shift + rows * (kb + extra),), float("nan"), device="cuda")
@@ -146,11 +147,12 @@ def test_scales_at_any_alignment(K, form, shift, extra):
     close(y, *plain(xv, wv, tok, off, 0, "none", N), F32)
 
 
-def test_strided_operands_and_neighbours_left_alone():
-    K, N, counts = 272, 136, [40, 7, 90]
+@pytest.mark.parametrize("N,counts", [(136, [40, 7, 90]), (1096, [40, 3000, 7, 900])])
+def test_strided_operands_and_neighbours_left_alone(N, counts):
+    K = 272
     y, _, (want, tol), (xq, xs, w, ws, tok, off) = case(5, counts, K, N, "none")
     bx = torch.full((xq.shape[0], K + 48), 0x7F, dtype=torch.uint8, device="cuda")
-    bw = torch.full((3, N + 5, K + 16), 0x7F, dtype=torch.uint8, device="cuda")
+    bw = torch.full((len(counts), N + 5, K + 16), 0x7F, dtype=torch.uint8, device="cuda")
     bx[:, 16:16 + K] = xq.view(torch.uint8)
     bw[:, :N, :K] = w.view(torch.uint8)
     by = torch.full((len(tok) + 2, N + 8), 7.0, device="cuda")
@@ -160,9 +162,10 @@ def test_strided_operands_and_neighbours_left_alone():
     assert (by[[0, -1]] == 7).all() and (by[:, N:] == 7).all()
 
 
-def test_values_that_are_no_numbers_stay_in_their_rows():
-    """A row whose scale is NaN, an expert with a NaN code in one weight row; zero scales."""
-    counts, K, N = [30, 50, 20], 384, 264
+@pytest.mark.parametrize("many,N", [(0, 264), (3000, 1032)])
+def test_values_that_are_no_numbers_stay_in_their_rows(many, N):
+    """A row whose scale is NaN, an expert with a NaN code in one weight row; zero scales; an expert of many rows besides."""
+    counts, K = [30, 50, 20] + [many] * (many > 0), 384
     y, _, (want, tol), (xq, xs, w, ws, tok, off) = case(9, counts, K, N, "none")
     xs[tok[10].item()] = float("nan")
     xs[tok[12].item(), 1] = 0
@@ -170,14 +173,14 @@ def test_values_that_are_no_numbers_stay_in_their_rows():
     ws[2] = 0
     got = torch.empty_like(y)
     dense.GroupedMm(x=xq, x_scales=xs, w=w, w_scales=ws, expert_offset=off, sorted_tok=tok, top_k=1, y=got).run(stream())
-    assert got[10].isnan().all() and got[30:80, 100].isnan().all() and not got[80:].any()
+    assert got[10].isnan().all() and got[30:80, 100].isnan().all() and not got[80:100].any()
     keep = torch.ones_like(got, dtype=torch.bool)
-    keep[[10, 12]] = keep[30:80, 100] = keep[80:] = False
+    keep[[10, 12]] = keep[80:100] = False
     keep[30:80, 100] = False
     assert torch.equal(got[keep], y[keep])
 
 
-@pytest.mark.parametrize("E,n,N", [(5, 1, 264), (5, 40, 264), (3, 900, 1056)])
+@pytest.mark.parametrize("E,n,N", [(5, 1, 264), (5, 40, 264), (3, 900, 1056), (3, 5000, 1056)])
 @pytest.mark.parametrize("start", [0, 1])
 def test_no_expert_has_a_row(E, n, N, start):
     xq, xs, w, ws, _ = operands(E + n, E, n, 512, N, "none")
@@ -196,39 +199,43 @@ def test_one_group_without_routing():
     close(y, *plain(xv, values_of(w, ws, 104), tok, off, 0, "none", 104), F32)
 
 
-def test_all_units_past_the_table():
-    """More units a CTA than its table holds: 40,000 rows of one expert over a wide output; rows repeat, so do results."""
-    n, K, N = 40000, 64, 16384
+@pytest.mark.parametrize("K", [64, 256])
+def test_all_units_past_the_table(K):
+    """More units a CTA than its table holds, in the narrow form (K 64) and the wide one: 40,000 rows of one expert over a wide
+    output; rows repeat, and so do results."""
+    n, N = 40000, 16384
     g = gen(4)
-    few = operands(4, 1, 16, K, N, "none")
+    xq16, xs16, w, ws, xv = operands(4, 1, 16, K, N, "none")
     pick = torch.randint(0, 16, (n,), generator=g, device="cuda")
     xq, xs = dense.f8_empty(n, K)
-    xq.view(torch.uint8).copy_(few[0].view(torch.uint8)[pick])
-    xs.copy_(few[1][pick])
+    xq.view(torch.uint8).copy_(xq16.view(torch.uint8)[pick])
+    xs.copy_(xs16[pick])
     y = torch.empty((n, N), dtype=F16, device="cuda")
-    dense.GroupedMm(x=xq, x_scales=xs, w=few[2], w_scales=few[3], y=y).run(stream())
-    small = torch.empty((16, N), dtype=F16, device="cuda")
-    dense.GroupedMm(x=few[0], x_scales=few[1], w=few[2], w_scales=few[3], y=small).run(stream())
+    dense.GroupedMm(x=xq, x_scales=xs, w=w, w_scales=ws, y=y).run(stream())
     tok, off = torch.arange(16, dtype=torch.int32, device="cuda"), torch.tensor([0, 16], dtype=torch.int32, device="cuda")
-    close(small, *plain(few[4], values_of(few[2], few[3], N), tok, off, 0, "none", N), F16)
-    assert torch.equal(y, small[pick])                         # one block of k: no order of additions to differ in
+    want, tol = plain(xv, values_of(w, ws, N), tok, off, 0, "none", N)
+    first = torch.stack([y[(pick == i).nonzero()[0, 0]] for i in range(16)])
+    close(first, want, tol, F16)
+    for r in range(0, n, 5000):
+        assert torch.equal(y[r:r + 5000], first[pick[r:r + 5000]])
 
 
-def test_offsets_past_32_bits():
-    """Experts, input rows and output rows that lie over 4 GiB into their tensors."""
-    K, N, far = 128, 32, 4_600_000_000
-    xq, xs, w, ws, xv = operands(6, 2, 3, K, N, "none")
+@pytest.mark.parametrize("rows,N", [(3, 32), (2100, 2048)])
+def test_offsets_past_32_bits(rows, N):
+    """Experts, input rows and output rows that lie over 4 GiB into their tensors, in the split and the wide form."""
+    K, far = 128, 4_600_000_000
+    xq, xs, w, ws, xv = operands(6, 2, rows, K, N, "none")
     wbuf = torch.empty(far + N * K, dtype=torch.uint8, device="cuda")
     wf = torch.as_strided(wbuf, (2, N, K), (far, K, 1))
     wf.copy_(w.view(torch.uint8))
-    pitch = 2_400_000_000
-    xbuf = torch.empty(2 * pitch + K, dtype=torch.uint8, device="cuda")
-    x = torch.as_strided(xbuf, (3, K), (pitch, 1))
+    pitch = 4_800_000_000 // rows // 16 * 16
+    xbuf = torch.empty((rows - 1) * pitch + K, dtype=torch.uint8, device="cuda")
+    x = torch.as_strided(xbuf, (rows, K), (pitch, 1))
     x.copy_(xq.view(torch.uint8))
-    ybuf = torch.empty(pitch + N, dtype=F16, device="cuda")
-    y = torch.as_strided(ybuf, (3, N), (pitch // 2, 1))
-    tok = torch.tensor([0, 2, 1], dtype=torch.int32, device="cuda")
-    off = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    ybuf = torch.empty((rows - 1) * (pitch // 2) + N, dtype=F16, device="cuda")
+    y = torch.as_strided(ybuf, (rows, N), (pitch // 2, 1))
+    tok = torch.randperm(rows, generator=gen(2), device="cuda").to(torch.int32)
+    off = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device="cuda")
     dense.GroupedMm(x=x.view(F8), x_scales=xs, w=wf.view(F8), w_scales=ws, y=y, expert_offset=off, sorted_tok=tok,
                     top_k=1).run(stream())
     close(y, *plain(xv, values_of(w, ws, N), tok, off, 1, "none", N), F16)
@@ -335,3 +342,70 @@ def test_f8_products_refuse():
         dense.GroupedMm(**{**kw, "y": torch.empty((4, 16), dtype=torch.uint8, device="cuda"),
                            "y_scales": torch.empty((4, 1), dtype=torch.uint8, device="cuda")}).run()
     assert (y == 5).all()
+
+
+@pytest.mark.parametrize("routed", [False, True])
+@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_an_fp8_block_is_its_entries(T, dtype, routed):
+    """The residual block over FP8 experts, with its own router and with grouped routing, against the entries it is made of, to
+    the bit; and in a graph."""
+    E, H, W, k = 32, 528, 272, 4
+    g = gen(T)
+    t = {"router_w": randn(g, E, H, dtype=dtype) * H ** -0.5, "pre_w": randn(g, H, dtype=dtype), "post_w": randn(g, H, dtype=dtype),
+         "gate": randn(g, H, dtype=dtype), "next_w": randn(g, H, dtype=dtype)}
+    _, _, t["gu_w"], t["gu_scales"], _ = operands(1, E, 1, H, W, "silu_mul")
+    _, _, t["dn_w"], t["dn_scales"], _ = operands(2, E, 1, W, H, "none")
+    routing = dict(score="sigmoid", bias=0.1 * randn(g, E), groups=8, keep_groups=3, group_top=2, renorm=True, scale=2.5)
+    block = dense.ExpertBlock(top_k=k, res_scale=0.5, max_tokens=300, router=routing if routed else None, **t)
+    x = randn(g, T, H, dtype=dtype)
+    out, nxt = torch.empty_like(x), torch.empty_like(x)
+    block.forward(x, out, nxt)
+    new = lambda *s, dt=dtype: torch.empty(s, dtype=dt, device="cuda")  # noqa: E731
+    P, nat = T * k, dense.native()
+    xn, logits, h, rows = new(T, H), new(T, E, dt=F32), new(P, W), new(P, H, dt=BF16)
+    ids, w, tok, off = new(T, k, dt=torch.int32), new(T, k, dt=F32), new(P, dt=torch.int32), new(E + 1, dt=torch.int32)
+    dense.BlockNorm(res=x, pre_w=t["pre_w"], y=xn).run()
+    dense.GroupedMm(x=xn, w=t["router_w"][None], y=logits).run()
+    if routed:
+        dense.Router(logits=logits, top_k=k, ids=ids, w=w, sorted_tok=tok, expert_offset=off, **routing).run()
+    else:
+        work = new(nat.scatter_work_bytes(P, E), dt=torch.uint8)
+        nat.router_scatter(logits.data_ptr(), T, E, k, ids.data_ptr(), w.data_ptr(), E, 0, tok.data_ptr(), off.data_ptr(),
+                           work.data_ptr(), stream())
+    (xq, xs), (hq, hs) = dense.f8_empty(T, H), dense.f8_empty(P, W)
+    dense.f8_quantize(xn, xq, xs)
+    dense.GroupedMm(x=xq, x_scales=xs, w=t["gu_w"], w_scales=t["gu_scales"], expert_offset=off, sorted_tok=tok, top_k=k,
+                    act="silu_mul", y=h).run()
+    dense.f8_quantize(h, hq, hs)
+    dense.GroupedMm(x=hq, x_scales=hs, w=t["dn_w"], w_scales=t["dn_scales"], expert_offset=off, sorted_tok=tok, y=rows).run()
+    branch, gw = new(T, H, dt=F32), new(nat.gather_work_bytes(T, k), dt=torch.uint8)
+    nat.moe_gather(rows.data_ptr(), H, tok.data_ptr(), P, w.data_ptr(), T, k, H, branch.data_ptr(), gw.data_ptr(), stream())
+    want, want_next = torch.empty_like(x), torch.empty_like(x)
+    dense.BlockNorm(branch=branch, post_w=t["post_w"], gate=t["gate"], gate_kind="channel", res=x, res_scale=0.5, out=want,
+                    pre_w=t["next_w"], y=want_next).run()
+    assert torch.equal(out, want) and torch.equal(nxt, want_next)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block.forward(x, out, nxt)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+
+
+def test_a_block_refuses_a_router_that_does_not_fit():
+    _, _, gu, gus, _ = operands(1, 16, 1, 64, 32, "silu_mul")
+    _, _, dn, dns, _ = operands(2, 16, 1, 32, 64, "none")
+    one = torch.ones(64, dtype=BF16, device="cuda")
+    t = dict(router_w=torch.zeros((16, 64), dtype=BF16, device="cuda"), gu_w=gu, gu_scales=gus, dn_w=dn, dn_scales=dns, pre_w=one,
+             top_k=4, max_tokens=8)
+    x = torch.zeros((8, 64), dtype=BF16, device="cuda")
+    out = torch.full_like(x, 5)
+    for bad in (dict(groups=3), dict(groups=8, keep_groups=1), dict(scale=float("inf"))):
+        with pytest.raises(RuntimeError):
+            dense.ExpertBlock(**t, router=bad).forward(x, out)
+    assert (out == 5).all()
+    for bad in (dict(router=dict(top=1)), dict(router=dict(bias=one)), dict(gu_scales=gus[:, :1]), dict(dn_scales=dns.double()),
+                dict(dn_w=dn.view(torch.uint8))):
+        with pytest.raises(ValueError):
+            dense.ExpertBlock(**{**t, **bad})

@@ -61,3 +61,31 @@ def test_f8_rows_refuse(want, kw):
                                     a["scales"], a["scales_pitch"], 0, None) == want
     assert lib.exl3b200_f8_dequantize(a["codes"], a["codes_pitch"], a["scales"], a["scales_pitch"], a["rows"], a["cols"],
                                       a["x"], a["dtype"], a["x_pitch"], None) == want
+
+
+def test_an_fp8_block_carves_disjoint_buffers_and_refuses_before_its_first_step():
+    from exl3b200.native import ExpertBlockDesc
+    nat = Native()
+    at = {n: 4096 for n in ("router_w", "gu_w", "dn_w", "gu_scales", "dn_scales", "pre_w")}
+    d = ExpertBlockDesc(n_expert=64, hidden=2064, width=528, top_k=10, dtype=3, weights=1024 + 0x3B8, eps=1e-6, res_scale=1.0, **at)
+    for T in (1, 33, 2048):
+        P, base, n = T * 10, 0x7F0000000010, nat.expert_block_work_bytes(d, T)
+        b = nat.expert_block_carve(d, T, base, n)
+        codes = b.h + (P * 528 * 2 + 255) // 256 * 256
+        spans = sorted((a, a + size) for a, size in (
+            (b.xn, T * 2064 * 2), (b.x_codes, T * 2064), (b.x_scales, T * 20 * 4), (b.logits, T * 64 * 4), (b.ids, P * 4), (b.w, P * 4),
+            (b.sorted_tok, P * 4), (b.expert_offset, 65 * 4), (b.h, P * 528 * 2), (codes, P * 528), (b.h_scales, P * 8 * 4),
+            (b.y_rows, P * 2064 * 2), (b.branch, T * 2064 * 4), (b.scatter_work, nat.scatter_work_bytes(P, 64)),
+            (b.gather_work, nat.gather_work_bytes(T, 10))))
+        assert spans[0][0] >= base and spans[-1][1] <= base + n and all(a % 256 == 0 for a, _ in spans)
+        assert all(e <= s for (_, e), (s, _) in zip(spans, spans[1:]))
+    f = nat.lib.exl3b200_expert_block_forward_routed
+    r = dict(score=1, n_group=8, group_keep=4, group_top=2, renorm=1, scale=2.5)
+    for want, k in ((E_DEVICE, {}), (E_SHAPE, dict(n_group=7)), (E_SHAPE, dict(group_keep=1)), (E_INVAL, dict(score=3)),
+                    (E_ALIGN, dict(bias=4097))):
+        assert f(d, RouterDesc(**{**r, **k}), b, 4096, 4, 4096, None, None) == want
+    assert f(d, None, b, 4096, 4, 4096, None, None) == E_DEVICE
+    for name, v, want in (("gu_scales", 4098, E_ALIGN), ("dn_scales", None, E_INVAL), ("gu_w", 4104, E_ALIGN), ("hidden", 2056, E_SHAPE)):
+        bad = ExpertBlockDesc.from_buffer_copy(d)
+        setattr(bad, name, v)
+        assert f(bad, None, b, 4096, 4, 4096, None, None) == want, name
