@@ -135,23 +135,29 @@ def f8_empty(rows, cols, device="cuda"):
 
 
 def _f8_rows(x, codes, scales, name):
-    """Both conversions' checks: (address, type, pitch) of x, (address, pitch) of the codes and of the scales."""
-    if x.dim() != 2:
-        raise ValueError(f"{name} has {x.dim()} dimensions, not 2")
-    rows, cols = x.shape
-    dev = x.get_device()
-    xp, pitch = _rows(x, name, dev)
-    at = _rows(codes, "codes", dev, (rows, cols), torch.float8_e4m3fn)
-    at += _rows(scales, "scales", dev, (rows, (cols + 127) // 128), torch.float32)
+    """Both conversions' checks: x's GPU, type and pitch, (address, pitch) of the codes and of the scales."""
+    dev, shape, xs, cs, ss = x.get_device(), x.shape, x.stride(), codes.stride(), scales.stride()
+    if (dev == codes.get_device() == scales.get_device() >= 0 and len(xs) == 2 and shape[0] > 1 and codes.shape == shape
+            and scales.shape == (shape[0], (shape[1] + 127) // 128) and 1 == xs[1] == cs[1] == ss[1]
+            and codes.dtype is torch.float8_e4m3fn and scales.dtype is torch.float32):
+        at = codes.data_ptr(), cs[0], scales.data_ptr(), ss[0]      # what _rows finds, in one go: a call costs a microsecond less
+        pitch = xs[0]
+    else:
+        if len(shape) != 2:
+            raise ValueError(f"{name} has {len(shape)} dimensions, not 2")
+        _, pitch = _rows(x, name, dev)
+        at = _rows(codes, "codes", dev, (shape[0], shape[1]), torch.float8_e4m3fn)
+        at += _rows(scales, "scales", dev, (shape[0], (shape[1] + 127) // 128), torch.float32)
     if _several:
         _check_current(dev)
-    return dev, (xp, _dtype(x), pitch), at
+    return dev, DTYPES.get(x.dtype) or _dtype(x), pitch, at
 
 
 def f8_quantize(x, codes, scales, pow2=False, stream=None):
     """x [rows, cols] in f32, f16 or bf16 -> its e4m3 codes and their scales (pow2: powers of two)."""
-    dev, (xp, dt, pitch), at = _f8_rows(x, codes, scales, "x")
-    rc = native().lib.exl3b200_f8_quantize(xp, dt, pitch, *x.shape, *at, pow2, _current_stream(dev) if stream is None else stream)
+    dev, dt, pitch, at = _f8_rows(x, codes, scales, "x")
+    rc = native().lib.exl3b200_f8_quantize(x.data_ptr(), dt, pitch, *x.shape, *at, pow2,
+                                           _current_stream(dev) if stream is None else stream)
     if rc:
         raise RuntimeError(f"exl3b200_f8_quantize: status {rc}")
     return codes, scales
@@ -159,8 +165,9 @@ def f8_quantize(x, codes, scales, pow2=False, stream=None):
 
 def f8_dequantize(codes, scales, y, stream=None):
     """The values that codes and scales stand for, into y [rows, cols] (f32, f16 or bf16)."""
-    dev, (yp, dt, pitch), at = _f8_rows(y, codes, scales, "y")
-    rc = native().lib.exl3b200_f8_dequantize(*at, *y.shape, yp, dt, pitch, _current_stream(dev) if stream is None else stream)
+    dev, dt, pitch, at = _f8_rows(y, codes, scales, "y")
+    rc = native().lib.exl3b200_f8_dequantize(*at, *y.shape, y.data_ptr(), dt, pitch,
+                                             _current_stream(dev) if stream is None else stream)
     if rc:
         raise RuntimeError(f"exl3b200_f8_dequantize: status {rc}")
     return y

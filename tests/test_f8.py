@@ -111,6 +111,7 @@ def test_extremes_zeros_and_values_that_are_no_numbers(dtype, pow2):
         x[12:20] = x[12:20] * 2.0 ** -112                       # about the least maximum
         x[20:] = x[20:] * 2.0 ** 120
     check(x, pow2)
+    check(x, pow2, torch.empty((24, 256), dtype=F8, device="cuda"), torch.empty((24, 2), device="cuda"))     # rows without gaps
 
 
 def test_values_on_the_midpoints():
