@@ -47,6 +47,24 @@ __device__ __forceinline__ void arrive_el(uint32_t bar) {
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(bar)
                  : "memory");
 }
+// 32 columns of this warp's 32 lanes, lane l's in thread l, and there when it returns: one load, 141 -> 135 us against two of 16
+// columns (16 experts, 16060 rows, 4096 -> 1536).
+__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 // A number from global memory if `ok`, else v as it was. In place: a value that met another one on the way would be waited for
 // where they meet.
 __device__ __forceinline__ void ld_if(float& v, const float* p, bool ok) {
@@ -294,20 +312,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
                 const uint32_t done = d_free[db.s];
                 db.next(2);
                 if (any) {
-                    uint32_t a[2][16];
+                    uint32_t a[32];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {             // 32 columns at a time
-                        tmem_ld16(d + 32 * c, a[0]);
-                        tmem_ld16(d + 32 * c + 16, a[1]);
-                        tmem_wait(a[0]);
-                        tmem_wait(a[1]);
+                        tmem_get32(d + 32 * c, a);
                         if (c == 3) {
                             fence_before();
                             arrive_el(done);
                         }
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            acc[2 * c + (k >> 3)][k & 7] = fma2(f2pk(__uint_as_float(a[k >> 3][2 * (k & 7)]), __uint_as_float(a[k >> 3][2 * (k & 7) + 1])), c < 2 ? f0 : f1, acc[2 * c + (k >> 3)][k & 7]);
+                            acc[2 * c + (k >> 3)][k & 7] =
+                                fma2(f2pk(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1])), c < 2 ? f0 : f1,
+                                     acc[2 * c + (k >> 3)][k & 7]);
                     }
                 } else {
                     arrive_el(done);

@@ -98,7 +98,7 @@ __device__ __forceinline__ void place_chunk_fast(const int32_t* ids, int64_t c0,
 constexpr int kPlaceFastExperts = 1024;
 
 // The whole sort in one block (few pairs): histogram, scan, stable placement, tail of -1.
-// `ids` carries no __restrict__: the fused router below writes the ids earlier in the same kernel, so they must not be
+// `ids` carries no __restrict__: a fused router writes the ids earlier in the same kernel, so they must not be
 // read through the read-only (non-coherent) path.
 __device__ __forceinline__ void scatter_block(const int32_t* ids, int64_t n_pairs, int n_expert,
                                               int64_t base, int32_t* __restrict__ sorted_tok,
