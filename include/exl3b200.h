@@ -165,8 +165,9 @@ int     exl3b200_moe_layer_forward(const Exl3bLayerDesc* desc, const Exl3bLayerB
  * row). desc->shared: n_expert = n_local = 1, expert_base 0, top_k 1, hidden = desc->routed.hidden, its own width and
  * bitrates; sgate_w f16 [hidden], 16-byte aligned. Buffers: one device block (exl3b200_moe_block_work_bytes), cut by
  * exl3b200_moe_block_carve into the routed layer's and the shared expert's Exl3bLayerBufs (shared.y_rows is the
- * shared arm's bf16 output). The forward enqueues only. Not built here: the protected experts (the reference serves
- * them with FP8 grouped GEMMs over the trailing run of the offsets) and the norm and residual add around the block.
+ * shared arm's bf16 output). The forward enqueues only. Not part of it: the norm and residual add around the
+ * block, and the protected experts, which the reference serves with FP8 grouped GEMMs over the trailing run of the
+ * offsets (exl3b200_grouped_mm over FP8 operands is such a product: it comes first, and exl3b200_moe_op_live after).
  *   exl3b200_moe_gather_fold: the fold alone (rows, sout, x, gate_w, y 16-byte aligned; row_pitch, width, x_cols
  *     multiples of 8; y_dtype RAD_F32 or RAD_BF16; work as exl3b200_moe_gather's).
  *   exl3b200_identity_routing: sorted_tok[i] = i for i < n_tok, expert_offset = {0, n_tok} (the shared expert's). */

@@ -15,6 +15,10 @@
 //   2, 3    nothing: they leave their registers to the summing warps
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok
 //   8..15   sums: 32 sorted rows and a group's 128 columns each, then their outputs
+// It is bounded by the summing warps: a stage's reads of tensor memory and FMAs take about 1000 cycles where its MMAs take 512,
+// and a unit's outputs (about 4000 cycles) find the tensor pipe with two stages to run ahead, what tensor memory holds: the pipe
+// is busy 37 to 41 % of a launch. In a graph 188 us at 418 experts of 20072 rows, 2048 -> 512 silu_mul (0.9 GB, 4.9 TB/s); 77 at
+// 64 experts of them; 135 at 16 experts, 16060 rows, 4096 -> 1536 (1520 TFLOP/s).
 #pragma once
 
 #include <cuda.h>

@@ -344,12 +344,12 @@ def test_f8_products_refuse():
     assert (y == 5).all()
 
 
-@pytest.mark.parametrize("routed", [False, True])
+@pytest.mark.parametrize("routed", [False, True, "masked"])
 @pytest.mark.parametrize("T", [1, 40, 300])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_an_fp8_block_is_its_entries(T, dtype, routed):
-    """The residual block over FP8 experts, with its own router and with grouped routing, against the entries it is made of, to
-    the bit; and in a graph."""
+    """The residual block over FP8 experts, with its own router, with grouped routing, and with a bias that leaves a token fewer
+    experts than slots, against the entries it is made of, to the bit; and in a graph."""
     E, H, W, k = 32, 528, 272, 4
     g = gen(T)
     t = {"router_w": randn(g, E, H, dtype=dtype) * H ** -0.5, "pre_w": randn(g, H, dtype=dtype), "post_w": randn(g, H, dtype=dtype),
@@ -357,6 +357,8 @@ def test_an_fp8_block_is_its_entries(T, dtype, routed):
     _, _, t["gu_w"], t["gu_scales"], _ = operands(1, E, 1, H, W, "silu_mul")
     _, _, t["dn_w"], t["dn_scales"], _ = operands(2, E, 1, W, H, "none")
     routing = dict(score="sigmoid", bias=0.1 * randn(g, E), groups=8, keep_groups=3, group_top=2, renorm=True, scale=2.5)
+    if routed == "masked":
+        routing["bias"][2:] = -float("inf")
     block = dense.ExpertBlock(top_k=k, res_scale=0.5, max_tokens=300, router=routing if routed else None, **t)
     x = randn(g, T, H, dtype=dtype)
     out, nxt = torch.empty_like(x), torch.empty_like(x)
@@ -369,6 +371,7 @@ def test_an_fp8_block_is_its_entries(T, dtype, routed):
     dense.GroupedMm(x=xn, w=t["router_w"][None], y=logits).run()
     if routed:
         dense.Router(logits=logits, top_k=k, ids=ids, w=w, sorted_tok=tok, expert_offset=off, **routing).run()
+        assert routed != "masked" or ((ids[:, 2:] == -1).all() and (ids[:, :2] >= 0).all() and (tok == -1).sum() == 2 * T)
     else:
         work = new(nat.scatter_work_bytes(P, E), dt=torch.uint8)
         nat.router_scatter(logits.data_ptr(), T, E, k, ids.data_ptr(), w.data_ptr(), E, 0, tok.data_ptr(), off.data_ptr(),
@@ -409,3 +412,32 @@ def test_a_block_refuses_a_router_that_does_not_fit():
                 dict(dn_w=dn.view(torch.uint8))):
         with pytest.raises(ValueError):
             dense.ExpertBlock(**{**t, **bad})
+
+
+@pytest.mark.parametrize("T,pad", [(1, 7), (40, 65), (300, 900)])
+def test_beside_exl3_experts_in_one_buffer(T, pad):
+    """Trailing experts in FP8 behind a layer's EXL3 ones: grouped_mm over their part of the offsets, which clears the rows
+    before them, then the EXL3 ops over their live rows alone, which leave the others."""
+    from exl3b200 import load_plugin
+    from exl3b200.layer import MoeLayer
+    lay = MoeLayer(load_plugin(), n_expert=16, hidden=2048, width=512, top_k=4, bits_gu=3, bits_dn=4, max_tokens=T, seed=3,
+                   max_rows=T * 4 + pad)
+    R, K, H, g = T * lay.k, 512, lay.H, gen(4)
+    lay.x.copy_(randn(g, *lay.x.shape, dtype=F16))
+    lay.logits.copy_(randn(g, *lay.logits.shape))
+    n = R + pad
+    lay.forward(T, stream())
+    lay.experts(T, n, stream(), live=True)    # alone, over as many rows: their number chooses the ops' form
+    torch.cuda.synchronize()
+    want = lay.y_rows[:R].view(torch.int16).clone()
+    off = torch.tensor([R, R + pad // 3, n], dtype=torch.int32, device="cuda")
+    y = lay.y_rows[:n].view(BF16)
+    xq, xs, w, ws, xv = operands(5, 2, n, K, H, "none")
+    dense.GroupedMm(x=xq, x_scales=xs, w=w, w_scales=ws, expert_offset=off, y=y).run(stream())
+    alone = y[R:].clone()
+    rows = torch.arange(n, dtype=torch.int32, device="cuda")
+    close(y, *plain(xv, values_of(w, ws, H), rows, off, 0, "none", H), BF16)
+    assert not y[:R].any()
+    lay.experts(T, n, stream(), live=True)
+    torch.cuda.synchronize()
+    assert torch.equal(y[R:], alone) and torch.equal(lay.y_rows[:R].view(torch.int16), want)
