@@ -398,7 +398,10 @@ class ExpertBlock:
                     raise ValueError(f"{name} is strided")
         if _several:
             _check_current(self._dev)
-        native().expert_block_forward(self.desc, self.bufs, x.data_ptr(), T, out.data_ptr(),
-                                      next_out.data_ptr() if next_out is not None else None,
-                                      _current_stream(self._dev) if stream is None else stream, self.router)
+        args = (self.bufs, x.data_ptr(), T, out.data_ptr(), next_out.data_ptr() if next_out is not None else None,
+                _current_stream(self._dev) if stream is None else stream)
+        if self.router is None:
+            native().expert_block_forward(self.desc, *args)
+        else:
+            native().expert_block_forward_routed(self.desc, self.router, *args)
         return out

@@ -470,7 +470,10 @@ class Native:
                     "exl3b200_expert_block_carve")
         return b
 
-    def expert_block_forward(self, desc, bufs, x, n_tok, out, next_, stream=0, router=None):
-        self._check(self.lib.exl3b200_expert_block_forward_routed(C.byref(desc), None if router is None else C.byref(router),
-                                                                  C.byref(bufs), x, n_tok, out, next_, stream),
-                    "exl3b200_expert_block_forward_routed")
+    def expert_block_forward(self, desc, bufs, x, n_tok, out, next_, stream=0):
+        self._check(self.lib.exl3b200_expert_block_forward(C.byref(desc), C.byref(bufs), x, n_tok, out, next_, stream),
+                    "exl3b200_expert_block_forward")
+
+    def expert_block_forward_routed(self, desc, router, bufs, x, n_tok, out, next_, stream=0):
+        self._check(self.lib.exl3b200_expert_block_forward_routed(C.byref(desc), C.byref(router), C.byref(bufs), x, n_tok, out,
+                                                                  next_, stream), "exl3b200_expert_block_forward_routed")
