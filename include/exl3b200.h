@@ -413,7 +413,7 @@ int     exl3b200_tp_step_forward(const Exl3bTpDesc* desc, const Exl3bLayerBufs* 
                                  const float* logits, int64_t n_tok, float* out, int64_t out_pitch, void* stream,
                                  void* const* marks);
 
-/* Experts whose weights are not EXL3 records (kept in f16 / bf16, or in MXFP4), and the norms around a block. No
+/* Experts whose weights are not EXL3 records (kept in f16 / bf16, FP8 or MXFP4), their routers, and the norms around a block. No
  * counterpart in the reference's kernels (its engine serves protected experts and norms); serving only, no gradients.
  *
  * MXFP4 (dtype EXL3B_MX4): blocks of 32 values along a row, each an e2m1 code -- two a byte, the lower index in the low

@@ -19,7 +19,7 @@ constexpr int kMaxTurn = 16;                      // slices a unit at most
 constexpr int kStage = 8;                        // ... and stages at once, where it stages in f32
 constexpr int kEpiLd = 128 + 4;                  // f32 a staged row, padded
 constexpr int kTab = 128;                        // a CTA's units held in a shared table (more: looked up)
-constexpr int kStatic = 3072;                    // the static shared arrays, up to the ring's alignment
+constexpr int kStatic = 3 * 1024;                // the static shared arrays, up to the ring's alignment
 constexpr int kMaxExpert = 2048;
 constexpr int kMaxSplit = 4;                     // CTAs a unit at most (SPLIT)
 constexpr int kMaxSt = 10;                       // stages at most
