@@ -273,9 +273,9 @@ class Router(_Plan):
         if sorted_tok is not None or expert_offset is not None:
             d.sorted_tok, _ = _rows(sorted_tok, "sorted_tok", dev, (d.n_tok * top_k,), torch.int32)
             d.expert_offset, _ = _rows(expert_offset, "expert_offset", dev, dtype=torch.int32)
-            if expert_offset.dim() != 1 or len(expert_offset) < 2:
+            if expert_offset.dim() != 1 or expert_offset.shape[0] < 2:
                 raise ValueError(f"expert_offset has shape {tuple(expert_offset.shape)}, not (local experts + 1,)")
-            d.n_local, d.expert_base = len(expert_offset) - 1, expert_base
+            d.n_local, d.expert_base = expert_offset.shape[0] - 1, expert_base
             work = torch.empty(native().scatter_work_bytes(d.n_tok * top_k, d.n_local), dtype=torch.uint8, device=logits.device)
             d.work = work.data_ptr()
             # a run may come on any stream: whatever used the buffer's memory before is done by then
