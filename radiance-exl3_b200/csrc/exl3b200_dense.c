@@ -18,7 +18,7 @@ int exl3b_cuda_gmm(const Exl3bGmmOp* p, int sm_count, void* stream);
 int exl3b_cuda_gmm8(const Exl3bGmmOp* p, int sm_count, void* stream);
 int exl3b_gmm_max_expert(void);
 /* exl3b200_route.cu, exl3b200_f8.cu */
-int exl3b_route_fuses(int64_t n_tok, int64_t n_local);
+int exl3b_route_fuses(int64_t n_tok, int64_t top_k, int64_t n_local);
 int exl3b_cuda_route(const Exl3bRouteOp* p, int dtype, int fused, void* stream);
 int exl3b_cuda_f8_quantize(const void* x, int dtype, int64_t x_pitch, int64_t rows, int64_t cols, uint8_t* q,
                            int64_t q_pitch, float* s, int64_t s_pitch, int pow2, void* stream);
@@ -203,7 +203,7 @@ int exl3b200_router(const Exl3bRouter* d, void* stream) {
     const int64_t E = d->n_expert, G = d->n_group;
     const int sort = d->expert_offset != 0;
     if (d->n_tok > 0) {
-        const int fused = sort && exl3b_route_fuses(d->n_tok, d->n_local);
+        const int fused = sort && exl3b_route_fuses(d->n_tok, d->top_k, d->n_local);
         int shift = 0;
         const int64_t per = lane_experts(d, &shift);
         Exl3bRouteOp p;

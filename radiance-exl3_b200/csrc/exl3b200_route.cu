@@ -372,23 +372,42 @@ __global__ void __launch_bounds__(128) k_route(const __grid_constant__ Exl3bRout
     if (t < p.n_tok) route<RPL, DT, WIDE>(p, t, threadIdx.x & 31);
 }
 
-// A few tokens: their routing and the whole sort in one block, as moe_scatter sorts: experts counted, the counts summed up, and
-// each pair placed behind those of its expert in earlier warps (whose leading lanes note their counts, a row a warp) and lanes.
-constexpr int kFusedTokens = 32, kFusedThreads = 512;
-__device__ __forceinline__ int32_t* fused_counts(int* sm, const Exl3bRouteOp& p) { return sm + ((int)p.n_tok * p.top_k + 3) / 4 * 4; }
+// A few tokens: their routing and the whole sort in one launch. A cluster of CTAs routes, a token a warp; its first CTA, to
+// whose shared memory they write the ids, sorts as moe_scatter does: experts counted, the counts summed up, and each pair placed
+// behind those of its expert in earlier warps (whose leading lanes note their counts, a row a warp) and lanes. The others are done
+// when they have routed: nothing reads their shared memory. A CTA for each four tokens, up to eight of them: a warp a scheduler as
+// long as it goes (32 tokens of 512 experts 7.4 us, all in one CTA 14.6, in two launches 9.7).
+constexpr int kFusedTokens = 128, kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
+__host__ __device__ __forceinline__ int64_t fused_ids(int64_t pairs) { return (pairs + 3) / 4 * 4; }
+size_t fused_bytes(int64_t pairs, int64_t n_local) { return (size_t)(fused_ids(pairs) + n_local + 1 + (pairs + 31) / 32 * n_local) * 4; }
 template <int RPL, int DT, bool WIDE>
 __global__ void __launch_bounds__(kFusedThreads) k_route_sort(const __grid_constant__ Exl3bRouteOp p) {
     extern __shared__ int sm[];
     __shared__ int wtot[32];
     int* const ids = sm;                                       // [n_tok * top_k]
-    int* const cnt = fused_counts(sm, p);                      // [n_local + 1], then [warps of pairs][n_local]
     const int tid = threadIdx.x, lane = tid & 31, E = p.n_local, P = (int)p.n_tok * p.top_k;
+    int* const cnt = sm + fused_ids(P);                        // [n_local + 1], then [warps of pairs][n_local]
     int* const wcnt = cnt + E + 1;
-    for (int x = tid; x < E + 1 + (P + 31) / 32 * E; x += kFusedThreads) cnt[x] = 0;
+    const bool several = gridDim.x > 1, first = blockIdx.x == 0;
+    if (several) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    if (first)
+        for (int x = tid; x < E + 1 + (P + 31) / 32 * E; x += kFusedThreads) cnt[x] = 0;
     chain_wait();
     chain_next();
-    for (int64_t t = tid >> 5; t < p.n_tok; t += kFusedThreads / 32) route<RPL, DT, WIDE>(p, t, lane, ids);
-    __syncthreads();
+    int* to = ids;
+    if (several) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");                // the first CTA is there
+        if (!first) asm volatile("mapa.u64 %0, %1, 0;" : "=l"(to) : "l"(ids));
+    }
+    for (int64_t t = blockIdx.x + gridDim.x * (tid >> 5); t < p.n_tok; t += gridDim.x * kFusedWarps)
+        route<RPL, DT, WIDE>(p, t, lane, to);
+    if (several) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (!first) return;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
     for (int f0 = 0; f0 < P; f0 += kFusedThreads) {
         const int f = f0 + tid, e = f < P ? local_expert(ids[f], p.expert_base, E) : -1;
         const unsigned peers = __match_any_sync(kAll, e);
@@ -424,11 +443,11 @@ template <int RPL, int DT, bool WIDE>
 int launch(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
     if (!fused) return chain_launch(k_route<RPL, DT, WIDE>, dim3((unsigned)((p->n_tok + 3) / 4)), dim3(128), 0, 1, st, *p);
     auto kern = k_route_sort<RPL, DT, WIDE>;
-    const int64_t pairs = p->n_tok * p->top_k;
-    const size_t smem = (size_t)((pairs + 3) / 4 * 4 + p->n_local + 1 + (pairs + 31) / 32 * p->n_local) * 4;
+    const size_t smem = fused_bytes(p->n_tok * p->top_k, p->n_local);
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return -6;
-    return chain_launch(kern, dim3(1), dim3(kFusedThreads), smem, 1, st, *p);
+    const int ctas = (int)(p->n_tok > 28 ? 8 : (p->n_tok + 3) / 4);
+    return chain_launch(kern, dim3(ctas), dim3(kFusedThreads), smem, ctas, st, *p);
 }
 template <int RPL, int DT>
 int launch_wide(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
@@ -445,8 +464,13 @@ int launch_type(const Exl3bRouteOp* p, int dtype, int fused, cudaStream_t st) {
 
 extern "C" {
 
-// Whether the sort comes in the same launch: few tokens, the placement's table in shared memory.
-int exl3b_route_fuses(int64_t n_tok, int64_t n_local) { return n_tok <= kFusedTokens && n_local <= kPlaceFastExperts; }
+// Whether the sort comes in the same launch: few tokens, the placement's table in shared memory. The table is one CTA's work, so
+// that from 64 tokens on a large one costs more than a launch: one launch against two at 64 tokens of 512 experts, ten each, 9.7
+// and 10.3 us, at 96 of them 11.2 and 10.8; at 128 of 256 experts, eight each (37 KB), 10.0 and 10.3.
+int exl3b_route_fuses(int64_t n_tok, int64_t top_k, int64_t n_local) {
+    return n_tok <= kFusedTokens && n_local <= kPlaceFastExperts &&
+           fused_bytes(n_tok * top_k, n_local) <= (n_tok <= 64 ? 200 : 40) * 1024;
+}
 
 int exl3b_cuda_route(const Exl3bRouteOp* p, int dtype, int fused, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);

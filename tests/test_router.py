@@ -120,10 +120,19 @@ def test_scores_biases_and_groups(E, k, groups, keep, top, renorm, bias, score):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("T", [1, 2, 31, 32, 33, 300, 2500])
 def test_types_and_token_counts_with_the_sort(T, dtype):
-    """16-bit logits hold equal ones; up to 32 tokens come with their sort in one launch."""
+    """16-bit logits hold equal ones."""
     kw = dict(score="sigmoid", groups=8, keep_groups=4, group_top=2, renorm=True, scale=2.5)
     check(logits_of(T, T, 256, dtype), 8, local=256, bias=bias_of(1, 256), **kw)
     check(logits_of(T + 1, T, 512, dtype), 10, local=512)
+
+
+@pytest.mark.parametrize("T", [3, 4, 5, 16, 17, 28, 29, 48, 63, 64, 65, 97, 127, 128, 129])
+@pytest.mark.parametrize("E,k,local,base", [(512, 10, 512, 0), (256, 8, 256, 0), (40, 5, 40, 0), (1024, 32, 1024, 0),
+                                            (2048, 16, 1024, 512), (64, 32, 8, 30)])
+def test_the_sort_in_one_launch_and_in_its_own(T, E, k, local, base):
+    """A CTA for each four tokens, up to eight of them with sixteen; by the size of the sort's table, launches of its own."""
+    check(logits_of(T, T, E), k, local=local, base=base, renorm=True)
+    check(logits_of(T, T, E, BF16), k, local=local, base=base, score="sigmoid", bias=bias_of(T, E))
 
 
 def test_the_sort_over_a_ranks_experts():
