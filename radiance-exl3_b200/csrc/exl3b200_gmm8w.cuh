@@ -44,6 +44,7 @@ constexpr int stages_of(int n_expert) {
     const int n = (227 * 1024 - kStatic - fixed_bytes(n_expert)) / kStageB;
     return n < kMaxSt ? n : kMaxSt;
 }
+constexpr int kPolls = 64;                                   // of a barrier, before a suspended wait
 static_assert(stages_of(kMaxExpert) >= 4 && (2 * kMaxSt + 2 * kDb) * 8 + 8 <= 512, "shared memory");
 
 // One arrival, by one lane of a whole warp.
@@ -51,9 +52,8 @@ __device__ __forceinline__ void arrive_el(uint32_t bar) {
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(bar)
                  : "memory");
 }
-// 32 columns of this warp's 32 lanes, lane l's in thread l, and there when it returns: one load, 141 -> 135 us against two of 16
-// columns (16 experts, 16060 rows, 4096 -> 1536).
-__device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t (&r)[32]) {
+// 32 or 16 columns of this warp's 32 lanes, lane l's in thread l; tmem_got before they are read.
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -61,11 +61,26 @@ __device__ __forceinline__ void tmem_get32(uint32_t taddr, uint32_t (&r)[32]) {
                    "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_got(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
                    "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_got(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
@@ -125,9 +140,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
     const int nck = sh.nck;
     volatile uint32_t* vdead = dead;
     // A bounded wait by a whole warp, which reports nothing: one that gives up marks the CTA dead, every other wait of the
-    // CTA then gives up at its next try, and the roles leave at their next unit.
+    // CTA then gives up at its next try, and the roles leave at their next unit. It asks a few times before it lets itself be
+    // suspended, which takes longer to wake from (132 against 128 us at 16 experts).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         const uint32_t a = smem_u32(bar);
+#pragma unroll 1
+        for (int j = 0; j < kPolls; ++j) {
+            uint32_t done;
+            asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                         " selp.u32 %0, 1, 0, p;\n}\n"
+                         : "=r"(done)
+                         : "r"(a), "r"(parity)
+                         : "memory");
+            if (done) {
+                __syncwarp();
+                return;
+            }
+        }
         uint64_t t0 = 0;
         for (;;) {
             uint32_t done;
@@ -149,10 +178,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
     };
     Pipe pipe;                                                // of the stages
 
-    // The summing warps' sums need more than the 128 registers a thread that 512 threads start with: 256 x 192 + 256 x 64 are
+    // The summing warps' sums need more than the 128 registers a thread that 512 threads start with: 256 x 208 + 256 x 48 are
     // the 512 x 128 of the launch.
     if (warp < kEpiWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 0) {
             // ------------------------------------------------------------ weights
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
@@ -240,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
         }
     } else {
         // ---------------------------------------------------------------- sums
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp & 3, g = (warp - kEpiWarp0) >> 2, ew = warp - kEpiWarp0;
         constexpr int es = OUT == RAD_F32 ? 4 : 2;
         clear_outside<OUT>(p, blockIdx.x * 4 * kGroups + ew, gridDim.x * 4 * kGroups, lane);
@@ -316,20 +345,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
                 const uint32_t done = d_free[db.s];
                 db.next(2);
                 if (any) {
-                    uint32_t a[32];
+                    // 32 and 16 columns in turn, the next ones' load in flight under the FMAs
+                    uint32_t a[32], b[16];
+                    auto sum = [&](const uint32_t* v, int c0, int n) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {             // 32 columns at a time
-                        tmem_get32(d + 32 * c, a);
-                        if (c == 3) {
-                            fence_before();
-                            arrive_el(done);
-                        }
+                        for (int k = 0; k < n; k += 2)
+                            acc[(c0 + k) >> 4][(c0 + k) >> 1 & 7] =
+                                fma2(f2pk(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c0 + k < 64 ? f0 : f1,
+                                     acc[(c0 + k) >> 4][(c0 + k) >> 1 & 7]);
+                    };
+                    tmem_get(d, a);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            acc[2 * c + (k >> 3)][k & 7] =
-                                fma2(f2pk(__uint_as_float(a[2 * k]), __uint_as_float(a[2 * k + 1])), c < 2 ? f0 : f1,
-                                     acc[2 * c + (k >> 3)][k & 7]);
+                    for (int c = 0; c < 96; c += 48) {
+                        tmem_got(a);
+                        tmem_get(d + c + 32, b);
+                        sum(a, c, 32);
+                        tmem_got(b);
+                        tmem_get(d + c + 48, a);
+                        sum(b, c + 32, 16);
                     }
+                    tmem_got(a);
+                    fence_before();
+                    arrive_el(done);
+                    sum(a, 96, 32);
                 } else {
                     arrive_el(done);
                 }
