@@ -6,19 +6,20 @@
 // 418 experts of 20072 rows, 2048 -> 512 silu_mul.)
 //
 // Persistent over units (expert, a group of up to 128 of its sorted rows, a block of 256 weight rows; silu_mul: 128 gate rows and
-// their 128 up rows), one CTA an SM. A unit's weight rows are two groups of 128, an MMA and four summing warps each: act NONE in
-// order; silu_mul 64 gate rows and their 64 up rows, and the next 64 of each, so that a thread has both of its 64 outputs.
+// their 128 up rows), one CTA an SM. A unit's weight rows are two groups of 128 columns of the accumulator, four summing warps each:
+// act NONE in order; silu_mul 64 gate rows and their 64 up rows, and the next 64 of each, so that a thread has both of its 64 outputs.
 // Warps of a CTA:
 //   0       weights: cp.async.bulk.tensor, 128-byte swizzled
-//   1       MMA issuer: eight tcgen05.mma (kind::f8f6f4, M 128, N 128, K 32) a stage of 128 k, four a group, into the group's
-//           next accumulator (two each, in tensor memory)
+//   1       MMA issuer: four tcgen05.mma (kind::f8f6f4, M 128, N 256, K 32) a stage of 128 k, into one of two accumulators in
+//           tensor memory (one of 128 columns a group instead, two each: 128.4 against 126.1 us at 16 experts)
 //   2, 3    nothing: they leave their registers to the summing warps
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok
 //   8..15   sums: 32 sorted rows and a group's 128 columns each, then their outputs
-// It is bounded by the summing warps: a stage's reads of tensor memory and FMAs take about 1000 cycles where its MMAs take 512,
-// and a unit's outputs (about 4000 cycles) find the tensor pipe with two stages to run ahead, what tensor memory holds: the pipe
-// is busy 37 to 41 % of a launch. In a graph 188 us at 418 experts of 20072 rows, 2048 -> 512 silu_mul (0.9 GB, 4.9 TB/s); 77 at
-// 64 experts of them; 135 at 16 experts, 16060 rows, 4096 -> 1536 (1520 TFLOP/s).
+// A stage's MMAs take 512 cycles, a stage about 1140 (16 experts). What is left is not the sums' instructions: with the sums left out
+// 128 us became 121, with the outputs too 112, with most of the loads as well 103. It is the round trip of an accumulator, of which
+// tensor memory holds two: the MMAs' completion, its barrier, the reads, their barrier and the next issue; then a unit's outputs, which
+// wait for its last stage. In a graph 184 us at 418 experts of 20072 rows, 2048 -> 512 silu_mul (0.9 GB, 4.9 TB/s); 72 at 64
+// experts of them; 126 at 16 experts, 16060 rows, 4096 -> 1536 (1630 TFLOP/s).
 #pragma once
 
 #include <cuda.h>
@@ -36,8 +37,8 @@ namespace wide {
 constexpr int kGroups = 2;                                   // of four summing warps, each for 128 weight rows
 constexpr int kThreads = (kEpiWarp0 + 4 * kGroups) * 32;
 constexpr int kRows = 128;                                   // sorted rows a unit at most: the MMA's lanes
-constexpr int kCols = 128;                                   // of an accumulator: a group's weight rows
-constexpr int kDb = 2 * kGroups;                             // accumulators: two of each group in turn
+constexpr int kCols = 128;                                   // of a group: its weight rows
+constexpr int kDb = 2;                                       // accumulators in turn, of both groups' columns
 constexpr int kWideW_B = kGroups * kW_B, kX_B = kRows * kRowB, kStageB = kWideW_B + kX_B;
 constexpr int fixed_bytes(int n_expert) { return 1024 + 512 + (n_expert + 4) * 4; }
 constexpr int stages_of(int n_expert) {
@@ -117,14 +118,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
         mbar_init(&empty[tid], 1);
     } else if (tid >= 32 && tid < 32 + kDb) {
         mbar_init(&d_full[tid - 32], 1);
-        mbar_init(&d_empty[tid - 32], 4);
+        mbar_init(&d_empty[tid - 32], 4 * kGroups);
     } else if (tid == 64) {
         *dead = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
-    if (warp == 1) tmem_alloc<false>(tmem_slot, kDb * kCols);
+    if (warp == 1) tmem_alloc<false>(tmem_slot, kDb * kGroups * kCols);
     chain_wait();                                             // all above needs no memory but the CTA's own
     scan_units<kThreads, 1>(p, sh, first, prefix, utab, wsum);
     fence_before();
@@ -204,21 +205,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
         } else if (warp == 1) {
             // ------------------------------------------------------------ MMA issuer
             const uint64_t wd0 = desc_sw128(smem_u32(w_ring)), xd0 = desc_sw128(smem_u32(x_ring));
-            // D f32, e4m3 both, both operands K-major, M 128, N 128
-            constexpr uint32_t idesc = (uint32_t)kCols >> 3 << 17 | 8u << 24 | 1u << 4;
+            // D f32, e4m3 both, both operands K-major, M 128, N 256
+            constexpr uint32_t idesc = (uint32_t)(kGroups * kCols) >> 3 << 17 | 8u << 24 | 1u << 4;
             Pipe db;
             for (uint32_t i = 0; i < n_mine && !*vdead; ++i) {
                 for (int ck = 0; ck < nck; ++ck, pipe.next(ST)) {
                     wait(&full[pipe.s], pipe.ph);
                     proxy_fence();
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g, db.next(kDb)) {
-                        wait(&d_empty[db.s], db.ph ^ 1);
-                        fence_after();
-                        mma4_f8<false>(tmem + db.s * kCols, xd0 + (uint64_t)(pipe.s * kX_B >> 4),
-                                      wd0 + (uint64_t)((pipe.s * kWideW_B + g * kW_B) >> 4), idesc, 0u);
-                        commit_el<false>(&d_full[db.s]);
-                    }
+                    wait(&d_empty[db.s], db.ph ^ 1);
+                    fence_after();
+                    mma4_f8<false>(tmem + db.s * kGroups * kCols, xd0 + (uint64_t)(pipe.s * kX_B >> 4),
+                                  wd0 + (uint64_t)(pipe.s * kWideW_B >> 4), idesc, 0u);
+                    commit_el<false>(&d_full[db.s]);
+                    db.next(kDb);
                     commit_el<false>(&empty[pipe.s]);
                 }
             }
@@ -309,12 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
             fetch(0);
             begin(0);
         }
-        // the group's accumulators: g, then g + 2; their barriers' addresses held, not worked out each stage (86 against 79 us at 64
-        // experts of 20072 rows, 2048 -> 512 silu_mul)
-        uint32_t d_free[2];
+        // the accumulators' barriers' addresses held, not worked out each stage (86 against 79 us at 64 experts of 20072 rows,
+        // 2048 -> 512 silu_mul)
+        uint32_t d_free[kDb];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            d_free[b] = smem_u32(&d_empty[2 * b + g]);
+        for (int b = 0; b < kDb; ++b) {
+            d_free[b] = smem_u32(&d_empty[b]);
             asm volatile("" : "+r"(d_free[b]));
         }
         Pipe db;
@@ -339,11 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
 #pragma unroll
                 for (int j = 0; j < (ACT ? 8 : 4); ++j)
                     if ((j & 3) < 3) f[j] = f[j + 1];
-                wait(&d_full[2 * db.s + g], db.ph);
+                wait(&d_full[db.s], db.ph);
                 fence_after();
-                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + (2 * db.s + g) * kCols;
+                const uint32_t d = tmem + ((uint32_t)(32 * q) << 16) + (kGroups * db.s + g) * kCols;
                 const uint32_t done = d_free[db.s];
-                db.next(2);
+                db.next(kDb);
                 if (any) {
                     // 32 and 16 columns in turn, the next ones' load in flight under the FMAs
                     uint32_t a[32], b[16];
@@ -430,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
     __syncthreads();
     if (warp == 1) {
         fence_after();
-        tmem_free<false>(tmem, kDb * kCols);
+        tmem_free<false>(tmem, kDb * kGroups * kCols);
     }
 }
 
