@@ -496,9 +496,9 @@ template <bool ACT>
 int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
     // The wide form where its units cost less: a unit's stage there takes 3.1 times as long as a narrow one's (2 times where the
     // SMs have a unit each at most), and its start and end as long as five of those; narrow units run two an SM. Narrow and wide,
-    // us: 64 experts, 2048 -> 512 silu_mul, 28 rows each 28.2 and 29.8, 40 rows 33.0 and 30.4, 130 rows 62.7 and 41.5; 640 ->
-    // 2560, 40 rows 27.4 and 30.8, 96 rows 47.6 and 41.5; 300 experts of 96 rows, 448 -> 160 silu_mul 30.9 and 33.4; one expert,
-    // 4096 -> 1536, 512 rows 17.7 and 25.0, 1024 rows 30.1 and 25.2.
+    // us: 64 experts, 2048 -> 512 silu_mul, 28 rows each 28.3 and 29.1, 40 rows 32.9 and 29.9, 130 rows 62.4 and 40.7; 640 ->
+    // 2560, 40 rows 27.5 and 27.8, 96 rows 47.4 and 36.9; 300 experts of 96 rows, 448 -> 160 silu_mul 30.9 and 32.1; one expert,
+    // 4096 -> 1536, 512 rows 17.8 and 22.3, 1024 rows 30.2 and 22.7.
     const int64_t nck = (p->n_in + 127) / 128, sm = sm_count;
     const int64_t wide_units = likely_units(p, 128, ACT ? 128 : 256), narrow_units = likely_units(p, 32, ACT ? 64 : 128);
     const int64_t wide_cost = wide_units > sm ? wide_units * (31 * nck + 50) : sm * (20 * nck + 50);
