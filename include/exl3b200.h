@@ -62,7 +62,8 @@ int exl3b200_decode_what(const void* record, int64_t rows, int64_t cols, int bit
  *                 lower id) as ids i32 [n_tok, top_k] and their probabilities w f32 [n_tok, top_k], in
  *                 descending order. n_expert <= 4096, top_k <= 32.
  *   moe_scatter:  a stable counting sort of the flattened pairs t*top_k + s by expert id - expert_base;
- *                 ids outside [0, n_expert) dropped; sorted_tok i32 [n_pairs] (-1 past the live count),
+ *                 negative ids and differences outside [0, n_expert) dropped; sorted_tok i32 [n_pairs] (-1 past
+ *                 the live count),
  *                 expert_offset i32 [n_expert + 1]. `work` is caller-provided device memory of
  *                 exl3b200_moe_scatter_work_bytes() bytes.
  *   moe_gather:   y f32 [n_tok][width] = sum over slots ascending of w * bf16 row of that slot's sorted row

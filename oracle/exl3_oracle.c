@@ -438,14 +438,14 @@ int orc_moe_scatter(const int32_t* expert_ids, int64_t n_pairs, int64_t n_expert
     if (!cnt) return -7;
     for (int64_t i = 0; i < n_pairs; ++i) {
         const int64_t e = (int64_t)expert_ids[i] - expert_base;
-        if (e >= 0 && e < n_expert) ++cnt[e + 1];
+        if (expert_ids[i] >= 0 && e >= 0 && e < n_expert) ++cnt[e + 1];
     }
     for (int64_t e = 0; e < n_expert; ++e) cnt[e + 1] += cnt[e];
     for (int64_t e = 0; e <= n_expert; ++e) expert_offset[e] = (int32_t)cnt[e];
     for (int64_t i = 0; i < n_pairs; ++i) sorted_tok[i] = -1;
     for (int64_t i = 0; i < n_pairs; ++i) {
         const int64_t e = (int64_t)expert_ids[i] - expert_base;
-        if (e >= 0 && e < n_expert) sorted_tok[cnt[e]++] = (int32_t)i;
+        if (expert_ids[i] >= 0 && e >= 0 && e < n_expert) sorted_tok[cnt[e]++] = (int32_t)i;
     }
     free(cnt);
     return 0;

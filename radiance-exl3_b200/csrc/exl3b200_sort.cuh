@@ -38,9 +38,10 @@ __device__ __forceinline__ int block_scan_excl(int* cnt, int n, int* wtot) {
     return total;
 }
 
+// A negative id is no expert's, also where a rank's first expert is a negative number.
 __device__ __forceinline__ int local_expert(int32_t id, int64_t base, int n_expert) {
     const int64_t e = (int64_t)id - base;
-    return e >= 0 && e < n_expert ? (int)e : -1;
+    return id >= 0 && e >= 0 && e < n_expert ? (int)e : -1;
 }
 
 // Stable placement of one chunk of up to 1024 pairs (one a thread, in order), the running per-expert
