@@ -22,6 +22,9 @@ __device__ int32_t g_err_word;   // set by a kernel whose bounded wait gave up
 
 constexpr int kScatterChunk = 1024;   // pairs a block of the large-sort path
 constexpr int kSmallPairs = 2048;     // at most this many pairs: one block does the whole sort
+// The most shared memory that a sort takes, the fast placement's table with its counts; a kernel's limit is set to it whatever a
+// call needs: a smaller one would fail another thread's launch between its own two steps.
+constexpr int kSortBytes = (33 * kPlaceFastExperts + 1) * 4;
 
 // ------------------------------------------------------------------------------------------ router
 // One warp a token: softmax over n_expert logits (max, then sum of exp in lane-strided order reduced by a
@@ -465,10 +468,8 @@ int exl3b200_moe_scatter(const int32_t* ids, int64_t n_pairs, int64_t n_expert, 
     // the small sort and the placement also hold the fast placement's [32][n_expert] table when it fits
     const size_t smem_place = smem + (n_expert <= kPlaceFastExperts ? (size_t)32 * n_expert * 4 : 0);
     if (smem_place > 48 * 1024 &&
-        (cudaFuncSetAttribute(k_scatter_small, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_place) !=
-             cudaSuccess ||
-         cudaFuncSetAttribute(k_scatter_place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_place) !=
-             cudaSuccess))
+        (cudaFuncSetAttribute(k_scatter_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess ||
+         cudaFuncSetAttribute(k_scatter_place, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess))
         return -6;
     if (n_pairs <= kSmallPairs) {
         k_scatter_small<<<1, 1024, smem_place, st>>>(ids, n_pairs, (int)n_expert, expert_base, sorted_tok,
@@ -500,7 +501,7 @@ int exl3b200_router_scatter(const float* logits, int64_t n_tok, int64_t n_route,
     do {                                                                                                             \
         auto kern = k_route_scatter_small<R>;                                                                        \
         if (smem > 48 * 1024 &&                                                                                      \
-            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)       \
+            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess)      \
             return -6;                                                                                               \
         kern<<<1, 1024, smem, st>>>(logits, n_tok, (int)n_route, (int)top_k, ids, w, (int)n_expert, expert_base,     \
                                     sorted_tok, expert_offset);                                                      \

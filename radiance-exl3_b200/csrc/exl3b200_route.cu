@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(128) k_route(const __grid_constant__ Exl3bRout
 // long as it goes (32 tokens of 512 experts 7.4 us, all in one CTA 14.6, in two launches 9.7).
 constexpr int kFusedTokens = 128, kFusedThreads = 512, kFusedWarps = kFusedThreads / 32;
 __host__ __device__ __forceinline__ int64_t fused_ids(int64_t pairs) { return (pairs + 3) / 4 * 4; }
+constexpr int kFusedBytes = 200 * 1024;          // the most that a sort takes
 size_t fused_bytes(int64_t pairs, int64_t n_local) { return (size_t)(fused_ids(pairs) + n_local + 1 + (pairs + 31) / 32 * n_local) * 4; }
 template <int RPL, int DT, bool WIDE>
 __global__ void __launch_bounds__(kFusedThreads) k_route_sort(const __grid_constant__ Exl3bRouteOp p) {
@@ -444,7 +445,8 @@ int launch(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
     if (!fused) return chain_launch(k_route<RPL, DT, WIDE>, dim3((unsigned)((p->n_tok + 3) / 4)), dim3(128), 0, 1, st, *p);
     auto kern = k_route_sort<RPL, DT, WIDE>;
     const size_t smem = fused_bytes(p->n_tok * p->top_k, p->n_local);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    // the same limit whatever this call needs: a smaller one would fail another thread's launch between its own two steps
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedBytes) != cudaSuccess)
         return -6;
     const int ctas = (int)(p->n_tok > 28 ? 8 : (p->n_tok + 3) / 4);
     return chain_launch(kern, dim3(ctas), dim3(kFusedThreads), smem, ctas, st, *p);
@@ -469,7 +471,7 @@ extern "C" {
 // and 10.3 us, at 96 of them 11.2 and 10.8; at 128 of 256 experts, eight each (37 KB), 10.0 and 10.3.
 int exl3b_route_fuses(int64_t n_tok, int64_t top_k, int64_t n_local) {
     return n_tok <= kFusedTokens && n_local <= kPlaceFastExperts &&
-           fused_bytes(n_tok * top_k, n_local) <= (n_tok <= 64 ? 200 : 40) * 1024;
+           fused_bytes(n_tok * top_k, n_local) <= (size_t)(n_tok <= 64 ? kFusedBytes : 40 * 1024);
 }
 
 int exl3b_cuda_route(const Exl3bRouteOp* p, int dtype, int fused, void* stream) {

@@ -1,5 +1,7 @@
 """The router on a GPU where its calls are unusual: slots without an expert before a rank whose first expert is a negative
 number, groups with a single expert left, calls from several threads at once, plans made under graph capture."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -31,3 +33,41 @@ def test_slots_without_an_expert_are_nobodys(T, local, base):
     tok, off = sorted_by_definition(got, local, base)
     assert np.array_equal(sort["expert_offset"].cpu().numpy(), off)
     assert np.array_equal(sort["sorted_tok"].cpu().numpy(), tok)
+
+
+def test_calls_from_several_threads_at_once():
+    """Threads whose sorts need different amounts of shared memory, each on a stream of its own: no call fails another's."""
+    shapes = [(60, 16, 1024), (20, 32, 1024), (64, 12, 700), (33, 8, 900)]      # tokens, slots, the rank's experts of 1024
+    failed, plans = [], []
+    for i, (T, k, local) in enumerate(shapes):
+        plan, ids, _, sort = run(logits_of(i, T, 1024), k, local)
+        plans.append((plan, torch.cuda.Stream(), ids, sort, local, ids.clone(), [sort[n].clone() for n in sorted(sort) if n != "expert_base"]))
+    flat = torch.randint(0, 1000, (2000,), dtype=torch.int32, device="cuda")
+    outs = [(n, torch.empty(2000, dtype=torch.int32, device="cuda"), torch.empty(n + 1, dtype=torch.int32, device="cuda"))
+            for n in (1000, 450)]
+    torch.cuda.synchronize()
+
+    def routes(plan, stream):
+        for _ in range(3000):
+            try:
+                plan.run(stream.cuda_stream)
+            except RuntimeError as e:
+                failed.append(e)
+
+    def sorts(n, tok, off, stream):
+        for _ in range(3000):
+            try:
+                dense.native().moe_scatter(flat.data_ptr(), 2000, n, 0, tok.data_ptr(), off.data_ptr(), None, stream.cuda_stream)
+            except RuntimeError as e:
+                failed.append(e)
+
+    threads = [threading.Thread(target=routes, args=p[:2]) for p in plans]
+    threads += [threading.Thread(target=sorts, args=(*o, torch.cuda.Stream())) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, (len(failed), failed[0])
+    for _, _, ids, sort, _, old, olds in plans:
+        assert torch.equal(ids, old) and all(torch.equal(sort[n], o) for n, o in zip([n for n in sorted(sort) if n != "expert_base"], olds))
