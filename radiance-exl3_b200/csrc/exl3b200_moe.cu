@@ -25,6 +25,11 @@ constexpr int kSmallPairs = 2048;     // at most this many pairs: one block does
 // The most shared memory that a sort takes, the fast placement's table with its counts; a kernel's limit is set to it whatever a
 // call needs: a smaller one would fail another thread's launch between its own two steps.
 constexpr int kSortBytes = (33 * kPlaceFastExperts + 1) * 4;
+constexpr int kUnasked = 40 * 1024;
+template <typename... P>
+bool ask(void (*kern)(P...)) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) == cudaSuccess;
+}
 
 // ------------------------------------------------------------------------------------------ router
 // One warp a token: softmax over n_expert logits (max, then sum of exp in lane-strided order reduced by a
@@ -467,9 +472,9 @@ int exl3b200_moe_scatter(const int32_t* ids, int64_t n_pairs, int64_t n_expert, 
     const size_t smem = (size_t)(n_expert + 1) * 4;
     // the small sort and the placement also hold the fast placement's [32][n_expert] table when it fits
     const size_t smem_place = smem + (n_expert <= kPlaceFastExperts ? (size_t)32 * n_expert * 4 : 0);
-    if (smem_place > 48 * 1024 &&
-        (cudaFuncSetAttribute(k_scatter_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess ||
-         cudaFuncSetAttribute(k_scatter_place, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess))
+    // 48 KB, their static arrays among them, are what kernels have without asking
+    if ((smem_place > kUnasked && (!ask(k_scatter_small) || !ask(k_scatter_place))) ||
+        (smem > kUnasked && (!ask(k_scatter_hist) || !ask(k_scatter_scan))))
         return -6;
     if (n_pairs <= kSmallPairs) {
         k_scatter_small<<<1, 1024, smem_place, st>>>(ids, n_pairs, (int)n_expert, expert_base, sorted_tok,
@@ -479,8 +484,11 @@ int exl3b200_moe_scatter(const int32_t* ids, int64_t n_pairs, int64_t n_expert, 
     if (!work) return -5;
     const int nb = (int)((n_pairs + kScatterChunk - 1) / kScatterChunk);
     int32_t* hist = static_cast<int32_t*>(work);
+    // a step comes only after the one whose results it takes for places to write to
     k_scatter_hist<<<nb, kScatterChunk, smem, st>>>(ids, n_pairs, (int)n_expert, expert_base, hist);
+    if (cudaGetLastError() != cudaSuccess) return -6;
     k_scatter_scan<<<1, 1024, smem, st>>>(hist, nb, (int)n_expert, expert_offset);
+    if (cudaGetLastError() != cudaSuccess) return -6;
     k_scatter_place<<<nb, kScatterChunk, smem_place, st>>>(ids, n_pairs, (int)n_expert, expert_base, hist,
                                                            expert_offset, sorted_tok);
     return cudaGetLastError() == cudaSuccess ? 0 : -6;
@@ -500,9 +508,7 @@ int exl3b200_router_scatter(const float* logits, int64_t n_tok, int64_t n_route,
 #define EXL3B_RS(R)                                                                                                  \
     do {                                                                                                             \
         auto kern = k_route_scatter_small<R>;                                                                        \
-        if (smem > 48 * 1024 &&                                                                                      \
-            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) != cudaSuccess)      \
-            return -6;                                                                                               \
+        if (smem > kUnasked && !ask(kern)) return -6;                                                                \
         kern<<<1, 1024, smem, st>>>(logits, n_tok, (int)n_route, (int)top_k, ids, w, (int)n_expert, expert_base,     \
                                     sorted_tok, expert_offset);                                                      \
     } while (0)

@@ -1,6 +1,9 @@
 """The router on a GPU where its calls are unusual: slots without an expert before a rank whose first expert is a negative
 number, groups with a single expert left, calls from several threads at once, plans made under graph capture."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -71,3 +74,41 @@ def test_calls_from_several_threads_at_once():
     assert not failed, (len(failed), failed[0])
     for _, _, ids, sort, _, old, olds in plans:
         assert torch.equal(ids, old) and all(torch.equal(sort[n], o) for n, o in zip([n for n in sorted(sort) if n != "expert_base"], olds))
+
+
+@pytest.mark.parametrize("local", [12287, 12288, 16384])
+@pytest.mark.parametrize("T", [40, 300])
+def test_the_largest_ranks(T, local):
+    """Counts of a rank's experts past the 48 KB of shared memory that a kernel has without asking."""
+    base = 100 - local                      # its last experts are the ones there are
+    _, ids, _, sort = run(logits_of(T, T, 100), 8, local, base)
+    tok, off = sorted_by_definition(ids.cpu().numpy(), local, base)
+    assert np.array_equal(sort["expert_offset"].cpu().numpy(), off)
+    assert np.array_equal(sort["sorted_tok"].cpu().numpy(), tok)
+
+
+def equal_sort(ids, local, base, tok, off):
+    for want, got in zip(sorted_by_definition(ids.cpu().numpy(), local, base), (tok, off)):
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
+def scatter_of_nearly_48_kilobytes():
+    native, stream = dense.native(), torch.cuda.current_stream().cuda_stream
+    for T in (20, 32):
+        for local in (371, 372, 373):
+            ids = torch.randint(-1, 400, (T, 8), generator=torch.Generator().manual_seed(T), dtype=torch.int32).cuda()
+            tok, off = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (T * 8, local + 1))
+            native.moe_scatter(ids.data_ptr(), T * 8, local, 0, tok.data_ptr(), off.data_ptr(), None, stream)
+            equal_sort(ids, local, 0, tok, off)
+            l, w = logits_of(T, T, 400), torch.empty((T, 8), device="cuda")
+            native.router_scatter(l.data_ptr(), T, 400, 8, ids.data_ptr(), w.data_ptr(), local, 0, tok.data_ptr(), off.data_ptr(),
+                                  None, stream)
+            equal_sort(ids, local, 0, tok, off)
+
+
+@pytest.mark.parametrize("what", ["scatter"])
+def test_a_sort_of_nearly_48_kilobytes(what):
+    """Tables of 48 KB less than a kernel's static arrays. In a process of its own: a kernel keeps the limit that a larger call
+    has set."""
+    code = f"import conftest, test_router_edges as t; t.{what}_of_nearly_48_kilobytes()"
+    subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parent, check=True, timeout=300)
