@@ -445,8 +445,9 @@ int launch(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
     if (!fused) return chain_launch(k_route<RPL, DT, WIDE>, dim3((unsigned)((p->n_tok + 3) / 4)), dim3(128), 0, 1, st, *p);
     auto kern = k_route_sort<RPL, DT, WIDE>;
     const size_t smem = fused_bytes(p->n_tok * p->top_k, p->n_local);
-    // the same limit whatever this call needs: a smaller one would fail another thread's launch between its own two steps
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedBytes) != cudaSuccess)
+    // 48 KB, the static array among them, need no asking. The same limit whatever this call needs: a smaller one would fail another
+    // thread's launch between its own two steps
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedBytes) != cudaSuccess)
         return -6;
     const int ctas = (int)(p->n_tok > 28 ? 8 : (p->n_tok + 3) / 4);
     return chain_launch(kern, dim3(ctas), dim3(kFusedThreads), smem, ctas, st, *p);

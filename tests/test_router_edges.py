@@ -106,7 +106,13 @@ def scatter_of_nearly_48_kilobytes():
             equal_sort(ids, local, 0, tok, off)
 
 
-@pytest.mark.parametrize("what", ["scatter"])
+def router_of_nearly_48_kilobytes():
+    for local in (992, 993, 994, 995):
+        _, ids, _, sort = run(logits_of(1, 44, 1000), 8, local, 3)
+        equal_sort(ids, local, 3, sort["sorted_tok"], sort["expert_offset"])
+
+
+@pytest.mark.parametrize("what", ["scatter", "router"])
 def test_a_sort_of_nearly_48_kilobytes(what):
     """Tables of 48 KB less than a kernel's static arrays. In a process of its own: a kernel keeps the limit that a larger call
     has set."""
