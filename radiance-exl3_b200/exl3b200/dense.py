@@ -19,6 +19,7 @@ F8 = 1024 + 0x3B8                       # EXL3B_F8
 DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
 ACTS = {"none": 0, "silu_mul": 1}
 SCORES = {"softmax": 0, "sigmoid": 1}
+SORT_PAIRS = 2048                       # a sort of up to so many pairs needs no work buffer
 GATES = {"none": 0, "token": 1, "channel": 2, "element": 3}
 
 _native = None
@@ -248,7 +249,8 @@ class Router(_Plan):
     (renorm), times scale. logits in f32, f16 or bf16.
 
     sorted_tok [tokens * top_k] and expert_offset [local experts + 1] i32 (both or neither): the pairs sorted over the experts
-    from expert_base on, as GroupedMm reads them. A plan that sorts has a work buffer: its runs come one after another."""
+    from expert_base on, as GroupedMm reads them. A plan that sorts more than 2048 pairs has a work buffer: its runs come one
+    after another, and one made under graph capture runs on the capturing stream, or on streams that wait for it."""
     _entry = "exl3b200_router"
 
     def __init__(self, *, logits, top_k, ids, w, score="softmax", bias=None, groups=1, keep_groups=1, group_top=1, renorm=False,
@@ -276,10 +278,13 @@ class Router(_Plan):
             if expert_offset.dim() != 1 or expert_offset.shape[0] < 2:
                 raise ValueError(f"expert_offset has shape {tuple(expert_offset.shape)}, not (local experts + 1,)")
             d.n_local, d.expert_base = expert_offset.shape[0] - 1, expert_base
-            work = torch.empty(native().scatter_work_bytes(d.n_tok * top_k, d.n_local), dtype=torch.uint8, device=logits.device)
-            d.work = work.data_ptr()
-            # a run may come on any stream: whatever used the buffer's memory before is done by then
-            torch.cuda.current_stream(dev).synchronize()
+            if d.n_tok * top_k > SORT_PAIRS:
+                work = torch.empty(native().scatter_work_bytes(d.n_tok * top_k, d.n_local), dtype=torch.uint8, device=logits.device)
+                d.work = work.data_ptr()
+                # a run may come on any stream: whatever used the buffer's memory before is done by then. Under capture it is
+                # the graph's own memory, in the capturing stream's order
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(dev).synchronize()
         self._finish(d, dev, logits, bias, ids, w, sorted_tok, expert_offset, work)
 
 

@@ -85,3 +85,15 @@ def test_a_router_sorts_with_both_arrays_or_neither(launched):
             dense.Router(top_k=2, **{**t, one: None})
     dense.Router(top_k=2, **{**t, "sorted_tok": None, "expert_offset": None}).run()
     assert len(enqueued(launched)) == 1
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+@pytest.mark.parametrize("T,waits", [(4, 0), (1024, 0), (1025, 1)])
+def test_a_router_waits_for_its_work_buffer_only_where_it_has_one(launched, monkeypatch, T, waits, capturing):
+    """Of up to 2048 pairs it has none; under capture there is nothing to wait for, and waiting would end the capture."""
+    monkeypatch.setattr(dense._native, "scatter_work_bytes", lambda *a: 4096, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    plan = dense.Router(top_k=2, logits=Fake(T, 16, dtype=F32), ids=Fake(T, 2, dtype=I32), w=Fake(T, 2, dtype=F32),
+                        sorted_tok=Fake(2 * T, dtype=I32), expert_offset=Fake(17, dtype=I32))
+    assert [n for n, _ in launched].count("synchronize") == (0 if capturing else waits)
+    assert bool(plan.desc.work) == bool(waits)

@@ -118,3 +118,18 @@ def test_a_sort_of_nearly_48_kilobytes(what):
     has set."""
     code = f"import conftest, test_router_edges as t; t.{what}_of_nearly_48_kilobytes()"
     subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parent, check=True, timeout=300)
+
+
+@pytest.mark.parametrize("T", [8, 200, 700])
+def test_a_plan_made_under_capture(T):
+    """As other plans can be: in one launch, with the one-block sort, and with the sort that has a work buffer."""
+    l = logits_of(1, T, 256)
+    _, want, _, want_sort = run(l, 8, 256)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, ids, _, sort = run(l, 8, 256)
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(ids, want)
+        assert all(torch.equal(sort[n], want_sort[n]) for n in ("sorted_tok", "expert_offset"))
+        ids.zero_()
