@@ -458,13 +458,15 @@ int     exl3b200_f8_dequantize(const uint8_t* codes, int64_t codes_pitch, const 
  *   the largest sum; of their experts the top_k with the largest c are chosen, in descending order -> ids i32 [n_tok][top_k]
  *   w f32 [n_tok][top_k] = scale * s of each, divided first by their sum over the chosen ones (renorm)
  * Ties go to the lower group and the lower expert, and scores compare as the real numbers do: by the logits, or in 64 bits
- * where a bias or a sum of two needs it. Masked experts, never chosen: a logit or a c that is -inf or NaN (their logits add
- * nothing to the softmax); +inf logits count as the largest f32. A slot for which no expert is left: id -1, w 0.
+ * where a bias or a sum of two needs it. Masked experts are never chosen: those whose logit is -inf or NaN (it adds nothing to
+ * the softmax) or whose c is (their logit counts in the softmax as any other). They are left out of their group's sum too: a
+ * group with one expert left is ranked by that c alone, a group with none comes last. +inf logits count as the largest f32.
+ * A slot for which no expert is left: id -1, w 0.
  * sorted_tok i32 [n_tok * top_k] and expert_offset i32 [n_local + 1], if given: moe_scatter of the ids over
  * [expert_base, expert_base + n_local), `work` as moe_scatter's (with up to 2048 pairs it may be NULL); one launch for up
- * to 128 tokens and 1024 local experts while the sort is small. logits f32 / f16 / bf16, their row pitch in elements. n_expert <= 2048, a multiple of n_group
- * <= 32 (no power of two of them: up to 1024 experts always, more while 64 a lane hold a group); top_k <= 32 and no more than
- * the kept groups hold. */
+ * to 128 tokens and 1024 local experts while the sort is small. logits f32 / f16 / bf16, their row pitch in elements.
+ * n_expert <= 2048, a multiple of n_group <= 32 (no power of two of them: up to 1024 experts always, more while 64 a lane hold
+ * a group); top_k <= 32 and no more than the kept groups hold. */
 enum { EXL3B_SCORE_SOFTMAX = 0, EXL3B_SCORE_SIGMOID = 1 };
 typedef struct Exl3bRouter {
     int64_t      n_tok, n_expert, top_k;

@@ -244,7 +244,7 @@ class GroupedMm(_Plan):
 
 class Router(_Plan):
     """Which experts a token goes to: scores ("softmax" or "sigmoid" of logits [tokens, experts]), compared with bias [experts]
-    f32 added, the keep_groups best of `groups` groups (by the sum of their group_top best), the top_k best of those ->
+    f32 added, the keep_groups best of `groups` groups (by the sum of their group_top best unmasked ones), the top_k best of those ->
     ids [tokens, top_k] i32 (-1 where none is left) and w [tokens, top_k] f32: the scores without the bias, divided by their sum
     (renorm), times scale. logits in f32, f16 or bf16.
 

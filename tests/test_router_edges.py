@@ -133,3 +133,43 @@ def test_a_plan_made_under_capture(T):
         assert torch.equal(ids, want)
         assert all(torch.equal(sort[n], want_sort[n]) for n in ("sorted_tok", "expert_offset"))
         ids.zero_()
+
+
+NONE = float("-inf")
+LONE = [                                                        # c by group, groups kept, the chosen experts
+    ([[.875], [.5, .25], [], [.125, .1875]], 1, [0, -1, -1]),
+    ([[.875], [.5, .25], [], [.125, .1875]], 2, [0, 4, 5]),
+    ([[], [.5], [], [.0625, .125]], 3, [4, 13, 12]),
+    ([[.75 + 2.0 ** -22], [.5, .25]], 1, [0, -1, -1]),          # sums that the 64-bit scores tell apart
+    ([[.75 - 2.0 ** -22], [.5, .25]], 1, [4, 5, -1]),
+    ([[.75], [.5, .25]], 1, [0, -1, -1]),                       # and equal ones
+    ([[.5, .25], [.75]], 1, [0, 1, -1]),
+    ([[-.125], [-.0625, -.125]], 1, [0, -1, -1])]
+
+
+@pytest.mark.parametrize("by", ["logit", "bias"])
+@pytest.mark.parametrize("c,keep,want", LONE)
+@pytest.mark.parametrize("T", [3, 300])
+def test_a_group_with_one_expert_left_is_ranked_by_it(T, c, keep, want, by):
+    """Masked experts, by their logit or by their bias, are left out of their group's sum of two. Sigmoid's s is 1/2 throughout."""
+    c = torch.tensor([(g + [NONE] * 4)[:4] for g in (c + [[]] * 4)[:4]]).reshape(16)
+    row, bias = torch.zeros(16), c - 0.5
+    if by == "logit":
+        row, bias = torch.where(c == NONE, NONE, row), bias.nan_to_num(neginf=0.25)
+    logits = row.expand(T, 16).contiguous().cuda()
+    _, ids, w, _ = run(logits, 3, score="sigmoid", bias=bias.cuda(), groups=4, keep_groups=keep, group_top=2)
+    assert ids.tolist() == [want] * T
+    assert w.tolist() == [[0.0 if e < 0 else 0.5 for e in want]] * T
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_an_expert_masked_by_its_bias_still_counts_in_the_softmax(score):
+    """Its logit does; a masked logit does not."""
+    l, bias = torch.zeros((2, 8), device="cuda"), torch.zeros(8, device="cuda")
+    bias[:4] = NONE
+    l[1, [0, 7]] = NONE
+    _, ids, w, _ = run(l, 4, score=score, bias=bias)
+    assert ids.tolist() == [[4, 5, 6, 7], [4, 5, 6, -1]]
+    of = [2.0 ** -3, 1 / 6] if score == "softmax" else [0.5, 0.5]
+    want = torch.tensor([[of[0]] * 4, [of[1]] * 3 + [0.0]], dtype=torch.float64)
+    assert ((w.cpu().double() - want).abs() <= 2.0 ** -24 * 88 * want).all()      # test_router's tolerance, z the largest logit
