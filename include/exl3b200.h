@@ -500,8 +500,9 @@ int     exl3b200_router(const Exl3bRouter* router, void* stream);
  * (MXFP4 out: 32); x, w and y rows on 16-byte boundaries (MXFP4 out: 4); n_expert <= 2048.
  * EXL3B_F8: x and w e4m3 codes, x_scales f32 [x_rows][ceil(n_in / 128)] as f8_quantize writes them, w_scales f32, dense,
  * [n_expert][blocks][ceil(n_in / 128)], one for 128 weight rows x 128 inputs (SILU_MUL: ceil(n_out / 128) blocks of gate rows
- * and then as many of up rows): z[n] = sum over blocks b of 128 k of x_scales[t][b] * w_scales[e][n / 128][b] * (the sum over
- * k of b), each such sum on the tensor cores, the blocks and their scales in f32. y in f32, f16 or bf16. */
+ * and then as many of up rows): z[n] = sum over blocks b of 128 k of (x_scales[t][b] * w_scales[e][n / 128][b]) * (the sum
+ * over k of b), each such sum on the tensor cores, the blocks and their scales in f32: the product of a block's two scales has
+ * to be a normal f32 number (2^-126 to 2^128) wherever the block's codes are not all zero. y in f32, f16 or bf16. */
 enum { EXL3B_ACT_NONE = 0, EXL3B_ACT_SILU_MUL = 1 };
 typedef struct Exl3bGroupedMm {
     int64_t        n_expert, n_rows, n_out, n_in;

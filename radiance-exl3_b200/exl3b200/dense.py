@@ -197,8 +197,9 @@ class GroupedMm(_Plan):
     x [x_rows, n_in] and w [experts, w_rows, n_in] in f16 or bf16; or MXFP4 codes (uint8, half as wide) with x_scales
     [x_rows, n_in / 32] and w_scales from mx4_tile_scales; or FP8 (float8_e4m3fn) with f32 x_scales [x_rows, ceil(n_in / 128)]
     and w_scales [experts, blocks, ceil(n_in / 128)], a block each 128 weight rows (silu_mul: ceil(n_out / 128) blocks of gate
-    rows, then as many of up rows). y [rows, n_out] in f32, f16 or bf16, or (not from FP8) MXFP4 codes with y_scales. expert_offset i32 [experts + 1] (None: one expert); sorted_tok i32 [rows] (None: no dropped slot). top_k:
-    row i reads x row sorted_tok[i] // top_k; 0: x is sorted already."""
+    rows, then as many of up rows), the two scales' product a normal f32 number. y [rows, n_out] in f32, f16 or bf16, or (not
+    from FP8) MXFP4 codes with y_scales. expert_offset i32 [experts + 1] (None: one expert); sorted_tok i32 [rows] (None: no
+    dropped slot). top_k: row i reads x row sorted_tok[i] // top_k; 0: x is sorted already."""
     _entry = "exl3b200_grouped_mm"
 
     def __init__(self, *, x, w, y, expert_offset=None, sorted_tok=None, top_k=0, act="none", x_scales=None,
