@@ -79,6 +79,10 @@ typedef struct Exl3bGmmOp {
     int32_t*       err;                  /* device word: set nonzero when a bounded wait gives up */
 } Exl3bGmmOp;
 
+/* The form that an FP8 product takes (exl3b200_gmm8.cu), for tests of each: 0 the wide one, otherwise the narrow one with as many
+ * CTAs a unit. */
+int exl3b_gmm8_form(int64_t n_expert, int64_t n_rows, int64_t n_out, int64_t n_in, int act, int sm_count);
+
 /* router (exl3b200_route.cu). A group has 2^group_shift lanes of a warp, each lane_experts neighbouring experts of it. */
 typedef struct Exl3bRouteOp {
     int64_t      n_tok;

@@ -492,28 +492,48 @@ int64_t likely_units(const Exl3bGmmOp* p, int nt, int64_t blk) {
     return (some > live ? some : live) * ((p->n_out + blk - 1) / blk);
 }
 
-template <bool ACT>
-int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
+// 0: the wide form; otherwise the narrow one, with as many CTAs a unit, each a part of its k.
+int form_of(const Exl3bGmmOp* p, int sm_count) {
     // The wide form where its units cost less: a unit's stage there takes 3.1 times as long as a narrow one's (2 times where the
     // SMs have a unit each at most), and its start and end as long as five of those; narrow units run two an SM. Narrow and wide,
     // us: 64 experts, 2048 -> 512 silu_mul, 28 rows each 28.3 and 29.1, 40 rows 32.9 and 29.9, 130 rows 62.4 and 40.7; 640 ->
     // 2560, 40 rows 27.5 and 27.8, 96 rows 47.4 and 36.9; 300 experts of 96 rows, 448 -> 160 silu_mul 30.9 and 32.1; one expert,
     // 4096 -> 1536, 512 rows 17.8 and 22.3, 1024 rows 30.2 and 22.7.
     const int64_t nck = (p->n_in + 127) / 128, sm = sm_count;
-    const int64_t wide_units = likely_units(p, 128, ACT ? 128 : 256), narrow_units = likely_units(p, 32, ACT ? 64 : 128);
+    const int64_t wide_units = likely_units(p, 128, p->act ? 128 : 256), narrow_units = likely_units(p, 32, p->act ? 64 : 128);
     const int64_t wide_cost = wide_units > sm ? wide_units * (31 * nck + 50) : sm * (20 * nck + 50);
-    if (wide_cost < 10 * nck * (narrow_units > 2 * sm ? narrow_units : 2 * sm)) return wide::launch<ACT>(p, sm_count, st);
-    const int64_t most = most_units(p, 32, 1);
-    int64_t split = sm_count / most;                          // so the grid has room for a cluster a unit: the kernel counts on it
+    if (wide_cost < 10 * nck * (narrow_units > 2 * sm ? narrow_units : 2 * sm)) return 0;
+    int64_t split = sm / most_units(p, 32, 1);                // so the grid has room for a cluster a unit: the kernel counts on it
     if (split > nck / 4) split = nck / 4;
     if (split > kMaxSplit) split = kMaxSplit;
-    if (split >= 2) return launch<true, ACT>(p, sm_count, (int)split, st);
+    return split >= 2 ? (int)split : 1;
+}
+
+template <bool ACT>
+int launch_form(const Exl3bGmmOp* p, int sm_count, cudaStream_t st) {
+    const int form = form_of(p, sm_count);
+    if (form == 0) return wide::launch<ACT>(p, sm_count, st);
+    if (form > 1) return launch<true, ACT>(p, sm_count, form, st);
     return launch<false, ACT>(p, sm_count, 1, st);
 }
 
 }  // namespace
 
-extern "C" int exl3b_cuda_gmm8(const Exl3bGmmOp* p, int sm_count, void* stream) {
+extern "C" {
+
+int exl3b_gmm8_form(int64_t n_expert, int64_t n_rows, int64_t n_out, int64_t n_in, int act, int sm_count) {
+    Exl3bGmmOp p = {};
+    p.n_expert = (int32_t)n_expert;
+    p.n_rows = n_rows;
+    p.n_out = n_out;
+    p.n_in = n_in;
+    p.act = act;
+    return form_of(&p, sm_count);
+}
+
+int exl3b_cuda_gmm8(const Exl3bGmmOp* p, int sm_count, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return p->act ? launch_form<true>(p, sm_count, st) : launch_form<false>(p, sm_count, st);
 }
+
+}  // extern "C"
