@@ -173,8 +173,6 @@ static int64_t lane_experts(const Exl3bRouter* d, int* shift) {
     return (d->n_expert / d->n_group + (1 << s) - 1) >> s;
 }
 
-/* Also exl3b200_expert_block.c's, before its first step. */
-int exl3b_router_check(const Exl3bRouter* d);
 int exl3b_router_check(const Exl3bRouter* d) {
     if (!d) return RAD_E_INVAL;
     if (!is_float(d->dtype)) return RAD_E_DTYPE;

@@ -101,6 +101,9 @@ typedef struct Exl3bRouteOp {
     int32_t      n_local;
 } Exl3bRouteOp;
 
+/* What exl3b200_router refuses (RAD_OK: nothing); the expert block asks before its first step. */
+int exl3b_router_check(const Exl3bRouter* router);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,10 +3,9 @@
  * the gather, and block_norm again into the residual stream. Nothing here allocates or synchronises: one caller block is sized and carved up front, and a
  * forward only enqueues. */
 #include "exl3b200.h"
+#include "exl3b200_dense.h"
 
 #include <string.h>
-
-int exl3b_router_check(const Exl3bRouter* d);      /* exl3b200_dense.c */
 
 static int mis(const void* p, int64_t a) { return (int)((uintptr_t)p % (uintptr_t)a); }
 static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }

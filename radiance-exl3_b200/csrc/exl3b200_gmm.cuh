@@ -141,10 +141,9 @@ __device__ __forceinline__ void mma4_f16(uint32_t d, uint64_t a, uint64_t b, uin
     if constexpr (PAIR) EXL3B_MMA4("2", "f16");
     else EXL3B_MMA4("1", "f16");
 }
-template <bool PAIR>
-__device__ __forceinline__ void mma4_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    if constexpr (PAIR) EXL3B_MMA4("2", "f8f6f4");
-    else EXL3B_MMA4("1", "f8f6f4");
+__device__ __forceinline__ void mma4_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    const uint32_t acc = 0;
+    EXL3B_MMA4("1", "f8f6f4");
 }
 // The MMAs issued so far done -> one arrival on bar (PAIR: on both CTAs' bar of that offset).
 template <bool PAIR>

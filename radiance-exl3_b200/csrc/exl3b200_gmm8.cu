@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(Cfg<SPLIT, ACT>::THREADS, Cfg<SPLIT, ACT>::PER
                 proxy_fence();
                 wait(&d_empty[db.s], db.ph ^ 1);
                 fence_after();
-                mma4_f8<false>(tmem + db.s * NT, wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd0 + (uint64_t)(pipe.s * C::X_B >> 4), idesc, 0u);
+                mma4_f8(tmem + db.s * NT, wd0 + (uint64_t)(pipe.s * kW_B >> 4), xd0 + (uint64_t)(pipe.s * C::X_B >> 4), idesc);
                 commit_el<false>(&d_full[db.s]);
                 commit_el<false>(&empty[pipe.s]);
             }

@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_gmm8w(const __grid_constant__ C
                     proxy_fence();
                     wait(&d_empty[db.s], db.ph ^ 1);
                     fence_after();
-                    mma4_f8<false>(tmem + db.s * kGroups * kCols, xd0 + (uint64_t)(pipe.s * kX_B >> 4),
-                                  wd0 + (uint64_t)(pipe.s * kWideW_B >> 4), idesc, 0u);
+                    mma4_f8(tmem + db.s * kGroups * kCols, xd0 + (uint64_t)(pipe.s * kX_B >> 4),
+                            wd0 + (uint64_t)(pipe.s * kWideW_B >> 4), idesc);
                     commit_el<false>(&d_full[db.s]);
                     db.next(kDb);
                     commit_el<false>(&empty[pipe.s]);
