@@ -592,11 +592,16 @@ int64_t skinny_smem(int bits, int gu, int mch, int64_t kc_max, int64_t n_expert)
     return 256 + skinny_prefix_bytes(n_expert) + kNst * stage + (xr > red ? xr : red);
 }
 
+// The most of it, beside the kernel's static array. A kernel's limit is set to that whatever a launch needs: a smaller one would
+// fail another thread's launch between its own two steps.
+constexpr int kSkinnyMost = 227 * 1024 - 128;
+static_assert(kThreads / 32 * 4 <= 128, "the static array");
+
 template <int BITS, int CB, bool GU, int MCH>
 int launch_skinny_t(const Exl3bOp* op, const Exl3bPlan* p, int kc_max, int n_blocks, cudaStream_t st) {
     auto kern = k_gemm_skinny<BITS, CB, GU, MCH>;
     const int smem = p->smem_bytes;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -6;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnyMost) != cudaSuccess) return -6;
     if (p->ksplit > 1 &&
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
         return -6;
@@ -755,7 +760,7 @@ int exl3b_plan_skinny(const Exl3bOp* op, int sm_count, Exl3bPlan* p) {
         mch /= 2;
         smem = skinny_smem(op->bits, gu, mch, kc_max, op->n_expert);
     }
-    if (smem > 227 * 1024) return -1;
+    if (smem > kSkinnyMost) return -1;
     const int64_t per_sm = smem <= 56 * 1024 ? 4 : smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
     int64_t clusters = sm_count * per_sm / S;
     const int64_t units_max = (live + op->T / (16 * mch) + 1) * n_blocks;

@@ -548,10 +548,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
+// Beside the kernel's static arrays. Its limit whatever a launch needs: a smaller one would fail another thread's launch between
+// its own two steps.
+constexpr int kTcMost = 223 * 1024;
+
 template <int BITS, int CB, bool GU>
 int launch_tc_t(const CUtensorMap& map, const Exl3bOp* op, int n_pairs, int grid, int smem, bool wide, cudaStream_t st) {
     auto kern = wide ? k_gemm_tc<BITS, CB, GU, true> : k_gemm_tc<BITS, CB, GU, false>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -6;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcMost) != cudaSuccess) return -6;
     kern<<<grid, kTcThreads, smem, st>>>(map, *op, n_pairs);
     return cudaGetLastError() == cudaSuccess ? 0 : -6;
 }
@@ -640,7 +644,7 @@ int exl3b_cuda_gemm_tc(const Exl3bOp* op, const void* xin, int64_t xin_pitch, in
     int rc = make_map(&map, xin, op->T, cols, xin_pitch);
     if (rc) return rc;
     const int64_t smem = exl3b_tc_smem_bytes(op->bits) + ((op->n_expert + 1) * 4 + 15) / 16 * 16 + 16;
-    if (smem > 227 * 1024) return -1;
+    if (smem > kTcMost) return -1;
     int grid = sm_count;
     // wide units (decode once a 128 rows) where experts hold many rows, the wide units still outnumber the SMs
     // several times over, and a unit's decode is long against its epilogue (an input of >= 1024 columns: gate_up's
