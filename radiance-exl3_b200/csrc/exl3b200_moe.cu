@@ -26,9 +26,13 @@ constexpr int kSmallPairs = 2048;     // at most this many pairs: one block does
 // call needs: a smaller one would fail another thread's launch between its own two steps.
 constexpr int kSortBytes = (33 * kPlaceFastExperts + 1) * 4;
 constexpr int kUnasked = 40 * 1024;
-template <typename... P>
-bool ask(void (*kern)(P...)) {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) == cudaSuccess;
+template <auto KERN>
+bool ask() {                          // once a device
+    static bool allowed[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (!allowed[dev]) allowed[dev] = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes) == cudaSuccess;
+    return allowed[dev];
 }
 
 // ------------------------------------------------------------------------------------------ router
@@ -473,8 +477,8 @@ int exl3b200_moe_scatter(const int32_t* ids, int64_t n_pairs, int64_t n_expert, 
     // the small sort and the placement also hold the fast placement's [32][n_expert] table when it fits
     const size_t smem_place = smem + (n_expert <= kPlaceFastExperts ? (size_t)32 * n_expert * 4 : 0);
     // 48 KB, their static arrays among them, are what kernels have without asking
-    if ((smem_place > kUnasked && (!ask(k_scatter_small) || !ask(k_scatter_place))) ||
-        (smem > kUnasked && (!ask(k_scatter_hist) || !ask(k_scatter_scan))))
+    if ((smem_place > kUnasked && (!ask<k_scatter_small>() || !ask<k_scatter_place>())) ||
+        (smem > kUnasked && (!ask<k_scatter_hist>() || !ask<k_scatter_scan>())))
         return -6;
     if (n_pairs <= kSmallPairs) {
         k_scatter_small<<<1, 1024, smem_place, st>>>(ids, n_pairs, (int)n_expert, expert_base, sorted_tok,
@@ -507,10 +511,9 @@ int exl3b200_router_scatter(const float* logits, int64_t n_tok, int64_t n_route,
         cudaStream_t st = as_stream(stream);
 #define EXL3B_RS(R)                                                                                                  \
     do {                                                                                                             \
-        auto kern = k_route_scatter_small<R>;                                                                        \
-        if (smem > kUnasked && !ask(kern)) return -6;                                                                \
-        kern<<<1, 1024, smem, st>>>(logits, n_tok, (int)n_route, (int)top_k, ids, w, (int)n_expert, expert_base,     \
-                                    sorted_tok, expert_offset);                                                      \
+        if (smem > kUnasked && !ask<k_route_scatter_small<R>>()) return -6;                                          \
+        k_route_scatter_small<R><<<1, 1024, smem, st>>>(logits, n_tok, (int)n_route, (int)top_k, ids, w,             \
+                                                        (int)n_expert, expert_base, sorted_tok, expert_offset);      \
     } while (0)
         if (n_route <= 256) EXL3B_RS(8);
         else EXL3B_RS(16);

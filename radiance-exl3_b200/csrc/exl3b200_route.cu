@@ -447,8 +447,14 @@ int launch(const Exl3bRouteOp* p, int fused, cudaStream_t st) {
     const size_t smem = fused_bytes(p->n_tok * p->top_k, p->n_local);
     // 48 KB, the static array among them, need no asking. The same limit whatever this call needs: a smaller one would fail another
     // thread's launch between its own two steps
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedBytes) != cudaSuccess)
-        return -6;
+    if (smem > 40 * 1024) {
+        static bool allowed[64];                              // once a device
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -6;
+        if (!allowed[dev] && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedBytes) != cudaSuccess)
+            return -6;
+        allowed[dev] = true;
+    }
     const int ctas = (int)(p->n_tok > 28 ? 8 : (p->n_tok + 3) / 4);
     return chain_launch(kern, dim3(ctas), dim3(kFusedThreads), smem, ctas, st, *p);
 }
