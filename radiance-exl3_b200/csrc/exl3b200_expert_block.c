@@ -1,7 +1,7 @@
 /* exl3b200_expert_block.c -- a residual MoE block over experts that are not EXL3 records, driven from C: block_norm (with
- * MXFP4 output, or FP8 rows behind it), the router's product, router_scatter or the router, the experts' two grouped products,
- * the gather, and block_norm again into the residual stream. Nothing here allocates or synchronises: one caller block is sized and carved up front, and a
- * forward only enqueues. */
+ * MXFP4 output, or FP8 rows behind it), the router's product, router_scatter or the router, the experts' two grouped
+ * products, the gather, and block_norm again into the residual stream. Nothing here allocates or synchronises: one caller
+ * block is sized and carved up front, and a forward only enqueues. */
 #include "exl3b200.h"
 #include "exl3b200_dense.h"
 

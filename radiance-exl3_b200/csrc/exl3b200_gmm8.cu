@@ -20,8 +20,9 @@
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok
 //   8..11   sums: each warp 32 weight rows, then its outputs
 // Every wait is bounded; one that gives up sets the error word, and every role then drains and leaves.
-// Few rows an expert are bounded by the weights' way from HBM: 191 live experts, 624 rows, 640 -> 2560, 313 MB in 50 us in a graph
-// (6.3 TB/s); one token's ten experts, 2048 -> 512 silu_mul, 21 MB, in 10 us, by the launch, the set-up and the first loads.
+// Few rows an expert are bounded by the weights' way from HBM: 173 live experts, 629 rows, 640 -> 2560, 286 MB in 50 us (5.7
+// TB/s); one token's ten experts, 2048 -> 512 silu_mul, 21 MB, in 10 us with its f8_quantize, by the launches, the set-up and
+// the first loads.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

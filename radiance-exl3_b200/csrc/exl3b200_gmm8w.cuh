@@ -5,9 +5,10 @@
 // shared memory, four bytes a lane a cycle: 174 against 138 us at 16 experts, 16060 rows, 4096 -> 1536, and 253 against 182 at
 // 418 experts of 20072 rows, 2048 -> 512 silu_mul.)
 //
-// Persistent over units (expert, a group of up to 128 of its sorted rows, a block of 256 weight rows; silu_mul: 128 gate rows and
-// their 128 up rows), one CTA an SM. A unit's weight rows are two groups of 128 columns of the accumulator, four summing warps each:
-// act NONE in order; silu_mul 64 gate rows and their 64 up rows, and the next 64 of each, so that a thread has both of its 64 outputs.
+// Persistent over units (expert, a group of up to 128 of its sorted rows, a block of 256 weight rows; silu_mul: 128 gate rows
+// and their 128 up rows), one CTA an SM. A unit's weight rows are two groups of 128 columns of the accumulator, four summing
+// warps each: act NONE in order; silu_mul 64 gate rows and their 64 up rows, and the next 64 of each, so that a thread has
+// both of its 64 outputs.
 // Warps of a CTA:
 //   0       weights: cp.async.bulk.tensor, 128-byte swizzled
 //   1       MMA issuer: four tcgen05.mma (kind::f8f6f4, M 128, N 256, K 32) a stage of 128 k, into one of two accumulators in
@@ -15,11 +16,15 @@
 //   2, 3    nothing: they leave their registers to the summing warps
 //   4..7    sorted rows: 16-byte cp.async through sorted_tok
 //   8..15   sums: 32 sorted rows and a group's 128 columns each, then their outputs
-// A stage's MMAs take 512 cycles, a stage about 1140 (16 experts). What is left is not the sums' instructions: with the sums left out
-// 128 us became 121, with the outputs too 112, with most of the loads as well 103. It is the round trip of an accumulator, of which
-// tensor memory holds two: the MMAs' completion, its barrier, the reads, their barrier and the next issue; then a unit's outputs, which
-// wait for its last stage. In a graph 184 us at 418 experts of 20072 rows, 2048 -> 512 silu_mul (0.9 GB, 4.9 TB/s); 72 at 64
-// experts of them; 126 at 16 experts, 16060 rows, 4096 -> 1536 (1630 TFLOP/s).
+// A stage's MMAs take 512 cycles, a stage 920 (16 experts; 64 experts 820) once a unit's first four are over, a unit 34700
+// (18700): 5200 (5500) besides its stages, for its outputs and the accumulators' refilling after them. What is left is not
+// the sums' instructions: with the sums left out 128 us became 121, with the outputs too 112, with most of the loads as well
+// 103. It is the round trip of an accumulator, of which tensor memory holds two: the MMAs' completion, its barrier, the
+// reads, their barrier and the next issue; then a unit's outputs, which wait for its last stage; then the last round, which
+// a third of the CTAs or fewer take part in (16 and 64 experts: five or six units a CTA).
+// 20 runs in a graph, the SMs at 1.6 to 1.75 GHz by the kernel's own clock: 177 us at 410 live experts of 20075 rows, 2048 ->
+// 512 silu_mul (0.88 GB, 5.0 TB/s); 75 at 64 experts of them (with the rows' f8_quantize); 130 at 16 experts, 16066 rows,
+// 4096 -> 1536 (202 GFLOP, 1560 TFLOP/s). Run on end, at the power limit's 1.3 to 1.5 GHz: 207, 83 and 148 us (1365 TFLOP/s).
 #pragma once
 
 #include <cuda.h>

@@ -10,17 +10,23 @@
 // a power of two of groups leaves each), so that a group's maximum is a few shuffles and the lower of two lanes has the lower
 // experts. Experts that are masked (a logit or a c that is -inf or NaN) have key 0, below every other key.
 //
-// Choices are made as the real numbers order them, not as their roundings do. Without a bias and without sums of two the logits
-// are compared (both scores grow with them), else c. Each expert has a 32-bit key that orders as the number does, but for its
-// last bits, which hold the expert's place in the lane: one maximum finds both. 16-bit logits leave room for the whole expert,
-// and their keys are exact. Where two neighbours among the chosen ones, or the last chosen and the next, or the worst group kept
-// and the best one dropped, are nearer than the keys and the f32 scores behind them can tell, the token is routed again with
-// 64-bit scores, exactly (`again`; about one token in a hundred at most, unless logits are equal).
+// Choices are made as the real numbers order them, not as their roundings do. Without a bias and without sums of two the
+// logits are compared (both scores grow with them), else c. Each expert has a 32-bit key that orders as the number does, but
+// for its last bits, which hold the expert's place in the lane: one maximum finds both. 16-bit logits that are compared leave
+// room for the whole expert, and their keys are exact. Where two neighbours among the chosen ones, or the last chosen and the
+// next, or the worst group kept and the best one dropped, are nearer than the keys and the f32 scores behind them can tell,
+// the token is routed again with 64-bit scores, exactly (`again`). How often that is, by the thresholds below at N(0, 1.5)
+// logits: two tokens in a thousand with a bias (256 experts, eight chosen, sums of two; or 512, ten chosen); f32 softmax sums
+// of two without a bias 0.3 % (256 experts, eight chosen) and 1.8 % (512, sixteen). 16-bit logits hold equal ones, which sums
+// of two without a bias, having c for keys, take for too near: f16 4 % and 14 % there, bf16 29 % and 71 %.
 //
 // Bound by instructions, about a thousand a token in this case, and by their latency: a round is a maximum over the warp, its
 // lane and that lane's next key. Measured on one B200: 16384 tokens, 256 experts, sigmoid, bias, four of eight groups, eight
-// chosen 26 us (all in 64 bits 43), of which the tokens routed again, a few us each at the grid's end, are 2 to 5; the 17 MB of
-// logits alone are 2.7. One token of 512 experts with its sort 5.6 us.
+// chosen 26 us (all in 64 bits 43), of which the tokens routed again, a few us each at the grid's end, are 2 to 5; the 17 MB
+// of logits alone are 2.7. Softmax without the bias 28 us in f32, 31 in f16, 49 in bf16; bf16, 512 experts, sixteen chosen
+// 201. One token of 512 experts with its sort 5.6 us. A lane's sixteen keys (257 to 512 experts) lie in local memory where
+// they are sorted, but for 16-bit logits compared by themselves without the sort of the tokens: a frame of 64 bytes; the
+// forms for over 1024 experts with that sort spill up to 380 bytes.
 #include <cuda_runtime.h>
 #include <float.h>
 #include <stdint.h>
@@ -72,7 +78,8 @@ __device__ __forceinline__ float warp_max_of(float v) {
 // 1 / (1 + e^-z); below -20 its exponential, which it is to within 2^-28, and which stays in range while the value does.
 __device__ __forceinline__ float sigmoid(float z) { return z < -20.f ? expf(z) : 1.f / (1.f + expf(-z)); }
 
-// e^x from the special-function unit: within 2^-22 + |x| 2^-24 of the value.
+// e^x from the special-function unit: within 2^-22 + 1.3 |x| 2^-24 of the value (the product's rounding, and the constant's,
+// which is 2^-26 of it).
 __device__ __forceinline__ float exp_near(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
@@ -273,9 +280,11 @@ __device__ __forceinline__ void route(const Exl3bRouteOp& p, int64_t t, int lane
         }
     }
     // Nearer than this two c cannot be told apart: twice an f32 score's error and, relative to c, its own rounding and the bits of
-    // the key that hold a place. A sigmoid s is off by s (1 - s) (2^-22 + |z| 2^-24) for the exponential and s 1.5 2^-23 for
-    // the sum and the reciprocal, below 2^-22 in all. A softmax's exponentials are off by 2^-22 + 0.4 2^-24 of the largest
-    // score, `inv`, at most, their sum (the same way for all) by as much and one rounding a term, at most 69 of 2^-24.
+    // the key that hold a place. A sigmoid s is off by s (1 - s) (2^-22 + 1.3 |z| 2^-24) for the exponential and s 1.5 2^-23 for
+    // the sum and the reciprocal, below 1.1 2^-22 in all. A softmax's exponentials are off by 2^-22 + 0.9 2^-24 of the largest
+    // score, `inv`, at most (|x| e^x is below 0.37, and the difference x is rounded too), the quotient and the product by one
+    // rounding each, their sum (the same way for all) by as much as a term and one rounding a term, at most 69 of 2^-24: 90 of
+    // 2^-24 for a difference, where 256 are taken.
     const float near = softmax ? 0x1p-16f * inv : 0x1p-20f;
     constexpr float near_rel = 0x1p-22f + (float)(LOW + 1) * 0x1p-23f;
     bool unsure = false;

@@ -244,10 +244,10 @@ class GroupedMm(_Plan):
 
 
 class Router(_Plan):
-    """Which experts a token goes to: scores ("softmax" or "sigmoid" of logits [tokens, experts]), compared with bias [experts]
-    f32 added, the keep_groups best of `groups` groups (by the sum of their group_top best unmasked ones), the top_k best of those ->
-    ids [tokens, top_k] i32 (-1 where none is left) and w [tokens, top_k] f32: the scores without the bias, divided by their sum
-    (renorm), times scale. logits in f32, f16 or bf16.
+    """Which experts a token goes to: scores ("softmax" or "sigmoid" of logits [tokens, experts]), compared with bias
+    [experts] f32 added, the keep_groups best of `groups` groups (by the sum of their group_top best, masked experts left
+    out), the top_k best of those -> ids [tokens, top_k] i32 (-1 where none is left) and w [tokens, top_k] f32: the scores
+    without the bias, divided by their sum (renorm), times scale. logits in f32, f16 or bf16.
 
     sorted_tok [tokens * top_k] and expert_offset [local experts + 1] i32 (both or neither): the pairs sorted over the experts
     from expert_base on, as GroupedMm reads them. A plan that sorts more than 2048 pairs has a work buffer: its runs come one
