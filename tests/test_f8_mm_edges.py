@@ -92,3 +92,14 @@ def test_the_narrow_forms_units_past_the_table():
         want = torch.einsum("ek,enk->en", xv[s], wv)
         tol = (128 + 1 + 5) * 2.0 ** -23 * torch.einsum("ek,enk->en", xv[s].abs(), wv.abs())
         close(y[s], want, tol, F32)
+
+
+@pytest.mark.parametrize("form,E,rows,N,K", FAR)
+def test_each_form_without_a_sort(form, E, rows, N, K):
+    """No sorted_tok: row i is slot i of token i / top_k, the last token's slots not all there."""
+    xq, xs, w, ws, xv = operands(5, E, -(-rows // 7), K, N, "none")
+    off = torch.tensor([rows * e // E for e in range(E + 1)], dtype=torch.int32, device="cuda")
+    y = torch.full((rows, N), float("nan"), dtype=F16, device="cuda")
+    dense.GroupedMm(x=xq, x_scales=xs, w=w, w_scales=ws, expert_offset=off, top_k=7, y=y).run(stream())
+    tok = torch.arange(rows, dtype=torch.int32, device="cuda")
+    close(y, *plain(xv, values_of(w, ws, N), tok, off, 7, "none", N), F16)
