@@ -22,8 +22,9 @@ def fill(x):
 
 def around(rows, lanes):
     """Rows at both ends and around the row of lane 2^31, `lanes` a row."""
-    at = (1 << 31) // lanes
-    return sorted({r for c in (0, 1024 // lanes, at - 1024 // lanes, at, rows // 2, rows - 1) for r in range(c - 2, c + 3) if 0 <= r < rows})
+    at, block = (1 << 31) // lanes, 1024 // lanes
+    near = {r for c in (0, block, at - block, at, rows // 2, rows - 1) for r in range(c - 2, c + 3)}
+    return sorted(r for r in near if 0 <= r < rows)
 
 
 def check(x, codes, scales, at):

@@ -15,8 +15,8 @@ from test_f8_mm import F8, F16, F32, FORMS, gpu, operands, plain, values_of  # n
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("x_by,w_by", [(-118, -2), (-3, -112), (-60, -60), (119, -20), (100, 2), (1, 100)])
 def test_scales_at_the_ends_of_their_range(form, x_by, w_by):
-    """x's scales times 2^x_by and the weight's times 2^w_by: from the least that f8_quantize makes to the largest of bf16 rows, with
-    products down to 2^-126 and values up to 2^120. A block of zeros may have a smaller product."""
+    """x's scales times 2^x_by and the weight's times 2^w_by: from the least that f8_quantize makes to the largest of bf16 rows,
+    with products down to 2^-126 and values up to 2^120. A block of zeros may have a smaller product."""
     counts, K, N = FORMS[form]
     rows = sum(counts)
     xq, xs, w, ws, xv = operands(3, len(counts), rows, K, N, "none")

@@ -44,10 +44,11 @@ def test_calls_from_several_threads_at_once():
     failed, plans = [], []
     for i, (T, k, local) in enumerate(shapes):
         plan, ids, _, sort = run(logits_of(i, T, 1024), k, local)
-        plans.append((plan, torch.cuda.Stream(), ids, sort, local, ids.clone(), [sort[n].clone() for n in sorted(sort) if n != "expert_base"]))
+        outs = [ids, sort["sorted_tok"], sort["expert_offset"]]
+        plans.append((plan, torch.cuda.Stream(), outs, [t.clone() for t in outs]))
     flat = torch.randint(0, 1000, (2000,), dtype=torch.int32, device="cuda")
-    outs = [(n, torch.empty(2000, dtype=torch.int32, device="cuda"), torch.empty(n + 1, dtype=torch.int32, device="cuda"))
-            for n in (1000, 450)]
+    scatters = [(n, torch.empty(2000, dtype=torch.int32, device="cuda"), torch.empty(n + 1, dtype=torch.int32, device="cuda"))
+                for n in (1000, 450)]
     torch.cuda.synchronize()
 
     def routes(plan, stream):
@@ -65,15 +66,15 @@ def test_calls_from_several_threads_at_once():
                 failed.append(e)
 
     threads = [threading.Thread(target=routes, args=p[:2]) for p in plans]
-    threads += [threading.Thread(target=sorts, args=(*o, torch.cuda.Stream())) for o in outs]
+    threads += [threading.Thread(target=sorts, args=(*o, torch.cuda.Stream())) for o in scatters]
     for t in threads:
         t.start()
     for t in threads:
         t.join()
     torch.cuda.synchronize()
     assert not failed, (len(failed), failed[0])
-    for _, _, ids, sort, _, old, olds in plans:
-        assert torch.equal(ids, old) and all(torch.equal(sort[n], o) for n, o in zip([n for n in sorted(sort) if n != "expert_base"], olds))
+    for _, _, outs, olds in plans:
+        assert all(torch.equal(t, old) for t, old in zip(outs, olds))
 
 
 @pytest.mark.parametrize("local", [12287, 12288, 16384])
